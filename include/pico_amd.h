@@ -172,6 +172,20 @@ void pico_relu_backward_gpu(struct PicoTensor* self);
 struct PicoTensor* pico_softmax_xent(struct PicoTensor* logits, const int32_t* labels);
 /* y = x * rstd * gain over the last dim of x [R, C], rstd = (mean(x^2) + eps)^-1/2 */
 struct PicoTensor* pico_rmsnorm(struct PicoTensor* x, struct PicoTensor* gain, float eps);
+/* y = (x - mean) * rstd * gain + bias over the last dim of x [R, C] (contiguous),
+ * rstd = (mean((x - mean)^2) + eps)^-1/2; bias may be NULL */
+struct PicoTensor* pico_layernorm(struct PicoTensor* x, struct PicoTensor* gain,
+                                  struct PicoTensor* bias, float eps);
+/* gated linear recurrence along the tokens of each sequence, channel by channel:
+ * h_t = s_t h_{t-1} + (1 - s_t) x_t, s = sigmoid(f); f, x token-major [batch*T, C]
+ * (contiguous or column views), h0 [batch, C] the state before the first token
+ * or NULL (zero).  f = -inf starts anew at a token.  Token by token: T = 1, and
+ * h0 the h before. */
+struct PicoTensor* pico_gated_scan(struct PicoTensor* f, struct PicoTensor* x,
+                                   struct PicoTensor* h0, int batch);
+/* the last token of each sequence of h [batch*T, C] (contiguous or a column view), as
+ * [batch, C]: the state a recurrence goes on from */
+struct PicoTensor* pico_last_token(struct PicoTensor* h, int batch);
 /* h = silu(a) * u, a and u of the same shape */
 struct PicoTensor* pico_swiglu(struct PicoTensor* a, struct PicoTensor* u);
 /* causal softmax(q k^T / sqrt(hd)) v per head; q, k, v token-major
@@ -205,6 +219,34 @@ struct PicoTensor* pico_matmul_add(struct PicoTensor* a, struct PicoTensor* b,
 struct PicoTensor* pico_matmul_gate_up(struct PicoTensor* a, struct PicoTensor* w);
 struct PicoTensor* pico_swiglu_matmul_add(struct PicoTensor* gate, struct PicoTensor* up,
                                           struct PicoTensor* w, struct PicoTensor* c);
+
+/* ---- mixture of experts (no reference counterpart) ----
+ * A feed-forward of E experts, each token choosing k of them:
+ *   gates = pico_route_topk(logits, k, &route)
+ *   xs = pico_expert_gather(x, route);  h = ... pico_expert_matmul(xs, w, route) ...
+ *   y  = pico_expert_combine(ys, gates, route, x)
+ * pico_route_topk: gates [tokens, k] = softmax over each token's k largest logits
+ *   [tokens, experts] (of equal ones the lowest index first); a logit of -inf is
+ *   never chosen, and where fewer than k are left the gate is 0 and the slot has
+ *   no expert (a row of -inf is a padding token).  *route lives in the current
+ *   arena.  Up to 1024 experts, k up to 64.
+ * pico_route_to_host: copies out the chosen experts [tokens*k] (-1: none) and the
+ *   experts' first rows [experts + 1]; either may be NULL.
+ * pico_expert_gather: the tokens' rows in expert order, [tokens*k, d]: a row for
+ *   every choice, zero rows behind the last expert's.
+ * pico_expert_matmul: rows of expert e times w[e], for w [experts, K, N].  Products
+ *   and their gradients take the matmul precision set when it is called
+ *   (PICO_MATMUL_FP8 runs them in bf16).
+ * pico_expert_combine: c + sum over a token's choices of gate times row, [tokens,
+ *   d]; c may be NULL. ---- */
+struct PicoRoute;
+struct PicoTensor* pico_route_topk(struct PicoTensor* logits, int k, struct PicoRoute** route);
+int pico_route_to_host(const struct PicoRoute* route, int32_t* experts, int32_t* offsets);
+struct PicoTensor* pico_expert_gather(struct PicoTensor* x, const struct PicoRoute* route);
+struct PicoTensor* pico_expert_matmul(struct PicoTensor* x, struct PicoTensor* w,
+                                      const struct PicoRoute* route);
+struct PicoTensor* pico_expert_combine(struct PicoTensor* ys, struct PicoTensor* gates,
+                                       const struct PicoRoute* route, struct PicoTensor* c);
 
 /* ---- nn (src/nn/linear.h:6-15) ---- */
 struct PicoLinear {

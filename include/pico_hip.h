@@ -369,6 +369,10 @@ int pk_fill_f32(int64_t n, float value, float* x, pk_stream_t stream);
  * zeros of a column-block view's gradient that nothing wrote) */
 int pk_fill2d_f32(int64_t rows, int64_t cols, float value, float* x, int64_t ld,
                   pk_stream_t stream);
+/* y[r*ldy + c] (+)= x[r*ldx + c] for r < rows, c < cols (no reference counterpart:
+ * rows taken out of a matrix, and their gradient put back) */
+int pk_copy2d_f32(int64_t rows, int64_t cols, const float* x, int64_t ldx, float* y, int64_t ldy,
+                  int flags, pk_stream_t stream);
 /* x[i] = mean + std * z_i, z_i ~ N(0,1) from a counter-based generator: element
  * i draws two uniforms from the 64-bit mix of (seed, i) and applies Box-Muller
  * (u1 in (0,1]), so the values do not depend on the launch shape.  Seeded
@@ -602,6 +606,107 @@ int pk_embed_fwd_f32(int64_t n, int64_t d, int64_t vocab, const int32_t* ids, co
 size_t pk_embed_bwd_workspace(int64_t n);
 int pk_embed_bwd_f32(int64_t n, int64_t d, int64_t vocab, const int32_t* ids, const float* dout,
                      float* dtable, void* workspace, size_t workspace_bytes, pk_stream_t stream);
+
+/* ---- layer norm (no reference counterpart) -------------------------------
+ * over rows of x [R, C], contiguous: y = (x - m) * r * g + b with m = mean(x),
+ * r = (mean((x - m)^2) + eps)^-1/2.  g [C]; b [C] or NULL (no bias).  mean and
+ * rstd [R] receive m and r for the backward; either may be NULL.
+ * backward, xh = (x - m) * r:
+ *   dx = dx_in + r*(g*dy - mean(g*dy) - xh*mean(g*dy*xh))  (dx_in NULL: without it;
+ *        dx_in may be dx)
+ *   dg (+)= sum_r dy*xh  (PK_ACCUM2),  db (+)= sum_r dy  (PK_ACCUM3)
+ * a NULL gradient is skipped; dg and db need pk_layernorm_bwd_workspace(R, C)
+ * bytes of device workspace.  Sums over rows in a fixed order. */
+int pk_layernorm_fwd_f32(int64_t R, int64_t C, float eps, const float* x, const float* g,
+                         const float* b, float* y, float* mean, float* rstd, pk_stream_t stream);
+size_t pk_layernorm_bwd_workspace(int64_t R, int64_t C);
+int pk_layernorm_bwd_f32(int64_t R, int64_t C, const float* x, const float* g, const float* mean,
+                         const float* rstd, const float* dy, const float* dx_in, float* dx, float* dg,
+                         float* db, int flags, void* workspace, size_t workspace_bytes,
+                         pk_stream_t stream);
+
+/* ---- gated linear recurrence (no reference counterpart) -------------------
+ * B sequences of T tokens, token t of sequence b in row b*T + t of [B*T, C]
+ * matrices; every channel on its own:
+ *   s_t = sigmoid(f_t),  h_t = s_t*h_{t-1} + (1 - s_t)*x_t,  h before the first
+ *   token = h0 [B, C], or zero when h0 is NULL
+ * f, x have row strides ldf, ldx >= C (column blocks of one projection are fine);
+ * h, dh are contiguous.  f = -inf starts anew (h_t = x_t), f = +inf keeps h.  One
+ * token at a time is T = 1 with h0 the state so far (h may be h0).
+ * backward: with G_t = dh_t + s_{t+1}*G_{t+1},
+ *   df (+)= G*(h_{t-1} - x)*s*(1 - s) (PK_ACCUM), dx (+)= (1 - s)*G (PK_ACCUM2),
+ *   dh0 (+)= s_1*G_1 (PK_ACCUM3); a NULL gradient is skipped.  The gradients'
+ *   buffers must not overlap each other.
+ * Both directions take pk_gated_scan_workspace(B, T, C) bytes of device workspace
+ * (0 for shapes that need none).  Sums in a fixed order. */
+size_t pk_gated_scan_workspace(int64_t B, int64_t T, int64_t C);
+int pk_gated_scan_fwd_f32(int64_t B, int64_t T, int64_t C, const float* f, int64_t ldf,
+                          const float* x, int64_t ldx, const float* h0, float* h, void* workspace,
+                          size_t workspace_bytes, pk_stream_t stream);
+int pk_gated_scan_bwd_f32(int64_t B, int64_t T, int64_t C, const float* f, int64_t ldf,
+                          const float* x, int64_t ldx, const float* h0, const float* h,
+                          const float* dh, float* df, int64_t lddf, float* dx, int64_t lddx,
+                          float* dh0, int flags, void* workspace, size_t workspace_bytes,
+                          pk_stream_t stream);
+
+/* ---- mixture of experts (no reference counterpart) ------------------------
+ * R tokens choose k of E experts each; slot t*k + j is token t's j-th choice,
+ * n = R*k.  Nothing is read back: group sizes stay on the device, so a captured
+ * graph replays with other routings.
+ * pk_route_topk_f32: experts[t, j] = the index of the j-th largest of token t's
+ *   logits [R, E] (row stride ldz; of equal ones the lowest index first, a NaN
+ *   above all), gates[t, j] = softmax over the chosen.  A logit of -inf is never
+ *   chosen: where fewer than k are left, the expert is -1 and the gate 0 (a
+ *   row of -inf, a padding token, has no expert at all).
+ * pk_route_topk_bwd_f32: dlogits (+)= g*(dg - sum_j g_j*dg_j) on the chosen experts
+ *   and 0 elsewhere (PK_ACCUM accumulates).
+ * pk_expert_plan: the slots in expert order, each expert's in increasing order.
+ *   offsets [E + 1]: expert e has the sorted positions offsets[e] ..
+ *   offsets[e + 1] - 1; order [n]: sorted position -> slot, the dropped slots
+ *   (expert outside [0, E)) last; place [n]: slot -> sorted position, -1 for a
+ *   dropped one.  Needs pk_expert_plan_workspace(n, E) bytes.
+ * pk_expert_gather_f32: out[r] = x[order[r] / k], r < offsets[E], zero rows from
+ *   there to n.
+ * pk_expert_combine_f32: out[t] = c[t] + sum_j gates[t, j]*ys[place[t, j]]; c NULL:
+ *   without it (c may be out); gates NULL: gates of 1, which makes it the gather's
+ *   backward.
+ * pk_expert_combine_bwd_f32: for slot = order[r], dys[r] (+)= gates[slot]*dout[slot / k]
+ *   (PK_ACCUM) and dgates[slot] (+)= dout[slot / k].ys[r] (PK_ACCUM2); 0 for dropped
+ *   slots.  dys or dgates may be NULL.
+ * pk_gemm_experts_f32: Y[r] (+)= X[r].op(W_e) for the rows r of every expert e, X
+ *   [n, K], W_e at W + e*sw: [K, N] for tb 'N', [N, K] for 'T' (row stride ldw), Y
+ *   [n, N].  Rows from offsets[E] to n become zero (accumulating: are left).
+ * pk_gemm_experts_dw_f32: dW_e (+)= X_e^T.dY_e, [K, N] at dW + e*sw, an expert without
+ *   rows getting zeros.  Needs pk_gemm_experts_dw_workspace(n, K, N, E) bytes.
+ *   precision: 0 fp32, 1 bf16, 2 three bf16 products, as in pk_gemm_add_f32 (no
+ *   fp8).  PK_ACCUM accumulates.
+ * Limits: E <= 1024, k <= 64, n < 2^31 (products: 2^30). */
+int pk_route_topk_f32(int64_t R, int64_t E, int64_t k, const float* logits, int64_t ldz,
+                      int32_t* experts, float* gates, pk_stream_t stream);
+int pk_route_topk_bwd_f32(int64_t R, int64_t E, int64_t k, const int32_t* experts,
+                          const float* gates, const float* dgates, float* dlogits, int64_t ldd,
+                          int flags, pk_stream_t stream);
+size_t pk_expert_plan_workspace(int64_t n, int64_t E);
+int pk_expert_plan(int64_t n, int64_t E, const int32_t* experts, int32_t* offsets, int32_t* order,
+                   int32_t* place, void* workspace, size_t workspace_bytes, pk_stream_t stream);
+int pk_expert_gather_f32(int64_t n, int64_t d, int64_t k, int64_t E, const int32_t* offsets,
+                         const int32_t* order, const float* x, int64_t ldx, float* out, int64_t ldo,
+                         pk_stream_t stream);
+int pk_expert_combine_f32(int64_t R, int64_t d, int64_t k, const int32_t* place, const float* gates,
+                          const float* ys, int64_t ldy, const float* c, int64_t ldc, float* out,
+                          int64_t ldo, pk_stream_t stream);
+int pk_expert_combine_bwd_f32(int64_t R, int64_t d, int64_t k, int64_t E, const int32_t* offsets,
+                              const int32_t* order, const float* gates, const float* ys, int64_t ldy,
+                              const float* dout, int64_t ldo, float* dys, int64_t ldd, float* dgates,
+                              int flags, pk_stream_t stream);
+int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int64_t E, const int32_t* offsets,
+                        const float* X, int64_t ldx, const float* W, int64_t ldw, int64_t sw,
+                        float* Y, int64_t ldy, int flags, int precision, pk_stream_t stream);
+size_t pk_gemm_experts_dw_workspace(int64_t n, int64_t K, int64_t N, int64_t E);
+int pk_gemm_experts_dw_f32(int64_t n, int64_t K, int64_t N, int64_t E, const int32_t* offsets,
+                           const float* X, int64_t ldx, const float* dY, int64_t ldy, float* dW,
+                           int64_t ldw, int64_t sw, int flags, int precision, void* workspace,
+                           size_t workspace_bytes, pk_stream_t stream);
 
 #ifdef __cplusplus
 }

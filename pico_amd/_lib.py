@@ -97,6 +97,7 @@ PK_SIGNATURES = {
     "pk_relu_bwd_f32": [c_i64, c_p, c_p, c_p, c_int, c_p],
     "pk_fill_f32": [c_i64, c_f, c_p, c_p],
     "pk_fill2d_f32": [c_i64, c_i64, c_f, c_p, c_i64, c_p],
+    "pk_copy2d_f32": [c_i64, c_i64, c_p, c_i64, c_p, c_i64, c_int, c_p],
     "pk_fill_normal_f32": [c_i64, ctypes.c_uint64, c_f, c_f, c_p, c_p],
     "pk_axpy_f32": [c_i64, c_f, c_p, c_p, c_p, c_int, c_p],
     "pk_reduce_sum_f32": [c_i64, c_p, c_f, c_p, c_int, c_p],
@@ -151,6 +152,29 @@ PK_SIGNATURES = {
     "pk_embed_fwd_f32": [c_i64, c_i64, c_i64, c_p, c_p, c_p, c_p],
     "pk_embed_bwd_workspace": [c_i64],
     "pk_embed_bwd_f32": [c_i64, c_i64, c_i64, c_p, c_p, c_p, c_p, c_size, c_p],
+    "pk_layernorm_fwd_f32": [c_i64, c_i64, c_f, c_p, c_p, c_p, c_p, c_p, c_p, c_p],
+    "pk_layernorm_bwd_workspace": [c_i64, c_i64],
+    "pk_layernorm_bwd_f32": [c_i64, c_i64, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_p, c_int, c_p,
+                             c_size, c_p],
+    "pk_gated_scan_workspace": [c_i64, c_i64, c_i64],
+    "pk_gated_scan_fwd_f32": [c_i64, c_i64, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p, c_p, c_size,
+                              c_p],
+    "pk_gated_scan_bwd_f32": [c_i64, c_i64, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_p, c_p, c_p, c_i64,
+                              c_p, c_i64, c_p, c_int, c_p, c_size, c_p],
+    "pk_route_topk_f32": [c_i64, c_i64, c_i64, c_p, c_i64, c_p, c_p, c_p],
+    "pk_route_topk_bwd_f32": [c_i64, c_i64, c_i64, c_p, c_p, c_p, c_p, c_i64, c_int, c_p],
+    "pk_expert_plan_workspace": [c_i64, c_i64],
+    "pk_expert_plan": [c_i64, c_i64, c_p, c_p, c_p, c_p, c_p, c_size, c_p],
+    "pk_expert_gather_f32": [c_i64, c_i64, c_i64, c_i64, c_p, c_p, c_p, c_i64, c_p, c_i64, c_p],
+    "pk_expert_combine_f32": [c_i64, c_i64, c_i64, c_p, c_p, c_p, c_i64, c_p, c_i64, c_p, c_i64,
+                              c_p],
+    "pk_expert_combine_bwd_f32": [c_i64, c_i64, c_i64, c_i64, c_p, c_p, c_p, c_p, c_i64, c_p, c_i64,
+                                  c_p, c_i64, c_p, c_int, c_p],
+    "pk_gemm_experts_f32": [c_char, c_i64, c_i64, c_i64, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_i64,
+                            c_p, c_i64, c_int, c_int, c_p],
+    "pk_gemm_experts_dw_workspace": [c_i64, c_i64, c_i64, c_i64],
+    "pk_gemm_experts_dw_f32": [c_i64, c_i64, c_i64, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_p, c_i64,
+                               c_i64, c_int, c_int, c_p, c_size, c_p],
     "pk_last_error": [],
 }
 _RESTYPES = {"pk_last_error": ctypes.c_char_p, "pk_rmsnorm_bwd_workspace": c_size,
@@ -161,7 +185,9 @@ _RESTYPES = {"pk_last_error": ctypes.c_char_p, "pk_rmsnorm_bwd_workspace": c_siz
              "pk_fp8_quantized_bytes": c_size, "pk_mx8_bytes": c_size,
              "pk_gemm_mx8_workspace": c_size, "pk_bf16q_bytes": c_size,
              "pk_gemm_bf16q_workspace": c_size, "pk_bf16x3q_bytes": c_size,
-             "pk_gemm_bf16x3q_workspace": c_size}
+             "pk_gemm_bf16x3q_workspace": c_size, "pk_layernorm_bwd_workspace": c_size,
+             "pk_gated_scan_workspace": c_size, "pk_expert_plan_workspace": c_size,
+             "pk_gemm_experts_dw_workspace": c_size}
 
 _hip = None
 

@@ -490,6 +490,18 @@ __global__ void fill2d_kernel(int64_t rows, int64_t cols, float v, float* __rest
         x[(i / cols) * ld + i % cols] = v;
 }
 
+__global__ void copy2d_kernel(int64_t rows, int64_t cols, const float* __restrict__ x, int64_t ldx,
+                              float* __restrict__ y, int64_t ldy, int accum) {
+    const int64_t n = rows * cols;
+    for(int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n;
+        i += (int64_t)gridDim.x * blockDim.x) {
+        const int64_t r = i / cols, c = i % cols;
+        float* o = y + r * ldy + c;
+        const float v = x[r * ldx + c];
+        *o = accum ? *o + v : v;
+    }
+}
+
 // splitmix64 finaliser: a bijective 64-bit mix (Steele, Lea & Flood 2014)
 __device__ __forceinline__ uint64_t mix64(uint64_t z) {
     z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
@@ -1169,6 +1181,17 @@ extern "C" int pk_fill2d_f32(int64_t rows, int64_t cols, float value, float* x, 
     fill2d_kernel<<<pk::grid_for(rows * cols, NT), NT, 0, pk::as_stream(stream)>>>(rows, cols,
                                                                                  value, x, ld);
     return pk::launch_status("pk_fill2d_f32");
+}
+
+extern "C" int pk_copy2d_f32(int64_t rows, int64_t cols, const float* x, int64_t ldx, float* y,
+                             int64_t ldy, int flags, pk_stream_t stream) {
+    if(rows < 0 || cols < 0 || (rows > 1 && (ldx < cols || ldy < cols)))
+        return pk::fail("pk_copy2d_f32: bad sizes");
+    if(rows == 0 || cols == 0) return PK_OK;
+    if(!x || !y) return pk::fail("pk_copy2d_f32: NULL pointer");
+    copy2d_kernel<<<pk::grid_for(rows * cols, NT), NT, 0, pk::as_stream(stream)>>>(
+        rows, cols, x, ldx, y, ldy, flags & PK_ACCUM);
+    return pk::launch_status("pk_copy2d_f32");
 }
 
 extern "C" int pk_fill_normal_f32(int64_t n, uint64_t seed, float mean, float std, float* x,

@@ -40,6 +40,7 @@
 #include <stdio.h>
 
 #include <algorithm>
+#include <cmath>
 #include <iterator>
 #include <mutex>
 #include <type_traits>
@@ -1511,6 +1512,33 @@ int gemm_impl(char ta, char tb, int64_t M, int64_t N, int64_t K, float alpha, co
 }
 
 }  // namespace
+
+namespace pkg {
+
+// An expert's last row tile is half empty on average; a tile holds rows of one
+// expert only.
+ExpertShape expert_shape(int prec, bool ta, double groups, double m, int64_t N, double k) {
+    const SplitShape* const shapes = prec == kFp32 ? kShapesF32 : prec == kBf16 ? kShapesBf16 : kShapesBf16x3;
+    const int n_shapes = prec == kFp32 ? (int)std::size(kShapesF32) : (int)std::size(kShapesBf16);
+    ExpertShape best = {kTile128, 128, 128};
+    double c = -1.0;
+    for(int i = 0; i < n_shapes; ++i) {
+        const SplitShape& t = shapes[i];
+        if(t.bn == 96 || (prec == kFp32 && (t.kind == kTile64 || t.kind == kTile64x1))) continue;
+        const double per = ta ? std::ceil(m / t.bm) : std::max(1.0, m / t.bm + 0.5);
+        const double n = groups * per * (double)((N + t.bn - 1) / t.bn);
+        const double rounds = 0.5 * (std::ceil(n / kCUs) + n / kCUs), kk = (ta ? t.ta : 1.0) * k;
+        const double own = std::max(t.one + t.edge + t.one_k * kk,
+                                    t.base + rounds * (t.round + t.edge + t.per_k * kk));
+        if(c < 0.0 || own < 0.97 * c) {
+            c = own;
+            best = {t.kind, t.bm, t.bn};
+        }
+    }
+    return best;
+}
+
+}  // namespace pkg
 
 extern "C" int pk_gemm_small_product_f32(int64_t M, int64_t N, int64_t K) {
     return M > 0 && N > 0 && K > 0 && K <= 1024 && small_product(M, N, K, false, false, K, N);

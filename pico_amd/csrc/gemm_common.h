@@ -118,6 +118,125 @@ __device__ __forceinline__ TileJob tile_job(const GemmParams& p) {
     return j;
 }
 
+// A product grouped by expert: the rows [offsets[e], offsets[e + 1]) of X belong to
+// expert e, and the numbers are known on the device only.
+//   rows: Y = X.op(W_e) for every expert's rows.  A is X, B is W (sBo from one
+//         expert to the next), C is Y, M all rows.
+//   else: dW_e = X_e^T.dY_e (sCo from one expert to the next).  A is X, B is dY, K
+//         all rows.
+struct ExpertParams : GemmParams {
+    const int32_t* offsets;
+    int experts;
+    int rows;
+};
+
+// Offsets are held to [0, n] and to increase, so that whatever they say no access
+// leaves the matrices.
+__device__ __forceinline__ void expert_range(const ExpertParams& p, int e, int64_t n, int64_t& lo,
+                                             int64_t& hi) {
+    lo = min(max((int64_t)p.offsets[e], (int64_t)0), n);
+    hi = e < p.experts ? min(max((int64_t)p.offsets[e + 1], lo), n) : n;
+}
+
+// The tile of workgroup blockIdx.x.  Its expert's matrices replace the whole ones in
+// p.  Of `rows` products the grid is the most row tiles that n rows and E experts
+// can need (tiles_m; 65 of it fit 32 bits); every wave adds up how many there are
+// and which expert has its own, 64 experts at a time.  The rows past the last expert's are a group of their own
+// that multiplies nothing, and so is filled with zeros (or, accumulating, left).
+template <class T>
+__device__ __forceinline__ TileJob tile_job(ExpertParams& p) {
+    TileJob j;
+    const int lane = threadIdx.x % 64;
+    int bid = blockIdx.x, e = 0, tm, tn;
+    int64_t lo, hi;
+    j.skip = true;
+    if(p.rows) {
+        const int64_t n = p.M;
+        auto tiles = [&](int q) {
+            if(q > p.experts) return 0;
+            expert_range(p, q, n, lo, hi);
+            return min((int)((hi - lo + T::BM - 1) / T::BM), p.tiles_m);
+        };
+        int all = 0;
+        for(int q = 0; q <= p.experts; q += 64) {
+            int c = tiles(q + lane);
+#pragma unroll
+            for(int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
+            all = min(all + c, p.tiles_m);
+        }
+        const int row_tiles = __builtin_amdgcn_readfirstlane(all);
+        const int ntiles = row_tiles * p.tiles_n, run = (ntiles + 7) >> 3;
+        bid = (bid & 7) * run + (bid >> 3);  // an XCD takes a run of tiles
+        if((int)(blockIdx.x >> 3) >= run || bid >= ntiles) return j;
+        const int group_span = GROUP_M * p.tiles_n;
+        const int first_m = (bid / group_span) * GROUP_M;
+        const int gm = min(row_tiles - first_m, GROUP_M);
+        const int local = bid % group_span;
+        tm = first_m + local % gm;
+        tn = local / gm;
+        // the expert of row tile tm
+        int before = 0;
+        for(int q = 0; q <= p.experts; q += 64) {
+            const int c = tiles(q + lane);
+            int sum = c;
+#pragma unroll
+            for(int o = 1; o < 64; o <<= 1) {
+                const int t = __shfl_up(sum, o, 64);
+                if(lane >= o) sum += t;
+            }
+            const uint64_t past = __ballot(before + sum > tm);
+            if(past) {
+                const int at = __builtin_ctzll(past);
+                e = q + at;
+                tm -= before + __shfl(sum - c, at, 64);
+                break;
+            }
+            before += __shfl(sum, 63, 64);
+        }
+        e = __builtin_amdgcn_readfirstlane(e);
+        tm = __builtin_amdgcn_readfirstlane(tm);
+        expert_range(p, e, n, lo, hi);
+        if(e == p.experts) {
+            if(p.beta != 0.0f) return j;
+            p.K = 0;
+        } else {
+            p.B += e * p.sBo;
+        }
+        p.A += lo * p.lda;
+        p.C += lo * p.ldc;
+        p.M = hi - lo;
+    } else {
+        const int ntiles = p.tiles_m * p.tiles_n;
+        const int total = ntiles * p.experts, run = (total + 7) >> 3;
+        bid = (bid & 7) * run + (bid >> 3);
+        if((int)(blockIdx.x >> 3) >= run || bid >= total) return j;
+        e = bid / ntiles;
+        bid %= ntiles;
+        tm = bid % p.tiles_m;
+        tn = bid / p.tiles_m;
+        expert_range(p, e, p.K, lo, hi);
+        p.A += lo * p.lda;
+        p.B += lo * p.ldb;
+        p.C += e * p.sCo;
+        p.K = hi - lo;
+    }
+    j.skip = false;
+    j.A = p.A;
+    j.B = p.B;
+    j.C = p.C;
+    j.ldc = p.ldc;
+    j.Cin = p.C;
+    j.ldcin = p.ldc;
+    j.alpha = p.alpha;
+    j.beta = p.beta;
+    j.row0 = (int64_t)tm * T::BM;
+    j.col0 = (int64_t)tn * T::BN;
+    j.kbeg = 0;
+    j.kend = p.K;
+    j.nslices = (int)((p.K + BK - 1) / BK);
+    return j;
+}
+
 // C block = alpha * acc (+ beta * C).  32x32 block accumulator r of lane l is
 // row 8*(r/4) + 4*(l/32) + r%4, column l%32: each half-wave writes 128
 // contiguous bytes per register.
@@ -320,6 +439,20 @@ enum TileKind { kTile128, kTile96, kTile256, kTile64, kTile256x96, kTile128x64, 
 int split_groups(TileKind kind);
 int launch_split(bool ta, bool tb, const GemmParams& gp, int64_t batch, bool edge, TileKind kind,
                  hipStream_t st);
+
+// products grouped by expert (A.B, A.B^T or A^T.B): kTile256, kTile128, kTile128x64
+// and kTile64 (fp32) or kTile64x2, the last one and the first two for bf16
+struct ExpertShape {
+    TileKind kind;
+    int bm, bn;
+};
+// the tile shape of a product of `groups` experts, [m, N] with k each on average
+// (gemm.hip's estimates)
+ExpertShape expert_shape(int prec, bool ta, double groups, double m, int64_t N, double k);
+int launch_split_experts(bool ta, bool tb, const ExpertParams& ep, unsigned grid, TileKind kind,
+                         hipStream_t st);
+int launch_narrow_experts(bool ta, bool tb, int parts, const ExpertParams& ep, unsigned grid,
+                          TileKind kind, hipStream_t st);
 
 // the bf16 (parts 1) and split-bf16 (parts 2) products (gemm_narrow.hip); with
 // gp.far, 64x64 tiles only

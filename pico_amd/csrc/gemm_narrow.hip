@@ -37,8 +37,8 @@ using namespace pkg;
 
 constexpr int W = 32;  // k per slice
 
-template <bool TA, bool TB, int EDGE, class T, int P, int EPI>
-__global__ __launch_bounds__(T::THREADS, T::WPS) void gemm_narrow_kernel(GemmParams p) {
+template <bool TA, bool TB, int EDGE, class T, int P, int EPI, class Params = GemmParams>
+__global__ __launch_bounds__(T::THREADS, T::WPS) void gemm_narrow_kernel(Params p) {
     constexpr int BM = T::BM, BN = T::BN, TM = T::TM, TN = T::TN, NT_ = T::THREADS;
     constexpr bool AK = !TA, BKF = TB, PAIR = EPI == kEpiSwigluFwd;
     using OA = SplitOperand<AK, BM, NT_, W>;
@@ -255,9 +255,38 @@ int launch_parts(bool ta, bool tb, const GemmParams& gp, int64_t batch, bool edg
     return launch_layout<true, true, P>(gp, batch, edge, kind, st);
 }
 
+template <bool TA, bool TB, int P>
+void launch_experts(const ExpertParams& ep, unsigned grid, TileKind kind, hipStream_t st) {
+    auto run = [&](auto shape) {
+        using T = decltype(shape);
+        gemm_narrow_kernel<TA, TB, kPartial, T, P, kEpiPlain, ExpertParams>
+            <<<grid, T::THREADS, 0, st>>>(ep);
+    };
+    switch(kind) {
+    case kTile256: run(Narrow256()); break;
+    case kTile128: run(Narrow128()); break;
+    default: run(Narrow64());
+    }
+}
+
+template <int P>
+void launch_experts_parts(bool ta, bool tb, const ExpertParams& ep, unsigned grid, TileKind kind,
+                          hipStream_t st) {
+    if(ta) launch_experts<true, false, P>(ep, grid, kind, st);
+    else if(tb) launch_experts<false, true, P>(ep, grid, kind, st);
+    else launch_experts<false, false, P>(ep, grid, kind, st);
+}
+
 }  // namespace
 
 namespace pkg {
+
+int launch_narrow_experts(bool ta, bool tb, int parts, const ExpertParams& ep, unsigned grid,
+                          TileKind kind, hipStream_t st) {
+    if(parts == 1) launch_experts_parts<1>(ta, tb, ep, grid, kind, st);
+    else launch_experts_parts<2>(ta, tb, ep, grid, kind, st);
+    return pk::launch_status("pk_gemm_experts_f32");
+}
 
 int launch_narrow(bool ta, bool tb, int parts, const GemmParams& gp, int64_t batch, bool edge,
                   TileKind kind, hipStream_t st) {

@@ -371,8 +371,9 @@ __device__ __forceinline__ void split_sched() {
     }
 }
 
-template <bool TA, bool TB, int EDGE, class T, int EPI>
-__global__ __launch_bounds__(T::THREADS, T::WPS) void gemm_split_kernel(GemmParams p) {
+// (Params: GemmParams, or ExpertParams for a product grouped by expert)
+template <bool TA, bool TB, int EDGE, class T, int EPI, class Params = GemmParams>
+__global__ __launch_bounds__(T::THREADS, T::WPS) void gemm_split_kernel(Params p) {
     constexpr int BM = T::BM, BN = T::BN, TM = T::TM, TN = T::TN, NT_ = T::GTHREADS, G = T::G,
                   SETS = T::A;
     constexpr bool AK = !TA, BKF = TB, PAIR = EPI == kEpiSwigluFwd;

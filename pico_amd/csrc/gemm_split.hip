@@ -66,9 +66,31 @@ int launch_layout(const GemmParams& gp, int64_t batch, bool edge, TileKind kind,
     }
 }
 
+template <bool TA, bool TB>
+void launch_experts(const ExpertParams& ep, unsigned grid, TileKind kind, hipStream_t st) {
+    auto run = [&](auto shape) {
+        using T = decltype(shape);
+        gemm_split_kernel<TA, TB, kPartial, T, kEpiPlain, ExpertParams><<<grid, T::THREADS, 0, st>>>(ep);
+    };
+    switch(kind) {
+    case kTile256: run(Split256()); break;
+    case kTile128: run(Split128()); break;
+    case kTile128x64: run(Split128x64()); break;
+    default: run(Split64x2());
+    }
+}
+
 }  // namespace
 
 namespace pkg {
+
+int launch_split_experts(bool ta, bool tb, const ExpertParams& ep, unsigned grid, TileKind kind,
+                         hipStream_t st) {
+    if(ta) launch_experts<true, false>(ep, grid, kind, st);
+    else if(tb) launch_experts<false, true>(ep, grid, kind, st);
+    else launch_experts<false, false>(ep, grid, kind, st);
+    return pk::launch_status("pk_gemm_experts_f32");
+}
 
 int split_groups(TileKind kind) {
     return kind == kTile64 ? Split64::G : kind == kTile256 || kind == kTile64x1 ? 1 : 2;

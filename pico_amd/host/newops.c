@@ -1,7 +1,8 @@
 /*
  * pico_amd/host/newops.c -- the hot-path ops pico does not have, in pico's op
  * style (src/ops.c:12-54) over GPU tensors: fused softmax cross-entropy,
- * RMSNorm, SwiGLU, causal attention, embedding, argmax.
+ * RMSNorm, layer norm, the gated recurrence, SwiGLU, causal attention,
+ * embedding, argmax.
  *
  * No reference code exists for these (the only traces are the softmax
  * Jacobian comment at src/autograd.h:38-40 and the plan at todo.md:95).
@@ -15,7 +16,7 @@
 
 #include "pk_host.h"
 
-static int need_gpu(const char* op, const struct PicoTensor* t) {
+int pkh_need_gpu(const char* op, const struct PicoTensor* t) {
     if(!t) {
         PKH_ERR("%s: NULL tensor!\n", op);
         return 1;
@@ -58,7 +59,7 @@ static void xent_backward(struct PicoTensor* self) {
 }
 
 struct PicoTensor* pico_softmax_xent(struct PicoTensor* logits, const int32_t* labels) {
-    if(need_gpu("pico_softmax_xent", logits)) return NULL;
+    if(pkh_need_gpu("pico_softmax_xent", logits)) return NULL;
     if(logits->ndim != 2 || logits->strides[1] != 1 || logits->strides[0] != logits->shape[1]) {
         PKH_ERR("softmax_xent expects contiguous 2-D logits [rows, classes]!\n");
         return NULL;
@@ -161,7 +162,7 @@ static void rms_backward(struct PicoTensor* self) {
 }
 
 struct PicoTensor* pico_rmsnorm(struct PicoTensor* x, struct PicoTensor* gain, float eps) {
-    if(need_gpu("pico_rmsnorm", x) || need_gpu("pico_rmsnorm", gain)) return NULL;
+    if(pkh_need_gpu("pico_rmsnorm", x) || pkh_need_gpu("pico_rmsnorm", gain)) return NULL;
     if(x->ndim < 1 || gain->numel != x->shape[x->ndim - 1] || x == gain) {
         PKH_ERR("rmsnorm expects x [rows, C] and gain [C]!\n");
         return NULL;
@@ -186,6 +187,185 @@ struct PicoTensor* pico_rmsnorm(struct PicoTensor* x, struct PicoTensor* gain, f
     if(pkh_status("pico_rmsnorm", st)) return NULL;
     struct PicoTensor* ps[2] = {x, gain};
     pkh_set_parents(arena, out, 2, ps, rms_backward);
+    return out;
+}
+
+/* -------------------------------------------------------------- layer norm
+ * y = (x - mean) * rstd * gain + bias over the last dim; the backward reads the
+ * saved mean and rstd */
+enum { LS_MEAN = 0, LS_RSTD = 1, LS_PARTS = 2 };
+
+static int contiguous(const struct PicoTensor* t) {
+    int64_t s = 1;
+    for(int i = t->ndim - 1; i >= 0; i--) {
+        if(t->shape[i] > 1 && t->strides[i] != s) return 0;
+        s *= t->shape[i];
+    }
+    return 1;
+}
+
+static void layernorm_backward(struct PicoTensor* self) {
+    struct PkNode* n = pkh_node(self);
+    struct PicoTensor *x = self->parents[0], *gain = self->parents[1];
+    struct PicoTensor* bias = self->num_parents > 2 ? self->parents[2] : NULL;
+    const float* dy = pkh_upstream(self);
+    if(!dy) return;
+    int64_t C = x->shape[x->ndim - 1], R = C ? x->numel / C : 0;
+    const float* dx_in = pkh_grad_base(x);
+    int flags = pkh_grad_flag(gain) ? PK_ACCUM2 : 0;
+    if(bias && pkh_grad_flag(bias)) flags |= PK_ACCUM3;
+    int st = pk_layernorm_bwd_f32(R, C, x->data, gain->data, (const float*)n->saved[LS_MEAN],
+                                  (const float*)n->saved[LS_RSTD], dy, dx_in, x->grad, gain->grad,
+                                  bias ? bias->grad : NULL, flags, n->saved[LS_PARTS],
+                                  pk_layernorm_bwd_workspace(R, C), pkh_stream());
+    if(pkh_status("pico_layernorm_backward", st)) return;
+    pkh_grad_mark(x);
+    pkh_grad_mark(gain);
+    if(bias) pkh_grad_mark(bias);
+}
+
+struct PicoTensor* pico_layernorm(struct PicoTensor* x, struct PicoTensor* gain,
+                                  struct PicoTensor* bias, float eps) {
+    if(pkh_need_gpu("pico_layernorm", x) || pkh_need_gpu("pico_layernorm", gain) ||
+       (bias && pkh_need_gpu("pico_layernorm", bias)))
+        return NULL;
+    if(x->ndim < 1 || gain->numel != x->shape[x->ndim - 1] || gain->numel < 1 ||
+       (bias && bias->numel != gain->numel) || x == gain || x == bias || gain == bias ||
+       !contiguous(x) || !contiguous(gain) || (bias && !contiguous(bias))) {
+        PKH_ERR("layernorm expects contiguous, different x [rows, C], gain [C] and bias [C] (or "
+                "NULL)!\n");
+        return NULL;
+    }
+    struct Arena* arena = pkh_need_arena();
+    if(!arena) return NULL;
+    int64_t C = x->shape[x->ndim - 1], R = x->numel / C;
+    struct PicoTensor* out = pkh_new_tensor(arena, x->shape, x->ndim);
+    if(!out) return NULL;
+    struct PkNode* n = pkh_node(out);
+    float* mean = (float*)arena_alloc_device(arena, sizeof(float) * (size_t)(R > 0 ? R : 1));
+    float* rstd = (float*)arena_alloc_device(arena, sizeof(float) * (size_t)(R > 0 ? R : 1));
+    /* (the backward's partial sums have a buffer of the node's own, so captured
+     * graphs share none) */
+    n->saved[LS_PARTS] = arena_alloc_device(arena, pk_layernorm_bwd_workspace(R, C));
+    if(!mean || !rstd || !n->saved[LS_PARTS]) return NULL;
+    n->saved[LS_MEAN] = mean;
+    n->saved[LS_RSTD] = rstd;
+    int st = pk_layernorm_fwd_f32(R, C, eps, x->data, gain->data, bias ? bias->data : NULL,
+                                  out->data, mean, rstd, pkh_stream());
+    if(pkh_status("pico_layernorm", st)) return NULL;
+    struct PicoTensor* ps[3] = {x, gain, bias};
+    pkh_set_parents(arena, out, bias ? 3 : 2, ps, layernorm_backward);
+    return out;
+}
+
+/* ------------------------------------------------- gated linear recurrence
+ * h_t = s_t h_{t-1} + (1 - s_t) x_t, s = sigmoid(f), token-major [batch*T, C];
+ * the backward reads f, x, h0 and the output */
+enum { GI_B = 0 };
+enum { GS_WS = 0 };
+
+static void gated_scan_backward(struct PicoTensor* self) {
+    struct PkNode* n = pkh_node(self);
+    struct PicoTensor *f = self->parents[0], *x = self->parents[1];
+    struct PicoTensor* h0 = self->num_parents > 2 ? self->parents[2] : NULL;
+    const float* dh = pkh_upstream(self);
+    if(!dh) return;
+    const int64_t B = n->ival[GI_B], T = x->shape[0] / B, C = x->shape[1];
+    void* ws = n->saved[GS_WS];
+    const size_t ws_bytes = pk_gated_scan_workspace(B, T, C);
+    /* one call writes every gradient, unless operands share a grad: then one
+     * call each, the later ones accumulating */
+    struct PicoTensor* const ps[3] = {f, x, h0};
+    const int bit[3] = {PK_ACCUM, PK_ACCUM2, PK_ACCUM3};
+    const int apart = f != x && f != h0 && x != h0;
+    for(int pass = 0; pass < (apart ? 1 : 3); pass++) {
+        float* g[3] = {NULL, NULL, NULL};
+        int flags = 0;
+        for(int i = 0; i < 3; i++) {
+            if(!ps[i] || !(apart || i == pass)) continue;
+            if(pkh_grad_flag(ps[i])) flags |= bit[i];
+            g[i] = ps[i]->grad;
+        }
+        if(!g[0] && !g[1] && !g[2]) continue;
+        int st = pk_gated_scan_bwd_f32(B, T, C, f->data, f->strides[0], x->data, x->strides[0],
+                                       h0 ? h0->data : NULL, self->data, dh, g[0], f->strides[0],
+                                       g[1], x->strides[0], g[2], flags, ws, ws_bytes,
+                                       pkh_stream());
+        if(pkh_status("pico_gated_scan_backward", st)) return;
+        for(int i = 0; i < 3; i++)
+            if(g[i]) pkh_grad_mark(ps[i]);
+    }
+}
+
+struct PicoTensor* pico_gated_scan(struct PicoTensor* f, struct PicoTensor* x,
+                                   struct PicoTensor* h0, int batch) {
+    if(pkh_need_gpu("pico_gated_scan", f) || pkh_need_gpu("pico_gated_scan", x) ||
+       (h0 && pkh_need_gpu("pico_gated_scan", h0)))
+        return NULL;
+    if(f->ndim != 2 || x->ndim != 2 || batch <= 0 || f->shape[0] != x->shape[0] ||
+       f->shape[1] != x->shape[1] || x->shape[0] % batch || f->strides[1] != 1 ||
+       x->strides[1] != 1 || f->strides[0] < f->shape[1] || x->strides[0] < x->shape[1]) {
+        PKH_ERR("gated_scan expects f and x [batch*T, C] with unit columns!\n");
+        return NULL;
+    }
+    const int64_t C = x->shape[1];
+    if(h0 && (h0->ndim != 2 || h0->shape[0] != batch || h0->shape[1] != C || !contiguous(h0))) {
+        PKH_ERR("gated_scan expects a contiguous state h0 [batch, C]!\n");
+        return NULL;
+    }
+    struct Arena* arena = pkh_need_arena();
+    if(!arena) return NULL;
+    const int64_t B = batch, T = x->shape[0] / batch;
+    struct PicoTensor* out = pkh_new_tensor(arena, x->shape, 2);
+    if(!out) return NULL;
+    pkh_node(out)->ival[GI_B] = B;
+    const size_t ws_bytes = pk_gated_scan_workspace(B, T, C);
+    void* ws = arena_alloc_device(arena, ws_bytes ? ws_bytes : 1);
+    if(!ws) return NULL;
+    pkh_node(out)->saved[GS_WS] = ws;
+    int st = pk_gated_scan_fwd_f32(B, T, C, f->data, f->strides[0], x->data, x->strides[0],
+                                   h0 ? h0->data : NULL, out->data, ws, ws_bytes, pkh_stream());
+    if(pkh_status("pico_gated_scan", st)) return NULL;
+    struct PicoTensor* ps[3] = {f, x, h0};
+    pkh_set_parents(arena, out, h0 ? 3 : 2, ps, gated_scan_backward);
+    return out;
+}
+
+/* the last token of every sequence: the state to go on from */
+static void last_token_backward(struct PicoTensor* self) {
+    struct PkNode* n = pkh_node(self);
+    struct PicoTensor* h = self->parents[0];
+    const float* g = pkh_upstream(self);
+    if(!g) return;
+    const int64_t B = n->ival[GI_B], C = h->shape[1], T = h->shape[0] / B, ld = h->strides[0];
+    if(!pkh_grad_flag(h)) {
+        /* the other tokens' gradients are zero */
+        if(pkh_status("pico_last_token_backward",
+                      pk_fill2d_f32(B * T, C, 0.0f, h->grad, ld, pkh_stream())))
+            return;
+        pkh_grad_mark(h);
+    }
+    pkh_status("pico_last_token_backward",
+               pk_copy2d_f32(B, C, g, C, h->grad + (T - 1) * ld, T * ld, PK_ACCUM, pkh_stream()));
+}
+
+struct PicoTensor* pico_last_token(struct PicoTensor* h, int batch) {
+    if(pkh_need_gpu("pico_last_token", h)) return NULL;
+    if(h->ndim != 2 || batch <= 0 || h->shape[0] < batch || h->shape[0] % batch ||
+       h->strides[1] != 1 || h->strides[0] < h->shape[1]) {
+        PKH_ERR("last_token expects h [batch*T, C] with unit columns and T >= 1!\n");
+        return NULL;
+    }
+    struct Arena* arena = pkh_need_arena();
+    if(!arena) return NULL;
+    const int64_t B = batch, C = h->shape[1], T = h->shape[0] / B, ld = h->strides[0];
+    int64_t shape[2] = {B, C};
+    struct PicoTensor* out = pkh_new_tensor(arena, shape, 2);
+    if(!out) return NULL;
+    pkh_node(out)->ival[GI_B] = B;
+    int st = pk_copy2d_f32(B, C, h->data + (T - 1) * ld, T * ld, out->data, C, 0, pkh_stream());
+    if(pkh_status("pico_last_token", st)) return NULL;
+    pkh_set_parents(arena, out, 1, &h, last_token_backward);
     return out;
 }
 
@@ -229,7 +409,7 @@ static void swiglu_backward(struct PicoTensor* self) {
 }
 
 struct PicoTensor* pico_swiglu(struct PicoTensor* a, struct PicoTensor* u) {
-    if(need_gpu("pico_swiglu", a) || need_gpu("pico_swiglu", u)) return NULL;
+    if(pkh_need_gpu("pico_swiglu", a) || pkh_need_gpu("pico_swiglu", u)) return NULL;
     if(a->numel != u->numel || a->ndim != u->ndim ||
        memcmp(a->shape, u->shape, sizeof(int64_t) * a->ndim) != 0) {
         PKH_ERR("swiglu expects gate and up of the same shape!\n");
@@ -366,8 +546,8 @@ static int wide_applies(struct PicoTensor* const* xs, int64_t B, int64_t H, int6
 
 struct PicoTensor* pico_attention_causal(struct PicoTensor* q, struct PicoTensor* k,
                                          struct PicoTensor* v, int batch, int n_heads) {
-    if(need_gpu("pico_attention_causal", q) || need_gpu("pico_attention_causal", k) ||
-       need_gpu("pico_attention_causal", v))
+    if(pkh_need_gpu("pico_attention_causal", q) || pkh_need_gpu("pico_attention_causal", k) ||
+       pkh_need_gpu("pico_attention_causal", v))
         return NULL;
     int layout_ok = 1;
     struct PicoTensor* xs[3] = {q, k, v};
@@ -459,7 +639,7 @@ static void emb_backward(struct PicoTensor* self) {
 }
 
 struct PicoTensor* pico_embedding(struct PicoTensor* table, const int32_t* ids, int64_t n_ids) {
-    if(need_gpu("pico_embedding", table)) return NULL;
+    if(pkh_need_gpu("pico_embedding", table)) return NULL;
     if(table->ndim != 2 || table->strides[1] != 1 || table->strides[0] != table->shape[1]) {
         PKH_ERR("embedding expects a contiguous 2-D table [vocab, d]!\n");
         return NULL;
@@ -485,7 +665,7 @@ struct PicoTensor* pico_embedding(struct PicoTensor* table, const int32_t* ids, 
 
 /* ----------------------------------------------------------------- argmax */
 int pico_argmax(struct PicoTensor* x, int32_t* idx) {
-    if(need_gpu("pico_argmax", x)) return PK_EINVAL;
+    if(pkh_need_gpu("pico_argmax", x)) return PK_EINVAL;
     if(x->ndim != 2 || x->strides[1] != 1 || !idx) {
         PKH_ERR("argmax expects 2-D x [rows, V] with contiguous rows and an output array!\n");
         return PK_EINVAL;

@@ -399,10 +399,11 @@ static int residual_ok(const struct PicoTensor* c, int64_t M, int64_t N) {
 
 /* d(out)/dc = 1: an empty grad takes out's grad by pointer (an alias),
  * otherwise out's grad is added to it */
-static int residual_backward(struct PicoTensor* self, struct PicoTensor* c, const float* g) {
+int pkh_residual_backward(const char* op, struct PicoTensor* self, struct PicoTensor* c,
+                          const float* g) {
     if(same_layout(c, self) && pkh_grad_alias(c, self)) return 0;
     int st = pk_axpy_f32(c->numel, 1.0f, NULL, g, c->grad, pkh_grad_flag(c), pkh_stream());
-    if(pkh_status("pico_matmul_add_backward", st)) return st;
+    if(pkh_status(op, st)) return st;
     pkh_grad_mark(c);
     return 0;
 }
@@ -412,7 +413,7 @@ static void matmul_add_backward(struct PicoTensor* self) {
     struct PicoTensor *a = self->parents[0], *b = self->parents[1], *c = self->parents[2];
     const float* g = pkh_upstream(self);
     if(!g) return;
-    if(residual_backward(self, c, g)) return;
+    if(pkh_residual_backward("pico_matmul_add_backward", self, c, g)) return;
     struct PkMat va, vb;
     if(matmul_views(a, b, &va, &vb)) return;
     int64_t M = a->shape[0], K = a->shape[1], N = b->shape[1];
@@ -694,7 +695,7 @@ static void swiglu_matmul_backward(struct PicoTensor* self) {
     struct PicoTensor *gate = self->parents[0], *up = self->parents[1], *w = self->parents[2];
     const float* g = pkh_upstream(self);
     if(!g) return;
-    if(n->ival[SM_RESID] && residual_backward(self, self->parents[3], g)) return;
+    if(n->ival[SM_RESID] && pkh_residual_backward("pico_matmul_add_backward", self, self->parents[3], g)) return;
     const int64_t M = gate->shape[0], F = gate->shape[1], N = w->shape[1];
     struct PkMat vh = {(const float*)n->saved[SM_H], 'N', F > 0 ? F : 1, 0};
     struct DaSwiglu ctx = {gate, up, w, g, M, F, N, n->ival[SM_LD]};

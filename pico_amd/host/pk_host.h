@@ -109,6 +109,13 @@ int pkh_copy_d2h(void* dst, const void* src, size_t bytes);
 /* device-to-device on the library's stream, not waited for */
 int pkh_copy_d2d_async(void* dst, const void* src, size_t bytes);
 
+/* 1, with a message, unless t is a GPU tensor (newops.c) */
+int pkh_need_gpu(const char* op, const struct PicoTensor* t);
+/* the gradient g of self = c + ...: an empty grad of c's takes self's by
+ * pointer, otherwise it is added (ops.c); `op` names a failure */
+int pkh_residual_backward(const char* op, struct PicoTensor* self, struct PicoTensor* c,
+                          const float* g);
+
 /* x . W + bias as one node (ops.c): pico's Linear forward in one product */
 struct PicoTensor* pkh_linear(struct PicoTensor* x, struct PicoTensor* w, struct PicoTensor* bias);
 

@@ -676,6 +676,291 @@ def embed_bwd(ids, dout, dtable):
     return dtable
 
 
+# ------------------------------------- layer norm, gated recurrence, experts
+ACCUM3 = 4
+PRECISIONS = {"fp32": 0, "bf16": 1, "bf16x3": 2}
+
+
+def _here(*ts):
+    """the launchers run on the current device: tensors of another are refused"""
+    for t in ts:
+        if t is not None and t.is_cuda and t.device.index != torch.cuda.current_device():
+            raise ValueError("a tensor lies on another device than the current one")
+
+
+def _i32(*ts):
+    for t in ts:
+        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
+            raise TypeError("expected a contiguous int32 CUDA tensor")
+
+
+def _rows(t, name):
+    """row stride of a 2-D tensor with unit columns and rows that do not overlap"""
+    ld = _rowmajor(t, name)
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}: rows overlap")
+    return ld
+
+
+def _dense(*ts):
+    for t in ts:
+        if t is not None and not t.is_contiguous():
+            raise ValueError("expected a contiguous tensor")
+
+
+def _ws(ws, need, device):
+    """a workspace of `need` bytes (ws itself when given) and its size"""
+    if ws is None:
+        ws = torch.empty(max(1, need), dtype=torch.uint8, device=device)
+    elif ws.device != device or not ws.is_contiguous():
+        raise ValueError("a workspace must be contiguous and on the operands' device")
+    return ws, ws.numel() * ws.element_size()
+
+
+def layernorm_fwd(x, g, b, y, mean, rstd, eps):
+    """y = (x - m) r g + b over the rows of x [R, C]; b, mean, rstd may be None"""
+    _f32(x, g, b, y, mean, rstd)
+    _here(x, g, b, y, mean, rstd)
+    _dense(x, g, b, y, mean, rstd)
+    R, C = x.shape
+    if g.numel() != C or (b is not None and b.numel() != C) or y.shape != x.shape or \
+            any(t is not None and t.numel() != R for t in (mean, rstd)):
+        raise ValueError("layernorm_fwd shape mismatch")
+    check("pk_layernorm_fwd_f32", hip_lib().pk_layernorm_fwd_f32(
+        R, C, eps, _ptr(x), _ptr(g), _ptr(b), _ptr(y), _ptr(mean), _ptr(rstd), _stream()))
+    return y
+
+
+def layernorm_bwd_workspace(R, C):
+    return int(hip_lib().pk_layernorm_bwd_workspace(R, C))
+
+
+def layernorm_bwd(x, g, mean, rstd, dy, dx, dg, db, ws=None, dx_in=None, accum_dg=False,
+                  accum_db=False):
+    """gradients of layernorm_fwd (a None one is skipped); dx_in is added to dx"""
+    _f32(x, g, mean, rstd, dy, dx, dg, db, dx_in)
+    _here(x, g, mean, rstd, dy, dx, dg, db, dx_in)
+    _dense(x, g, mean, rstd, dy, dx, dg, db, dx_in)
+    R, C = x.shape
+    if g.numel() != C or any(t is not None and t.shape != x.shape for t in (dy, dx, dx_in)) or \
+            any(t is not None and t.numel() != C for t in (dg, db)) or \
+            mean.numel() != R or rstd.numel() != R:
+        raise ValueError("layernorm_bwd shape mismatch")
+    ws, wsb = _ws(ws, layernorm_bwd_workspace(R, C), x.device)
+    flags = (ACCUM2 if accum_dg else 0) | (ACCUM3 if accum_db else 0)
+    check("pk_layernorm_bwd_f32", hip_lib().pk_layernorm_bwd_f32(
+        R, C, _ptr(x), _ptr(g), _ptr(mean), _ptr(rstd), _ptr(dy), _ptr(dx_in), _ptr(dx), _ptr(dg),
+        _ptr(db), flags, _ptr(ws), wsb, _stream()))
+
+
+def gated_scan_workspace(B, T, C):
+    return int(hip_lib().pk_gated_scan_workspace(B, T, C))
+
+
+def _scan_layout(B, f, x, h0, *rows):
+    """(T, C) of [B*T, C] matrices"""
+    N, C = x.shape
+    if B < 1 or N % B or f.shape != x.shape or any(t is not None and t.shape != x.shape for t in rows):
+        raise ValueError("gated_scan: f, x and h must be [B*T, C]")
+    if h0 is not None and tuple(h0.shape) != (B, C):
+        raise ValueError("gated_scan: h0 must be [B, C]")
+    return N // B, C
+
+
+def gated_scan_fwd(B, f, x, h, h0=None, ws=None):
+    """h_t = s_t h_{t-1} + (1 - s_t) x_t, s = sigmoid(f), over B sequences"""
+    _f32(f, x, h, h0)
+    _here(f, x, h, h0)
+    _dense(h, h0)
+    T, C = _scan_layout(B, f, x, h0, h)
+    ws, wsb = _ws(ws, gated_scan_workspace(B, T, C), x.device)
+    check("pk_gated_scan_fwd_f32", hip_lib().pk_gated_scan_fwd_f32(
+        B, T, C, _ptr(f), _rows(f, "f"), _ptr(x), _rows(x, "x"), _ptr(h0), _ptr(h), _ptr(ws),
+        wsb, _stream()))
+    return h
+
+
+def gated_scan_bwd(B, f, x, h, dh, df, dx, h0=None, dh0=None, ws=None, accum_df=False,
+                   accum_dx=False, accum_dh0=False):
+    """gradients of gated_scan_fwd (a None one is skipped)"""
+    _f32(f, x, h, dh, df, dx, h0, dh0)
+    _here(f, x, h, dh, df, dx, h0, dh0)
+    _dense(h, dh, h0, dh0)
+    T, C = _scan_layout(B, f, x, h0, h, dh, df, dx)
+    if dh0 is not None and tuple(dh0.shape) != (B, C):
+        raise ValueError("gated_scan: dh0 must be [B, C]")
+    ws, wsb = _ws(ws, gated_scan_workspace(B, T, C), x.device)
+    flags = (ACCUM if accum_df else 0) | (ACCUM2 if accum_dx else 0) | (ACCUM3 if accum_dh0 else 0)
+    check("pk_gated_scan_bwd_f32", hip_lib().pk_gated_scan_bwd_f32(
+        B, T, C, _ptr(f), _rows(f, "f"), _ptr(x), _rows(x, "x"), _ptr(h0), _ptr(h), _ptr(dh),
+        _ptr(df), C if df is None else _rows(df, "df"), _ptr(dx),
+        C if dx is None else _rows(dx, "dx"), _ptr(dh0), flags, _ptr(ws), wsb, _stream()))
+
+
+def route_topk(logits, experts, gates):
+    """experts [R, k] int32 and gates [R, k]: the k largest logits of each token
+    and the softmax over them"""
+    _f32(logits, gates)
+    _here(logits, gates)
+    _i32(experts)
+    _here(experts)
+    _dense(gates)
+    if experts.dim() != 2 or gates.shape != experts.shape or experts.shape[0] != logits.shape[0]:
+        raise ValueError("route_topk: experts and gates must be [R, k]")
+    check("pk_route_topk_f32", hip_lib().pk_route_topk_f32(
+        logits.shape[0], logits.shape[1], experts.shape[1], _ptr(logits),
+        _rows(logits, "logits"), _ptr(experts), _ptr(gates), _stream()))
+
+
+def route_topk_bwd(experts, gates, dgates, dlogits, accum=False):
+    _f32(gates, dgates, dlogits)
+    _here(gates, dgates, dlogits)
+    _i32(experts)
+    _here(experts)
+    _dense(gates, dgates)
+    if gates.shape != experts.shape or dgates.shape != experts.shape or \
+            experts.shape[0] != dlogits.shape[0]:
+        raise ValueError("route_topk_bwd: experts, gates and dgates must be [R, k]")
+    check("pk_route_topk_bwd_f32", hip_lib().pk_route_topk_bwd_f32(
+        dlogits.shape[0], dlogits.shape[1], experts.shape[1], _ptr(experts), _ptr(gates),
+        _ptr(dgates), _ptr(dlogits), _rows(dlogits, "dlogits"), ACCUM if accum else 0,
+        _stream()))
+    return dlogits
+
+
+def expert_plan_workspace(n, E):
+    return int(hip_lib().pk_expert_plan_workspace(n, E))
+
+
+def expert_plan(experts, offsets, order, place, ws=None):
+    """the slots of experts [R, k] in expert order: offsets [E + 1], order and
+    place [R*k], all int32"""
+    _i32(experts, offsets, order, place)
+    _here(experts, offsets, order, place)
+    n, E = experts.numel(), offsets.numel() - 1
+    if order.numel() != n or place.numel() != n or E < 1:
+        raise ValueError("expert_plan: order and place must hold a value a slot, offsets E + 1")
+    ws, wsb = _ws(ws, expert_plan_workspace(n, E), experts.device)
+    check("pk_expert_plan", hip_lib().pk_expert_plan(
+        n, E, _ptr(experts), _ptr(offsets), _ptr(order), _ptr(place), _ptr(ws), wsb, _stream()))
+
+
+def _expert_rows(n, d, *ts):
+    for t in ts:
+        if t is not None and tuple(t.shape) != (n, d):
+            raise ValueError(f"expected a [{n}, {d}] matrix, got {tuple(t.shape)}")
+
+
+def expert_gather(x, k, offsets, order, out):
+    """out[r] = x[order[r] // k]; zero rows behind the last expert's"""
+    _f32(x, out)
+    _here(x, out)
+    _i32(offsets, order)
+    _here(offsets, order)
+    n, d = x.shape[0] * k, x.shape[1]
+    _expert_rows(n, d, out)
+    if order.numel() != n or offsets.numel() < 2:
+        raise ValueError("expert_gather: order must hold a value a slot, offsets E + 1")
+    check("pk_expert_gather_f32", hip_lib().pk_expert_gather_f32(
+        n, d, k, offsets.numel() - 1, _ptr(offsets), _ptr(order), _ptr(x), _rows(x, "x"),
+        _ptr(out), _rows(out, "out"), _stream()))
+    return out
+
+
+def expert_combine(place, gates, ys, out, c=None):
+    """out[t] = c[t] + sum_j gates[t, j] ys[place[t, j]] (gates None: 1)"""
+    _f32(gates, ys, out, c)
+    _here(gates, ys, out, c)
+    _i32(place)
+    _here(place)
+    _dense(gates)
+    R, d = out.shape
+    n = place.numel()
+    if R == 0:
+        return out
+    if n % R or (gates is not None and gates.numel() != n):
+        raise ValueError("expert_combine: place and gates must hold k values a token")
+    _expert_rows(n, d, ys)
+    _expert_rows(R, d, c)
+    check("pk_expert_combine_f32", hip_lib().pk_expert_combine_f32(
+        R, d, n // R, _ptr(place), _ptr(gates), _ptr(ys), _rows(ys, "ys"), _ptr(c),
+        d if c is None else _rows(c, "c"), _ptr(out), _rows(out, "out"), _stream()))
+    return out
+
+
+def expert_combine_bwd(offsets, order, gates, ys, dout, dys, dgates, accum_dys=False,
+                       accum_dgates=False):
+    _f32(gates, ys, dout, dys, dgates)
+    _here(gates, ys, dout, dys, dgates)
+    _i32(offsets, order)
+    _here(offsets, order)
+    _dense(gates, dgates)
+    R, d = dout.shape
+    n = order.numel()
+    if R == 0:
+        return
+    if n % R or gates.numel() != n or (dgates is not None and dgates.numel() != n) or \
+            offsets.numel() < 2:
+        raise ValueError("expert_combine_bwd: order and gates must hold k values a token")
+    _expert_rows(n, d, ys, dys)
+    flags = (ACCUM if accum_dys else 0) | (ACCUM2 if accum_dgates else 0)
+    check("pk_expert_combine_bwd_f32", hip_lib().pk_expert_combine_bwd_f32(
+        R, d, n // R, offsets.numel() - 1, _ptr(offsets), _ptr(order), _ptr(gates), _ptr(ys),
+        d if ys is None else _rows(ys, "ys"), _ptr(dout), _rows(dout, "dout"), _ptr(dys),
+        d if dys is None else _rows(dys, "dys"), _ptr(dgates), flags, _stream()))
+
+
+def _expert_stack(w, name):
+    """(row stride, expert stride) of w [E, rows, cols] with unit columns"""
+    if w.dim() != 3 or (w.shape[2] > 1 and w.stride(2) != 1) or \
+            (w.shape[1] > 1 and w.stride(1) < w.shape[2]):
+        raise ValueError(f"{name} must be [E, rows, cols] with unit column stride")
+    return max(w.stride(1), w.shape[2]), w.stride(0)
+
+
+def gemm_experts(tb, x, w, offsets, y, precision="fp32", accum=False):
+    """y[r] = x[r] @ op(w[e]) for every expert's rows r (op = transpose for 'T')"""
+    _f32(x, w, y)
+    _here(x, w, y)
+    _i32(offsets)
+    _here(offsets)
+    ldw, sw = _expert_stack(w, "w")
+    E, K, N = w.shape if tb == "N" else (w.shape[0], w.shape[2], w.shape[1])
+    n = x.shape[0]
+    if offsets.numel() != E + 1 or x.shape[1] != K:
+        raise ValueError(f"gemm_experts: x {tuple(x.shape)}, w {tuple(w.shape)} ({tb}) and "
+                         f"{offsets.numel()} offsets do not fit")
+    _expert_rows(n, N, y)
+    check("pk_gemm_experts_f32", hip_lib().pk_gemm_experts_f32(
+        tb.encode(), n, N, K, E, _ptr(offsets), _ptr(x), _rows(x, "x"), _ptr(w), ldw, sw,
+        _ptr(y), _rows(y, "y"), ACCUM if accum else 0, PRECISIONS[precision], _stream()))
+    return y
+
+
+def gemm_experts_dw_workspace(n, K, N, E):
+    return int(hip_lib().pk_gemm_experts_dw_workspace(n, K, N, E))
+
+
+def gemm_experts_dw(x, dy, offsets, dw, precision="fp32", accum=False, ws=None):
+    """dw[e] = x_e^T @ dy_e over every expert's rows"""
+    _f32(x, dy, dw)
+    _here(x, dy, dw)
+    _i32(offsets)
+    _here(offsets)
+    ldw, sw = _expert_stack(dw, "dw")
+    E, K, N = dw.shape
+    n = x.shape[0]
+    if offsets.numel() != E + 1:
+        raise ValueError("gemm_experts_dw: offsets must hold E + 1 values")
+    _expert_rows(n, K, x)
+    _expert_rows(n, N, dy)
+    ws, wsb = _ws(ws, gemm_experts_dw_workspace(n, K, N, E), x.device)
+    check("pk_gemm_experts_dw_f32", hip_lib().pk_gemm_experts_dw_f32(
+        n, K, N, E, _ptr(offsets), _ptr(x), _rows(x, "x"), _ptr(dy), _rows(dy, "dy"),
+        _ptr(dw), ldw, sw, ACCUM if accum else 0, PRECISIONS[precision], _ptr(ws), wsb, _stream()))
+    return dw
+
+
 def device_info():
     cu, clk = ctypes.c_int(0), ctypes.c_int(0)
     arch = ctypes.create_string_buffer(64)

@@ -124,6 +124,14 @@ _GPU_SIGS = {
     "pico_matmul_add": (TP, [TP, TP, TP]),
     "pico_swiglu_matmul_add": (TP, [TP, TP, TP, TP]),
     "pico_matmul_gate_up": (TP, [TP, TP]),
+    "pico_layernorm": (TP, [TP, TP, TP, c_f]),
+    "pico_gated_scan": (TP, [TP, TP, TP, ctypes.c_int]),
+    "pico_last_token": (TP, [TP, ctypes.c_int]),
+    "pico_route_topk": (TP, [TP, ctypes.c_int, ctypes.POINTER(c_p)]),
+    "pico_route_to_host": (ctypes.c_int, [c_p, c_p, c_p]),
+    "pico_expert_gather": (TP, [TP, c_p]),
+    "pico_expert_matmul": (TP, [TP, TP, c_p]),
+    "pico_expert_combine": (TP, [TP, TP, c_p, TP]),
     "pico_set_matmul_precision": (ctypes.c_int, [ctypes.c_int]),
     "pico_get_matmul_precision": (ctypes.c_int, []),
     "pico_checkpoint_save": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(TP),
@@ -314,6 +322,20 @@ class Pico:
         if self.lib.pico_split_cols(t, n, outs):
             raise PicoError("pico_split_cols failed")
         return list(outs)
+
+    def route_topk(self, logits, k):
+        """pico_route_topk: (gates [tokens, k], the route)"""
+        route = c_p()
+        gates = self._check(self.lib.pico_route_topk(logits, k, ctypes.byref(route)),
+                            "pico_route_topk")
+        return gates, route
+
+    def route_to_host(self, route, tokens, k, experts):
+        """(chosen experts [tokens, k], first rows [experts + 1])"""
+        e, o = np.empty((tokens, k), np.int32), np.empty(experts + 1, np.int32)
+        if self.lib.pico_route_to_host(route, e.ctypes.data_as(c_p), o.ctypes.data_as(c_p)):
+            raise PicoError("pico_route_to_host failed")
+        return e, o
 
     def xent(self, logits, labels):
         return self._check(self.lib.pico_softmax_xent(logits, self.ids(labels)),
