@@ -5,9 +5,22 @@
 // and backwards, with the gradient u that a token hands to the one before it,
 //   G_t = dh_t + u_{t+1},  u_t = s_t G_t
 //   dx_t = (1 - s_t) G_t,  df_t = G_t (h_{t-1} - x_t) s_t (1 - s_t),  dh_0 = u_1
+//
+// Both directions are chains of p -> A p + H (forward A = s, H = q x; backward A = s,
+// H = s dh), and a run of steps is again one: (A2, H2) after (A1, H1) is
+// (A1 A2, A2 H1 + H2).  A workgroup walks its steps in tiles: a thread has 4
+// consecutive steps of 4 channels, composes them, the threads' results are scanned
+// across the lanes and through LDS, and every thread goes over its steps again, in
+// registers, from the value that reaches it.  The next tile's loads are in flight
+// meanwhile, so memory is read once: 12 bytes an element forward, 24 backward.
+// Sums are fp32, in an order that depends on the sizes alone.
 #include "pk_common.h"
 
 namespace {
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kThreads = 256, kWaves = kThreads / 64, LT = 4;  // LT steps a thread
 
 // s = sigmoid(f) and q = 1 - s = sigmoid(-f), each to its own last bits: the
 // smaller one is not got by subtraction
@@ -18,61 +31,422 @@ __device__ __forceinline__ void gate(float f, float& s, float& q) {
     q = f >= 0.0f ? small : big;
 }
 
-__global__ __launch_bounds__(256) void scan_fwd_serial(int64_t B, int64_t T, int64_t C,
-                                                       const float* __restrict__ f, int64_t ldf,
-                                                       const float* __restrict__ x, int64_t ldx,
-                                                       const float* __restrict__ h0,
-                                                       float* __restrict__ h) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if(i >= B * C) return;
-    const int64_t b = i / C, c = i % C;
-    float p = h0 ? h0[i] : 0.0f;
-    for(int64_t t = 0; t < T; ++t) {
-        const int64_t row = b * T + t;
-        float s, q;
-        gate(f[row * ldf + c], s, q);
-        p = s * p + q * x[row * ldx + c];
-        h[row * C + c] = p;
+// V channels from `at`.  A lane at the end of a row with fewer than 4 left reads the
+// row's last 4 (rows of fewer than 4 channels have V = 1): `skip` of them belong
+// to the lane before it and are not stored.
+template <int V>
+__device__ __forceinline__ void load(const float* at, float (&v)[V]) {
+    if constexpr(V == 4) {
+        const f32x4 x = *reinterpret_cast<const f32x4u*>(at);
+#pragma unroll
+        for(int i = 0; i < 4; ++i) v[i] = x[i];
+    } else {
+        v[0] = *at;
+    }
+}
+template <int V>
+__device__ __forceinline__ void store(float* at, const float (&v)[V], int skip, bool accum) {
+    if constexpr(V == 4) {
+        if(skip == 0) {
+            f32x4 x = {v[0], v[1], v[2], v[3]};
+            f32x4u* o = reinterpret_cast<f32x4u*>(at);
+            if(accum) x = *o + x;
+            *o = x;
+            return;
+        }
+    }
+#pragma unroll
+    for(int i = 0; i < V; ++i)
+        if(i >= skip) at[i] = accum ? at[i] + v[i] : v[i];
+}
+
+struct ScanParams {
+    int64_t B, T, C;
+    const float *f, *x, *h0, *h, *dh;
+    int64_t ldf, ldx, lddf, lddx;
+    float *out, *df, *dx, *dh0;  // forward: out
+    int flags;
+    float* ws;      // [S][B][C] A, then the same of H
+    int S;          // chunks along the tokens
+    int64_t L;      // steps of a chunk
+    int groups;     // channel groups of a sequence
+};
+
+// CL lanes along the channels, V channels each
+template <int V, int CL>
+struct Place {
+    static constexpr int TL = kThreads / CL, TT = TL * LT;  // lanes along the steps, steps of a tile
+    int64_t b, c, chunk;
+    int tl, cl, skip;
+    bool on;
+
+    // a run of channel groups to each XCD: groups narrower than a cache line meet
+    // in one L2
+    __device__ __forceinline__ explicit Place(const ScanParams& p) {
+        const int64_t n = p.B * p.groups, run = (n + 7) / 8;
+        const int64_t id = (blockIdx.x & 7) * run + (blockIdx.x >> 3);
+        on = (blockIdx.x >> 3) < run && id < n;
+        b = id / p.groups;
+        tl = threadIdx.x / CL;
+        cl = threadIdx.x % CL;
+        chunk = blockIdx.y;
+        c = ((id % p.groups) * CL + cl) * V;
+        skip = 0;
+        if(c + V > p.C) {
+            // (lanes wholly past the row repeat its last channels and store nothing)
+            skip = (int)min(c + V - p.C, (int64_t)V);
+            c = p.C - V;
+        }
+    }
+};
+
+// (A, H) of the lanes' steps, in step order -> the value that reaches each lane
+// from `carry`; carry becomes the one behind the last lane.  One barrier; `turn`
+// alternates between calls.
+template <int V, int CL>
+__device__ __forceinline__ void through(float (&A)[V], float (&H)[V], float (&carry)[V], float (&in)[V],
+                                        float (*lds)[kWaves][2][V * CL], int turn) {
+    const int lane = threadIdx.x % 64, w = threadIdx.x / 64, cl = threadIdx.x % CL;
+#pragma unroll
+    for(int o = CL; o < 64; o <<= 1) {
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            const float a = __shfl_up(A[i], o, 64), h = __shfl_up(H[i], o, 64);
+            if(lane >= o) {
+                H[i] = fmaf(A[i], h, H[i]);
+                A[i] *= a;
+            }
+        }
+    }
+    if(lane >= 64 - CL) {
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            lds[turn][w][0][cl * V + i] = A[i];
+            lds[turn][w][1][cl * V + i] = H[i];
+        }
+    }
+    __syncthreads();
+    float own[V];
+#pragma unroll
+    for(int i = 0; i < V; ++i) {
+        own[i] = carry[i];
+#pragma unroll
+        for(int q = 0; q < kWaves; ++q) {
+            if(q == w) own[i] = carry[i];
+            carry[i] = fmaf(lds[turn][q][0][cl * V + i], carry[i], lds[turn][q][1][cl * V + i]);
+        }
+        const float a = __shfl_up(A[i], CL, 64), h = __shfl_up(H[i], CL, 64);
+        in[i] = lane >= CL ? fmaf(a, own[i], h) : own[i];
     }
 }
 
-__global__ __launch_bounds__(256) void scan_bwd_serial(int64_t B, int64_t T, int64_t C,
-                                                       const float* __restrict__ f, int64_t ldf,
-                                                       const float* __restrict__ x, int64_t ldx,
-                                                       const float* __restrict__ h0,
-                                                       const float* __restrict__ h,
-                                                       const float* __restrict__ dh, float* df,
-                                                       int64_t lddf, float* dx, int64_t lddx,
-                                                       float* dh0, int flags) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if(i >= B * C) return;
-    const int64_t b = i / C, c = i % C;
-    float u = 0.0f;
-    for(int64_t t = T - 1; t >= 0; --t) {
-        const int64_t row = b * T + t;
-        float s, q;
-        gate(f[row * ldf + c], s, q);
-        const float G = dh[row * C + c] + u;
-        const float before = t > 0 ? h[(row - 1) * C + c] : h0 ? h0[i] : 0.0f;
-        if(df) {
-            const float v = G * (before - x[row * ldx + c]) * (s * q);
-            float* o = df + row * lddf + c;
-            *o = (flags & PK_ACCUM) ? *o + v : v;
-        }
-        if(dx) {
-            float* o = dx + row * lddx + c;
-            *o = (flags & PK_ACCUM2) ? *o + q * G : q * G;
-        }
-        u = s * G;
+// one step of the chain
+template <bool BWD>
+__device__ __forceinline__ float step(float p, float s, float v) {
+    return BWD ? s * (v + p) : fmaf(s, p, v);
+}
+
+// the composed (A, H) of every chunk but the last: thread tl has the steps
+// tl n .. tl n + n - 1 of the chunk, n = L / TL
+template <int V, int CL, bool BWD>
+__global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
+    using Pl = Place<V, CL>;
+    __shared__ float lds[1][kWaves][2][V * CL];
+    const Pl at(p);
+    if(!at.on) return;
+    const int64_t n = p.L / Pl::TL, g0 = at.chunk * p.L + at.tl * n;
+    const float* const f = p.f + at.b * p.T * p.ldf + at.c;
+    const float* const v = BWD ? p.dh + at.b * p.T * p.C + at.c : p.x + at.b * p.T * p.ldx + at.c;
+    const int64_t ldv = BWD ? p.C : p.ldx;
+    float A[V], H[V];
+#pragma unroll
+    for(int i = 0; i < V; ++i) {
+        A[i] = 1.0f;
+        H[i] = 0.0f;
     }
-    if(dh0) dh0[i] = (flags & PK_ACCUM3) ? dh0[i] + u : u;
+    float fr[LT][V], vr[LT][V];
+    auto fetch = [&](int64_t k) {
+#pragma unroll
+        for(int e = 0; e < LT; ++e) {
+            const int64_t g = min(g0 + k + e, p.T - 1), t = BWD ? p.T - 1 - g : g;
+            load<V>(f + t * p.ldf, fr[e]);
+            load<V>(v + t * ldv, vr[e]);
+        }
+    };
+    fetch(0);
+    for(int64_t k = 0; k < n; k += LT) {
+        float fc[LT][V], vc[LT][V];
+#pragma unroll
+        for(int e = 0; e < LT; ++e)
+#pragma unroll
+            for(int i = 0; i < V; ++i) {
+                fc[e][i] = fr[e][i];
+                vc[e][i] = vr[e][i];
+            }
+        fetch(k + LT);
+#pragma unroll
+        for(int e = 0; e < LT; ++e)
+#pragma unroll
+            for(int i = 0; i < V; ++i) {
+                float s, q;
+                gate(fc[e][i], s, q);
+                A[i] *= s;
+                H[i] = step<BWD>(H[i], s, BWD ? vc[e][i] : q * vc[e][i]);
+            }
+    }
+    float a[V], none[V], in[V];
+#pragma unroll
+    for(int i = 0; i < V; ++i) none[i] = 0.0f;
+    // (the last lane's scanned A and its H from nothing are the chunk's)
+    through<V, CL>(A, H, none, in, lds, 0);
+#pragma unroll
+    for(int i = 0; i < V; ++i) {
+        a[i] = 1.0f;
+#pragma unroll
+        for(int q = 0; q < kWaves; ++q) a[i] *= lds[0][q][0][at.cl * V + i];
+    }
+    if(at.tl == 0) {
+        float* const o = p.ws + (at.chunk * p.B + at.b) * p.C + at.c;
+        store<V>(o, a, at.skip, false);
+        store<V>(o + (int64_t)p.S * p.B * p.C, none, at.skip, false);
+    }
+}
+
+template <int V, int CL, bool BWD>
+__global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
+    using Pl = Place<V, CL>;
+    __shared__ float lds[2][kWaves][2][V * CL];
+    const Pl at(p);
+    if(!at.on) return;
+    const int64_t g0 = at.chunk * p.L, g1 = min(p.T, g0 + p.L);
+    const float* const f = p.f + at.b * p.T * p.ldf + at.c;
+    const float* const x = p.x + at.b * p.T * p.ldx + at.c;
+    const float* const h = BWD ? p.h + at.b * p.T * p.C + at.c : nullptr;
+    const float* const dh = BWD ? p.dh + at.b * p.T * p.C + at.c : nullptr;
+    const float* const h0 = p.h0 ? p.h0 + at.b * p.C + at.c : nullptr;
+    float* const out = BWD ? nullptr : p.out + at.b * p.T * p.C + at.c;
+
+    float carry[V], in[V];
+#pragma unroll
+    for(int i = 0; i < V; ++i) carry[i] = 0.0f;
+    if(!BWD && h0) load<V>(h0, carry);
+    int turn = 0;
+
+    struct Regs {
+        float f[LT][V], x[LT][V], h[BWD ? LT : 1][V], dh[BWD ? LT : 1][V];
+    };
+    Regs next;
+    auto fetch = [&](int64_t tile) {
+#pragma unroll
+        for(int e = 0; e < LT; ++e) {
+            const int64_t g = min(tile + at.tl * LT + e, p.T - 1), t = BWD ? p.T - 1 - g : g;
+            load<V>(f + t * p.ldf, next.f[e]);
+            load<V>(x + t * p.ldx, next.x[e]);
+            if constexpr(BWD) {
+                load<V>(dh + t * p.C, next.dh[e]);
+                if(t > 0) load<V>(h + (t - 1) * p.C, next.h[e]);
+                else if(h0) load<V>(h0, next.h[e]);
+                else
+#pragma unroll
+                    for(int i = 0; i < V; ++i) next.h[e][i] = 0.0f;
+            }
+        }
+    };
+    fetch(g0);
+    if(at.chunk > 0) {
+        // the value behind the chunks before this one
+        const int64_t m = (at.chunk + Pl::TL - 1) / Pl::TL;
+        float A[V], H[V];
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            A[i] = 1.0f;
+            H[i] = 0.0f;
+        }
+        for(int64_t k = at.tl * m; k < min(at.tl * m + m, at.chunk); ++k) {
+            const float* o = p.ws + (k * p.B + at.b) * p.C + at.c;
+            float a[V], e[V];
+            load<V>(o, a);
+            load<V>(o + (int64_t)p.S * p.B * p.C, e);
+#pragma unroll
+            for(int i = 0; i < V; ++i) {
+                H[i] = fmaf(a[i], H[i], e[i]);
+                A[i] *= a[i];
+            }
+        }
+        through<V, CL>(A, H, carry, in, lds, turn);
+        turn ^= 1;
+    }
+    for(int64_t tile = g0; tile < g1; tile += Pl::TT) {
+        Regs r = next;
+        fetch(tile + Pl::TT);
+        const int64_t first = tile + at.tl * LT;
+        float s[LT][V], q[LT][V], A[V], H[V];
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            A[i] = 1.0f;
+            H[i] = 0.0f;
+        }
+#pragma unroll
+        for(int e = 0; e < LT; ++e) {
+            const bool past = first + e >= g1;  // a step that changes nothing
+#pragma unroll
+            for(int i = 0; i < V; ++i) {
+                gate(r.f[e][i], s[e][i], q[e][i]);
+                if(past) {
+                    s[e][i] = 1.0f;
+                    q[e][i] = r.x[e][i] = 0.0f;
+                    if(BWD) r.dh[BWD ? e : 0][i] = 0.0f;
+                }
+                A[i] *= s[e][i];
+                H[i] = step<BWD>(H[i], s[e][i], BWD ? r.dh[BWD ? e : 0][i] : q[e][i] * r.x[e][i]);
+            }
+        }
+        through<V, CL>(A, H, carry, in, lds, turn);
+        turn ^= 1;
+#pragma unroll
+        for(int e = 0; e < LT; ++e) {
+            const int64_t g = first + e, t = BWD ? p.T - 1 - g : g;
+            if(g >= g1) continue;
+            if constexpr(!BWD) {
+#pragma unroll
+                for(int i = 0; i < V; ++i) in[i] = step<false>(in[i], s[e][i], q[e][i] * r.x[e][i]);
+                store<V>(out + t * p.C, in, at.skip, false);
+            } else {
+                float df[V], dx[V];
+#pragma unroll
+                for(int i = 0; i < V; ++i) {
+                    const float G = r.dh[e][i] + in[i];
+                    dx[i] = q[e][i] * G;
+                    df[i] = G * (r.h[e][i] - r.x[e][i]) * (s[e][i] * q[e][i]);
+                    in[i] = s[e][i] * G;
+                }
+                const int64_t row = at.b * p.T + t;
+                if(p.df) store<V>(p.df + row * p.lddf + at.c, df, at.skip, p.flags & PK_ACCUM);
+                if(p.dx) store<V>(p.dx + row * p.lddx + at.c, dx, at.skip, p.flags & PK_ACCUM2);
+            }
+        }
+    }
+    if(BWD && p.dh0 && at.tl == 0 && g1 == p.T)
+        store<V>(p.dh0 + at.b * p.C + at.c, carry, at.skip, p.flags & PK_ACCUM3);
+}
+
+// a few tokens of many sequences: a thread to V channels, token after token
+template <int V, bool BWD>
+__global__ __launch_bounds__(kThreads) void scan_serial(ScanParams p) {
+    const int64_t per = (p.C + V - 1) / V, id = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+    if(id >= p.B * per) return;
+    const int64_t b = id / per;
+    int64_t c = (id % per) * V;
+    int skip = 0;
+    if(c + V > p.C) {
+        skip = (int)(c + V - p.C);
+        c = p.C - V;
+    }
+    float state[V];
+#pragma unroll
+    for(int i = 0; i < V; ++i) state[i] = 0.0f;
+    if(!BWD && p.h0) load<V>(p.h0 + b * p.C + c, state);
+    for(int64_t g = 0; g < p.T; ++g) {
+        const int64_t t = BWD ? p.T - 1 - g : g, row = b * p.T + t;
+        float f[V], x[V];
+        load<V>(p.f + row * p.ldf + c, f);
+        load<V>(p.x + row * p.ldx + c, x);
+        if constexpr(!BWD) {
+#pragma unroll
+            for(int i = 0; i < V; ++i) {
+                float s, q;
+                gate(f[i], s, q);
+                state[i] = step<false>(state[i], s, q * x[i]);
+            }
+            store<V>(p.out + row * p.C + c, state, skip, false);
+        } else {
+            float dh[V], h[V], df[V], dx[V];
+            load<V>(p.dh + row * p.C + c, dh);
+#pragma unroll
+            for(int i = 0; i < V; ++i) h[i] = 0.0f;
+            if(t > 0) load<V>(p.h + (row - 1) * p.C + c, h);
+            else if(p.h0) load<V>(p.h0 + b * p.C + c, h);
+#pragma unroll
+            for(int i = 0; i < V; ++i) {
+                float s, q;
+                gate(f[i], s, q);
+                const float G = dh[i] + state[i];
+                dx[i] = q * G;
+                df[i] = G * (h[i] - x[i]) * (s * q);
+                state[i] = s * G;
+            }
+            if(p.df) store<V>(p.df + row * p.lddf + c, df, skip, p.flags & PK_ACCUM);
+            if(p.dx) store<V>(p.dx + row * p.lddx + c, dx, skip, p.flags & PK_ACCUM2);
+        }
+    }
+    if(BWD && p.dh0) store<V>(p.dh0 + b * p.C + c, state, skip, p.flags & PK_ACCUM3);
+}
+
+// How a shape is split: serial (lanes 0), or groups of `lanes` lanes along the
+// channels (4 channels each, 1 below 4) and S chunks of L steps.
+struct Plan {
+    int lanes, S;
+    int64_t L;
+};
+
+Plan plan_of(int64_t B, int64_t T, int64_t C) {
+    const int V = C < 4 ? 1 : 4;
+    if(T <= 8) return {0, 1, T};
+    auto groups = [&](int lanes) { return B * ((C + V * lanes - 1) / (V * lanes)); };
+    constexpr int64_t kBlocks = 512;
+    // one chunk: the widest rows that still give every CU two workgroups
+    if(groups(16) >= kBlocks) return {16, 1, T};
+    if(groups(4) >= kBlocks / 2) return {groups(8) >= kBlocks ? 8 : 4, 1, T};
+    // chunks of at least 256 steps, a multiple of a thread's steps in them
+    const int64_t most = (T + 255) / 256, want = (kBlocks + groups(16) - 1) / groups(16);
+    const int64_t S = most < want ? most : want;
+    if(S <= 1) return {4, 1, T};
+    const int64_t L = ((T + S - 1) / S + 63) / 64 * 64;
+    return {16, (int)((T + L - 1) / L), L};
+}
+
+template <int V, int CL, bool BWD>
+void launch(ScanParams& p, const Plan& plan, hipStream_t st) {
+    p.groups = (int)((p.C + V * CL - 1) / (V * CL));
+    const unsigned grid = (unsigned)((p.B * p.groups + 7) / 8 * 8);
+    if constexpr(CL == 16) {
+        if(plan.S > 1) scan_chunks<V, CL, BWD><<<dim3(grid, plan.S - 1), kThreads, 0, st>>>(p);
+    }
+    scan_tiles<V, CL, BWD><<<dim3(grid, plan.S), kThreads, 0, st>>>(p);
+}
+
+template <bool BWD>
+int run(const char* who, ScanParams& p, void* workspace, size_t workspace_bytes, pk_stream_t stream) {
+    const Plan plan = plan_of(p.B, p.T, p.C);
+    const size_t need = pk_gated_scan_workspace(p.B, p.T, p.C);
+    if(need && (!workspace || workspace_bytes < need)) return pk::fail("%s: workspace needs %zu bytes", who, need);
+    hipStream_t st = pk::as_stream(stream);
+    p.ws = static_cast<float*>(workspace);
+    p.S = plan.S;
+    p.L = plan.L;
+    if(plan.lanes == 0) {
+        const int64_t V = p.C < 4 ? 1 : 4;
+        const unsigned grid = (unsigned)((p.B * ((p.C + V - 1) / V) + kThreads - 1) / kThreads);
+        if(V == 1) scan_serial<1, BWD><<<grid, kThreads, 0, st>>>(p);
+        else scan_serial<4, BWD><<<grid, kThreads, 0, st>>>(p);
+    } else if(p.C < 4) {
+        if(plan.lanes == 16) launch<1, 16, BWD>(p, plan, st);
+        else launch<1, 4, BWD>(p, plan, st);
+    } else if(plan.lanes == 16) {
+        launch<4, 16, BWD>(p, plan, st);
+    } else if(plan.lanes == 8) {
+        launch<4, 8, BWD>(p, plan, st);
+    } else {
+        launch<4, 4, BWD>(p, plan, st);
+    }
+    return pk::launch_status(who);
 }
 
 int check(const char* who, int64_t B, int64_t T, int64_t C, const float* f, int64_t ldf,
           const float* x, int64_t ldx) {
     if(B < 0 || T < 0 || C < 0) return pk::fail("%s: negative size", who);
     if(B > INT32_MAX || T > INT32_MAX || C > INT32_MAX || B * T > INT32_MAX ||
-       B * C > (int64_t)INT32_MAX * 64)
+       B * ((C + 3) / 4) > INT32_MAX - 8)
         return pk::fail("%s: B*T rows or B*C channels too many for one call", who);
     if(B == 0 || T == 0 || C == 0) return PK_OK;
     if(!f || !x) return pk::fail("%s: NULL f or x", who);
@@ -83,10 +457,9 @@ int check(const char* who, int64_t B, int64_t T, int64_t C, const float* f, int6
 }  // namespace
 
 extern "C" size_t pk_gated_scan_workspace(int64_t B, int64_t T, int64_t C) {
-    (void)B;
-    (void)T;
-    (void)C;
-    return 0;
+    if(B <= 0 || T <= 0 || C <= 0) return 0;
+    const Plan plan = plan_of(B, T, C);
+    return plan.S > 1 ? (size_t)plan.S * (size_t)B * (size_t)C * 2 * sizeof(float) : 0;
 }
 
 extern "C" int pk_gated_scan_fwd_f32(int64_t B, int64_t T, int64_t C, const float* f, int64_t ldf,
@@ -95,9 +468,17 @@ extern "C" int pk_gated_scan_fwd_f32(int64_t B, int64_t T, int64_t C, const floa
     if(int st = check("pk_gated_scan_fwd_f32", B, T, C, f, ldf, x, ldx)) return st;
     if(B == 0 || T == 0 || C == 0) return PK_OK;
     if(!h) return pk::fail("pk_gated_scan_fwd_f32: NULL h");
-    scan_fwd_serial<<<(unsigned)((B * C + 255) / 256), 256, 0, pk::as_stream(stream)>>>(B, T, C, f, ldf, x,
-                                                                                   ldx, h0, h);
-    return pk::launch_status("pk_gated_scan_fwd_f32");
+    ScanParams p = {};
+    p.B = B;
+    p.T = T;
+    p.C = C;
+    p.f = f;
+    p.ldf = ldf;
+    p.x = x;
+    p.ldx = ldx;
+    p.h0 = h0;
+    p.out = h;
+    return run<false>("pk_gated_scan_fwd_f32", p, workspace, workspace_bytes, stream);
 }
 
 extern "C" int pk_gated_scan_bwd_f32(int64_t B, int64_t T, int64_t C, const float* f, int64_t ldf,
@@ -112,7 +493,22 @@ extern "C" int pk_gated_scan_bwd_f32(int64_t B, int64_t T, int64_t C, const floa
     if(!h || !dh) return pk::fail("pk_gated_scan_bwd_f32: NULL h or dh");
     if((df && lddf < C) || (dx && lddx < C))
         return pk::fail("pk_gated_scan_bwd_f32: row stride of a gradient < C");
-    scan_bwd_serial<<<(unsigned)((B * C + 255) / 256), 256, 0, pk::as_stream(stream)>>>(
-        B, T, C, f, ldf, x, ldx, h0, h, dh, df, lddf, dx, lddx, dh0, flags);
-    return pk::launch_status("pk_gated_scan_bwd_f32");
+    ScanParams p = {};
+    p.B = B;
+    p.T = T;
+    p.C = C;
+    p.f = f;
+    p.ldf = ldf;
+    p.x = x;
+    p.ldx = ldx;
+    p.h0 = h0;
+    p.h = h;
+    p.dh = dh;
+    p.df = df;
+    p.lddf = lddf;
+    p.dx = dx;
+    p.lddx = lddx;
+    p.dh0 = dh0;
+    p.flags = flags;
+    return run<true>("pk_gated_scan_bwd_f32", p, workspace, workspace_bytes, stream);
 }
