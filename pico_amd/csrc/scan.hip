@@ -423,8 +423,9 @@ __global__ __launch_bounds__(kThreads) void scan_serial(ScanParams p) {
     if(BWD && p.dh0) store<V>(p.dh0 + b * p.C + c, state, skip, p.flags & PK_ACCUM3);
 }
 
-// How a shape is split: serial (lanes 0), or groups of `lanes` lanes along the
-// channels (4 channels each, 1 below 4) and S chunks of L steps.
+// How a shape is split: token after token (lanes 0), or groups of `lanes` lanes along
+// the channels (4 channels each, 1 below 4) and S chunks of L steps.  Times are
+// forward + backward, us, from graphs of 20 calls.
 struct Plan {
     int lanes, S;
     int64_t L;
@@ -434,25 +435,36 @@ Plan plan_of(int64_t B, int64_t T, int64_t C) {
     const int V = C < 4 ? 1 : 4;
     if(T <= 8) return {0, 1, T};
     auto groups = [&](int lanes) { return B * ((C + V * lanes - 1) / (V * lanes)); };
-    constexpr int64_t kBlocks = 512;
-    // one chunk: the widest rows that still give every CU two workgroups
-    if(groups(16) >= kBlocks) return {16, 1, T};
-    if(groups(4) >= kBlocks / 2) return {groups(8) >= kBlocks ? 8 : 4, 1, T};
-    // chunks of at least 256 steps, a multiple of a thread's steps in them
-    const int64_t most = (T + 255) / 256, want = (kBlocks + groups(16) - 1) / groups(16);
-    const int64_t S = most < want ? most : want;
-    if(S <= 1) return {4, 1, T};
-    const int64_t L = ((T + S - 1) / S + 63) / 64 * 64;
-    return {16, (int)((T + L - 1) / L), L};
+    auto steps = [](int lanes) { return (int64_t)(kThreads / lanes * LT); };  // of a tile
+    // One chunk, which reads everything once, where it fills most of the chip, with
+    // the widest rows that do: 8x1024x768 8 lanes 50.5, 4 lanes 53.4, 2 chunks 59.2;
+    // 4x2000x768 4 lanes 55.8, 16 chunks 60.1; 16x512x512 8 lanes 32.9, 2 chunks 41.6
+    for(const int lanes : {16, 8, 4})
+        if(groups(lanes) >= 192) return {lanes, 1, T};
+    // ... and where it is a tile or two long: 8x64x768 9.3 (2 chunks of 32: a second
+    // launch), 1x300x2048 4 lanes 15.0, 3 chunks 18.8
+    for(const int lanes : {16, 8})
+        if(T <= steps(lanes)) return {lanes, 1, T};
+    if(T <= 2 * steps(4)) return {4, 1, T};
+    // Chunks.  Few tiles in all: one to a chunk, narrow ones, so that the chunks to
+    // gather the state from are few (3x1001x333 4 lanes 23.8, 16 lanes 27.3, one chunk
+    // 29.6; 1x9000x20 24.0).  Else 512 workgroups: rows of 128 bytes (1x32768x256 8
+    // lanes 78.3, 16 lanes 106, 4 lanes 85.9; 1x4096x768 38.3, 42.0, 38.8), of 64 where
+    // few channels would leave chunks many (1x20000x64 41.2, 8 lanes 47.6), of 256
+    // beyond what the last-level cache holds (1x65536x512 323, 8 lanes 355)
+    const int64_t tiles = groups(8) * ((T + steps(8) - 1) / steps(8));
+    const int lanes = tiles <= 384 || groups(8) < 4 ? 4 : tiles >= 8192 && groups(16) >= 8 ? 16 : 8;
+    const int64_t want = tiles <= 384 ? T : (512 + groups(lanes) - 1) / groups(lanes);
+    const int64_t per = ((T + want - 1) / want + steps(lanes) - 1) / steps(lanes);
+    const int64_t L = per * steps(lanes);
+    return {lanes, (int)((T + L - 1) / L), L};
 }
 
 template <int V, int CL, bool BWD>
 void launch(ScanParams& p, const Plan& plan, hipStream_t st) {
     p.groups = (int)((p.C + V * CL - 1) / (V * CL));
     const unsigned grid = (unsigned)((p.B * p.groups + 7) / 8 * 8);
-    if constexpr(CL == 16) {
-        if(plan.S > 1) scan_chunks<V, CL, BWD><<<dim3(grid, plan.S - 1), kThreads, 0, st>>>(p);
-    }
+    if(plan.S > 1) scan_chunks<V, CL, BWD><<<dim3(grid, plan.S - 1), kThreads, 0, st>>>(p);
     scan_tiles<V, CL, BWD><<<dim3(grid, plan.S), kThreads, 0, st>>>(p);
 }
 
@@ -470,15 +482,15 @@ int run(const char* who, ScanParams& p, void* workspace, size_t workspace_bytes,
         const unsigned grid = (unsigned)((p.B * ((p.C + V - 1) / V) + kThreads - 1) / kThreads);
         if(V == 1) scan_serial<1, BWD><<<grid, kThreads, 0, st>>>(p);
         else scan_serial<4, BWD><<<grid, kThreads, 0, st>>>(p);
-    } else if(p.C < 4) {
-        if(plan.lanes == 16) launch<1, 16, BWD>(p, plan, st);
-        else launch<1, 4, BWD>(p, plan, st);
-    } else if(plan.lanes == 16) {
-        launch<4, 16, BWD>(p, plan, st);
-    } else if(plan.lanes == 8) {
-        launch<4, 8, BWD>(p, plan, st);
     } else {
-        launch<4, 4, BWD>(p, plan, st);
+        auto with = [&](auto v) {
+            constexpr int V = decltype(v)::value;
+            if(plan.lanes == 16) launch<V, 16, BWD>(p, plan, st);
+            else if(plan.lanes == 8) launch<V, 8, BWD>(p, plan, st);
+            else launch<V, 4, BWD>(p, plan, st);
+        };
+        if(p.C < 4) with(std::integral_constant<int, 1>());
+        else with(std::integral_constant<int, 4>());
     }
     return pk::launch_status(who);
 }
