@@ -47,16 +47,19 @@ __device__ __forceinline__ void gate(float f, float& s, float& q) {
 // V channels from `at`.  A lane at the end of a row with fewer than 4 left reads the
 // row's last 4 (rows of fewer than 4 channels have V = 1): `skip` of them belong
 // to the lane before it and are not stored.
-template <int V>
+template <int V, bool NT = false>
 __device__ __forceinline__ void load(const float* at, float (&v)[V]) {
     if constexpr(V == 4) {
-        const f32x4 x = *reinterpret_cast<const f32x4u*>(at);
+        const f32x4u* const a = reinterpret_cast<const f32x4u*>(at);
+        const f32x4 x = NT ? __builtin_nontemporal_load(a) : *a;
 #pragma unroll
         for(int i = 0; i < 4; ++i) v[i] = x[i];
     } else {
         v[0] = *at;
     }
 }
+// (nontemporal: outputs that stay in the cache cost the inputs their place there; 32x2048x256
+// backward 93 -> 68 us, 1x65536x512 forward 116 -> 104)
 template <int V>
 __device__ __forceinline__ void store(float* at, const float (&v)[V], int skip, bool accum) {
     if constexpr(V == 4) {
@@ -64,7 +67,7 @@ __device__ __forceinline__ void store(float* at, const float (&v)[V], int skip, 
             f32x4 x = {v[0], v[1], v[2], v[3]};
             f32x4u* o = reinterpret_cast<f32x4u*>(at);
             if(accum) x = *o + x;
-            *o = x;
+            __builtin_nontemporal_store(x, o);
             return;
         }
     }
@@ -159,76 +162,78 @@ __device__ __forceinline__ float step(float p, float s, float v) {
     return BWD ? s * (v + p) : fmaf(s, p, v);
 }
 
-// the composed (A, H) of every chunk but the last: thread tl has the steps
-// tl n .. tl n + n - 1 of the chunk, n = L / TL
+// the composed (A, H) of every chunk but the last, tile by tile as scan_tiles walks
+// them (a thread with a run of the chunk of its own read 64 rows apart: 4.1
+// TB/s)
 template <int V, int CL, bool BWD>
 __global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
     using Pl = Place<V, CL>;
-    __shared__ float lds[1][kWaves][2][V * CL];
+    __shared__ float lds[2][kWaves][2][V * CL];
     const Pl at(p);
     if(!at.on) return;
-    const int64_t n = p.L / Pl::TL, g0 = at.chunk * p.L + at.tl * n;
-    const float* const f = p.f + at.b * p.T * p.ldf + at.c;
-    const float* const v = BWD ? p.dh + at.b * p.T * p.C + at.c : p.x + at.b * p.T * p.ldx + at.c;
-    const int64_t ldv = BWD ? p.C : p.ldx;
-    float A[V], H[V];
+    const int64_t g0 = at.chunk * p.L + at.tl * LT, t0 = BWD ? p.T - 1 - g0 : g0;
+    const int64_t ldv = BWD ? p.C : p.ldx, df = BWD ? -p.ldf : p.ldf, dv = BWD ? -ldv : ldv;
+    const float* fp = p.f + (at.b * p.T + t0) * p.ldf + at.c;
+    const float* vp = (BWD ? p.dh : p.x) + (at.b * p.T + t0) * ldv + at.c;
+    float all[V], carry[V], in[V], fr[LT][V], vr[LT][V];
 #pragma unroll
     for(int i = 0; i < V; ++i) {
-        A[i] = 1.0f;
-        H[i] = 0.0f;
+        all[i] = 1.0f;
+        carry[i] = 0.0f;
     }
-    float fr[LT][V], vr[LT][V];
-    const int64_t t0 = BWD ? p.T - 1 - g0 : g0, df = BWD ? -p.ldf : p.ldf, dv = BWD ? -ldv : ldv;
-    const float *fp = f + t0 * p.ldf, *vp = v + t0 * ldv;
     auto fetch = [&]() {
 #pragma unroll
         for(int e = 0; e < LT; ++e) {
             load<V>(fp + e * df, fr[e]);
             load<V>(vp + e * dv, vr[e]);
         }
-        fp += LT * df;
-        vp += LT * dv;
+        fp += Pl::TT * df;
+        vp += Pl::TT * dv;
     };
     fetch();
-    for(int64_t k = 0; k < n; k += LT) {
-        float fc[LT][V], vc[LT][V];
+    int turn = 0;
+    for(int64_t k = 0; k < p.L; k += Pl::TT) {
+        float s[LT][V], A[V], H[V];
 #pragma unroll
         for(int e = 0; e < LT; ++e)
 #pragma unroll
             for(int i = 0; i < V; ++i) {
-                fc[e][i] = fr[e][i];
-                vc[e][i] = vr[e][i];
+                float q;
+                gate(fr[e][i], s[e][i], q);
+                if(!BWD) vr[e][i] *= q;
             }
-        if(k + LT < n) fetch();
 #pragma unroll
-        for(int e = 0; e < LT; ++e)
+        for(int i = 0; i < V; ++i) {
+            A[i] = s[0][i];
+            H[i] = BWD ? s[0][i] * vr[0][i] : vr[0][i];
+        }
+#pragma unroll
+        for(int e = 1; e < LT; ++e)
 #pragma unroll
             for(int i = 0; i < V; ++i) {
-                float s, q;
-                gate(fc[e][i], s, q);
-                A[i] *= s;
-                H[i] = step<BWD>(H[i], s, BWD ? vc[e][i] : q * vc[e][i]);
+                A[i] *= s[e][i];
+                H[i] = step<BWD>(H[i], s[e][i], vr[e][i]);
             }
-    }
-    float a[V], none[V], in[V];
+        if(k + Pl::TT < p.L) fetch();
+        through<V, CL>(A, H, carry, in, lds, turn);
 #pragma unroll
-    for(int i = 0; i < V; ++i) none[i] = 0.0f;
-    // (the last lane's scanned A and its H from nothing are the chunk's)
-    through<V, CL>(A, H, none, in, lds, 0);
+        for(int i = 0; i < V; ++i)
 #pragma unroll
-    for(int i = 0; i < V; ++i) {
-        a[i] = 1.0f;
-#pragma unroll
-        for(int q = 0; q < kWaves; ++q) a[i] *= lds[0][q][0][at.cl * V + i];
+            for(int q = 0; q < kWaves; ++q) all[i] *= lds[turn][q][0][at.cl * V + i];
+        turn ^= 1;
     }
     if(at.tl == 0) {
         float* const o = p.ws + (at.chunk * p.B + at.b) * p.C + at.c;
-        store<V>(o, a, at.skip, false);
-        store<V>(o + (int64_t)p.S * p.B * p.C, none, at.skip, false);
+        store<V>(o, all, at.skip, false);
+        store<V>(o + (int64_t)p.S * p.B * p.C, carry, at.skip, false);
     }
 }
 
-template <int V, int CL, bool BWD>
+// BIG: x and h, which only this pass of the backward reads, leave the caches to f and
+// dh and to the next kernel (1x65536x512 backward 195 -> 167 us, 4x8192x1024 214 ->
+// 200; tensors that fit the last-level cache are better read from there: 8x1024x768
+// 30 against 37, 32x2048x256 68 against 75)
+template <int V, int CL, bool BWD, bool BIG>
 __global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
     using Pl = Place<V, CL>;
     __shared__ float lds[2][kWaves][2][V * CL];
@@ -267,14 +272,14 @@ __global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
 #pragma unroll
         for(int e = 0; e < LT; ++e) {
             load<V>(fp, next.f[e]);
-            load<V>(xp, next.x[e]);
+            load<V, BIG>(xp, next.x[e]);
             fp += BWD ? -p.ldf : p.ldf;
             xp += BWD ? -p.ldx : p.ldx;
             if constexpr(BWD) {
                 // (before the first token: h0, or a zero put in later)
                 if(e == LT - 1 && t0 == LT - 1) hp = h0 ? h0 : dp;
                 load<V>(dp, next.dh[e]);
-                load<V>(hp, next.h[e]);
+                load<V, BIG>(hp, next.h[e]);
                 dp -= p.C;
                 hp -= p.C;
             }
@@ -465,7 +470,11 @@ void launch(ScanParams& p, const Plan& plan, hipStream_t st) {
     p.groups = (int)((p.C + V * CL - 1) / (V * CL));
     const unsigned grid = (unsigned)((p.B * p.groups + 7) / 8 * 8);
     if(plan.S > 1) scan_chunks<V, CL, BWD><<<dim3(grid, plan.S - 1), kThreads, 0, st>>>(p);
-    scan_tiles<V, CL, BWD><<<dim3(grid, plan.S), kThreads, 0, st>>>(p);
+    // (values of a tensor: between 17 and 33 million)
+    if(BWD && p.B * p.T * p.C >= (int64_t)24 << 20)
+        scan_tiles<V, CL, BWD, BWD><<<dim3(grid, plan.S), kThreads, 0, st>>>(p);
+    else
+        scan_tiles<V, CL, BWD, false><<<dim3(grid, plan.S), kThreads, 0, st>>>(p);
 }
 
 template <bool BWD>
