@@ -681,25 +681,37 @@ ACCUM3 = 4
 PRECISIONS = {"fp32": 0, "bf16": 1, "bf16x3": 2}
 
 
-def _here(*ts):
-    """the launchers run on the current device: tensors of another are refused"""
+def _ready(dtype, *ts):
+    """each of `ts` (None aside) is a `dtype` tensor on the current device, where the
+    launchers run; returns the device's index"""
+    dev = torch.cuda.current_device()
     for t in ts:
-        if t is not None and t.is_cuda and t.device.index != torch.cuda.current_device():
+        if t is not None and (t.dtype is not dtype or t.get_device() != dev):
+            if t.dtype is not dtype or not t.is_cuda:
+                raise TypeError(f"expected a {dtype} CUDA tensor, got {t.dtype} on {t.device}")
             raise ValueError("a tensor lies on another device than the current one")
+    return dev
 
 
-def _i32(*ts):
-    for t in ts:
-        if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
-            raise TypeError("expected a contiguous int32 CUDA tensor")
+def _at(t):
+    """a tensor's address for a launcher (None: NULL)"""
+    return None if t is None else t.data_ptr()
+
+
+def _raw_stream(dev):
+    """the current stream's handle (torch.cuda.current_stream(), in 0.1 us)"""
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _rows(t, name):
     """row stride of a 2-D tensor with unit columns and rows that do not overlap"""
-    ld = _rowmajor(t, name)
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
-        raise ValueError(f"{name}: rows overlap")
-    return ld
+    if t.dim() == 2:
+        rows, cols = t.shape
+        if t.is_contiguous():
+            return max(1, cols)
+        if (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols):
+            return max(t.stride(0), cols)
+    raise ValueError(f"{name} must be a 2-D tensor with unit column stride and rows apart")
 
 
 def _dense(*ts):
@@ -708,26 +720,26 @@ def _dense(*ts):
             raise ValueError("expected a contiguous tensor")
 
 
-def _ws(ws, need, device):
-    """a workspace of `need` bytes (ws itself when given) and its size"""
+def _ws(ws, dev, size, *shape):
+    """a workspace of size(*shape) bytes (ws itself when given: the launcher says
+    when it is too small) and its size"""
     if ws is None:
-        ws = torch.empty(max(1, need), dtype=torch.uint8, device=device)
-    elif ws.device != device or not ws.is_contiguous():
+        ws = torch.empty(max(1, size(*shape)), dtype=torch.uint8, device=dev)
+    elif ws.get_device() != dev or not ws.is_contiguous():
         raise ValueError("a workspace must be contiguous and on the operands' device")
-    return ws, ws.numel() * ws.element_size()
+    return ws, ws.nbytes
 
 
 def layernorm_fwd(x, g, b, y, mean, rstd, eps):
     """y = (x - m) r g + b over the rows of x [R, C]; b, mean, rstd may be None"""
-    _f32(x, g, b, y, mean, rstd)
-    _here(x, g, b, y, mean, rstd)
+    dev = _ready(torch.float32, x, g, b, y, mean, rstd)
     _dense(x, g, b, y, mean, rstd)
     R, C = x.shape
     if g.numel() != C or (b is not None and b.numel() != C) or y.shape != x.shape or \
             any(t is not None and t.numel() != R for t in (mean, rstd)):
         raise ValueError("layernorm_fwd shape mismatch")
     check("pk_layernorm_fwd_f32", hip_lib().pk_layernorm_fwd_f32(
-        R, C, eps, _ptr(x), _ptr(g), _ptr(b), _ptr(y), _ptr(mean), _ptr(rstd), _stream()))
+        R, C, eps, _at(x), _at(g), _at(b), _at(y), _at(mean), _at(rstd), _raw_stream(dev)))
     return y
 
 
@@ -738,19 +750,18 @@ def layernorm_bwd_workspace(R, C):
 def layernorm_bwd(x, g, mean, rstd, dy, dx, dg, db, ws=None, dx_in=None, accum_dg=False,
                   accum_db=False):
     """gradients of layernorm_fwd (a None one is skipped); dx_in is added to dx"""
-    _f32(x, g, mean, rstd, dy, dx, dg, db, dx_in)
-    _here(x, g, mean, rstd, dy, dx, dg, db, dx_in)
+    dev = _ready(torch.float32, x, g, mean, rstd, dy, dx, dg, db, dx_in)
     _dense(x, g, mean, rstd, dy, dx, dg, db, dx_in)
     R, C = x.shape
     if g.numel() != C or any(t is not None and t.shape != x.shape for t in (dy, dx, dx_in)) or \
             any(t is not None and t.numel() != C for t in (dg, db)) or \
             mean.numel() != R or rstd.numel() != R:
         raise ValueError("layernorm_bwd shape mismatch")
-    ws, wsb = _ws(ws, layernorm_bwd_workspace(R, C), x.device)
+    ws, wsb = _ws(ws, dev, layernorm_bwd_workspace, R, C)
     flags = (ACCUM2 if accum_dg else 0) | (ACCUM3 if accum_db else 0)
     check("pk_layernorm_bwd_f32", hip_lib().pk_layernorm_bwd_f32(
-        R, C, _ptr(x), _ptr(g), _ptr(mean), _ptr(rstd), _ptr(dy), _ptr(dx_in), _ptr(dx), _ptr(dg),
-        _ptr(db), flags, _ptr(ws), wsb, _stream()))
+        R, C, _at(x), _at(g), _at(mean), _at(rstd), _at(dy), _at(dx_in), _at(dx), _at(dg),
+        _at(db), flags, _at(ws), wsb, _raw_stream(dev)))
 
 
 def gated_scan_workspace(B, T, C):
@@ -769,62 +780,56 @@ def _scan_layout(B, f, x, h0, *rows):
 
 def gated_scan_fwd(B, f, x, h, h0=None, ws=None):
     """h_t = s_t h_{t-1} + (1 - s_t) x_t, s = sigmoid(f), over B sequences"""
-    _f32(f, x, h, h0)
-    _here(f, x, h, h0)
+    dev = _ready(torch.float32, f, x, h, h0)
     _dense(h, h0)
     T, C = _scan_layout(B, f, x, h0, h)
-    ws, wsb = _ws(ws, gated_scan_workspace(B, T, C), x.device)
+    ws, wsb = _ws(ws, dev, gated_scan_workspace, B, T, C)
     check("pk_gated_scan_fwd_f32", hip_lib().pk_gated_scan_fwd_f32(
-        B, T, C, _ptr(f), _rows(f, "f"), _ptr(x), _rows(x, "x"), _ptr(h0), _ptr(h), _ptr(ws),
-        wsb, _stream()))
+        B, T, C, _at(f), _rows(f, "f"), _at(x), _rows(x, "x"), _at(h0), _at(h), _at(ws),
+        wsb, _raw_stream(dev)))
     return h
 
 
 def gated_scan_bwd(B, f, x, h, dh, df, dx, h0=None, dh0=None, ws=None, accum_df=False,
                    accum_dx=False, accum_dh0=False):
     """gradients of gated_scan_fwd (a None one is skipped)"""
-    _f32(f, x, h, dh, df, dx, h0, dh0)
-    _here(f, x, h, dh, df, dx, h0, dh0)
+    dev = _ready(torch.float32, f, x, h, dh, df, dx, h0, dh0)
     _dense(h, dh, h0, dh0)
     T, C = _scan_layout(B, f, x, h0, h, dh, df, dx)
     if dh0 is not None and tuple(dh0.shape) != (B, C):
         raise ValueError("gated_scan: dh0 must be [B, C]")
-    ws, wsb = _ws(ws, gated_scan_workspace(B, T, C), x.device)
+    ws, wsb = _ws(ws, dev, gated_scan_workspace, B, T, C)
     flags = (ACCUM if accum_df else 0) | (ACCUM2 if accum_dx else 0) | (ACCUM3 if accum_dh0 else 0)
     check("pk_gated_scan_bwd_f32", hip_lib().pk_gated_scan_bwd_f32(
-        B, T, C, _ptr(f), _rows(f, "f"), _ptr(x), _rows(x, "x"), _ptr(h0), _ptr(h), _ptr(dh),
-        _ptr(df), C if df is None else _rows(df, "df"), _ptr(dx),
-        C if dx is None else _rows(dx, "dx"), _ptr(dh0), flags, _ptr(ws), wsb, _stream()))
+        B, T, C, _at(f), _rows(f, "f"), _at(x), _rows(x, "x"), _at(h0), _at(h), _at(dh),
+        _at(df), C if df is None else _rows(df, "df"), _at(dx),
+        C if dx is None else _rows(dx, "dx"), _at(dh0), flags, _at(ws), wsb, _raw_stream(dev)))
 
 
 def route_topk(logits, experts, gates):
     """experts [R, k] int32 and gates [R, k]: the k largest logits of each token
     and the softmax over them"""
-    _f32(logits, gates)
-    _here(logits, gates)
-    _i32(experts)
-    _here(experts)
-    _dense(gates)
+    dev = _ready(torch.float32, logits, gates)
+    _ready(torch.int32, experts)
+    _dense(experts, gates)
     if experts.dim() != 2 or gates.shape != experts.shape or experts.shape[0] != logits.shape[0]:
         raise ValueError("route_topk: experts and gates must be [R, k]")
     check("pk_route_topk_f32", hip_lib().pk_route_topk_f32(
-        logits.shape[0], logits.shape[1], experts.shape[1], _ptr(logits),
-        _rows(logits, "logits"), _ptr(experts), _ptr(gates), _stream()))
+        logits.shape[0], logits.shape[1], experts.shape[1], _at(logits),
+        _rows(logits, "logits"), _at(experts), _at(gates), _raw_stream(dev)))
 
 
 def route_topk_bwd(experts, gates, dgates, dlogits, accum=False):
-    _f32(gates, dgates, dlogits)
-    _here(gates, dgates, dlogits)
-    _i32(experts)
-    _here(experts)
-    _dense(gates, dgates)
+    dev = _ready(torch.float32, gates, dgates, dlogits)
+    _ready(torch.int32, experts)
+    _dense(experts, gates, dgates)
     if gates.shape != experts.shape or dgates.shape != experts.shape or \
             experts.shape[0] != dlogits.shape[0]:
         raise ValueError("route_topk_bwd: experts, gates and dgates must be [R, k]")
     check("pk_route_topk_bwd_f32", hip_lib().pk_route_topk_bwd_f32(
-        dlogits.shape[0], dlogits.shape[1], experts.shape[1], _ptr(experts), _ptr(gates),
-        _ptr(dgates), _ptr(dlogits), _rows(dlogits, "dlogits"), ACCUM if accum else 0,
-        _stream()))
+        dlogits.shape[0], dlogits.shape[1], experts.shape[1], _at(experts), _at(gates),
+        _at(dgates), _at(dlogits), _rows(dlogits, "dlogits"), ACCUM if accum else 0,
+        _raw_stream(dev)))
     return dlogits
 
 
@@ -835,14 +840,14 @@ def expert_plan_workspace(n, E):
 def expert_plan(experts, offsets, order, place, ws=None):
     """the slots of experts [R, k] in expert order: offsets [E + 1], order and
     place [R*k], all int32"""
-    _i32(experts, offsets, order, place)
-    _here(experts, offsets, order, place)
+    dev = _ready(torch.int32, experts, offsets, order, place)
+    _dense(experts, offsets, order, place)
     n, E = experts.numel(), offsets.numel() - 1
     if order.numel() != n or place.numel() != n or E < 1:
         raise ValueError("expert_plan: order and place must hold a value a slot, offsets E + 1")
-    ws, wsb = _ws(ws, expert_plan_workspace(n, E), experts.device)
+    ws, wsb = _ws(ws, dev, expert_plan_workspace, n, E)
     check("pk_expert_plan", hip_lib().pk_expert_plan(
-        n, E, _ptr(experts), _ptr(offsets), _ptr(order), _ptr(place), _ptr(ws), wsb, _stream()))
+        n, E, _at(experts), _at(offsets), _at(order), _at(place), _at(ws), wsb, _raw_stream(dev)))
 
 
 def _expert_rows(n, d, *ts):
@@ -853,27 +858,24 @@ def _expert_rows(n, d, *ts):
 
 def expert_gather(x, k, offsets, order, out):
     """out[r] = x[order[r] // k]; zero rows behind the last expert's"""
-    _f32(x, out)
-    _here(x, out)
-    _i32(offsets, order)
-    _here(offsets, order)
+    dev = _ready(torch.float32, x, out)
+    _ready(torch.int32, offsets, order)
+    _dense(offsets, order)
     n, d = x.shape[0] * k, x.shape[1]
     _expert_rows(n, d, out)
     if order.numel() != n or offsets.numel() < 2:
         raise ValueError("expert_gather: order must hold a value a slot, offsets E + 1")
     check("pk_expert_gather_f32", hip_lib().pk_expert_gather_f32(
-        n, d, k, offsets.numel() - 1, _ptr(offsets), _ptr(order), _ptr(x), _rows(x, "x"),
-        _ptr(out), _rows(out, "out"), _stream()))
+        n, d, k, offsets.numel() - 1, _at(offsets), _at(order), _at(x), _rows(x, "x"),
+        _at(out), _rows(out, "out"), _raw_stream(dev)))
     return out
 
 
 def expert_combine(place, gates, ys, out, c=None):
     """out[t] = c[t] + sum_j gates[t, j] ys[place[t, j]] (gates None: 1)"""
-    _f32(gates, ys, out, c)
-    _here(gates, ys, out, c)
-    _i32(place)
-    _here(place)
-    _dense(gates)
+    dev = _ready(torch.float32, gates, ys, out, c)
+    _ready(torch.int32, place)
+    _dense(place, gates)
     R, d = out.shape
     n = place.numel()
     if R == 0:
@@ -883,18 +885,16 @@ def expert_combine(place, gates, ys, out, c=None):
     _expert_rows(n, d, ys)
     _expert_rows(R, d, c)
     check("pk_expert_combine_f32", hip_lib().pk_expert_combine_f32(
-        R, d, n // R, _ptr(place), _ptr(gates), _ptr(ys), _rows(ys, "ys"), _ptr(c),
-        d if c is None else _rows(c, "c"), _ptr(out), _rows(out, "out"), _stream()))
+        R, d, n // R, _at(place), _at(gates), _at(ys), _rows(ys, "ys"), _at(c),
+        d if c is None else _rows(c, "c"), _at(out), _rows(out, "out"), _raw_stream(dev)))
     return out
 
 
 def expert_combine_bwd(offsets, order, gates, ys, dout, dys, dgates, accum_dys=False,
                        accum_dgates=False):
-    _f32(gates, ys, dout, dys, dgates)
-    _here(gates, ys, dout, dys, dgates)
-    _i32(offsets, order)
-    _here(offsets, order)
-    _dense(gates, dgates)
+    dev = _ready(torch.float32, gates, ys, dout, dys, dgates)
+    _ready(torch.int32, offsets, order)
+    _dense(offsets, order, gates, dgates)
     R, d = dout.shape
     n = order.numel()
     if R == 0:
@@ -905,9 +905,9 @@ def expert_combine_bwd(offsets, order, gates, ys, dout, dys, dgates, accum_dys=F
     _expert_rows(n, d, ys, dys)
     flags = (ACCUM if accum_dys else 0) | (ACCUM2 if accum_dgates else 0)
     check("pk_expert_combine_bwd_f32", hip_lib().pk_expert_combine_bwd_f32(
-        R, d, n // R, offsets.numel() - 1, _ptr(offsets), _ptr(order), _ptr(gates), _ptr(ys),
-        d if ys is None else _rows(ys, "ys"), _ptr(dout), _rows(dout, "dout"), _ptr(dys),
-        d if dys is None else _rows(dys, "dys"), _ptr(dgates), flags, _stream()))
+        R, d, n // R, offsets.numel() - 1, _at(offsets), _at(order), _at(gates), _at(ys),
+        d if ys is None else _rows(ys, "ys"), _at(dout), _rows(dout, "dout"), _at(dys),
+        d if dys is None else _rows(dys, "dys"), _at(dgates), flags, _raw_stream(dev)))
 
 
 def _expert_stack(w, name):
@@ -920,10 +920,9 @@ def _expert_stack(w, name):
 
 def gemm_experts(tb, x, w, offsets, y, precision="fp32", accum=False):
     """y[r] = x[r] @ op(w[e]) for every expert's rows r (op = transpose for 'T')"""
-    _f32(x, w, y)
-    _here(x, w, y)
-    _i32(offsets)
-    _here(offsets)
+    dev = _ready(torch.float32, x, w, y)
+    _ready(torch.int32, offsets)
+    _dense(offsets)
     ldw, sw = _expert_stack(w, "w")
     E, K, N = w.shape if tb == "N" else (w.shape[0], w.shape[2], w.shape[1])
     n = x.shape[0]
@@ -932,8 +931,8 @@ def gemm_experts(tb, x, w, offsets, y, precision="fp32", accum=False):
                          f"{offsets.numel()} offsets do not fit")
     _expert_rows(n, N, y)
     check("pk_gemm_experts_f32", hip_lib().pk_gemm_experts_f32(
-        tb.encode(), n, N, K, E, _ptr(offsets), _ptr(x), _rows(x, "x"), _ptr(w), ldw, sw,
-        _ptr(y), _rows(y, "y"), ACCUM if accum else 0, PRECISIONS[precision], _stream()))
+        tb.encode(), n, N, K, E, _at(offsets), _at(x), _rows(x, "x"), _at(w), ldw, sw,
+        _at(y), _rows(y, "y"), ACCUM if accum else 0, PRECISIONS[precision], _raw_stream(dev)))
     return y
 
 
@@ -943,10 +942,9 @@ def gemm_experts_dw_workspace(n, K, N, E):
 
 def gemm_experts_dw(x, dy, offsets, dw, precision="fp32", accum=False, ws=None):
     """dw[e] = x_e^T @ dy_e over every expert's rows"""
-    _f32(x, dy, dw)
-    _here(x, dy, dw)
-    _i32(offsets)
-    _here(offsets)
+    dev = _ready(torch.float32, x, dy, dw)
+    _ready(torch.int32, offsets)
+    _dense(offsets)
     ldw, sw = _expert_stack(dw, "dw")
     E, K, N = dw.shape
     n = x.shape[0]
@@ -954,10 +952,10 @@ def gemm_experts_dw(x, dy, offsets, dw, precision="fp32", accum=False, ws=None):
         raise ValueError("gemm_experts_dw: offsets must hold E + 1 values")
     _expert_rows(n, K, x)
     _expert_rows(n, N, dy)
-    ws, wsb = _ws(ws, gemm_experts_dw_workspace(n, K, N, E), x.device)
+    ws, wsb = _ws(ws, dev, gemm_experts_dw_workspace, n, K, N, E)
     check("pk_gemm_experts_dw_f32", hip_lib().pk_gemm_experts_dw_f32(
-        n, K, N, E, _ptr(offsets), _ptr(x), _rows(x, "x"), _ptr(dy), _rows(dy, "dy"),
-        _ptr(dw), ldw, sw, ACCUM if accum else 0, PRECISIONS[precision], _ptr(ws), wsb, _stream()))
+        n, K, N, E, _at(offsets), _at(x), _rows(x, "x"), _at(dy), _rows(dy, "dy"),
+        _at(dw), ldw, sw, ACCUM if accum else 0, PRECISIONS[precision], _at(ws), wsb, _raw_stream(dev)))
     return dw
 
 
