@@ -4,57 +4,334 @@
 //   xh = (x - m) r
 //   dx = r (g dy - mean(g dy) - xh mean(g dy xh))
 //   dg = sum over rows of dy xh,  db = sum over rows of dy
+//
+// Bound by memory: 8 bytes a value forward, 12 backward, each row read once and
+// kept in registers between the sums and the result.  W waves share a row, NV 4-value
+// vectors a lane; the mean and the squares around it are each wave's own, put
+// together as
+//   M2 = sum of M2_w + n_w (m_w - m)^2
+// so that a row takes one exchange through LDS and no difference of squares.  128-bit
+// accesses at any 4-byte alignment; of a row whose length is no multiple of 4 the
+// last lane reads the last 4 values and leaves those before its own out.
+#include <type_traits>
+
 #include "pk_common.h"
 
 namespace {
 
-__global__ __launch_bounds__(256) void layernorm_fwd_any(int64_t R, int64_t C, float eps,
-                                                         const float* __restrict__ x,
-                                                         const float* __restrict__ g,
-                                                         const float* __restrict__ b,
-                                                         float* __restrict__ y,
-                                                         float* __restrict__ mean,
-                                                         float* __restrict__ rstd) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const int lane = threadIdx.x % 64;
-    if(row >= R) return;
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+template <bool NT>
+__device__ __forceinline__ f32x4 load4(const float* p) {
+    const f32x4u* const a = reinterpret_cast<const f32x4u*>(p);
+    return NT ? __builtin_nontemporal_load(a) : *a;
+}
+
+// A lane's share of a row: vector v starts at column `at[v]` and holds `skip[v]` values
+// (0 to 3) of the lane before it, or lies past the row (4).  EXACT: every vector
+// is whole.
+template <int NV, int W, bool EXACT>
+struct Share {
+    int at[NV], skip[NV];
+    float count;  // the wave's values
+
+    __device__ __forceinline__ explicit Share(int C) {
+        const int t = threadIdx.x % (64 * W);
+        int mine = 0;
+#pragma unroll
+        for(int v = 0; v < NV; ++v) {
+            const int c = 4 * (v * 64 * W + t);
+            at[v] = EXACT ? c : min(c, C - 4);
+            skip[v] = EXACT ? 0 : min(c - at[v], 4);
+            mine += 4 - skip[v];
+        }
+        count = EXACT ? 256.0f * NV : pk::wave_sum((float)mine);
+    }
+    template <bool NT>
+    __device__ __forceinline__ void load(const float* row, f32x4 (&x)[NV]) const {
+#pragma unroll
+        for(int v = 0; v < NV; ++v) x[v] = load4<NT>(row + at[v]);
+    }
+    // whether value i of vector v is the lane's own
+    __device__ __forceinline__ bool own(int v, int i) const { return EXACT || i >= skip[v]; }
+    __device__ __forceinline__ void store(float* row, int v, f32x4 y) const {
+        if(EXACT || skip[v] == 0) {
+            __builtin_nontemporal_store(y, reinterpret_cast<f32x4u*>(row + at[v]));
+        } else {
+#pragma unroll
+            for(int i = 1; i < 4; ++i)
+                if(i >= skip[v]) row[at[v] + i] = y[i];
+        }
+    }
+};
+
+// rows of W waves each, 4 / W of them in a workgroup of 4 waves, the next one's
+// values in flight
+template <int NV, int W, bool EXACT, bool NT>
+__global__ __launch_bounds__(W > 4 ? 64 * W : 256) void layernorm_fwd(int R, int C, float eps,
+                                                                      const float* __restrict__ x,
+                                                                      const float* __restrict__ g,
+                                                                      const float* __restrict__ b,
+                                                                      float* __restrict__ y,
+                                                                      float* __restrict__ mean,
+                                                                      float* __restrict__ rstd) {
+    constexpr int ROWS = W > 4 ? 1 : 4 / W;
+    __shared__ float part[2][ROWS][W][3];
+    const Share<NV, W, EXACT> me(C);
+    const int group = threadIdx.x / (64 * W), w = threadIdx.x / 64 % W;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    const float inv = 1.0f / me.count;
+    int64_t row = (int64_t)blockIdx.x * ROWS + group;
+    f32x4 cur[NV], next[NV];
+    if(W > 1 || row < R) me.template load<NT>(x + min(row, (int64_t)R - 1) * C, cur);
+    // (the waves of a workgroup meet in every turn, so all take the same ones)
+    for(int turn = 0; row - group < R; row += step, turn ^= 1) {
+        if(W == 1 && row >= R) return;
+        const int64_t after = min(row + step, (int64_t)R - 1);
+        if(row - group + step < R) me.template load<NT>(x + after * C, next);
+        float s = 0.0f;
+#pragma unroll
+        for(int v = 0; v < NV; ++v)
+#pragma unroll
+            for(int i = 0; i < 4; ++i) s += me.own(v, i) ? cur[v][i] : 0.0f;
+        float m = pk::wave_sum(s) / me.count, q = 0.0f;
+        if(!EXACT && me.count == 0.0f) m = 0.0f;
+#pragma unroll
+        for(int v = 0; v < NV; ++v)
+#pragma unroll
+            for(int i = 0; i < 4; ++i) {
+                const float d = me.own(v, i) ? cur[v][i] - m : 0.0f;
+                q = fmaf(d, d, q);
+            }
+        q = pk::wave_sum(q);
+        if constexpr(W > 1) {
+            if(threadIdx.x % 64 == 0) {
+                part[turn][group][w][0] = me.count;
+                part[turn][group][w][1] = m;
+                part[turn][group][w][2] = q;
+            }
+            __syncthreads();
+            s = 0.0f;
+#pragma unroll
+            for(int i = 0; i < W; ++i) s = fmaf(part[turn][group][i][0], part[turn][group][i][1], s);
+            m = s / (float)C;
+            q = 0.0f;
+#pragma unroll
+            for(int i = 0; i < W; ++i) {
+                const float d = part[turn][group][i][1] - m;
+                q += fmaf(part[turn][group][i][0] * d, d, part[turn][group][i][2]);
+            }
+        }
+        const float r = 1.0f / sqrtf(q / (float)C + eps);
+        if(row < R) {
+            if(threadIdx.x % (64 * W) == 0) {
+                if(mean) mean[row] = m;
+                if(rstd) rstd[row] = r;
+            }
+            float* const yr = y + row * C;
+#pragma unroll
+            for(int v = 0; v < NV; ++v) {
+                if(!EXACT && me.skip[v] == 4) continue;
+                f32x4 o = (cur[v] - m) * r * load4<false>(g + me.at[v]);
+                if(b) o = o + load4<false>(b + me.at[v]);
+                me.store(yr, v, o);
+            }
+        }
+#pragma unroll
+        for(int v = 0; v < NV; ++v) cur[v] = next[v];
+    }
+}
+
+// dx of every row, and the workgroup's part of dg and db in ws [P][2][C] (or, P = 1,
+// dg and db themselves): a workgroup of 8 waves walks rows 8 / W at a time, its
+// lanes keeping the sums of their own columns; at the end the row groups' sums meet
+// in LDS, in a fixed order.
+constexpr int kBwdWaves = 8;
+enum { kDx = 1, kSums = 2, kDirect = 4 };
+
+template <int NV, int W, bool EXACT, bool NT>
+__global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
+    int R, int C, const float* __restrict__ x, const float* __restrict__ g,
+    const float* __restrict__ mean, const float* __restrict__ rstd, const float* __restrict__ dy,
+    const float* dxin, float* dx, float* __restrict__ ws, float* dg, float* db, int what, int flags) {
+    constexpr int ROWS = kBwdWaves / W;
+    __shared__ float part[2][ROWS][W][2];
+    extern __shared__ float sums[];  // [ROWS / 2][2][C]
+    const Share<NV, W, EXACT> me(C);
+    const int group = threadIdx.x / (64 * W), w = threadIdx.x / 64 % W;
+    const int64_t step = (int64_t)gridDim.x * ROWS;
+    f32x4 gv[NV], sg[NV], sb[NV], xc[NV], dc[NV], xn[NV], dn[NV];
+#pragma unroll
+    for(int v = 0; v < NV; ++v) {
+        gv[v] = load4<false>(g + me.at[v]);
+#pragma unroll
+        for(int i = 0; i < 4; ++i) gv[v][i] = me.own(v, i) ? gv[v][i] : 0.0f;
+        sg[v] = sb[v] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    int64_t row = (int64_t)blockIdx.x * ROWS + group;
+    float mn, rn;
+    auto fetch = [&](int64_t r, f32x4 (&a)[NV], f32x4 (&d)[NV]) {
+        r = min(r, (int64_t)R - 1);
+        me.template load<NT>(x + r * C, a);
+        me.template load<NT>(dy + r * C, d);
+        mn = mean[r];
+        rn = rstd[r];
+    };
+    // (8 vectors of every array leave no registers for the next row's)
+    constexpr bool AHEAD = NV <= 4;
+    if(AHEAD) fetch(row, xn, dn);
+    for(int turn = 0; row - group < R; row += step, turn ^= 1) {
+        if(!AHEAD) fetch(row, xc, dc);
+        const float m = mn, r = rn;
+        if(AHEAD) {
+#pragma unroll
+            for(int v = 0; v < NV; ++v) {
+                xc[v] = xn[v];
+                dc[v] = dn[v];
+            }
+            if(row - group + step < R) fetch(row + step, xn, dn);
+        }
+        const bool on = row < R;
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for(int v = 0; v < NV; ++v) {
+            xc[v] = (xc[v] - m) * r;
+#pragma unroll
+            for(int i = 0; i < 4; ++i) {
+                // (g is 0 where the value is not the lane's, which an infinity or NaN
+                // there would not respect)
+                const float t = me.own(v, i) ? gv[v][i] * dc[v][i] : 0.0f;
+                s1 += t;
+                s2 = fmaf(t, me.own(v, i) ? xc[v][i] : 0.0f, s2);
+            }
+        }
+        if(what & kDx) {
+            s1 = pk::wave_sum(s1);
+            s2 = pk::wave_sum(s2);
+            if constexpr(W > 1) {
+                if(threadIdx.x % 64 == 0) {
+                    part[turn][group][w][0] = s1;
+                    part[turn][group][w][1] = s2;
+                }
+                __syncthreads();
+                s1 = s2 = 0.0f;
+#pragma unroll
+                for(int i = 0; i < W; ++i) {
+                    s1 += part[turn][group][i][0];
+                    s2 += part[turn][group][i][1];
+                }
+            }
+            s1 /= (float)C;
+            s2 /= (float)C;
+        }
+        if(!on) continue;
+#pragma unroll
+        for(int v = 0; v < NV; ++v) {
+            if(!EXACT && me.skip[v] == 4) continue;
+            sg[v] = sg[v] + dc[v] * xc[v];
+            sb[v] = sb[v] + dc[v];
+            if(what & kDx) {
+                f32x4 o = r * (gv[v] * dc[v] - s1 - xc[v] * s2);
+                if(dxin) o = o + load4<NT>(dxin + row * C + me.at[v]);
+                me.store(dx + row * C, v, o);
+            }
+        }
+    }
+    if(!(what & kSums)) return;
+    // the row groups' sums, by halves: the upper half puts its own down, the lower
+    // adds them (a column belongs to one lane of every group)
+#pragma unroll
+    for(int half = ROWS / 2; half > 0; half /= 2) {
+        float* const slot = sums + (int64_t)(group % half) * 2 * C;
+        if(half < ROWS / 2) __syncthreads();
+        if(group >= half && group < 2 * half) {
+#pragma unroll
+            for(int v = 0; v < NV; ++v)
+#pragma unroll
+                for(int i = 0; i < 4; ++i) {
+                    if(!me.own(v, i)) continue;
+                    slot[me.at[v] + i] = sg[v][i];
+                    slot[C + me.at[v] + i] = sb[v][i];
+                }
+        }
+        __syncthreads();
+        if(group < half) {
+#pragma unroll
+            for(int v = 0; v < NV; ++v)
+#pragma unroll
+                for(int i = 0; i < 4; ++i) {
+                    if(!me.own(v, i)) continue;
+                    sg[v][i] += slot[me.at[v] + i];
+                    sb[v][i] += slot[C + me.at[v] + i];
+                }
+        }
+    }
+    if(group != 0) return;
+#pragma unroll
+    for(int v = 0; v < NV; ++v)
+#pragma unroll
+        for(int i = 0; i < 4; ++i) {
+            if(!me.own(v, i)) continue;
+            const int c = me.at[v] + i;
+            if(what & kDirect) {
+                if(dg) dg[c] = (flags & PK_ACCUM2) ? dg[c] + sg[v][i] : sg[v][i];
+                if(db) db[c] = (flags & PK_ACCUM3) ? db[c] + sb[v][i] : sb[v][i];
+            } else {
+                float* out = ws + (int64_t)blockIdx.x * 2 * C;
+                out[c] = sg[v][i];
+                out[C + c] = sb[v][i];
+            }
+        }
+}
+
+// ------------------------------------- rows of fewer than 4 or too many values
+// a row to NW waves, read again for every sum
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void layernorm_fwd_any(int64_t C, float eps,
+                                                             const float* __restrict__ x,
+                                                             const float* __restrict__ g,
+                                                             const float* __restrict__ b,
+                                                             float* __restrict__ y,
+                                                             float* __restrict__ mean,
+                                                             float* __restrict__ rstd) {
+    __shared__ float red[NW];
+    const int64_t row = blockIdx.x;
     const float* xr = x + row * C;
     float s = 0.0f;
-    for(int64_t c = lane; c < C; c += 64) s += xr[c];
-    const float m = pk::wave_sum(s) / (float)C;
+    for(int64_t c = threadIdx.x; c < C; c += 64 * NW) s += xr[c];
+    const float m = pk::block_sum<NW>(s, red) / (float)C;
     s = 0.0f;
-    for(int64_t c = lane; c < C; c += 64) s += (xr[c] - m) * (xr[c] - m);
-    const float r = 1.0f / sqrtf(pk::wave_sum(s) / (float)C + eps);
-    if(lane == 0) {
+    for(int64_t c = threadIdx.x; c < C; c += 64 * NW) s = fmaf(xr[c] - m, xr[c] - m, s);
+    const float r = 1.0f / sqrtf(pk::block_sum<NW>(s, red) / (float)C + eps);
+    if(threadIdx.x == 0) {
         if(mean) mean[row] = m;
         if(rstd) rstd[row] = r;
     }
-    for(int64_t c = lane; c < C; c += 64)
+    for(int64_t c = threadIdx.x; c < C; c += 64 * NW)
         y[row * C + c] = (xr[c] - m) * r * g[c] + (b ? b[c] : 0.0f);
 }
 
-__global__ __launch_bounds__(256) void layernorm_dx_any(int64_t R, int64_t C,
-                                                        const float* __restrict__ x,
-                                                        const float* __restrict__ g,
-                                                        const float* __restrict__ mean,
-                                                        const float* __restrict__ rstd,
-                                                        const float* __restrict__ dy,
-                                                        const float* dxin, float* dx) {
-    const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const int lane = threadIdx.x % 64;
-    if(row >= R) return;
+template <int NW>
+__global__ __launch_bounds__(64 * NW) void layernorm_dx_any(int64_t C, const float* __restrict__ x,
+                                                            const float* __restrict__ g,
+                                                            const float* __restrict__ mean,
+                                                            const float* __restrict__ rstd,
+                                                            const float* __restrict__ dy,
+                                                            const float* dxin, float* dx) {
+    __shared__ float red[2][NW];
+    const int64_t row = blockIdx.x;
     const float* xr = x + row * C;
     const float* dr = dy + row * C;
     const float m = mean[row], r = rstd[row];
     float s1 = 0.0f, s2 = 0.0f;
-    for(int64_t c = lane; c < C; c += 64) {
+    for(int64_t c = threadIdx.x; c < C; c += 64 * NW) {
         const float t = g[c] * dr[c];
         s1 += t;
         s2 += t * ((xr[c] - m) * r);
     }
-    s1 = pk::wave_sum(s1) / (float)C;
-    s2 = pk::wave_sum(s2) / (float)C;
-    for(int64_t c = lane; c < C; c += 64) {
+    s1 = pk::block_sum<NW>(s1, red[0]) / (float)C;
+    s2 = pk::block_sum<NW>(s2, red[1]) / (float)C;
+    for(int64_t c = threadIdx.x; c < C; c += 64 * NW) {
         const float v = r * (g[c] * dr[c] - s1 - (xr[c] - m) * r * s2);
         dx[row * C + c] = dxin ? dxin[row * C + c] + v : v;
     }
@@ -107,7 +384,42 @@ __global__ __launch_bounds__(64 * kSumWaves) void layernorm_sum(int64_t P, int64
     *o = (flags & (c < C ? PK_ACCUM2 : PK_ACCUM3)) ? *o + s : s;
 }
 
-int64_t parts_of(int64_t R) { return R < 256 ? R : 256; }
+// f(NV, W, EXACT) for rows of C values, 4 <= C <= 16384
+template <class F>
+void with_shape(int64_t C, F f) {
+    auto shape = [&](auto nv, auto w) {
+        constexpr int N = decltype(nv)::value, W = decltype(w)::value;
+        if(C == 256 * N * W) f(nv, w, std::true_type());
+        else f(nv, w, std::false_type());
+    };
+    using std::integral_constant;
+    const int64_t v = (C + 255) / 256;  // vectors a lane of one wave would have
+    if(v <= 1) shape(integral_constant<int, 1>(), integral_constant<int, 1>());
+    else if(v <= 2) shape(integral_constant<int, 2>(), integral_constant<int, 1>());
+    else if(v <= 3) shape(integral_constant<int, 3>(), integral_constant<int, 1>());
+    else if(v <= 4) shape(integral_constant<int, 4>(), integral_constant<int, 1>());
+    else if(v <= 6) shape(integral_constant<int, 3>(), integral_constant<int, 2>());
+    else if(v <= 8) shape(integral_constant<int, 4>(), integral_constant<int, 2>());
+    else if(v <= 12) shape(integral_constant<int, 3>(), integral_constant<int, 4>());
+    else if(v <= 16) shape(integral_constant<int, 4>(), integral_constant<int, 4>());
+    else if(v <= 24) shape(integral_constant<int, 3>(), integral_constant<int, 8>());
+    else if(v <= 32) shape(integral_constant<int, 4>(), integral_constant<int, 8>());
+    else shape(integral_constant<int, 8>(), integral_constant<int, 8>());
+}
+
+bool cached(int64_t C) { return C >= 4 && C <= 16384; }
+
+// the workgroups of the backward, each of which leaves a partial sum: one on every
+// CU at most, and one in all where a second launch would take longer
+int64_t parts_of(int64_t R, int64_t C) {
+    if(cached(C) && R * C <= 16384) return 1;
+    const int64_t waves = (C + 1023) / 1024;
+    const int64_t rows = !cached(C) ? 1 : waves <= 1 ? 8 : waves <= 2 ? 4 : waves <= 4 ? 2 : 1;
+    const int64_t p = (R + rows - 1) / rows;
+    return p < 256 ? p : 256;
+}
+
+bool big(int64_t R, int64_t C) { return R * C >= (int64_t)24 << 20; }
 
 }  // namespace
 
@@ -118,14 +430,29 @@ extern "C" int pk_layernorm_fwd_f32(int64_t R, int64_t C, float eps, const float
     if(R > (int64_t)INT32_MAX) return pk::fail("pk_layernorm_fwd_f32: R above 2^31 - 1");
     if(R == 0) return PK_OK;
     if(!x || !g || !y) return pk::fail("pk_layernorm_fwd_f32: NULL pointer");
-    layernorm_fwd_any<<<(unsigned)((R + 3) / 4), 256, 0, pk::as_stream(stream)>>>(R, C, eps, x, g, b, y,
-                                                                             mean, rstd);
+    hipStream_t st = pk::as_stream(stream);
+    if(!cached(C)) {
+        if(C < 4) layernorm_fwd_any<1><<<(unsigned)R, 64, 0, st>>>(C, eps, x, g, b, y, mean, rstd);
+        else layernorm_fwd_any<16><<<(unsigned)R, 1024, 0, st>>>(C, eps, x, g, b, y, mean, rstd);
+        return pk::launch_status("pk_layernorm_fwd_f32");
+    }
+    with_shape(C, [&](auto nv, auto w, auto exact) {
+        constexpr int N = decltype(nv)::value, W = decltype(w)::value;
+        constexpr bool EXACT = decltype(exact)::value;
+        constexpr int rows = W > 4 ? 1 : 4 / W, threads = W > 4 ? 64 * W : 256;
+        const int64_t blocks = (R + rows - 1) / rows;
+        const unsigned grid = (unsigned)(blocks < 2048 ? blocks : 2048);
+        if(big(R, C))
+            layernorm_fwd<N, W, EXACT, true><<<grid, threads, 0, st>>>((int)R, (int)C, eps, x, g, b, y, mean, rstd);
+        else
+            layernorm_fwd<N, W, EXACT, false><<<grid, threads, 0, st>>>((int)R, (int)C, eps, x, g, b, y, mean, rstd);
+    });
     return pk::launch_status("pk_layernorm_fwd_f32");
 }
 
 extern "C" size_t pk_layernorm_bwd_workspace(int64_t R, int64_t C) {
     if(R <= 0 || C <= 0) return 0;
-    return (size_t)parts_of(R) * 2 * (size_t)C * sizeof(float);
+    return (size_t)parts_of(R, C) * 2 * (size_t)C * sizeof(float);
 }
 
 extern "C" int pk_layernorm_bwd_f32(int64_t R, int64_t C, const float* x, const float* g,
@@ -144,9 +471,29 @@ extern "C" int pk_layernorm_bwd_f32(int64_t R, int64_t C, const float* x, const 
     }
     hipStream_t st = pk::as_stream(stream);
     float* ws = static_cast<float*>(workspace);
-    const int64_t P = R > 0 ? parts_of(R) : 0;
-    if(R > 0 && dx)
-        layernorm_dx_any<<<(unsigned)((R + 3) / 4), 256, 0, st>>>(R, C, x, g, mean, rstd, dy, dx_in, dx);
+    const int64_t P = R > 0 ? parts_of(R, C) : 0;
+    if(R > 0 && cached(C)) {
+        if(!dx && !sums) return PK_OK;
+        const int what = (dx ? kDx : 0) | (sums ? kSums : 0) | (P == 1 ? kDirect : 0);
+        with_shape(C, [&](auto nv, auto w, auto exact) {
+            constexpr int N = decltype(nv)::value, W = decltype(w)::value;
+            constexpr bool EXACT = decltype(exact)::value;
+            const size_t lds = kBwdWaves / W / 2 * 2 * (size_t)C * sizeof(float);
+            if(big(R, C))
+                layernorm_bwd<N, W, EXACT, true><<<(unsigned)P, 64 * kBwdWaves, lds, st>>>(
+                    (int)R, (int)C, x, g, mean, rstd, dy, dx_in, dx, ws, dg, db, what, flags);
+            else
+                layernorm_bwd<N, W, EXACT, false><<<(unsigned)P, 64 * kBwdWaves, lds, st>>>(
+                    (int)R, (int)C, x, g, mean, rstd, dy, dx_in, dx, ws, dg, db, what, flags);
+        });
+        if(sums && P > 1)
+            layernorm_sum<<<(unsigned)((2 * C + 63) / 64), 64 * kSumWaves, 0, st>>>(P, C, ws, dg, db, flags);
+        return pk::launch_status("pk_layernorm_bwd_f32");
+    }
+    if(R > 0 && dx) {
+        if(C < 4) layernorm_dx_any<1><<<(unsigned)R, 64, 0, st>>>(C, x, g, mean, rstd, dy, dx_in, dx);
+        else layernorm_dx_any<16><<<(unsigned)R, 1024, 0, st>>>(C, x, g, mean, rstd, dy, dx_in, dx);
+    }
     if(sums) {
         if(R > 0)
             layernorm_parts_any<<<dim3((unsigned)((C + 255) / 256), (unsigned)P), 256, 0, st>>>(
