@@ -21,11 +21,9 @@ namespace {
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
-template <bool NT>
-__device__ __forceinline__ f32x4 load4(const float* p) {
-    const f32x4u* const a = reinterpret_cast<const f32x4u*>(p);
-    return NT ? __builtin_nontemporal_load(a) : *a;
-}
+// (plain loads and nontemporal stores: with nontemporal loads 8192x4096 took 48 + 78 us
+// forward and backward, with these 41 + 73)
+__device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4u*>(p); }
 
 // A lane's share of a row: vector v starts at column `at[v]` and holds `skip[v]` values
 // (0 to 3) of the lane before it, or lies past the row (4).  EXACT: every vector
@@ -47,10 +45,9 @@ struct Share {
         }
         count = EXACT ? 256.0f * NV : pk::wave_sum((float)mine);
     }
-    template <bool NT>
     __device__ __forceinline__ void load(const float* row, f32x4 (&x)[NV]) const {
 #pragma unroll
-        for(int v = 0; v < NV; ++v) x[v] = load4<NT>(row + at[v]);
+        for(int v = 0; v < NV; ++v) x[v] = load4(row + at[v]);
     }
     // whether value i of vector v is the lane's own
     __device__ __forceinline__ bool own(int v, int i) const { return EXACT || i >= skip[v]; }
@@ -67,7 +64,7 @@ struct Share {
 
 // rows of W waves each, 4 / W of them in a workgroup of 4 waves, the next one's
 // values in flight
-template <int NV, int W, bool EXACT, bool NT>
+template <int NV, int W, bool EXACT>
 __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void layernorm_fwd(int R, int C, float eps,
                                                                       const float* __restrict__ x,
                                                                       const float* __restrict__ g,
@@ -83,12 +80,12 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void layernorm_fwd(int R, int
     const float inv = 1.0f / me.count;
     int64_t row = (int64_t)blockIdx.x * ROWS + group;
     f32x4 cur[NV], next[NV];
-    if(W > 1 || row < R) me.template load<NT>(x + min(row, (int64_t)R - 1) * C, cur);
+    if(W > 1 || row < R) me.load(x + min(row, (int64_t)R - 1) * C, cur);
     // (the waves of a workgroup meet in every turn, so all take the same ones)
     for(int turn = 0; row - group < R; row += step, turn ^= 1) {
         if(W == 1 && row >= R) return;
         const int64_t after = min(row + step, (int64_t)R - 1);
-        if(row - group + step < R) me.template load<NT>(x + after * C, next);
+        if(row - group + step < R) me.load(x + after * C, next);
         float s = 0.0f;
 #pragma unroll
         for(int v = 0; v < NV; ++v)
@@ -132,8 +129,8 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void layernorm_fwd(int R, int
 #pragma unroll
             for(int v = 0; v < NV; ++v) {
                 if(!EXACT && me.skip[v] == 4) continue;
-                f32x4 o = (cur[v] - m) * r * load4<false>(g + me.at[v]);
-                if(b) o = o + load4<false>(b + me.at[v]);
+                f32x4 o = (cur[v] - m) * r * load4(g + me.at[v]);
+                if(b) o = o + load4(b + me.at[v]);
                 me.store(yr, v, o);
             }
         }
@@ -149,7 +146,7 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void layernorm_fwd(int R, int
 constexpr int kBwdWaves = 8;
 enum { kDx = 1, kSums = 2, kDirect = 4 };
 
-template <int NV, int W, bool EXACT, bool NT>
+template <int NV, int W, bool EXACT>
 __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
     int R, int C, const float* __restrict__ x, const float* __restrict__ g,
     const float* __restrict__ mean, const float* __restrict__ rstd, const float* __restrict__ dy,
@@ -163,7 +160,7 @@ __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
     f32x4 gv[NV], sg[NV], sb[NV], xc[NV], dc[NV], xn[NV], dn[NV];
 #pragma unroll
     for(int v = 0; v < NV; ++v) {
-        gv[v] = load4<false>(g + me.at[v]);
+        gv[v] = load4(g + me.at[v]);
 #pragma unroll
         for(int i = 0; i < 4; ++i) gv[v][i] = me.own(v, i) ? gv[v][i] : 0.0f;
         sg[v] = sb[v] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -172,8 +169,8 @@ __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
     float mn, rn;
     auto fetch = [&](int64_t r, f32x4 (&a)[NV], f32x4 (&d)[NV]) {
         r = min(r, (int64_t)R - 1);
-        me.template load<NT>(x + r * C, a);
-        me.template load<NT>(dy + r * C, d);
+        me.load(x + r * C, a);
+        me.load(dy + r * C, d);
         mn = mean[r];
         rn = rstd[r];
     };
@@ -232,7 +229,7 @@ __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
             sb[v] = sb[v] + dc[v];
             if(what & kDx) {
                 f32x4 o = r * (gv[v] * dc[v] - s1 - xc[v] * s2);
-                if(dxin) o = o + load4<NT>(dxin + row * C + me.at[v]);
+                if(dxin) o = o + load4(dxin + row * C + me.at[v]);
                 me.store(dx + row * C, v, o);
             }
         }
@@ -410,16 +407,16 @@ void with_shape(int64_t C, F f) {
 bool cached(int64_t C) { return C >= 4 && C <= 16384; }
 
 // the workgroups of the backward, each of which leaves a partial sum: one on every
-// CU at most, and one in all where a second launch would take longer
+// CU at most (8192x4096 73 us, two 78; of short rows two: 65536x128 25, one 32), and
+// one in all where a second launch would take longer
 int64_t parts_of(int64_t R, int64_t C) {
     if(cached(C) && R * C <= 16384) return 1;
     const int64_t waves = (C + 1023) / 1024;
     const int64_t rows = !cached(C) ? 1 : waves <= 1 ? 8 : waves <= 2 ? 4 : waves <= 4 ? 2 : 1;
     const int64_t p = (R + rows - 1) / rows;
-    return p < 256 ? p : 256;
+    const int64_t most = C <= 256 ? 512 : 256;
+    return p < most ? p : most;
 }
-
-bool big(int64_t R, int64_t C) { return R * C >= (int64_t)24 << 20; }
 
 }  // namespace
 
@@ -441,11 +438,12 @@ extern "C" int pk_layernorm_fwd_f32(int64_t R, int64_t C, float eps, const float
         constexpr bool EXACT = decltype(exact)::value;
         constexpr int rows = W > 4 ? 1 : 4 / W, threads = W > 4 ? 64 * W : 256;
         const int64_t blocks = (R + rows - 1) / rows;
-        const unsigned grid = (unsigned)(blocks < 2048 ? blocks : 2048);
-        if(big(R, C))
-            layernorm_fwd<N, W, EXACT, true><<<grid, threads, 0, st>>>((int)R, (int)C, eps, x, g, b, y, mean, rstd);
-        else
-            layernorm_fwd<N, W, EXACT, false><<<grid, threads, 0, st>>>((int)R, (int)C, eps, x, g, b, y, mean, rstd);
+        // workgroups walk the rows, the next one's loads under the present one's sums: four
+        // on a CU (8192x1024 9.1 us, eight 10.6), eight of short rows (65536x128 18.5,
+        // four 26.0)
+        const int64_t most = C >= 512 ? 1024 : 2048;
+        const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+        layernorm_fwd<N, W, EXACT><<<grid, threads, 0, st>>>((int)R, (int)C, eps, x, g, b, y, mean, rstd);
     });
     return pk::launch_status("pk_layernorm_fwd_f32");
 }
@@ -479,12 +477,8 @@ extern "C" int pk_layernorm_bwd_f32(int64_t R, int64_t C, const float* x, const 
             constexpr int N = decltype(nv)::value, W = decltype(w)::value;
             constexpr bool EXACT = decltype(exact)::value;
             const size_t lds = kBwdWaves / W / 2 * 2 * (size_t)C * sizeof(float);
-            if(big(R, C))
-                layernorm_bwd<N, W, EXACT, true><<<(unsigned)P, 64 * kBwdWaves, lds, st>>>(
-                    (int)R, (int)C, x, g, mean, rstd, dy, dx_in, dx, ws, dg, db, what, flags);
-            else
-                layernorm_bwd<N, W, EXACT, false><<<(unsigned)P, 64 * kBwdWaves, lds, st>>>(
-                    (int)R, (int)C, x, g, mean, rstd, dy, dx_in, dx, ws, dg, db, what, flags);
+            layernorm_bwd<N, W, EXACT><<<(unsigned)P, 64 * kBwdWaves, lds, st>>>(
+                (int)R, (int)C, x, g, mean, rstd, dy, dx_in, dx, ws, dg, db, what, flags);
         });
         if(sums && P > 1)
             layernorm_sum<<<(unsigned)((2 * C + 63) / 64), 64 * kSumWaves, 0, st>>>(P, C, ws, dg, db, flags);
