@@ -677,7 +677,9 @@ int pk_gated_scan_bwd_f32(int64_t B, int64_t T, int64_t C, const float* f, int64
  *   [n, K], W_e at W + e*sw: [K, N] for tb 'N', [N, K] for 'T' (row stride ldw), Y
  *   [n, N].  Rows from offsets[E] to n become zero (accumulating: are left).
  * pk_gemm_experts_dw_f32: dW_e (+)= X_e^T.dY_e, [K, N] at dW + e*sw, an expert without
- *   rows getting zeros.  Needs pk_gemm_experts_dw_workspace(n, K, N, E) bytes.
+ *   rows getting zeros.  Where few tiles would leave the chip idle the rows are
+ *   split, in pk_gemm_experts_dw_workspace(n, K, N, E) bytes of device workspace (0: no
+ *   split; NULL or fewer bytes: unsplit); parts are added in a fixed order.
  *   precision: 0 fp32, 1 bf16, 2 three bf16 products, as in pk_gemm_add_f32 (no
  *   fp8).  PK_ACCUM accumulates.
  * Limits: E <= 1024, k <= 64, n < 2^31 (products: 2^30). */

@@ -1515,26 +1515,63 @@ int gemm_impl(char ta, char tb, int64_t M, int64_t N, int64_t K, float alpha, co
 
 namespace pkg {
 
-// An expert's last row tile is half empty on average; a tile holds rows of one
-// expert only.
-ExpertShape expert_shape(int prec, bool ta, double groups, double m, int64_t N, double k) {
+namespace {
+
+template <class F>
+void expert_shapes(int prec, F f) {
     const SplitShape* const shapes = prec == kFp32 ? kShapesF32 : prec == kBf16 ? kShapesBf16 : kShapesBf16x3;
-    const int n_shapes = prec == kFp32 ? (int)std::size(kShapesF32) : (int)std::size(kShapesBf16);
+    const int n = prec == kFp32 ? (int)std::size(kShapesF32) : (int)std::size(kShapesBf16);
+    for(int i = 0; i < n; ++i)
+        if(shapes[i].bn != 96 && !(prec == kFp32 && (shapes[i].kind == kTile64 || shapes[i].kind == kTile64x1)))
+            f(shapes[i]);
+}
+
+}  // namespace
+
+// A tile holds rows of one expert only, whose last one is half empty on average.
+ExpertShape expert_rows_shape(int prec, double groups, double m, int64_t N, double k) {
     ExpertShape best = {kTile128, 128, 128};
     double c = -1.0;
-    for(int i = 0; i < n_shapes; ++i) {
-        const SplitShape& t = shapes[i];
-        if(t.bn == 96 || (prec == kFp32 && (t.kind == kTile64 || t.kind == kTile64x1))) continue;
-        const double per = ta ? std::ceil(m / t.bm) : std::max(1.0, m / t.bm + 0.5);
-        const double n = groups * per * (double)((N + t.bn - 1) / t.bn);
-        const double rounds = 0.5 * (std::ceil(n / kCUs) + n / kCUs), kk = (ta ? t.ta : 1.0) * k;
-        const double own = std::max(t.one + t.edge + t.one_k * kk,
-                                    t.base + rounds * (t.round + t.edge + t.per_k * kk));
+    expert_shapes(prec, [&](const SplitShape& t) {
+        const double n = groups * std::max(1.0, m / t.bm + 0.5) * (double)((N + t.bn - 1) / t.bn);
+        const double rounds = 0.5 * (std::ceil(n / kCUs) + n / kCUs);
+        const double own = std::max(t.one + t.edge + t.one_k * k,
+                                    t.base + rounds * (t.round + t.edge + t.per_k * k));
         if(c < 0.0 || own < 0.97 * c) {
             c = own;
             best = {t.kind, t.bm, t.bn};
         }
-    }
+    });
+    return best;
+}
+
+// The estimates with an expert of 2.5 times the mean rows, whose workgroups start
+// first: 8 experts of [768, 4096], 16384 rows in all, the largest with 2048 / 3827
+// / 4273: 256x256 550 / 519 / 536 us, 128x128 576 / 586 / 572; [2048, 768], largest
+// 2048 / 5016 / 7698: 256x256 266 / 553 / 841, 128x128 (taken) 287 / 300 / 345.
+ExpertShape expert_dw_shape(int prec, int64_t groups, int64_t m, int64_t N, int64_t n, bool split,
+                            int* splits) {
+    const double mean = (double)n / groups, most = std::min((double)n, 2.5 * mean);
+    const double plane = (double)groups * (double)m * (double)N * 4.0 / 6.7e6;
+    ExpertShape best = {kTile128, 128, 128};
+    *splits = 1;
+    double c = -1.0;
+    expert_shapes(prec, [&](const SplitShape& t) {
+        const double tiles = (double)groups * ((m + t.bm - 1) / t.bm) * ((N + t.bn - 1) / t.bn);
+        for(const int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+            // (parts of at least 128 rows, planes of at most 64 MiB in all)
+            if(s > 1 && (!split || most < 128.0 * s || s * plane > 10.0)) break;
+            const double own = std::max(t.one + t.edge + t.one_k * t.ta * most / s,
+                                        t.base + std::max(1.0, tiles * s / kCUs) *
+                                                     (t.round + t.edge + t.per_k * t.ta * mean / s)) +
+                               (s > 1 ? 3.0 + 0.3 * s + (s + 1) * plane : 0.0);
+            if(c < 0.0 || own < 0.97 * c) {
+                c = own;
+                best = {t.kind, t.bm, t.bn};
+                *splits = s;
+            }
+        }
+    });
     return best;
 }
 

@@ -123,7 +123,8 @@ __device__ __forceinline__ TileJob tile_job(const GemmParams& p) {
 //   rows: Y = X.op(W_e) for every expert's rows.  A is X, B is W (sBo from one
 //         expert to the next), C is Y, M all rows.
 //   else: dW_e = X_e^T.dY_e (sCo from one expert to the next).  A is X, B is dY, K
-//         all rows.
+//         all rows.  With splits > 1 blockIdx.y is one of as many equal parts of each
+//         expert's rows, whose product goes to plane [blockIdx.y][e] of ws.
 struct ExpertParams : GemmParams {
     const int32_t* offsets;
     int experts;
@@ -206,18 +207,43 @@ __device__ __forceinline__ TileJob tile_job(ExpertParams& p) {
         p.C += lo * p.ldc;
         p.M = hi - lo;
     } else {
-        const int ntiles = p.tiles_m * p.tiles_n;
-        const int total = ntiles * p.experts, run = (total + 7) >> 3;
-        bid = (bid & 7) * run + (bid >> 3);
-        if((int)(blockIdx.x >> 3) >= run || bid >= total) return j;
-        e = bid / ntiles;
-        bid %= ntiles;
-        tm = bid % p.tiles_m;
-        tn = bid / p.tiles_m;
+        // An expert's tiles are dealt to the XCDs in runs, the experts one after another,
+        // the one with the most rows first (of up to 64, which one wave can put in
+        // order): the workgroups that start last have the shortest sums
+        const int ntiles = p.tiles_m * p.tiles_n, per = (ntiles + 7) >> 3, used = (ntiles + per - 1) / per;
+        const int q = (int)(blockIdx.x >> 3) / per;
+        const int tile = ((((int)blockIdx.x & 7) + q * used) & 7) * per + (int)(blockIdx.x >> 3) % per;
+        if(q >= p.experts || tile >= ntiles) return j;
+        e = q;
+        if(p.experts <= 64) {
+            int64_t mine = -1;
+            if(lane < p.experts) {
+                expert_range(p, lane, p.K, lo, hi);
+                mine = hi - lo;
+            }
+            const int size = (int)mine;
+            int rank = 0;
+            for(int o = 0; o < p.experts; ++o) {
+                const int other = __builtin_amdgcn_readlane(size, o);
+                rank += other > size || (other == size && o < lane);
+            }
+            e = (int)__builtin_ctzll(__ballot(lane < p.experts && rank == q));
+        }
+        tm = tile % p.tiles_m;
+        tn = tile / p.tiles_m;
         expert_range(p, e, p.K, lo, hi);
+        if(p.splits > 1) {
+            const int64_t len = ((hi - lo + p.splits - 1) / p.splits + 31) / 32 * 32;
+            lo = min(lo + (int64_t)blockIdx.y * len, hi);
+            hi = min(lo + len, hi);
+            p.C = p.ws + ((int64_t)blockIdx.y * p.experts + e) * p.M * p.N;
+            p.ldc = p.N;
+            p.beta = 0.0f;
+        } else {
+            p.C += e * p.sCo;
+        }
         p.A += lo * p.lda;
         p.B += lo * p.ldb;
-        p.C += e * p.sCo;
         p.K = hi - lo;
     }
     j.skip = false;
@@ -446,12 +472,15 @@ struct ExpertShape {
     TileKind kind;
     int bm, bn;
 };
-// the tile shape of a product of `groups` experts, [m, N] with k each on average
-// (gemm.hip's estimates)
-ExpertShape expert_shape(int prec, bool ta, double groups, double m, int64_t N, double k);
-int launch_split_experts(bool ta, bool tb, const ExpertParams& ep, unsigned grid, TileKind kind,
+// the tile shape of the products of `groups` experts with m rows of [N, k] each on
+// average, and that of their A^T.B products, [m, N] with k rows, which may split
+// them (gemm.hip's estimates)
+ExpertShape expert_rows_shape(int prec, double groups, double m, int64_t N, double k);
+ExpertShape expert_dw_shape(int prec, int64_t groups, int64_t m, int64_t N, int64_t n, bool split,
+                            int* splits);
+int launch_split_experts(bool ta, bool tb, const ExpertParams& ep, dim3 grid, TileKind kind,
                          hipStream_t st);
-int launch_narrow_experts(bool ta, bool tb, int parts, const ExpertParams& ep, unsigned grid,
+int launch_narrow_experts(bool ta, bool tb, int parts, const ExpertParams& ep, dim3 grid,
                           TileKind kind, hipStream_t st);
 
 // the bf16 (parts 1) and split-bf16 (parts 2) products (gemm_narrow.hip); with

@@ -21,8 +21,24 @@ int check(const char* who, int64_t n, int64_t M, int64_t N, int64_t E, const int
 
 int run(bool ta, bool tb, const ExpertParams& ep, int64_t grid, TileKind kind, int precision,
         hipStream_t st) {
-    if(precision == 0) return launch_split_experts(ta, tb, ep, (unsigned)grid, kind, st);
-    return launch_narrow_experts(ta, tb, precision, ep, (unsigned)grid, kind, st);
+    const dim3 g((unsigned)grid, (unsigned)ep.splits);
+    if(precision == 0) return launch_split_experts(ta, tb, ep, g, kind, st);
+    return launch_narrow_experts(ta, tb, precision, ep, g, kind, st);
+}
+
+// dW_e (+)= the sum of the S planes [S][E][K][N], in plane order
+__global__ __launch_bounds__(256) void experts_dw_sum(int64_t E, int64_t K, int64_t N, int S,
+                                                      const float* __restrict__ ws, float* dW,
+                                                      int64_t ldw, int64_t sw, int accum) {
+    const int64_t plane = E * K * N;
+    for(int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < plane; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / N, e = r / K;
+        float* const o = dW + e * sw + (r - e * K) * ldw + (i - r * N);
+        float sum = 0.0f;
+#pragma unroll 8
+        for(int s = 0; s < S; ++s) sum += ws[s * plane + i];
+        *o = accum ? *o + sum : sum;
+    }
 }
 
 }  // namespace
@@ -63,7 +79,7 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     ep.experts = (int)E;
     ep.rows = 1;
     const int64_t groups = E < n ? E : n;
-    const ExpertShape s = expert_shape(precision, false, (double)groups, (double)n / groups, N, (double)K);
+    const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K);
     // every expert with rows, and the rows behind the last one's, end in a partial tile
     const int64_t tiles_m = (n + s.bm - 1) / s.bm + groups + 1, tiles_n = (N + s.bn - 1) / s.bn;
     if(tiles_m * tiles_n > (int64_t)1 << 30)
@@ -74,11 +90,14 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
 }
 
 extern "C" size_t pk_gemm_experts_dw_workspace(int64_t n, int64_t K, int64_t N, int64_t E) {
-    (void)n;
-    (void)K;
-    (void)N;
-    (void)E;
-    return 0;
+    if(n <= 0 || K <= 0 || N <= 0 || E < 1 || E > kMaxExperts) return 0;
+    int most = 1;
+    for(int precision = 0; precision < 3; ++precision) {
+        int splits;
+        expert_dw_shape(precision, E, K, N, n, true, &splits);
+        if(splits > most) most = splits;
+    }
+    return most > 1 ? (size_t)most * (size_t)E * (size_t)K * (size_t)N * sizeof(float) : 0;
 }
 
 extern "C" int pk_gemm_experts_dw_f32(int64_t n, int64_t K, int64_t N, int64_t E,
@@ -112,11 +131,22 @@ extern "C" int pk_gemm_experts_dw_f32(int64_t n, int64_t K, int64_t N, int64_t E
     ep.kchunk = n;
     ep.offsets = offsets;
     ep.experts = (int)E;
-    const ExpertShape s = expert_shape(precision, true, (double)E, (double)K, N, (double)n / E);
+    int splits;
+    ExpertShape s = expert_dw_shape(precision, E, K, N, n, workspace != nullptr, &splits);
+    if(workspace_bytes < (size_t)splits * (size_t)E * (size_t)K * (size_t)N * sizeof(float))
+        s = expert_dw_shape(precision, E, K, N, n, false, &splits);
+    ep.splits = splits;
+    ep.ws = static_cast<float*>(workspace);
     const int64_t tiles_m = (K + s.bm - 1) / s.bm, tiles_n = (N + s.bn - 1) / s.bn;
     if(tiles_m > (int64_t)1 << 30 || tiles_n > (int64_t)1 << 30 || tiles_m * tiles_n * E > (int64_t)1 << 30)
         return pk::fail("pk_gemm_experts_dw_f32: problem too large for one launch");
     ep.tiles_m = (int)tiles_m;
     ep.tiles_n = (int)tiles_n;
-    return run(true, false, ep, (tiles_m * tiles_n * E + 7) / 8 * 8, s.kind, precision, pk::as_stream(stream));
+    // (an expert's tiles in 8 runs, one to an XCD)
+    hipStream_t st = pk::as_stream(stream);
+    if(int rc = run(true, false, ep, (tiles_m * tiles_n + 7) / 8 * 8 * E, s.kind, precision, st)) return rc;
+    if(splits == 1) return PK_OK;
+    experts_dw_sum<<<pk::grid_for(E * K * N, 256), 256, 0, st>>>(E, K, N, splits, ep.ws, dW, ldw, sw,
+                                                                flags & PK_ACCUM);
+    return pk::launch_status("pk_gemm_experts_dw_f32");
 }

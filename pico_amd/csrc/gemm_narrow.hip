@@ -256,7 +256,7 @@ int launch_parts(bool ta, bool tb, const GemmParams& gp, int64_t batch, bool edg
 }
 
 template <bool TA, bool TB, int P>
-void launch_experts(const ExpertParams& ep, unsigned grid, TileKind kind, hipStream_t st) {
+void launch_experts(const ExpertParams& ep, dim3 grid, TileKind kind, hipStream_t st) {
     auto run = [&](auto shape) {
         using T = decltype(shape);
         gemm_narrow_kernel<TA, TB, kPartial, T, P, kEpiPlain, ExpertParams>
@@ -270,7 +270,7 @@ void launch_experts(const ExpertParams& ep, unsigned grid, TileKind kind, hipStr
 }
 
 template <int P>
-void launch_experts_parts(bool ta, bool tb, const ExpertParams& ep, unsigned grid, TileKind kind,
+void launch_experts_parts(bool ta, bool tb, const ExpertParams& ep, dim3 grid, TileKind kind,
                           hipStream_t st) {
     if(ta) launch_experts<true, false, P>(ep, grid, kind, st);
     else if(tb) launch_experts<false, true, P>(ep, grid, kind, st);
@@ -281,7 +281,7 @@ void launch_experts_parts(bool ta, bool tb, const ExpertParams& ep, unsigned gri
 
 namespace pkg {
 
-int launch_narrow_experts(bool ta, bool tb, int parts, const ExpertParams& ep, unsigned grid,
+int launch_narrow_experts(bool ta, bool tb, int parts, const ExpertParams& ep, dim3 grid,
                           TileKind kind, hipStream_t st) {
     if(parts == 1) launch_experts_parts<1>(ta, tb, ep, grid, kind, st);
     else launch_experts_parts<2>(ta, tb, ep, grid, kind, st);

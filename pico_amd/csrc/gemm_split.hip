@@ -67,7 +67,7 @@ int launch_layout(const GemmParams& gp, int64_t batch, bool edge, TileKind kind,
 }
 
 template <bool TA, bool TB>
-void launch_experts(const ExpertParams& ep, unsigned grid, TileKind kind, hipStream_t st) {
+void launch_experts(const ExpertParams& ep, dim3 grid, TileKind kind, hipStream_t st) {
     auto run = [&](auto shape) {
         using T = decltype(shape);
         gemm_split_kernel<TA, TB, kPartial, T, kEpiPlain, ExpertParams><<<grid, T::THREADS, 0, st>>>(ep);
@@ -84,7 +84,7 @@ void launch_experts(const ExpertParams& ep, unsigned grid, TileKind kind, hipStr
 
 namespace pkg {
 
-int launch_split_experts(bool ta, bool tb, const ExpertParams& ep, unsigned grid, TileKind kind,
+int launch_split_experts(bool ta, bool tb, const ExpertParams& ep, dim3 grid, TileKind kind,
                          hipStream_t st) {
     if(ta) launch_experts<true, false>(ep, grid, kind, st);
     else if(tb) launch_experts<false, true>(ep, grid, kind, st);

@@ -24,7 +24,7 @@ static int rows_of(const struct PicoTensor* t, int64_t rows) {
 
 /* ------------------------------------------------------------- the router
  * gates [R, k] = softmax over the k largest of the E logits */
-enum { RS_ROUTE = 0 };
+enum { RS_ROUTE = 0, ES_WS = 1 };
 
 static void route_backward(struct PicoTensor* self) {
     const struct PicoRoute* r = (const struct PicoRoute*)pkh_node(self)->saved[RS_ROUTE];
@@ -140,11 +140,9 @@ static void expert_matmul_backward(struct PicoTensor* self) {
                                  x->strides[0], pkh_grad_flag(x), prec, pkh_stream());
     if(pkh_status("pico_expert_matmul_backward", st)) return;
     pkh_grad_mark(x);
-    const size_t ws_bytes = pk_gemm_experts_dw_workspace(rows, K, N, r->E);
-    void* ws = ws_bytes ? pkh_workspace(ws_bytes) : NULL;
-    if(!ws && ws_bytes) return;
     st = pk_gemm_experts_dw_f32(rows, K, N, r->E, r->offsets, x->data, x->strides[0], g, N, w->grad,
-                                N, K * N, pkh_grad_flag(w), prec, ws, ws_bytes, pkh_stream());
+                                N, K * N, pkh_grad_flag(w), prec, n->saved[ES_WS],
+                                pk_gemm_experts_dw_workspace(rows, K, N, r->E), pkh_stream());
     if(pkh_status("pico_expert_matmul_backward", st)) return;
     pkh_grad_mark(w);
 }
@@ -176,6 +174,9 @@ struct PicoTensor* pico_expert_matmul(struct PicoTensor* x, struct PicoTensor* w
                                  N, K * N, out->data, N, 0, (int)n->ival[EI_PREC], pkh_stream());
     if(pkh_status("pico_expert_matmul", st)) return NULL;
     n->saved[RS_ROUTE] = (void*)r;
+    /* (of the node's own, so captured graphs share none; small where rows split) */
+    const size_t ws_bytes = pk_gemm_experts_dw_workspace(rows, K, N, r->E);
+    if(ws_bytes && !(n->saved[ES_WS] = arena_alloc_device(arena, ws_bytes))) return NULL;
     struct PicoTensor* ps[2] = {x, w};
     pkh_set_parents(arena, out, 2, ps, expert_matmul_backward);
     return out;
