@@ -1530,7 +1530,7 @@ void expert_shapes(int prec, F f) {
 
 // A tile holds rows of one expert only, whose last one is half empty on average.
 ExpertShape expert_rows_shape(int prec, double groups, double m, int64_t N, double k) {
-    ExpertShape best = {kTile128, 128, 128};
+    ExpertShape best = {kTile128, 128, 128, 0.0};
     double c = -1.0;
     expert_shapes(prec, [&](const SplitShape& t) {
         const double n = groups * std::max(1.0, m / t.bm + 0.5) * (double)((N + t.bn - 1) / t.bn);
@@ -1539,7 +1539,7 @@ ExpertShape expert_rows_shape(int prec, double groups, double m, int64_t N, doub
                                     t.base + rounds * (t.round + t.edge + t.per_k * k));
         if(c < 0.0 || own < 0.97 * c) {
             c = own;
-            best = {t.kind, t.bm, t.bn};
+            best = {t.kind, t.bm, t.bn, own};
         }
     });
     return best;
@@ -1553,7 +1553,7 @@ ExpertShape expert_dw_shape(int prec, int64_t groups, int64_t m, int64_t N, int6
                             int* splits) {
     const double mean = (double)n / groups, most = std::min((double)n, 2.5 * mean);
     const double plane = (double)groups * (double)m * (double)N * 4.0 / 6.7e6;
-    ExpertShape best = {kTile128, 128, 128};
+    ExpertShape best = {kTile128, 128, 128, 0.0};
     *splits = 1;
     double c = -1.0;
     expert_shapes(prec, [&](const SplitShape& t) {
@@ -1567,7 +1567,7 @@ ExpertShape expert_dw_shape(int prec, int64_t groups, int64_t m, int64_t N, int6
                                (s > 1 ? 3.0 + 0.3 * s + (s + 1) * plane : 0.0);
             if(c < 0.0 || own < 0.97 * c) {
                 c = own;
-                best = {t.kind, t.bm, t.bn};
+                best = {t.kind, t.bm, t.bn, own};
                 *splits = s;
             }
         }

@@ -471,6 +471,7 @@ int launch_split(bool ta, bool tb, const GemmParams& gp, int64_t batch, bool edg
 struct ExpertShape {
     TileKind kind;
     int bm, bn;
+    double us;  // estimated
 };
 // the tile shape of the products of `groups` experts with m rows of [N, k] each on
 // average, and that of their A^T.B products, [m, N] with k rows, which may split

@@ -1,6 +1,8 @@
 // pico_amd/csrc/gemm_experts.hip -- matrix products grouped by expert: the launches
 // of the fp32 (gemm_split.h), bf16 and split-bf16 (gemm_narrow.hip) tiles over
 // groups of rows whose sizes only the device knows.
+#include <algorithm>
+
 #include "gemm_common.h"
 
 namespace {
@@ -24,6 +26,124 @@ int run(bool ta, bool tb, const ExpertParams& ep, int64_t grid, TileKind kind, i
     const dim3 g((unsigned)grid, (unsigned)ep.splits);
     if(precision == 0) return launch_split_experts(ta, tb, ep, g, kind, st);
     return launch_narrow_experts(ta, tb, precision, ep, g, kind, st);
+}
+
+// ------------------------------------------------ a few rows to an expert
+// Y = X.W_e where every expert's weights are read for a handful of rows (tokens being
+// generated): bound by W's bytes.  A workgroup takes 4 rows of an expert and 64
+// columns; its lanes lie 16 along the columns, the others along k, 4 k at a time, so W
+// is read in runs of 256 bytes with two steps in flight, and each value is used 4
+// times in fp32 multiply-adds, which take less time than its bytes.  (bf16: operands
+// rounded first, products exact.)  The partial sums meet across the lanes, then the
+// waves, in a fixed order.
+constexpr int kThinWaves = 8, kThinRows = 4;
+
+struct ThinTile {
+    static constexpr int BM = kThinRows, BN = 64;
+};
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+template <bool BF16>
+__device__ __forceinline__ f32x4 rounded(f32x4 x) {
+    if constexpr(BF16) {
+        const bf16x4 b = __builtin_convertvector(x, bf16x4);
+        return __builtin_convertvector(b, f32x4);
+    }
+    return x;
+}
+
+template <bool BF16>
+__global__ __launch_bounds__(64 * kThinWaves) void experts_thin(ExpertParams p) {
+    using T = ThinTile;
+    constexpr int RM = kThinRows, CL = 16, KL = 64 / CL, STEP = 4 * KL * kThinWaves;  // k of a workgroup's step
+    __shared__ float part[kThinWaves][RM][4 * CL];
+    const TileJob j = tile_job<T>(p);
+    if(j.skip) return;
+    const int w = threadIdx.x / 64, lane = threadIdx.x % 64, cl = lane % CL;
+    const int rows = (int)min(p.M - j.row0, (int64_t)RM);
+    const int64_t col = j.col0 + 4 * cl, at = min(col, p.N - 4);
+    const float* const wp = j.B + at;
+    const float* xp[RM];
+#pragma unroll
+    for(int r = 0; r < RM; ++r) xp[r] = j.A + (j.row0 + min(r, rows - 1)) * p.lda;
+    f32x4 acc[RM];
+#pragma unroll
+    for(int r = 0; r < RM; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 wv[4], xv[RM];
+    auto load = [&](int64_t k) {
+#pragma unroll
+        for(int i = 0; i < 4; ++i) wv[i] = *reinterpret_cast<const f32x4u*>(wp + (k + i) * p.ldb);
+#pragma unroll
+        for(int r = 0; r < RM; ++r) xv[r] = *reinterpret_cast<const f32x4u*>(xp[r] + k);
+    };
+    auto add = [&](const f32x4 (&a)[4], const f32x4 (&x)[RM]) {
+#pragma unroll
+        for(int i = 0; i < 4; ++i) {
+            const f32x4 b = rounded<BF16>(a[i]);
+#pragma unroll
+            for(int r = 0; r < RM; ++r)
+#pragma unroll
+                for(int c = 0; c < 4; ++c) acc[r][c] = fmaf(x[r][i], b[c], acc[r][c]);
+        }
+    };
+    int64_t k = 4 * (w * KL + lane / CL);
+    if(k + 4 <= p.K) load(k);
+    for(; k + 4 <= p.K; k += STEP) {
+        f32x4 a[4], x[RM];
+#pragma unroll
+        for(int i = 0; i < 4; ++i) a[i] = wv[i];
+#pragma unroll
+        for(int r = 0; r < RM; ++r) x[r] = rounded<BF16>(xv[r]);
+        if(k + STEP + 4 <= p.K) load(k + STEP);
+        add(a, x);
+    }
+    if(k < p.K) {
+        // the last one to three k
+        f32x4 a[4], x[RM];
+#pragma unroll
+        for(int i = 0; i < 4; ++i) {
+            const bool on = k + i < p.K;
+            a[i] = on ? *reinterpret_cast<const f32x4u*>(wp + (k + i) * p.ldb) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for(int r = 0; r < RM; ++r) x[r][i] = on ? xp[r][k + i] : 0.0f;
+        }
+#pragma unroll
+        for(int r = 0; r < RM; ++r) x[r] = rounded<BF16>(x[r]);
+        add(a, x);
+    }
+#pragma unroll
+    for(int o = CL; o < 64; o <<= 1)
+#pragma unroll
+        for(int r = 0; r < RM; ++r)
+#pragma unroll
+            for(int c = 0; c < 4; ++c) acc[r][c] += __shfl_xor(acc[r][c], o, 64);
+    if(lane < CL) {
+#pragma unroll
+        for(int r = 0; r < RM; ++r) *reinterpret_cast<f32x4*>(&part[w][r][4 * cl]) = acc[r];
+    }
+    __syncthreads();
+    for(int i = threadIdx.x; i < rows * 4 * CL; i += 64 * kThinWaves) {
+        const int r = i / (4 * CL), c = i % (4 * CL);
+        float sum = part[0][r][c];
+#pragma unroll
+        for(int q = 1; q < kThinWaves; ++q) sum += part[q][r][c];
+        // (a lane past N - 4 holds the row's last four)
+        const int64_t n = j.col0 + c / 4 * 4, shift = max(n - (p.N - 4), (int64_t)0);
+        if(c % 4 < shift) continue;
+        float* const y = j.C + (j.row0 + r) * p.ldc + n - shift + c % 4;
+        *y = j.beta != 0.0f ? *y + sum : sum;
+    }
+}
+
+// Microseconds: W once from memory, or once for every row tile from the caches, and a
+// start.  8 experts, rows each 1 / 4 / 8 / 16, us against those of matrix-core tiles:
+// [768, 4096] 15 / 22 / 28 / 40 against 27 / 29 / 28 / 28, [2048, 768] - / 13 / 14 / 22
+// against 37 (96 tiles, each all of K).  Workgroups of 8 or 16 rows read W less often
+// but are fewer and hold more: [768, 4096] with 4 rows each 24 and 31.
+double thin_us(double groups, double m, int64_t N, int64_t K) {
+    const double mb = (double)K * (double)N * 4e-6, tiles = groups * std::max(1.0, m / kThinRows + 0.5);
+    return 4.0 + mb * std::max(groups / 6.5, tiles / 11.0);
 }
 
 // dW_e (+)= the sum of the S planes [S][E][K][N], in plane order
@@ -80,6 +200,20 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     ep.rows = 1;
     const int64_t groups = E < n ? E : n;
     const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K);
+    // (the estimates are of up to 32 rows to an expert)
+    if(!TB && N >= 4 && K > 0 && n <= 32 * groups &&
+       thin_us((double)groups, (double)n / groups, N, K) < s.us) {
+        const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 63) / 64;
+        if(tiles_m * tiles_n > (int64_t)1 << 30)
+            return pk::fail("pk_gemm_experts_f32: problem too large for one launch");
+        ep.tiles_m = (int)tiles_m;
+        ep.tiles_n = (int)tiles_n;
+        const unsigned grid = (unsigned)((tiles_m * tiles_n + 7) / 8 * 8);
+        hipStream_t st = pk::as_stream(stream);
+        if(precision == 1) experts_thin<true><<<grid, 64 * kThinWaves, 0, st>>>(ep);
+        else experts_thin<false><<<grid, 64 * kThinWaves, 0, st>>>(ep);
+        return pk::launch_status("pk_gemm_experts_f32");
+    }
     // every expert with rows, and the rows behind the last one's, end in a partial tile
     const int64_t tiles_m = (n + s.bm - 1) / s.bm + groups + 1, tiles_n = (N + s.bn - 1) / s.bn;
     if(tiles_m * tiles_n > (int64_t)1 << 30)

@@ -128,6 +128,21 @@ struct PicoTensor* pico_expert_gather(struct PicoTensor* x, const struct PicoRou
  * the backward uses the precision the forward ran in */
 enum { EI_PREC = 0 };
 
+static int expert_dw(struct PicoTensor* self, const float* g, int flags, pk_stream_t stream) {
+    const struct PkNode* n = pkh_node(self);
+    const struct PicoRoute* r = (const struct PicoRoute*)n->saved[RS_ROUTE];
+    const struct PicoTensor *x = self->parents[0], *w = self->parents[1];
+    const int64_t rows = x->shape[0], K = w->shape[1], N = w->shape[2];
+    return pkh_status("pico_expert_matmul_backward",
+                      pk_gemm_experts_dw_f32(rows, K, N, r->E, r->offsets, x->data, x->strides[0], g,
+                                             N, w->grad, N, K * N, flags, (int)n->ival[EI_PREC],
+                                             n->saved[ES_WS],
+                                             pk_gemm_experts_dw_workspace(rows, K, N, r->E), stream));
+}
+
+/* dW of a parameter goes to the side stream, beside dX and what follows it, in the
+ * order matmul_backward_body (ops.c) explains: eagerly before dX is issued, under
+ * graph capture after it, waiting for the point before it */
 static void expert_matmul_backward(struct PicoTensor* self) {
     struct PkNode* n = pkh_node(self);
     const struct PicoRoute* r = (const struct PicoRoute*)n->saved[RS_ROUTE];
@@ -135,15 +150,31 @@ static void expert_matmul_backward(struct PicoTensor* self) {
     const float* g = pkh_upstream(self);
     if(!g) return;
     const int64_t rows = x->shape[0], K = w->shape[1], N = w->shape[2];
-    const int prec = (int)n->ival[EI_PREC];
+    struct PkNode* nw = pkh_node(w);
+    const int to_side = nw && w->is_persistent && !x->is_persistent;
+    pk_stream_t side = to_side && !pkh_capturing() ? pkh_side_fork() : NULL;
+    const int done = side != NULL;
+    if(side) {
+        if(expert_dw(self, g, nw->grad_live ? PK_ACCUM : 0, side)) return;
+        nw->side_seq = pkh_side_seq();
+        pkh_grad_mark(w);
+    } else if(to_side) {
+        pkh_side_prepare();
+    }
     int st = pk_gemm_experts_f32('T', rows, K, N, r->E, r->offsets, g, N, w->data, N, K * N, x->grad,
-                                 x->strides[0], pkh_grad_flag(x), prec, pkh_stream());
+                                 x->strides[0], pkh_grad_flag(x), (int)n->ival[EI_PREC],
+                                 pkh_stream());
     if(pkh_status("pico_expert_matmul_backward", st)) return;
     pkh_grad_mark(x);
-    st = pk_gemm_experts_dw_f32(rows, K, N, r->E, r->offsets, x->data, x->strides[0], g, N, w->grad,
-                                N, K * N, pkh_grad_flag(w), prec, n->saved[ES_WS],
-                                pk_gemm_experts_dw_workspace(rows, K, N, r->E), pkh_stream());
-    if(pkh_status("pico_expert_matmul_backward", st)) return;
+    if(done) return;
+    side = to_side ? pkh_side_fork() : NULL;
+    if(side) {
+        st = expert_dw(self, g, nw->grad_live ? PK_ACCUM : 0, side);
+        nw->side_seq = pkh_side_seq();
+    } else {
+        st = expert_dw(self, g, pkh_grad_flag(w), pkh_stream());
+    }
+    if(st) return;
     pkh_grad_mark(w);
 }
 
