@@ -1528,18 +1528,41 @@ void expert_shapes(int prec, F f) {
 
 }  // namespace
 
-// A tile holds rows of one expert only, whose last one is half empty on average.
-ExpertShape expert_rows_shape(int prec, double groups, double m, int64_t N, double k) {
+// A tile holds rows of one expert only, whose last one is half empty on average.  Where
+// the experts have many rows those last tiles often make a round of their own (1088
+// tiles on 256 CUs take 5 rounds, the 1024 of as many rows in one 4): then 256x256 tiles
+// take the whole 256 rows, without bounds where N and k allow, and a second launch of
+// smaller tiles the rest.  16384 rows of 8 experts, us: see expert_rows in
+// gemm_experts.hip.
+ExpertShape expert_rows_shape(int prec, double groups, double m, int64_t N, double k, ExpertShape* rest) {
     ExpertShape best = {kTile128, 128, 128, 0.0};
     double c = -1.0;
-    expert_shapes(prec, [&](const SplitShape& t) {
-        const double n = groups * std::max(1.0, m / t.bm + 0.5) * (double)((N + t.bn - 1) / t.bn);
+    auto time = [&](const SplitShape& t, double row_tiles, double edge) {
+        const double n = row_tiles * (double)((N + t.bn - 1) / t.bn);
         const double rounds = 0.5 * (std::ceil(n / kCUs) + n / kCUs);
-        const double own = std::max(t.one + t.edge + t.one_k * k,
-                                    t.base + rounds * (t.round + t.edge + t.per_k * k));
+        return std::max(t.one + edge + t.one_k * k, t.base + rounds * (t.round + edge + t.per_k * k));
+    };
+    expert_shapes(prec, [&](const SplitShape& t) {
+        const double own = time(t, groups * std::max(1.0, m / t.bm + 0.5), t.edge);
         if(c < 0.0 || own < 0.97 * c) {
             c = own;
             best = {t.kind, t.bm, t.bn, own};
+        }
+    });
+    *rest = {kTile128, 0, 0, 0.0};
+    if(m < 512.0) return best;
+    const bool full = N % 256 == 0 && (int64_t)k % 32 == 0 && prec != kBf16x3;
+    double large = 0.0;
+    expert_shapes(prec, [&](const SplitShape& t) {
+        if(t.kind == kTile256) large = time(t, std::floor(groups * (m / 256.0 - 0.5)), full ? 0.0 : t.edge);
+    });
+    expert_shapes(prec, [&](const SplitShape& t) {
+        if(t.kind == kTile256) return;
+        const double own = large + 3.0 + time(t, groups * (128.0 / t.bm + 0.5), t.edge);
+        if(own < 0.97 * c) {
+            c = own;
+            best = {kTile256, 256, 256, own};
+            *rest = {t.kind, t.bm, t.bn, own};
         }
     });
     return best;

@@ -121,15 +121,17 @@ __device__ __forceinline__ TileJob tile_job(const GemmParams& p) {
 // A product grouped by expert: the rows [offsets[e], offsets[e + 1]) of X belong to
 // expert e, and the numbers are known on the device only.
 //   rows: Y = X.op(W_e) for every expert's rows.  A is X, B is W (sBo from one
-//         expert to the next), C is Y, M all rows.
+//         expert to the next), C is Y, M all rows.  whole and rest: of every expert
+//         only the rows in whole tiles of 256, or those after them.
 //   else: dW_e = X_e^T.dY_e (sCo from one expert to the next).  A is X, B is dY, K
 //         all rows.  With splits > 1 blockIdx.y is one of as many equal parts of each
 //         expert's rows, whose product goes to plane [blockIdx.y][e] of ws.
 struct ExpertParams : GemmParams {
     const int32_t* offsets;
     int experts;
-    int rows;
+    int rows;  // kDw, kRows, kRowsWhole or kRowsRest
 };
+constexpr int kDw = 0, kRows = 1, kRowsWhole = 2, kRowsRest = 3;
 
 // Offsets are held to [0, n] and to increase, so that whatever they say no access
 // leaves the matrices.
@@ -137,13 +139,21 @@ __device__ __forceinline__ void expert_range(const ExpertParams& p, int e, int64
                                              int64_t& hi) {
     lo = min(max((int64_t)p.offsets[e], (int64_t)0), n);
     hi = e < p.experts ? min(max((int64_t)p.offsets[e + 1], lo), n) : n;
+    if(p.rows >= kRowsWhole) {
+        const int64_t cut = e < p.experts ? lo + (hi - lo) / 256 * 256 : lo;
+        if(p.rows == kRowsWhole) hi = cut;
+        else lo = cut;
+    }
 }
 
+// The rows past the last expert's are a group of their own of at most kZeroTiles row
+// tiles, which fill them with zeros (or, accumulating, leave them).
+constexpr int kZeroTiles = 32;
+
 // The tile of workgroup blockIdx.x.  Its expert's matrices replace the whole ones in
-// p.  Of `rows` products the grid is the most row tiles that n rows and E experts
+// p.  Of products of rows the grid is the most row tiles that n rows and E experts
 // can need (tiles_m; 65 of it fit 32 bits); every wave adds up how many there are
-// and which expert has its own, 64 experts at a time.  The rows past the last expert's are a group of their own
-// that multiplies nothing, and so is filled with zeros (or, accumulating, left).
+// and which expert has its own, 64 experts at a time.
 template <class T>
 __device__ __forceinline__ TileJob tile_job(ExpertParams& p) {
     TileJob j;
@@ -154,9 +164,9 @@ __device__ __forceinline__ TileJob tile_job(ExpertParams& p) {
     if(p.rows) {
         const int64_t n = p.M;
         auto tiles = [&](int q) {
-            if(q > p.experts) return 0;
+            if(q > p.experts || (q == p.experts && p.beta != 0.0f)) return 0;
             expert_range(p, q, n, lo, hi);
-            return min((int)((hi - lo + T::BM - 1) / T::BM), p.tiles_m);
+            return min((int)((hi - lo + T::BM - 1) / T::BM), q < p.experts ? p.tiles_m : kZeroTiles);
         };
         int all = 0;
         for(int q = 0; q <= p.experts; q += 64) {
@@ -198,11 +208,13 @@ __device__ __forceinline__ TileJob tile_job(ExpertParams& p) {
         tm = __builtin_amdgcn_readfirstlane(tm);
         expert_range(p, e, n, lo, hi);
         if(e == p.experts) {
-            if(p.beta != 0.0f) return j;
-            p.K = 0;
-        } else {
-            p.B += e * p.sBo;
+            const int64_t c = (int64_t)tn * T::BN, width = min(p.N - c, (int64_t)T::BN);
+            const int step = min((int)((hi - lo + T::BM - 1) / T::BM), kZeroTiles);
+            for(int64_t r = lo + tm; r < hi; r += step)
+                for(int64_t i = threadIdx.x; i < width; i += blockDim.x) p.C[r * p.ldc + c + i] = 0.0f;
+            return j;
         }
+        p.B += e * p.sBo;
         p.A += lo * p.lda;
         p.C += lo * p.ldc;
         p.M = hi - lo;
@@ -466,23 +478,25 @@ int split_groups(TileKind kind);
 int launch_split(bool ta, bool tb, const GemmParams& gp, int64_t batch, bool edge, TileKind kind,
                  hipStream_t st);
 
-// products grouped by expert (A.B, A.B^T or A^T.B): kTile256, kTile128, kTile128x64
-// and kTile64 (fp32) or kTile64x2, the last one and the first two for bf16
+// products grouped by expert (A.B, A.B^T or A^T.B): kTile256, kTile128, kTile128x64 and
+// kTile64x2 (fp32), kTile256, kTile128 and kTile64 (bf16).  full: tiles that need no
+// bounds (of rows, kTile256 only)
 struct ExpertShape {
     TileKind kind;
     int bm, bn;
     double us;  // estimated
 };
 // the tile shape of the products of `groups` experts with m rows of [N, k] each on
-// average, and that of their A^T.B products, [m, N] with k rows, which may split
-// them (gemm.hip's estimates)
-ExpertShape expert_rows_shape(int prec, double groups, double m, int64_t N, double k);
+// average, or, where `rest` gets a shape, 256x256 tiles of the whole 256 rows of each
+// and that one for the rest; and the shape of their A^T.B products, [m, N] with n
+// rows in all, which may split them (gemm.hip's estimates)
+ExpertShape expert_rows_shape(int prec, double groups, double m, int64_t N, double k, ExpertShape* rest);
 ExpertShape expert_dw_shape(int prec, int64_t groups, int64_t m, int64_t N, int64_t n, bool split,
                             int* splits);
 int launch_split_experts(bool ta, bool tb, const ExpertParams& ep, dim3 grid, TileKind kind,
-                         hipStream_t st);
+                         bool full, hipStream_t st);
 int launch_narrow_experts(bool ta, bool tb, int parts, const ExpertParams& ep, dim3 grid,
-                          TileKind kind, hipStream_t st);
+                          TileKind kind, bool full, hipStream_t st);
 
 // the bf16 (parts 1) and split-bf16 (parts 2) products (gemm_narrow.hip); with
 // gp.far, 64x64 tiles only

@@ -21,11 +21,11 @@ int check(const char* who, int64_t n, int64_t M, int64_t N, int64_t E, const int
     return PK_OK;
 }
 
-int run(bool ta, bool tb, const ExpertParams& ep, int64_t grid, TileKind kind, int precision,
-        hipStream_t st) {
+int run(bool ta, bool tb, const ExpertParams& ep, int64_t grid, TileKind kind, bool full,
+        int precision, hipStream_t st) {
     const dim3 g((unsigned)grid, (unsigned)ep.splits);
-    if(precision == 0) return launch_split_experts(ta, tb, ep, g, kind, st);
-    return launch_narrow_experts(ta, tb, precision, ep, g, kind, st);
+    if(precision == 0) return launch_split_experts(ta, tb, ep, g, kind, full, st);
+    return launch_narrow_experts(ta, tb, precision, ep, g, kind, full, st);
 }
 
 // ------------------------------------------------ a few rows to an expert
@@ -197,9 +197,10 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     ep.kchunk = K;
     ep.offsets = offsets;
     ep.experts = (int)E;
-    ep.rows = 1;
+    ep.rows = kRows;
     const int64_t groups = E < n ? E : n;
-    const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K);
+    ExpertShape rest;
+    const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K, &rest);
     // (the estimates are of up to 32 rows to an expert)
     if(!TB && N >= 4 && K > 0 && n <= 32 * groups &&
        thin_us((double)groups, (double)n / groups, N, K) < s.us) {
@@ -214,13 +215,21 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
         else experts_thin<false><<<grid, 64 * kThinWaves, 0, st>>>(ep);
         return pk::launch_status("pk_gemm_experts_f32");
     }
+    // `most` row tiles at most
+    auto tiles = [&](const ExpertShape& t, int64_t most, int which, bool full) {
+        const int64_t tiles_n = (N + t.bn - 1) / t.bn;
+        if(most * tiles_n > (int64_t)1 << 30)
+            return pk::fail("pk_gemm_experts_f32: problem too large for one launch");
+        ep.rows = which;
+        ep.tiles_m = (int)most;
+        ep.tiles_n = (int)tiles_n;
+        return run(false, TB, ep, (most * tiles_n + 7) / 8 * 8, t.kind, full, precision, pk::as_stream(stream));
+    };
     // every expert with rows, and the rows behind the last one's, end in a partial tile
-    const int64_t tiles_m = (n + s.bm - 1) / s.bm + groups + 1, tiles_n = (N + s.bn - 1) / s.bn;
-    if(tiles_m * tiles_n > (int64_t)1 << 30)
-        return pk::fail("pk_gemm_experts_f32: problem too large for one launch");
-    ep.tiles_m = (int)tiles_m;
-    ep.tiles_n = (int)tiles_n;
-    return run(false, TB, ep, (tiles_m * tiles_n + 7) / 8 * 8, s.kind, precision, pk::as_stream(stream));
+    if(!rest.bm) return tiles(s, (n + s.bm - 1) / s.bm + groups + 1, kRows, false);
+    if(int st = tiles(s, n / s.bm, kRowsWhole, N % s.bn == 0 && K % 32 == 0)) return st;
+    // up to 255 rows of every expert
+    return tiles(rest, groups * ((254 + rest.bm) / rest.bm) + kZeroTiles, kRowsRest, false);
 }
 
 extern "C" size_t pk_gemm_experts_dw_workspace(int64_t n, int64_t K, int64_t N, int64_t E) {
@@ -278,7 +287,7 @@ extern "C" int pk_gemm_experts_dw_f32(int64_t n, int64_t K, int64_t N, int64_t E
     ep.tiles_n = (int)tiles_n;
     // (an expert's tiles in 8 runs, one to an XCD)
     hipStream_t st = pk::as_stream(stream);
-    if(int rc = run(true, false, ep, (tiles_m * tiles_n + 7) / 8 * 8 * E, s.kind, precision, st)) return rc;
+    if(int rc = run(true, false, ep, (tiles_m * tiles_n + 7) / 8 * 8 * E, s.kind, false, precision, st)) return rc;
     if(splits == 1) return PK_OK;
     experts_dw_sum<<<pk::grid_for(E * K * N, 256), 256, 0, st>>>(E, K, N, splits, ep.ws, dW, ldw, sw,
                                                                 flags & PK_ACCUM);

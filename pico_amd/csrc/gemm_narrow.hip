@@ -256,7 +256,14 @@ int launch_parts(bool ta, bool tb, const GemmParams& gp, int64_t batch, bool edg
 }
 
 template <bool TA, bool TB, int P>
-void launch_experts(const ExpertParams& ep, dim3 grid, TileKind kind, hipStream_t st) {
+void launch_experts(const ExpertParams& ep, dim3 grid, TileKind kind, bool full, hipStream_t st) {
+    if constexpr(!TA && P == 1) {
+        if(full && kind == kTile256) {
+            gemm_narrow_kernel<TA, TB, kWhole, Narrow256, P, kEpiPlain, ExpertParams>
+                <<<grid, Narrow256::THREADS, 0, st>>>(ep);
+            return;
+        }
+    }
     auto run = [&](auto shape) {
         using T = decltype(shape);
         gemm_narrow_kernel<TA, TB, kPartial, T, P, kEpiPlain, ExpertParams>
@@ -271,10 +278,10 @@ void launch_experts(const ExpertParams& ep, dim3 grid, TileKind kind, hipStream_
 
 template <int P>
 void launch_experts_parts(bool ta, bool tb, const ExpertParams& ep, dim3 grid, TileKind kind,
-                          hipStream_t st) {
-    if(ta) launch_experts<true, false, P>(ep, grid, kind, st);
-    else if(tb) launch_experts<false, true, P>(ep, grid, kind, st);
-    else launch_experts<false, false, P>(ep, grid, kind, st);
+                          bool full, hipStream_t st) {
+    if(ta) launch_experts<true, false, P>(ep, grid, kind, full, st);
+    else if(tb) launch_experts<false, true, P>(ep, grid, kind, full, st);
+    else launch_experts<false, false, P>(ep, grid, kind, full, st);
 }
 
 }  // namespace
@@ -282,9 +289,9 @@ void launch_experts_parts(bool ta, bool tb, const ExpertParams& ep, dim3 grid, T
 namespace pkg {
 
 int launch_narrow_experts(bool ta, bool tb, int parts, const ExpertParams& ep, dim3 grid,
-                          TileKind kind, hipStream_t st) {
-    if(parts == 1) launch_experts_parts<1>(ta, tb, ep, grid, kind, st);
-    else launch_experts_parts<2>(ta, tb, ep, grid, kind, st);
+                          TileKind kind, bool full, hipStream_t st) {
+    if(parts == 1) launch_experts_parts<1>(ta, tb, ep, grid, kind, full, st);
+    else launch_experts_parts<2>(ta, tb, ep, grid, kind, full, st);
     return pk::launch_status("pk_gemm_experts_f32");
 }
 

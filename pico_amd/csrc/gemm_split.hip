@@ -67,7 +67,14 @@ int launch_layout(const GemmParams& gp, int64_t batch, bool edge, TileKind kind,
 }
 
 template <bool TA, bool TB>
-void launch_experts(const ExpertParams& ep, dim3 grid, TileKind kind, hipStream_t st) {
+void launch_experts(const ExpertParams& ep, dim3 grid, TileKind kind, bool full, hipStream_t st) {
+    if constexpr(!TA) {
+        if(full && kind == kTile256) {
+            gemm_split_kernel<TA, TB, kWhole, Split256, kEpiPlain, ExpertParams>
+                <<<grid, Split256::THREADS, 0, st>>>(ep);
+            return;
+        }
+    }
     auto run = [&](auto shape) {
         using T = decltype(shape);
         gemm_split_kernel<TA, TB, kPartial, T, kEpiPlain, ExpertParams><<<grid, T::THREADS, 0, st>>>(ep);
@@ -85,10 +92,10 @@ void launch_experts(const ExpertParams& ep, dim3 grid, TileKind kind, hipStream_
 namespace pkg {
 
 int launch_split_experts(bool ta, bool tb, const ExpertParams& ep, dim3 grid, TileKind kind,
-                         hipStream_t st) {
-    if(ta) launch_experts<true, false>(ep, grid, kind, st);
-    else if(tb) launch_experts<false, true>(ep, grid, kind, st);
-    else launch_experts<false, false>(ep, grid, kind, st);
+                         bool full, hipStream_t st) {
+    if(ta) launch_experts<true, false>(ep, grid, kind, full, st);
+    else if(tb) launch_experts<false, true>(ep, grid, kind, full, st);
+    else launch_experts<false, false>(ep, grid, kind, full, st);
     return pk::launch_status("pk_gemm_experts_f32");
 }
 
