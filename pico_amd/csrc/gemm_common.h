@@ -146,6 +146,23 @@ __device__ __forceinline__ void expert_range(const ExpertParams& p, int e, int64
     }
 }
 
+// inclusive sums over a wave's lanes, without the trip through LDS that shuffles take
+__device__ __forceinline__ int wave_prefix(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);  // lanes 1, 2, 4, 8 before
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // lane 15 of the row before
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31
+    return v;
+}
+// lane `at`'s value, in every lane
+__device__ __forceinline__ int64_t wave_value(int64_t v, int at) {
+    const unsigned a = (unsigned)__builtin_amdgcn_readlane((int)v, at),
+                   b = (unsigned)__builtin_amdgcn_readlane((int)(v >> 32), at);
+    return (int64_t)((uint64_t)b << 32 | a);
+}
+
 // The rows past the last expert's are a group of their own of at most kZeroTiles row
 // tiles, which fill them with zeros (or, accumulating, leave them).
 constexpr int kZeroTiles = 32;
@@ -168,14 +185,12 @@ __device__ __forceinline__ TileJob tile_job(ExpertParams& p) {
             expert_range(p, q, n, lo, hi);
             return min((int)((hi - lo + T::BM - 1) / T::BM), q < p.experts ? p.tiles_m : kZeroTiles);
         };
-        int all = 0;
+        int all = 0, sum = 0;  // sum: of the lane's expert and those before it, of the last 64
         for(int q = 0; q <= p.experts; q += 64) {
-            int c = tiles(q + lane);
-#pragma unroll
-            for(int o = 32; o > 0; o >>= 1) c += __shfl_xor(c, o, 64);
-            all = min(all + c, p.tiles_m);
+            sum = wave_prefix(tiles(q + lane));
+            all = min(all + __builtin_amdgcn_readlane(sum, 63), p.tiles_m);
         }
-        const int row_tiles = __builtin_amdgcn_readfirstlane(all);
+        const int row_tiles = all;
         const int ntiles = row_tiles * p.tiles_n, run = (ntiles + 7) >> 3;
         bid = (bid & 7) * run + (bid >> 3);  // an XCD takes a run of tiles
         if((int)(blockIdx.x >> 3) >= run || bid >= ntiles) return j;
@@ -185,28 +200,27 @@ __device__ __forceinline__ TileJob tile_job(ExpertParams& p) {
         const int local = bid % group_span;
         tm = first_m + local % gm;
         tn = local / gm;
-        // the expert of row tile tm
+        // the expert of row tile tm (up to 63 experts: found in the sums at hand)
         int before = 0;
         for(int q = 0; q <= p.experts; q += 64) {
-            const int c = tiles(q + lane);
-            int sum = c;
-#pragma unroll
-            for(int o = 1; o < 64; o <<= 1) {
-                const int t = __shfl_up(sum, o, 64);
-                if(lane >= o) sum += t;
-            }
+            if(p.experts > 63) sum = wave_prefix(tiles(q + lane));
             const uint64_t past = __ballot(before + sum > tm);
             if(past) {
                 const int at = __builtin_ctzll(past);
                 e = q + at;
-                tm -= before + __shfl(sum - c, at, 64);
+                tm -= before + (at ? __builtin_amdgcn_readlane(sum, at - 1) : 0);
+                lo = wave_value(lo, at);
+                hi = wave_value(hi, at);
                 break;
             }
-            before += __shfl(sum, 63, 64);
+            before += __builtin_amdgcn_readlane(sum, 63);
         }
+        // (the same in every lane, which the compiler does not see; held in vector
+        // registers they cost the main loop up to half its rate)
         e = __builtin_amdgcn_readfirstlane(e);
         tm = __builtin_amdgcn_readfirstlane(tm);
-        expert_range(p, e, n, lo, hi);
+        lo = wave_value(lo, 0);
+        hi = wave_value(hi, 0);
         if(e == p.experts) {
             const int64_t c = (int64_t)tn * T::BN, width = min(p.N - c, (int64_t)T::BN);
             const int step = min((int)((hi - lo + T::BM - 1) / T::BM), kZeroTiles);
