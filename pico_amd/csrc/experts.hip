@@ -275,7 +275,11 @@ int64_t plan_chunk(int64_t n) {
 }
 
 // ------------------------------------------------------------ rows
-// V floats to a lane (1 or 4), one wave to a row
+// V floats to a lane (1 or 4), L lanes to a row: a wave, or for a few rows a
+// workgroup.  Bound by the rows' bytes (8192 tokens of 768, 2 choices, us: gather 17.5,
+// combine 20, its backward 24.5, 5.0 to 6.1 TB/s); a few rows by the loads that wait
+// for each other (a row's place, its values), which are issued together where they
+// can be.
 template <int V>
 struct Row;
 template <>
@@ -292,43 +296,58 @@ struct Row<4> {
 };
 
 // out[r] = x[order[r] / k] for r < offsets[E]; zeros from there on
-template <int V>
-__global__ __launch_bounds__(256) void expert_gather_kernel(int64_t n, int64_t d, int k,
+template <int V, int L>
+__global__ __launch_bounds__(256) void expert_gather_kernel(int n, int64_t d, int k,
                                                             const int32_t* __restrict__ kept,
                                                             const int32_t* __restrict__ order,
                                                             const float* __restrict__ x, int64_t ldx,
                                                             float* __restrict__ out, int64_t ldo) {
     typedef typename Row<V>::T T;
-    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    const int r = (int)(blockIdx.x * (256 / L) + threadIdx.x / L);
     if(r >= n) return;
-    const int64_t slot = r < *kept ? order[r] : -1;
-    const bool on = slot >= 0 && slot < n;
-    const T* src = reinterpret_cast<const T*>(x + (on ? slot / k : 0) * ldx);
-    T* dst = reinterpret_cast<T*>(out + r * ldo);
-    for(int64_t c = threadIdx.x % 64; c < d / V; c += 64) dst[c] = on ? src[c] : T{};
+    const int slot = order[r], count = *kept;
+    const bool on = r < count && (unsigned)slot < (unsigned)n;
+    const T* src = reinterpret_cast<const T*>(x + (int64_t)(on ? slot / k : 0) * ldx);
+    T* dst = reinterpret_cast<T*>(out + (int64_t)r * ldo);
+    const int m = (int)(d / V);
+#pragma unroll 4
+    for(int c = threadIdx.x % L; c < m; c += L) dst[c] = on ? src[c] : T{};
 }
 
 // out[t] = c[t] + sum over j of gates[t, j] ys[place[t, j]]  (gates NULL: 1)
-template <int V>
-__global__ __launch_bounds__(256) void expert_combine_kernel(int64_t R, int64_t n, int64_t d, int k,
+template <int V, int L>
+__global__ __launch_bounds__(256) void expert_combine_kernel(int R, int n, int64_t d, int k,
                                                              const int32_t* __restrict__ place,
                                                              const float* __restrict__ gates,
                                                              const float* __restrict__ ys, int64_t ldy,
                                                              const float* c, int64_t ldc, float* out,
                                                              int64_t ldo) {
     typedef typename Row<V>::T T;
-    const int64_t t = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    const int t = (int)(blockIdx.x * (256 / L) + threadIdx.x / L);
     if(t >= R) return;
-    for(int64_t i = threadIdx.x % 64; i < d / V; i += 64) {
+    const int m = (int)(d / V);
+    const int32_t* const pt = place + (int64_t)t * k;
+    const float* const gt = gates ? gates + (int64_t)t * k : nullptr;
+    for(int i = threadIdx.x % L; i < m; i += L) {
+        const T base = c ? reinterpret_cast<const T*>(c + (int64_t)t * ldc)[i] : T{};
         T acc = T{};
-        for(int j = 0; j < k; ++j) {
-            const int64_t p = place[t * k + j];
-            if(p < 0 || p >= n) continue;
-            const T v = reinterpret_cast<const T*>(ys + p * ldy)[i];
-            acc = acc + (gates ? gates[t * k + j] * v : v);
+        // four choices at a time, their rows in flight together
+        for(int j = 0; j < k; j += 4) {
+            T v[4];
+            float g[4];
+            bool on[4];
+#pragma unroll
+            for(int e = 0; e < 4; ++e) {
+                const int q = j + e < k ? pt[j + e] : -1;
+                on[e] = (unsigned)q < (unsigned)n;
+                g[e] = gt && j + e < k ? gt[j + e] : 1.0f;
+                v[e] = reinterpret_cast<const T*>(ys + (int64_t)(on[e] ? q : 0) * ldy)[i];
+            }
+#pragma unroll
+            for(int e = 0; e < 4; ++e)
+                if(on[e]) acc = acc + g[e] * v[e];
         }
-        if(c) acc = acc + reinterpret_cast<const T*>(c + t * ldc)[i];
-        reinterpret_cast<T*>(out + t * ldo)[i] = acc;
+        reinterpret_cast<T*>(out + (int64_t)t * ldo)[i] = c ? acc + base : acc;
     }
 }
 
@@ -336,21 +355,21 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(int64_t R, int64_t 
 // slot = order[r]; zeros for dropped slots
 template <int V>
 __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(
-    int64_t n, int64_t d, int k, const int32_t* __restrict__ kept, const int32_t* __restrict__ order,
+    int n, int64_t d, int k, const int32_t* __restrict__ kept, const int32_t* __restrict__ order,
     const float* __restrict__ gates, const float* __restrict__ ys, int64_t ldy,
     const float* __restrict__ dout, int64_t ldo, float* dys, int64_t ldd, float* dgates, int flags) {
     typedef typename Row<V>::T T;
-    const int64_t r = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+    const int r = (int)(blockIdx.x * 4 + threadIdx.x / 64);
     if(r >= n) return;
-    const int lane = threadIdx.x % 64;
-    const int64_t slot = order[r];
-    const bool known = slot >= 0 && slot < n, on = known && r < *kept;
+    const int lane = threadIdx.x % 64, m = (int)(d / V);
+    const int slot = order[r], count = *kept;
+    const bool known = (unsigned)slot < (unsigned)n, on = known && r < count;
     const float g = on ? gates[slot] : 0.0f;
-    const T* up = reinterpret_cast<const T*>(dout + (on ? slot / k : 0) * ldo);
-    const T* yr = reinterpret_cast<const T*>(ys + r * ldy);
-    T* dr = reinterpret_cast<T*>(dys + r * ldd);
+    const T* up = reinterpret_cast<const T*>(dout + (int64_t)(on ? slot / k : 0) * ldo);
+    const T* yr = reinterpret_cast<const T*>(ys + (int64_t)r * ldy);
+    T* dr = reinterpret_cast<T*>(dys + (int64_t)r * ldd);
     float dot = 0.0f;
-    for(int64_t c = lane; c < d / V; c += 64) {
+    for(int c = lane; c < m; c += 64) {
         const T u = on ? up[c] : T{};
         if(dys) {
             const T v = on ? g * u : T{};
@@ -363,15 +382,28 @@ __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(
     if(lane == 0) dgates[slot] = (flags & PK_ACCUM2) ? dgates[slot] + dot : dot;
 }
 
+// rows to which a workgroup each is better than a wave (us, d 768: 32 rows gathered
+// 4.0 as waves, 16 combined 5.5)
+bool few(int64_t rows) { return rows <= 1024; }
+
 bool vec4(int64_t d, std::initializer_list<std::pair<const void*, int64_t>> xs) {
     bool v = d % 4 == 0;
     for(auto& x : xs) v = v && (!x.first || (pk::aligned16(x.first) && x.second % 4 == 0));
     return v;
 }
 
+template <class F>
+void with_rows(bool vec, bool workgroup, F f) {
+    using std::integral_constant;
+    if(vec && workgroup) f(integral_constant<int, 4>(), integral_constant<int, 256>());
+    else if(vec) f(integral_constant<int, 4>(), integral_constant<int, 64>());
+    else if(workgroup) f(integral_constant<int, 1>(), integral_constant<int, 256>());
+    else f(integral_constant<int, 1>(), integral_constant<int, 64>());
+}
+
 int check_rows(const char* who, int64_t n, int64_t d, int64_t k) {
-    if(n < 0 || n > INT32_MAX || d < 1 || k < 1 || k > kMaxTopk)
-        return pk::fail("%s: need 0 <= n < 2^31 slots, d >= 1 and 1 <= k <= %d", who, kMaxTopk);
+    if(n < 0 || n > INT32_MAX || d < 1 || d > INT32_MAX || k < 1 || k > kMaxTopk)
+        return pk::fail("%s: need 0 <= n < 2^31 slots, 1 <= d < 2^31 and 1 <= k <= %d", who, kMaxTopk);
     return PK_OK;
 }
 
@@ -440,13 +472,11 @@ extern "C" int pk_expert_gather_f32(int64_t n, int64_t d, int64_t k, int64_t E, 
     if(n == 0) return PK_OK;
     if(!offsets || !order || !x || !out || ldx < d || ldo < d)
         return pk::fail("pk_expert_gather_f32: NULL pointer or row stride < d");
-    const unsigned grid = (unsigned)((n + 3) / 4);
-    if(vec4(d, {{x, ldx}, {out, ldo}}))
-        expert_gather_kernel<4><<<grid, 256, 0, pk::as_stream(stream)>>>(n, d, (int)k, offsets + E, order, x,
-                                                                        ldx, out, ldo);
-    else
-        expert_gather_kernel<1><<<grid, 256, 0, pk::as_stream(stream)>>>(n, d, (int)k, offsets + E, order, x,
-                                                                        ldx, out, ldo);
+    with_rows(vec4(d, {{x, ldx}, {out, ldo}}), few(n), [&](auto v, auto l) {
+        constexpr int V = decltype(v)::value, L = decltype(l)::value;
+        expert_gather_kernel<V, L><<<(unsigned)((n * L + 255) / 256), 256, 0, pk::as_stream(stream)>>>(
+            (int)n, d, (int)k, offsets + E, order, x, ldx, out, ldo);
+    });
     return pk::launch_status("pk_expert_gather_f32");
 }
 
@@ -458,13 +488,11 @@ extern "C" int pk_expert_combine_f32(int64_t R, int64_t d, int64_t k, const int3
     if(R == 0) return PK_OK;
     if(!place || !ys || !out || ldy < d || ldo < d || (c && ldc < d))
         return pk::fail("pk_expert_combine_f32: NULL pointer or row stride < d");
-    const unsigned grid = (unsigned)((R + 3) / 4);
-    if(vec4(d, {{ys, ldy}, {c, ldc}, {out, ldo}}))
-        expert_combine_kernel<4><<<grid, 256, 0, pk::as_stream(stream)>>>(R, R * k, d, (int)k, place, gates,
-                                                                         ys, ldy, c, ldc, out, ldo);
-    else
-        expert_combine_kernel<1><<<grid, 256, 0, pk::as_stream(stream)>>>(R, R * k, d, (int)k, place, gates,
-                                                                         ys, ldy, c, ldc, out, ldo);
+    with_rows(vec4(d, {{ys, ldy}, {c, ldc}, {out, ldo}}), few(R), [&](auto v, auto l) {
+        constexpr int V = decltype(v)::value, L = decltype(l)::value;
+        expert_combine_kernel<V, L><<<(unsigned)((R * L + 255) / 256), 256, 0, pk::as_stream(stream)>>>(
+            (int)R, (int)(R * k), d, (int)k, place, gates, ys, ldy, c, ldc, out, ldo);
+    });
     return pk::launch_status("pk_expert_combine_f32");
 }
 
@@ -484,9 +512,9 @@ extern "C" int pk_expert_combine_bwd_f32(int64_t R, int64_t d, int64_t k, int64_
     const unsigned grid = (unsigned)((n + 3) / 4);
     if(vec4(d, {{ys, ldy}, {dout, ldo}, {dys, ldd}}))
         expert_combine_bwd_kernel<4><<<grid, 256, 0, pk::as_stream(stream)>>>(
-            n, d, (int)k, offsets + E, order, gates, ys, ldy, dout, ldo, dys, ldd, dgates, flags);
+            (int)n, d, (int)k, offsets + E, order, gates, ys, ldy, dout, ldo, dys, ldd, dgates, flags);
     else
         expert_combine_bwd_kernel<1><<<grid, 256, 0, pk::as_stream(stream)>>>(
-            n, d, (int)k, offsets + E, order, gates, ys, ldy, dout, ldo, dys, ldd, dgates, flags);
+            (int)n, d, (int)k, offsets + E, order, gates, ys, ldy, dout, ldo, dys, ldd, dgates, flags);
     return pk::launch_status("pk_expert_combine_bwd_f32");
 }
