@@ -23,8 +23,14 @@ def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
+def _raw_stream(dev):
+    """the current stream's handle on device `dev` (what torch.cuda.current_stream()
+    wraps, at 0.1 us rather than 3)"""
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    return ctypes.c_void_p(_raw_stream(torch.cuda.current_device()))
 
 
 def _f32(*ts):
@@ -696,11 +702,6 @@ def _ready(dtype, *ts):
 def _at(t):
     """a tensor's address for a launcher (None: NULL)"""
     return None if t is None else t.data_ptr()
-
-
-def _raw_stream(dev):
-    """the current stream's handle (torch.cuda.current_stream(), in 0.1 us)"""
-    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _rows(t, name):
