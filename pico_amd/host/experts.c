@@ -154,14 +154,16 @@ static void expert_matmul_backward(struct PicoTensor* self) {
     const int to_side = nw && w->is_persistent && !x->is_persistent;
     pk_stream_t side = to_side && !pkh_capturing() ? pkh_side_fork() : NULL;
     const int done = side != NULL;
+    int st;
     if(side) {
-        if(expert_dw(self, g, nw->grad_live ? PK_ACCUM : 0, side)) return;
+        st = expert_dw(self, g, nw->grad_live ? PK_ACCUM : 0, side);
         nw->side_seq = pkh_side_seq();
+        if(st) return;
         pkh_grad_mark(w);
     } else if(to_side) {
         pkh_side_prepare();
     }
-    int st = pk_gemm_experts_f32('T', rows, K, N, r->E, r->offsets, g, N, w->data, N, K * N, x->grad,
+    st = pk_gemm_experts_f32('T', rows, K, N, r->E, r->offsets, g, N, w->data, N, K * N, x->grad,
                                  x->strides[0], pkh_grad_flag(x), (int)n->ival[EI_PREC],
                                  pkh_stream());
     if(pkh_status("pico_expert_matmul_backward", st)) return;
