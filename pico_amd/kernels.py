@@ -690,7 +690,7 @@ PRECISIONS = {"fp32": 0, "bf16": 1, "bf16x3": 2}
 def _ready(dtype, *ts):
     """each of `ts` (None aside) is a `dtype` tensor on the current device, where the
     launchers run; returns the device's index"""
-    dev = torch.cuda.current_device()
+    dev = torch._C._cuda_getDevice()
     for t in ts:
         if t is not None and (t.dtype is not dtype or t.get_device() != dev):
             if t.dtype is not dtype or not t.is_cuda:
