@@ -607,7 +607,9 @@ size_t pk_embed_bwd_workspace(int64_t n);
 int pk_embed_bwd_f32(int64_t n, int64_t d, int64_t vocab, const int32_t* ids, const float* dout,
                      float* dtable, void* workspace, size_t workspace_bytes, pk_stream_t stream);
 
-/* ---- layer norm (no reference counterpart) -------------------------------
+/* In the three sections below outputs overlap neither inputs nor each other, except
+ * where a call says that they may.
+ * ---- layer norm (no reference counterpart) -------------------------------
  * over rows of x [R, C], contiguous: y = (x - m) * r * g + b with m = mean(x),
  * r = (mean((x - m)^2) + eps)^-1/2.  g [C]; b [C] or NULL (no bias).  mean and
  * rstd [R] receive m and r for the backward; either may be NULL.
@@ -682,7 +684,10 @@ int pk_gated_scan_bwd_f32(int64_t B, int64_t T, int64_t C, const float* f, int64
  *   split; NULL or fewer bytes: unsplit); parts are added in a fixed order.
  *   precision: 0 fp32, 1 bf16, 2 three bf16 products, as in pk_gemm_add_f32 (no
  *   fp8).  PK_ACCUM accumulates.
- * Limits: E <= 1024, k <= 64, n < 2^31 (products: 2^30). */
+ *   Row strides up to 2^21 (W [K, N], and dw's X and dY: 2^24).
+ * Limits: E <= 1024, k <= 64, n < 2^31 (products: 2^30).  What experts, offsets, order
+ * and place hold is checked on the device: values out of range reach no memory out
+ * of bounds (rows of overlapping experts have no defined result). */
 int pk_route_topk_f32(int64_t R, int64_t E, int64_t k, const float* logits, int64_t ldz,
                       int32_t* experts, float* gates, pk_stream_t stream);
 int pk_route_topk_bwd_f32(int64_t R, int64_t E, int64_t k, const int32_t* experts,

@@ -278,7 +278,13 @@ def _factor(k, precision):
 SIZES = [([1], 8, 8), ([3, 0, 2], 5, 7), ([64], 64, 64), ([0, 0, 1], 33, 65), ([17, 40, 0, 130], 96, 100),
          ([300, 1, 2, 0, 0, 77], 130, 257), ([256, 512, 0, 256], 256, 256), ([1, 1, 1, 1, 1, 1, 1, 1], 768, 128),
          ([700, 90, 13], 1000, 33), ([5] * 70, 40, 36), ([2000, 3, 500], 64, 520), ([129] * 3, 1, 1),
-         ([40, 2], 2, 300), ([60, 0, 61], 3, 1)]
+         ([40, 2], 2, 300), ([60, 0, 61], 3, 1),
+         # many rows: whole tiles of 256 apart from the rest, with and without bounds
+         ([1500, 700, 0, 900], 64, 256), ([1025, 511], 40, 300), ([2048], 32, 512), ([512, 1024], 96, 256),
+         # a few rows, streamed weights: sizes around the vectors' and steps'
+         ([4, 4], 128, 64), ([5, 3, 9], 131, 68), ([1], 4, 4), ([2, 7], 130, 66), ([30, 2], 515, 6),
+         # more experts than a wave's lanes, tiles of several rows each
+         ([45] * 70, 96, 130), ([0] * 40 + [200] * 30, 32, 40)]
 
 
 @pytest.mark.parametrize("sizes,kk,nn", SIZES)
@@ -442,6 +448,52 @@ def test_layer_captured_and_replayed_with_other_routings(dev):
         step()
         assert all(torch.equal(a, b) for a, b in zip(got, outs))
     assert len(seen) == 4
+
+
+@pytest.mark.parametrize("bad", [[-7, 3, 2, 400], [0, 1 << 30, 1 << 30, 1 << 30], [90, 60, 30, 0],
+                                 [-(1 << 31)] * 4])
+@pytest.mark.parametrize("kk,nn", [(64, 256), (40, 20)])
+def test_offsets_out_of_range_stay_in_bounds(dev, bad, kk, nn):
+    """offsets are held to the rows there are and to increase: nothing outside the
+    outputs is written, and rows that one expert has alone are right"""
+    n, E = 100, 3
+    g = _gen(3)
+    offsets = torch.tensor(bad, dtype=torch.int32).cuda()
+    x, w = torch.randn(n, kk, generator=g).cuda(), torch.randn(E, kk, nn, generator=g).cuda()
+    y, dw = _empty(n + 2, nn), _empty(E + 2, kk, nn)
+    K.gemm_experts("N", x, w, offsets, y[1:n + 1])
+    dy = torch.randn(n, nn, generator=g).cuda()
+    K.gemm_experts_dw(x, dy, offsets, dw[1:E + 1])
+    assert bool((y[[0, n + 1]] == 7).all()) and bool((dw[[0, E + 1]] == 7).all())
+    lo = [min(max(b, 0), n) for b in bad]
+    hi = [max(lo[e + 1], lo[e]) for e in range(E)]
+    own = torch.zeros(n, dtype=torch.int32)
+    for e in range(E):
+        own[lo[e]:hi[e]] += 1
+        a, b = x[lo[e]:hi[e]].double().cpu(), dy[lo[e]:hi[e]].double().cpu()
+        _close(dw[e + 1], a.t() @ b, _factor(len(a), "fp32") * (a.t().abs() @ b.abs()), e)
+    for e in range(E):
+        r = [i for i in range(lo[e], hi[e]) if own[i] == 1 and i < lo[E]]
+        a, b = x[r].double().cpu(), w[e].double().cpu()
+        _close(y[1:n + 1][r], a @ b, _factor(kk, "fp32") * (a.abs() @ b.abs()), e)
+
+
+def test_dw_workspace_is_optional(dev):
+    """few tiles and many rows: split with a workspace, unsplit without; both right"""
+    offsets, n = _offsets([3000, 0, 5000])
+    g = _gen(4)
+    x, dy = torch.randn(n, 64, generator=g).cuda(), torch.randn(n, 48, generator=g).cuda()
+    need = K.gemm_experts_dw_workspace(n, 64, 48, 3)
+    assert need > 0
+    out = []
+    for size in (need, need - 1, 1):
+        dw = _empty(3, 64, 48)
+        K.gemm_experts_dw(x, dy, offsets, dw, ws=torch.empty(size, dtype=torch.uint8, device="cuda:0"))
+        out.append(dw)
+        for e, r in ((0, slice(0, 3000)), (1, slice(0, 0)), (2, slice(3000, 8000))):
+            a, b = x[r].double().cpu(), dy[r].double().cpu()
+            _close(dw[e], a.t() @ b, _factor(len(a), "fp32") * (a.t().abs() @ b.abs()), (size, e))
+    assert torch.equal(out[1], out[2])
 
 
 def test_refusals(dev):

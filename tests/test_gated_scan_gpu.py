@@ -95,6 +95,43 @@ def test_forward_and_gradients(dev, B, T, C, state):
         assert bool((t == 7.0).all())  # nothing behind the outputs is written
 
 
+def _chain(a, b):
+    """y_t = a_t y_{t-1} + b_t along dim 0 from zero, in log2(T) passes"""
+    step = 1
+    a, b = a.clone(), b.clone()
+    while step < a.shape[0]:
+        b[step:] = b[step:] + a[step:] * b[:-step]
+        a[step:] = a[step:] * a[:-step]
+        step *= 2
+    return b
+
+
+def test_larger_than_the_caches(dev):
+    """one sequence of 25 million values a tensor, which takes the backward's own kernel"""
+    T, C = 50000, 512
+    g = torch.Generator(device="cuda:0").manual_seed(1)
+    f = torch.randn(T, C, device="cuda:0", generator=g) + 2
+    x, dh = (torch.randn(T, C, device="cuda:0", generator=g) for _ in range(2))
+    h, df, dx = _empty(T, C), _empty(T, C), _empty(T, C)
+    K.gated_scan_fwd(1, f, x, h)
+    K.gated_scan_bwd(1, f, x, h, dh, df, dx)
+    for c in range(0, C, 64):
+        cut = slice(c, c + 64)
+        fd, xd, gd = (t[:, cut].double() for t in (f, x, dh))
+        s, q = torch.sigmoid(fd), torch.sigmoid(-fd)
+        zero = torch.zeros_like(s[:1])
+        want, ab = _chain(s, q * xd), _chain(s, q * xd.abs())
+        eh = _chain(s, 20 * U * (ab + s * torch.cat([zero, ab[:-1]])))
+        _close(h[:, cut], want, eh, "h")
+        after = torch.cat([s[1:], zero]).flip(0)
+        G, aG = _chain(after, gd.flip(0)).flip(0), _chain(after, gd.abs().flip(0)).flip(0)
+        eG = _chain(after, 40 * U * aG.flip(0)).flip(0)
+        _close(dx[:, cut], q * G, q * (eG + 12 * U * aG), "dx")
+        hp, ehp = torch.cat([zero, want[:-1]]), torch.cat([zero, eh[:-1]])
+        _close(df[:, cut], G * (hp - xd) * s * q,
+               s * q * (eG * (hp - xd).abs() + aG * ehp + 30 * U * aG * (hp.abs() + xd.abs())), "df")
+
+
 @pytest.mark.parametrize("B,T,C", [(2, 70, 24), (1, 3000, 17), (3, 1, 64), (4, 600, 64)])
 def test_views_accumulation_and_single_gradients(dev, B, T, C):
     """f and x as column blocks of one projection, the gradients as columns of its
