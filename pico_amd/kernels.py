@@ -924,6 +924,8 @@ def gemm_experts(tb, x, w, offsets, y, precision="fp32", accum=False):
     dev = _ready(torch.float32, x, w, y)
     _ready(torch.int32, offsets)
     _dense(offsets)
+    if tb not in ("N", "T"):
+        raise ValueError(f"gemm_experts: the transpose flag must be 'N' or 'T' (got {tb!r})")
     ldw, sw = _expert_stack(w, "w")
     E, K, N = w.shape if tb == "N" else (w.shape[0], w.shape[2], w.shape[1])
     n = x.shape[0]

@@ -496,6 +496,13 @@ def test_dw_workspace_is_optional(dev):
     assert torch.equal(out[1], out[2])
 
 
+def test_transpose_flag(dev):
+    offsets, n = _offsets([4, 9])
+    for tb in ("n", "t", "C", ""):
+        with pytest.raises(ValueError):
+            K.gemm_experts(tb, _empty(n, 8), _empty(2, 8, 8), offsets, _empty(n, 8))
+
+
 def test_refusals(dev):
     offsets, n = _offsets([4, 9])
     x, w, y = _empty(n, 8), _empty(2, 8, 12), _empty(n, 12)
