@@ -116,6 +116,8 @@ __global__ __launch_bounds__(256) void route_topk_bwd_kernel(int64_t R, int E, i
 }
 
 constexpr int kMaxExperts = 1024, kMaxTopk = 64;
+// slots, at up to 64 lanes each (a launch has fewer than 2^32 threads)
+constexpr int64_t kMaxSlots = (int64_t)1 << 25;
 
 // f(G, N) as compile-time numbers: 4 logits a lane where that leaves at least 8 lanes
 // to a token and k of them, so that a wave has several tokens and an exchange few
@@ -143,7 +145,7 @@ int check_route(const char* who, int64_t R, int64_t E, int64_t k) {
     if(R < 0 || E < 1 || E > kMaxExperts || k < 1 || k > E || k > kMaxTopk)
         return pk::fail("%s: need R >= 0, 1 <= E <= %d experts and 1 <= k <= min(E, %d) choices", who,
                         kMaxExperts, kMaxTopk);
-    if(R * k > (int64_t)INT32_MAX) return pk::fail("%s: R*k above 2^31 - 1", who);
+    if(R > kMaxSlots || R * k > kMaxSlots) return pk::fail("%s: R*k above 2^25", who);
     return PK_OK;
 }
 
@@ -410,8 +412,8 @@ void with_rows(bool vec, bool workgroup, F f) {
 }
 
 int check_rows(const char* who, int64_t n, int64_t d, int64_t k) {
-    if(n < 0 || n > INT32_MAX || d < 1 || d > INT32_MAX || k < 1 || k > kMaxTopk)
-        return pk::fail("%s: need 0 <= n < 2^31 slots, 1 <= d < 2^31 and 1 <= k <= %d", who, kMaxTopk);
+    if(n < 0 || n > kMaxSlots || d < 1 || d > (int64_t)1 << 30 || k < 1 || k > kMaxTopk)
+        return pk::fail("%s: need 0 <= n <= 2^25 slots, 1 <= d <= 2^30 and 1 <= k <= %d", who, kMaxTopk);
     return PK_OK;
 }
 
@@ -491,7 +493,7 @@ extern "C" int pk_expert_gather_f32(int64_t n, int64_t d, int64_t k, int64_t E, 
 extern "C" int pk_expert_combine_f32(int64_t R, int64_t d, int64_t k, const int32_t* place,
                                      const float* gates, const float* ys, int64_t ldy, const float* c,
                                      int64_t ldc, float* out, int64_t ldo, pk_stream_t stream) {
-    if(R < 0 || R > INT32_MAX) return pk::fail("pk_expert_combine_f32: need 0 <= R < 2^31");
+    if(R < 0 || R > kMaxSlots) return pk::fail("pk_expert_combine_f32: need 0 <= R <= 2^25");
     if(int st = check_rows("pk_expert_combine_f32", R * k, d, k)) return st;
     if(R == 0) return PK_OK;
     if(!place || !ys || !out || ldy < d || ldo < d || (c && ldc < d))
@@ -509,7 +511,7 @@ extern "C" int pk_expert_combine_bwd_f32(int64_t R, int64_t d, int64_t k, int64_
                                          const float* gates, const float* ys, int64_t ldy,
                                          const float* dout, int64_t ldo, float* dys, int64_t ldd,
                                          float* dgates, int flags, pk_stream_t stream) {
-    if(R < 0 || R > INT32_MAX) return pk::fail("pk_expert_combine_bwd_f32: need 0 <= R < 2^31");
+    if(R < 0 || R > kMaxSlots) return pk::fail("pk_expert_combine_bwd_f32: need 0 <= R <= 2^25");
     if(int st = check_rows("pk_expert_combine_bwd_f32", R * k, d, k)) return st;
     if(E < 1) return pk::fail("pk_expert_combine_bwd_f32: need E >= 1");
     if(R == 0 || (!dys && !dgates)) return PK_OK;

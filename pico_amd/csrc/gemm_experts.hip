@@ -10,6 +10,8 @@ namespace {
 using namespace pkg;
 
 constexpr int kMaxExperts = 1024;
+// workgroups of a launch, at up to 512 threads (fewer than 2^32 in all)
+constexpr int64_t kMaxTiles = (int64_t)1 << 22;
 
 int check(const char* who, int64_t n, int64_t M, int64_t N, int64_t E, const int32_t* offsets,
           int precision) {
@@ -202,11 +204,9 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     ExpertShape rest;
     const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K, &rest);
     // (the estimates are of up to 32 rows to an expert)
-    if(!TB && N >= 4 && K > 0 && n <= 32 * groups &&
+    const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 63) / 64;
+    if(!TB && N >= 4 && K > 0 && n <= 32 * groups && tiles_n <= kMaxTiles / tiles_m &&
        thin_us((double)groups, (double)n / groups, N, K) < s.us) {
-        const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 63) / 64;
-        if(tiles_m * tiles_n > (int64_t)1 << 30)
-            return pk::fail("pk_gemm_experts_f32: problem too large for one launch");
         ep.tiles_m = (int)tiles_m;
         ep.tiles_n = (int)tiles_n;
         const unsigned grid = (unsigned)((tiles_m * tiles_n + 7) / 8 * 8);
@@ -218,7 +218,7 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     // `most` row tiles at most
     auto tiles = [&](const ExpertShape& t, int64_t most, int which, bool full) {
         const int64_t tiles_n = (N + t.bn - 1) / t.bn;
-        if(most * tiles_n > (int64_t)1 << 30)
+        if(most > 0 && tiles_n > kMaxTiles / most)
             return pk::fail("pk_gemm_experts_f32: problem too large for one launch");
         ep.rows = which;
         ep.tiles_m = (int)most;
@@ -281,7 +281,7 @@ extern "C" int pk_gemm_experts_dw_f32(int64_t n, int64_t K, int64_t N, int64_t E
     ep.splits = splits;
     ep.ws = static_cast<float*>(workspace);
     const int64_t tiles_m = (K + s.bm - 1) / s.bm, tiles_n = (N + s.bn - 1) / s.bn;
-    if(tiles_m > (int64_t)1 << 30 || tiles_n > (int64_t)1 << 30 || tiles_m * tiles_n * E > (int64_t)1 << 30)
+    if(tiles_m > kMaxTiles || tiles_n > kMaxTiles || tiles_m * tiles_n > kMaxTiles / E)
         return pk::fail("pk_gemm_experts_dw_f32: problem too large for one launch");
     ep.tiles_m = (int)tiles_m;
     ep.tiles_n = (int)tiles_n;

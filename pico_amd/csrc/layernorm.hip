@@ -77,7 +77,6 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void layernorm_fwd(int R, int
     const Share<NV, W, EXACT> me(C);
     const int group = threadIdx.x / (64 * W), w = threadIdx.x / 64 % W;
     const int64_t step = (int64_t)gridDim.x * ROWS;
-    const float inv = 1.0f / me.count;
     int64_t row = (int64_t)blockIdx.x * ROWS + group;
     f32x4 cur[NV], next[NV];
     if(W > 1 || row < R) me.load(x + min(row, (int64_t)R - 1) * C, cur);
@@ -429,6 +428,8 @@ extern "C" int pk_layernorm_fwd_f32(int64_t R, int64_t C, float eps, const float
     if(!x || !g || !y) return pk::fail("pk_layernorm_fwd_f32: NULL pointer");
     hipStream_t st = pk::as_stream(stream);
     if(!cached(C)) {
+        if(!pk::grid_fits(R, C < 4 ? 64 : 1024))
+            return pk::fail("pk_layernorm_fwd_f32: too many rows of %lld values for one launch", (long long)C);
         if(C < 4) layernorm_fwd_any<1><<<(unsigned)R, 64, 0, st>>>(C, eps, x, g, b, y, mean, rstd);
         else layernorm_fwd_any<16><<<(unsigned)R, 1024, 0, st>>>(C, eps, x, g, b, y, mean, rstd);
         return pk::launch_status("pk_layernorm_fwd_f32");
@@ -485,6 +486,8 @@ extern "C" int pk_layernorm_bwd_f32(int64_t R, int64_t C, const float* x, const 
         return pk::launch_status("pk_layernorm_bwd_f32");
     }
     if(R > 0 && dx) {
+        if(!pk::grid_fits(R, C < 4 ? 64 : 1024))
+            return pk::fail("pk_layernorm_bwd_f32: too many rows of %lld values for one launch", (long long)C);
         if(C < 4) layernorm_dx_any<1><<<(unsigned)R, 64, 0, st>>>(C, x, g, mean, rstd, dy, dx_in, dx);
         else layernorm_dx_any<16><<<(unsigned)R, 1024, 0, st>>>(C, x, g, mean, rstd, dy, dx_in, dx);
     }

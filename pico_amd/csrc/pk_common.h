@@ -122,4 +122,7 @@ inline unsigned grid_for(int64_t work_items, int threads, int64_t cap = 256 * 16
     return (unsigned)g;
 }
 
+// a launch has fewer than 2^32 threads along x
+inline bool grid_fits(int64_t blocks, int64_t threads) { return blocks < ((int64_t)1 << 32) / threads; }
+
 }  // namespace pk

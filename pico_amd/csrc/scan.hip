@@ -507,10 +507,15 @@ int run(const char* who, ScanParams& p, void* workspace, size_t workspace_bytes,
 int check(const char* who, int64_t B, int64_t T, int64_t C, const float* f, int64_t ldf,
           const float* x, int64_t ldx) {
     if(B < 0 || T < 0 || C < 0) return pk::fail("%s: negative size", who);
-    if(B > INT32_MAX || T > INT32_MAX || C > INT32_MAX || B * T > INT32_MAX ||
-       B * ((C + 3) / 4) > INT32_MAX - 8)
-        return pk::fail("%s: B*T rows or B*C channels too many for one call", who);
+    if(B > INT32_MAX || T > INT32_MAX || C > INT32_MAX || B * T > INT32_MAX)
+        return pk::fail("%s: B*T rows too many for one call", who);
     if(B == 0 || T == 0 || C == 0) return PK_OK;
+    // (4 channels to a thread, and 256 threads to a workgroup of at least a sequence)
+    const Plan plan = plan_of(B, T, C);
+    const int64_t V = C < 4 ? 1 : 4, lanes = plan.lanes ? plan.lanes : 1,
+                  groups = (C + V * lanes - 1) / (V * lanes);
+    if(groups > (((int64_t)1 << 32) / (plan.lanes ? kThreads : 1) - 2 * kThreads) / B)
+        return pk::fail("%s: B*C channels too many for one launch", who);
     if(!f || !x) return pk::fail("%s: NULL f or x", who);
     if(ldf < C || ldx < C) return pk::fail("%s: row stride < C", who);
     return PK_OK;

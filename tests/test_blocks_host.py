@@ -142,3 +142,21 @@ def test_products(L):
     for bad in (dict(X=None), dict(dY=None), dict(dW=None), dict(ldx=3), dict(ldy=11), dict(ldw=11), dict(sw=47),
                 dict(ldx=1 << 25), dict(ldy=1 << 25)):
         _refused(L, dw(**bad), "pk_gemm_experts_dw_f32")
+
+
+def test_more_threads_than_a_launch_has(L):
+    """sizes whose launch would have 2^32 threads or more"""
+    for C, R in ((3, 1 << 26), (20000, 1 << 22)):
+        _refused(L, L.pk_layernorm_fwd_f32(R, C, 1e-5, PTR, PTR, None, PTR, None, None, None), "rows")
+        _refused(L, L.pk_layernorm_bwd_f32(R, C, PTR, PTR, PTR, PTR, PTR, None, PTR, None, None, 0, None, 0, None),
+                 "rows")
+    for B, T, C in (((1 << 31) - 1, 1, 3), (1 << 24, 9, 4), (1 << 28, 2, 64)):
+        _refused(L, L.pk_gated_scan_fwd_f32(B, T, C, PTR, 64, PTR, 64, None, PTR, PTR, 1 << 60, None), "channels")
+    _refused(L, L.pk_route_topk_f32((1 << 25) + 1, 64, 1, PTR, 64, PTR, PTR, None), "2^25")
+    _refused(L, L.pk_expert_gather_f32(1 << 26, 4, 2, 4, PTR, PTR, PTR, 8, PTR, 8, None), "2^25")
+    _refused(L, L.pk_expert_combine_f32(1 << 25, 4, 2, PTR, PTR, PTR, 8, None, 8, PTR, 8, None), "2^25")
+    # 32768 rows of 1024 experts: more tiles than a launch has, streamed or not
+    _refused(L, L.pk_gemm_experts_f32(b"N", 32768, 1 << 24, 4, 1024, PTR, PTR, 4, PTR, 1 << 24, 1 << 26, PTR, 1 << 24,
+                                      0, 0, None), "too large")
+    _refused(L, L.pk_gemm_experts_dw_f32(32768, 1 << 12, 1 << 20, 1024, PTR, PTR, 1 << 12, PTR, 1 << 20, PTR, 1 << 20,
+                                         1 << 32, 0, 0, None, 0, None), "too large")
