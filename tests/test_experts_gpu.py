@@ -496,6 +496,83 @@ def test_dw_workspace_is_optional(dev):
     assert torch.equal(out[1], out[2])
 
 
+def test_rows_past_32_bit_offsets(dev):
+    """1100 rows 2^21 values apart: element offsets beyond 2^31, byte offsets beyond 2^33"""
+    n, E, ld, kk, nn = 1100, 3, 1 << 21, 36, 40
+    g = _gen(8)
+    far = torch.empty(n, ld, device="cuda:0")
+    x, y, dys = far[:, :kk], far[:, 64:64 + nn], far[:, 128:128 + kk]
+    x.copy_(torch.randn(n, kk, generator=g).cuda())
+    experts = torch.randint(0, E, (n, 1), generator=g, dtype=torch.int32).cuda()
+    offsets, order, place = (_empty(m, dtype=torch.int32) for m in (E + 1, n, n))
+    K.expert_plan(experts, offsets, order, place)
+    w = torch.randn(E, kk, nn, generator=g).cuda()
+    gates, dout = torch.rand(n, 1, generator=g).cuda(), torch.randn(n, kk, generator=g).cuda()
+    near = x.contiguous()
+    for a, b in ((lambda t, o: K.expert_gather(t, 1, offsets, order, o), kk),
+                 (lambda t, o: K.gemm_experts("N", t, w, offsets, o), nn),
+                 (lambda t, o: K.expert_combine(place, gates, t, o), kk)):
+        out = far[:, 192:192 + b]
+        want = _empty(n, b)
+        a(near, want)
+        a(x, out)
+        assert torch.equal(out, want)
+    dw, want, dgates, dwant = _empty(E, kk, kk), _empty(E, kk, kk), _empty(n, 1), _empty(n, 1)
+    K.expert_combine_bwd(offsets, order, gates, x, dout, dys, dgates)
+    ndys = _empty(n, kk)
+    K.expert_combine_bwd(offsets, order, gates, near, dout, ndys, dwant)
+    assert torch.equal(dys, ndys) and torch.equal(dgates, dwant)
+    K.gemm_experts_dw(x, dys, offsets, dw)
+    K.gemm_experts_dw(near, ndys, offsets, want)
+    assert torch.equal(dw, want)
+    logits, dlogits = far[:, 256:256 + E], far[:, 320:320 + E]
+    logits.copy_(torch.randn(n, E, generator=g).cuda())
+    out = [(_empty(n, 2, dtype=torch.int32), _empty(n, 2)) for _ in range(2)]
+    K.route_topk(logits, *out[0])
+    K.route_topk(logits.contiguous(), *out[1])
+    assert torch.equal(out[0][0], out[1][0]) and torch.equal(out[0][1], out[1][1])
+    dg, dz = torch.randn(n, 2, generator=g).cuda(), _empty(n, E)
+    K.route_topk_bwd(*out[0], dg, dlogits)
+    K.route_topk_bwd(*out[0], dg, dz)
+    assert torch.equal(dlogits, dz)
+
+
+def test_two_streams(dev):
+    """the same layer on two streams at once, each with other tokens, as on one"""
+    E, k, d, f = 6, 2, 96, 160
+    g = _gen(9)
+    w, w2 = torch.randn(E, d, f, generator=g).cuda(), torch.randn(E, f, d, generator=g).cuda()
+    inputs = [(torch.randn(R, d, generator=g).cuda(), torch.randn(R, E, generator=g).cuda()) for R in (700, 3000)]
+
+    def layer(x, z):
+        R = len(x)
+        experts, gates = _empty(R, k, dtype=torch.int32), _empty(R, k)
+        offsets, order, place = (_empty(m, dtype=torch.int32) for m in (E + 1, R * k, R * k))
+        K.route_topk(z, experts, gates)
+        K.expert_plan(experts, offsets, order, place)
+        xs, h, ys, y = _empty(R * k, d), _empty(R * k, f), _empty(R * k, d), _empty(R, d)
+        K.expert_gather(x, k, offsets, order, xs)
+        K.gemm_experts("N", xs, w, offsets, h)
+        K.gemm_experts("N", h, w2, offsets, ys)
+        K.expert_combine(place, gates, ys, y, c=x)
+        dw = _empty(E, d, f)
+        K.gemm_experts_dw(xs, h, offsets, dw)
+        return y, dw
+
+    want = [layer(*i) for i in inputs]
+    streams = [torch.cuda.Stream() for _ in inputs]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for st, i in zip(streams, inputs):
+            with torch.cuda.stream(st):
+                got.append(layer(*i))
+    torch.cuda.synchronize()
+    for i, pair in enumerate(got):
+        for a, b in zip(pair, want[i % 2]):
+            assert torch.equal(a, b)
+
+
 def test_transpose_flag(dev):
     offsets, n = _offsets([4, 9])
     for tb in ("n", "t", "C", ""):
@@ -615,4 +692,49 @@ def test_pico_product_precisions(P, precision):
             for got, a, b in ((gy[r], xr[r], wr[e]), (gx[r], dr[r], wr[e].t()), (gw[e], xr[r].t(), dr[r])):
                 _close(got, a @ b, _factor(a.shape[1], name) * (a.abs() @ b.abs()), e)
     for t in (zp, xp, wp):
+        P.free(t)
+
+
+def test_pico_shared_weights_padding_and_two_backwards(P):
+    """two layers over one route with the same weights and gates, a padded batch, and the
+    gradients of two backward passes added up"""
+    R, E, k, d = 37, 4, 2, 48
+    g = _gen(12)
+    x, z = torch.randn(R, d, generator=g), torch.randn(R, E, generator=g)
+    w = torch.randn(E, d, d, generator=g) * d ** -0.5
+    z[30:] = -INF
+    dy = torch.randn(R, d, generator=g)
+    vx, vz, vw = leaves = [t.double().requires_grad_() for t in (x, z, w)]
+    experts = torch.from_numpy(_choose(z, k)[0]).long()
+    gone = experts < 0
+    picked = torch.gather(torch.where(vz == -INF, 0.0, vz), 1, experts.clamp(min=0))
+    gates = torch.where(gone, 0.0, torch.softmax(picked, 1))
+
+    def layer(h):
+        y = h
+        for e in range(E):
+            t, j = torch.nonzero(experts == e, as_tuple=True)
+            y = y.index_add(0, t, (h[t] @ vw[e]) * gates[t, j][:, None])
+        return y
+
+    y = layer(layer(vx))
+    (2 * y * dy.double()).sum().backward()
+    xp, zp, wp = ps = [P.param(list(t.shape), t.numpy()) for t in (x, z, w)]
+    for _ in range(2):
+        with P.arena():
+            gp, route = P.route_topk(zp, k)
+            h = xp
+            for _ in range(2):
+                h = P.expert_combine(P.expert_matmul(P.expert_gather(h, route), wp, route), gp, route, h)
+            P.backward(P.mul(h, P.tensor([R, d], dy.numpy())))
+            got = P.value(h)
+    assert np.array_equal(got[30:], x[30:].numpy())  # no expert: the residual alone
+    # every value passes at most four products, of at most d + R terms, whose absolute
+    # values are within 40 times the largest result's
+    bound = 40 * (2 * d + 2 * R + 50) * 2 * U
+    _close(torch.from_numpy(got), y.detach(), bound * y.detach().abs().max(), "y")
+    for t, leaf, name in zip(ps, leaves, ("dx", "dlogits", "dw")):
+        _close(torch.from_numpy(P.grad_value(t)), leaf.grad, bound * leaf.grad.abs().max(), name)
+    assert not P.grad_value(zp)[30:].any()
+    for t in ps:
         P.free(t)

@@ -132,6 +132,25 @@ def test_larger_than_the_caches(dev):
                s * q * (eG * (hp - xd).abs() + aG * ehp + 30 * U * aG * (hp.abs() + xd.abs())), "df")
 
 
+@pytest.mark.parametrize("B,T", [(1, 1100), (275, 4)])
+def test_rows_past_32_bit_offsets(dev, B, T):
+    """rows 2^21 values apart: element offsets beyond 2^31"""
+    C = 20
+    far = torch.empty(B * T, 1 << 21, device="cuda:0")
+    f, x, h0, dh = _data(B, T, C, 3)
+    ff, fx, fdf, fdx = (far[:, i:i + C] for i in (0, 64, 128, 192))
+    ff.copy_(f)
+    fx.copy_(x)
+    h, want = _empty(B * T, C), _empty(B * T, C)
+    K.gated_scan_fwd(B, ff, fx, h, h0=h0)
+    K.gated_scan_fwd(B, f, x, want, h0=h0)
+    assert torch.equal(h, want)
+    df, dx, d0, d1 = _empty(B * T, C), _empty(B * T, C), _empty(B, C), _empty(B, C)
+    K.gated_scan_bwd(B, ff, fx, h, dh, fdf, fdx, h0=h0, dh0=d0)
+    K.gated_scan_bwd(B, f, x, h, dh, df, dx, h0=h0, dh0=d1)
+    assert torch.equal(fdf, df) and torch.equal(fdx, dx) and torch.equal(d0, d1)
+
+
 @pytest.mark.parametrize("B,T,C", [(2, 70, 24), (1, 3000, 17), (3, 1, 64), (4, 600, 64)])
 def test_views_accumulation_and_single_gradients(dev, B, T, C):
     """f and x as column blocks of one projection, the gradients as columns of its

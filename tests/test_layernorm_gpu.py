@@ -213,6 +213,33 @@ def test_captured_and_replayed(dev):
         assert all(torch.equal(a, c) for a, c in zip(got, out))
 
 
+def test_values_past_32_bit_offsets(dev):
+    """more than 2^31 values: the last rows as by themselves"""
+    R, C = 1100000, 2048
+    x = torch.empty(R, C, device="cuda:0")
+    last = torch.randn(64, C, generator=torch.Generator().manual_seed(1)).cuda()
+    x.fill_(1)
+    x[-64:] = last
+    g, b = torch.randn(C, device="cuda:0"), torch.randn(C, device="cuda:0")
+    y, mean, rstd = torch.empty_like(x), torch.empty(R, device="cuda:0"), torch.empty(R, device="cuda:0")
+    K.layernorm_fwd(x, g, b, y, mean, rstd, 1e-5)
+    want, m, r = torch.empty_like(last), torch.empty(64, device="cuda:0"), torch.empty(64, device="cuda:0")
+    K.layernorm_fwd(last, g, b, want, m, r, 1e-5)
+    assert torch.equal(y[-64:], want) and torch.equal(mean[-64:], m) and torch.equal(rstd[-64:], r)
+    assert torch.equal(y[:-64].amax(0), b) and torch.equal(y[:-64].amin(0), b)
+    # the same rows' gradients; those of the others are zero
+    dy = y.zero_()
+    dy[-64:] = want
+    dg, db, dg1, db1 = (torch.empty(C, device="cuda:0") for _ in range(4))
+    dx, dx1 = torch.full_like(x, 7), torch.empty_like(last)
+    K.layernorm_bwd(x, g, mean, rstd, dy, dx, dg, db)
+    K.layernorm_bwd(last, g, m, r, want, dx1, dg1, db1)
+    assert torch.equal(dx[-64:], dx1) and not dx[:-64].any()
+    # (64 values a column, added in two orders)
+    for a, c, each in ((dg, dg1, want * (last - m[:, None]) * r[:, None]), (db, db1, want)):
+        assert bool(((a - c).abs() <= 2 * 66 * 2.0 ** -24 * each.abs().sum(0)).all())
+
+
 def test_refusals(dev):
     x, g, b, dy = _data(4, 8, 2)
     m = _empty(4)
