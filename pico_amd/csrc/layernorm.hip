@@ -22,7 +22,7 @@ namespace {
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 // (plain loads and nontemporal stores: with nontemporal loads 8192x4096 took 48 + 78 us
-// forward and backward, with these 41 + 73)
+// forward and backward, with these 41 + 73, now 41 + 66)
 __device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4u*>(p); }
 
 // A lane's share of a row: vector v starts at column `at[v]` and holds `skip[v]` values
@@ -83,8 +83,12 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void layernorm_fwd(int R, int
     // (the waves of a workgroup meet in every turn, so all take the same ones)
     for(int turn = 0; row - group < R; row += step, turn ^= 1) {
         if(W == 1 && row >= R) return;
+        // (of one wave's rows the last is read twice: with a load that a branch may leave
+        // out, the waits for this row's values wait for the next one's.  65536x512 us 39.5
+        // against 41; of several waves, which wait for each other, 8192x4096 43.3 against
+        // 41.0)
         const int64_t after = min(row + step, (int64_t)R - 1);
-        if(row - group + step < R) me.load(x + after * C, next);
+        if(W == 1 || row - group + step < R) me.load(x + after * C, next);
         float s = 0.0f;
 #pragma unroll
         for(int v = 0; v < NV; ++v)
@@ -165,7 +169,7 @@ __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
         sg[v] = sb[v] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
     int64_t row = (int64_t)blockIdx.x * ROWS + group;
-    float mn, rn;
+    float m, r, mn, rn;
     auto fetch = [&](int64_t r, f32x4 (&a)[NV], f32x4 (&d)[NV]) {
         r = min(r, (int64_t)R - 1);
         me.load(x + r * C, a);
@@ -175,17 +179,21 @@ __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
     };
     // (8 vectors of every array leave no registers for the next row's)
     constexpr bool AHEAD = NV <= 4;
-    if(AHEAD) fetch(row, xn, dn);
+    if(AHEAD) {
+        fetch(row, xc, dc);
+        m = mn;
+        r = rn;
+    }
     for(int turn = 0; row - group < R; row += step, turn ^= 1) {
-        if(!AHEAD) fetch(row, xc, dc);
-        const float m = mn, r = rn;
         if(AHEAD) {
-#pragma unroll
-            for(int v = 0; v < NV; ++v) {
-                xc[v] = xn[v];
-                dc[v] = dn[v];
-            }
-            if(row - group + step < R) fetch(row + step, xn, dn);
+            // (a last row is read twice: with a load that a branch may leave out, the
+            // waits for this row's values wait for the next one's; 8192x4096 66 us, so
+            // 73, but 100x4096 10.3 and so 9.7)
+            fetch(row - group + step < R ? row + step : row, xn, dn);
+        } else {
+            fetch(row, xc, dc);
+            m = mn;
+            r = rn;
         }
         const bool on = row < R;
         float s1 = 0.0f, s2 = 0.0f;
@@ -220,10 +228,9 @@ __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
             s1 /= (float)C;
             s2 /= (float)C;
         }
-        if(!on) continue;
 #pragma unroll
         for(int v = 0; v < NV; ++v) {
-            if(!EXACT && me.skip[v] == 4) continue;
+            if(!on || (!EXACT && me.skip[v] == 4)) continue;
             sg[v] = sg[v] + dc[v] * xc[v];
             sb[v] = sb[v] + dc[v];
             if(what & kDx) {
@@ -231,6 +238,15 @@ __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
                 if(dxin) o = o + load4(dxin + row * C + me.at[v]);
                 me.store(dx + row * C, v, o);
             }
+        }
+        if(AHEAD) {
+#pragma unroll
+            for(int v = 0; v < NV; ++v) {
+                xc[v] = xn[v];
+                dc[v] = dn[v];
+            }
+            m = mn;
+            r = rn;
         }
     }
     if(!(what & kSums)) return;
@@ -380,8 +396,12 @@ __global__ __launch_bounds__(64 * kSumWaves) void layernorm_sum(int64_t P, int64
     *o = (flags & (c < C ? PK_ACCUM2 : PK_ACCUM3)) ? *o + s : s;
 }
 
-// f(NV, W, EXACT) for rows of C values, 4 <= C <= 16384
-template <class F>
+// f(NV, W, EXACT) for rows of C values, 4 <= C <= 16384: up to 4 vectors a lane, and as
+// few waves as hold the row so (33.5 million values forward, us: C 512 2 vectors of one
+// wave 41, 1 of two 55; 1024 4x1 41, 2x2 41, 1x4 55; 2048 4x2 41, 2x4 41, 2x8 62;
+// 4096 4x4 40, 2x8 46).  The backward has two waves from C 769 on (1024 2x2 64.0, 4x1
+// 66.4, with bounds 64.2 and 69.5; 768 3x1 65.5, 2x2 64.1).
+template <bool BWD, class F>
 void with_shape(int64_t C, F f) {
     auto shape = [&](auto nv, auto w) {
         constexpr int N = decltype(nv)::value, W = decltype(w)::value;
@@ -393,7 +413,7 @@ void with_shape(int64_t C, F f) {
     if(v <= 1) shape(integral_constant<int, 1>(), integral_constant<int, 1>());
     else if(v <= 2) shape(integral_constant<int, 2>(), integral_constant<int, 1>());
     else if(v <= 3) shape(integral_constant<int, 3>(), integral_constant<int, 1>());
-    else if(v <= 4) shape(integral_constant<int, 4>(), integral_constant<int, 1>());
+    else if(v <= 4) shape(integral_constant<int, BWD ? 2 : 4>(), integral_constant<int, BWD ? 2 : 1>());
     else if(v <= 6) shape(integral_constant<int, 3>(), integral_constant<int, 2>());
     else if(v <= 8) shape(integral_constant<int, 4>(), integral_constant<int, 2>());
     else if(v <= 12) shape(integral_constant<int, 3>(), integral_constant<int, 4>());
@@ -406,12 +426,13 @@ void with_shape(int64_t C, F f) {
 bool cached(int64_t C) { return C >= 4 && C <= 16384; }
 
 // the workgroups of the backward, each of which leaves a partial sum: one on every
-// CU at most (8192x4096 73 us, two 78; of short rows two: 65536x128 25, one 32), and
-// one in all where a second launch would take longer
+// CU at most (8192x4096 67 us, two 75; of short rows two: 65536x128 25, one 32), and
+// one in all where a second launch would take longer than a second turn (16x768 6.4 us,
+// two launches 6.8; of four turns 32x512 6.9 against 6.2, of eight 64x128 8.4 against
+// 5.2)
 int64_t parts_of(int64_t R, int64_t C) {
-    if(cached(C) && R * C <= 16384) return 1;
-    const int64_t waves = (C + 1023) / 1024;
-    const int64_t rows = !cached(C) ? 1 : waves <= 1 ? 8 : waves <= 2 ? 4 : waves <= 4 ? 2 : 1;
+    const int64_t rows = !cached(C) ? 1 : C <= 768 ? 8 : C <= 2048 ? 4 : C <= 4096 ? 2 : 1;
+    if(cached(C) && R <= 2 * rows) return 1;
     const int64_t p = (R + rows - 1) / rows;
     const int64_t most = C <= 256 ? 512 : 256;
     return p < most ? p : most;
@@ -434,7 +455,7 @@ extern "C" int pk_layernorm_fwd_f32(int64_t R, int64_t C, float eps, const float
         else layernorm_fwd_any<16><<<(unsigned)R, 1024, 0, st>>>(C, eps, x, g, b, y, mean, rstd);
         return pk::launch_status("pk_layernorm_fwd_f32");
     }
-    with_shape(C, [&](auto nv, auto w, auto exact) {
+    with_shape<false>(C, [&](auto nv, auto w, auto exact) {
         constexpr int N = decltype(nv)::value, W = decltype(w)::value;
         constexpr bool EXACT = decltype(exact)::value;
         constexpr int rows = W > 4 ? 1 : 4 / W, threads = W > 4 ? 64 * W : 256;
@@ -474,7 +495,7 @@ extern "C" int pk_layernorm_bwd_f32(int64_t R, int64_t C, const float* x, const 
     if(R > 0 && cached(C)) {
         if(!dx && !sums) return PK_OK;
         const int what = (dx ? kDx : 0) | (sums ? kSums : 0) | (P == 1 ? kDirect : 0);
-        with_shape(C, [&](auto nv, auto w, auto exact) {
+        with_shape<true>(C, [&](auto nv, auto w, auto exact) {
             constexpr int N = decltype(nv)::value, W = decltype(w)::value;
             constexpr bool EXACT = decltype(exact)::value;
             const size_t lds = kBwdWaves / W / 2 * 2 * (size_t)C * sizeof(float);
