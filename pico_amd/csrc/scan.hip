@@ -192,7 +192,7 @@ __global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
     };
     fetch();
     int turn = 0;
-    for(int64_t k = 0; k < p.L; k += Pl::TT) {
+    auto walk = [&](auto last) {
         float s[LT][V], A[V], H[V];
 #pragma unroll
         for(int e = 0; e < LT; ++e)
@@ -214,14 +214,16 @@ __global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
                 A[i] *= s[e][i];
                 H[i] = step<BWD>(H[i], s[e][i], vr[e][i]);
             }
-        if(k + Pl::TT < p.L) fetch();
+        if constexpr(!decltype(last)::value) fetch();
         through<V, CL>(A, H, carry, in, lds, turn);
 #pragma unroll
         for(int i = 0; i < V; ++i)
 #pragma unroll
             for(int q = 0; q < kWaves; ++q) all[i] *= lds[turn][q][0][at.cl * V + i];
         turn ^= 1;
-    }
+    };
+    for(int64_t k = Pl::TT; k < p.L; k += Pl::TT) walk(std::false_type());
+    walk(std::true_type());
     if(at.tl == 0) {
         float* const o = p.ws + (at.chunk * p.B + at.b) * p.C + at.c;
         store<V>(o, all, at.skip, false);
@@ -309,12 +311,18 @@ __global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
         through<V, CL>(A, H, carry, in, lds, turn);
         turn ^= 1;
     }
-    for(int64_t tile = g0; tile < g1; tile += Pl::TT) {
+    // (the last tile apart: were its fetch a branch's, the waits for one tile's values
+    // would be for the next one's as well)
+    auto walk = [&](int64_t tile, auto last) {
+        constexpr bool LAST = decltype(last)::value;
         Regs r = next;
-        if(tile + Pl::TT < g1) fetch(tile + Pl::TT);
+        if constexpr(!LAST) {
+            fetch(tile + Pl::TT);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         const int64_t first = start(tile);
         const int shift = (int)min(tile + at.tl * LT - first, (int64_t)LT);
-        const bool whole = tile + Pl::TT <= g1;
+        const bool whole = !LAST || tile + Pl::TT <= g1;
         float s[LT][V], q[LT][V], A[V], H[V];
 #pragma unroll
         for(int e = 0; e < LT; ++e)
@@ -371,7 +379,10 @@ __global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
                 if(p.dx) store<V>(p.dx + row * p.lddx + at.c, dx, at.skip, p.flags & PK_ACCUM2);
             }
         }
-    }
+    };
+    int64_t tile = g0;
+    for(; tile + Pl::TT < g1; tile += Pl::TT) walk(tile, std::false_type());
+    walk(tile, std::true_type());
     if(BWD && p.dh0 && at.tl == 0 && g1 == p.T)
         store<V>(p.dh0 + at.b * p.C + at.c, carry, at.skip, p.flags & PK_ACCUM3);
 }
