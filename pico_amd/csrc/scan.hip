@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
 
 // BIG: x and h, which only this pass of the backward reads, leave the caches to f and
 // dh and to the next kernel (1x65536x512 backward 195 -> 167 us, 4x8192x1024 214 ->
-// 200; tensors that fit the last-level cache are better read from there: 8x1024x768
+// 200; now 164 and 194; tensors that fit the last-level cache are better read from there: 8x1024x768
 // 30 against 37, 32x2048x256 68 against 75)
 template <int V, int CL, bool BWD, bool BIG>
 __global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
@@ -449,25 +449,29 @@ struct Plan {
 
 Plan plan_of(int64_t B, int64_t T, int64_t C) {
     const int V = C < 4 ? 1 : 4;
-    if(T <= 8) return {0, 1, T};
     auto groups = [&](int lanes) { return B * ((C + V * lanes - 1) / (V * lanes)); };
     auto steps = [](int lanes) { return (int64_t)(kThreads / lanes * LT); };  // of a tile
+    // Token after token where there are few, and up to some tens of them where the
+    // sequences are so many that tiles mostly empty fill the chip more than once:
+    // 64x8x768 11.6, tiles 14.7; 128x9x768 12.9, 23.4; 128x16x768 22.7, 23.6; 512x32x768
+    // 72.8, 90.7 (but 32x12x768 15.2, tiles 11.1; 128x24x768 34.6, 27.7; 512x64x768 176, 157)
+    if(T <= 8 || (T <= 16 && groups(16) >= 1024) || (T <= 40 && groups(16) >= 4096)) return {0, 1, T};
     // One chunk, which reads everything once, where it fills most of the chip, with
-    // the widest rows that do: 8x1024x768 8 lanes 50.5, 4 lanes 53.4, 2 chunks 59.2;
-    // 4x2000x768 4 lanes 55.8, 16 chunks 60.1; 16x512x512 8 lanes 32.9, 2 chunks 41.6
+    // the widest rows that do: 8x1024x768 8 lanes 46.6, 4 lanes 52.8, 2 chunks 59.1;
+    // 4x2000x768 4 lanes 53.5, 16 chunks 62.0; 16x512x512 8 lanes 29.9, 2 chunks 37.7
     for(const int lanes : {16, 8, 4})
         if(groups(lanes) >= 192) return {lanes, 1, T};
-    // ... and where it is a tile or two long: 8x64x768 9.3 (2 chunks of 32: a second
-    // launch), 1x300x2048 4 lanes 15.0, 3 chunks 18.8
+    // ... and where it is a tile or two long: 8x64x768 9.9 (8 lanes 10.1), 1x300x2048
+    // 4 lanes 14.4, 3 chunks 19.1
     for(const int lanes : {16, 8})
         if(T <= steps(lanes)) return {lanes, 1, T};
     if(T <= 2 * steps(4)) return {4, 1, T};
     // Chunks.  Few tiles in all: one to a chunk, narrow ones, so that the chunks to
-    // gather the state from are few (3x1001x333 4 lanes 23.8, 16 lanes 27.3, one chunk
-    // 29.6; 1x9000x20 24.0).  Else 512 workgroups: rows of 128 bytes (1x32768x256 8
-    // lanes 78.3, 16 lanes 106, 4 lanes 85.9; 1x4096x768 38.3, 42.0, 38.8), of 64 where
-    // few channels would leave chunks many (1x20000x64 41.2, 8 lanes 47.6), of 256
-    // beyond what the last-level cache holds (1x65536x512 323, 8 lanes 355)
+    // gather the state from are few (3x1001x333 4 lanes 24.3, 16 lanes 23.5, one chunk
+    // 28.2; 1x9000x20 23.4, 8 lanes 27.8).  Else 512 workgroups: rows of 128 bytes (1x32768x256 8
+    // lanes 80.5, 16 lanes 105, 4 lanes 87.5; 1x4096x768 34.9, 39.7, 39.2), of 64 where
+    // few channels would leave chunks many (1x20000x64 40.8, 8 lanes 52.0), of 256
+    // beyond what the last-level cache holds (1x65536x512 267, 8 lanes 292)
     const int64_t tiles = groups(8) * ((T + steps(8) - 1) / steps(8));
     const int lanes = tiles <= 384 || groups(8) < 4 ? 4 : tiles >= 8192 && groups(16) >= 8 ? 16 : 8;
     const int64_t want = tiles <= 384 ? T : (512 + groups(lanes) - 1) / groups(lanes);

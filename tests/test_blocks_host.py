@@ -150,7 +150,7 @@ def test_more_threads_than_a_launch_has(L):
         _refused(L, L.pk_layernorm_fwd_f32(R, C, 1e-5, PTR, PTR, None, PTR, None, None, None), "rows")
         _refused(L, L.pk_layernorm_bwd_f32(R, C, PTR, PTR, PTR, PTR, PTR, None, PTR, None, None, 0, None, 0, None),
                  "rows")
-    for B, T, C in (((1 << 31) - 1, 1, 3), (1 << 24, 9, 4), (1 << 28, 2, 64)):
+    for B, T, C in (((1 << 31) - 1, 1, 3), (1 << 24, 41, 4), (1 << 28, 2, 64)):
         _refused(L, L.pk_gated_scan_fwd_f32(B, T, C, PTR, 64, PTR, 64, None, PTR, PTR, 1 << 60, None), "channels")
     _refused(L, L.pk_route_topk_f32((1 << 25) + 1, 64, 1, PTR, 64, PTR, PTR, None), "2^25")
     _refused(L, L.pk_expert_gather_f32(1 << 26, 4, 2, 4, PTR, PTR, PTR, 8, PTR, 8, None), "2^25")

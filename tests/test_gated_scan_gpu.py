@@ -73,7 +73,9 @@ def _empty(*shape):
 SHAPES = [(1, 1, 1), (2, 1, 3), (64, 1, 768), (3, 2, 5), (1, 3, 64), (2, 7, 63), (5, 8, 100),
           (2, 9, 65), (1, 33, 257), (3, 64, 128), (2, 65, 16), (1, 127, 4), (4, 128, 12), (2, 200, 333),
           (8, 256, 96), (1, 257, 1), (2, 300, 130), (1, 1000, 48), (3, 1001, 33), (1, 2049, 64),
-          (1, 5000, 7), (1, 9000, 20), (70, 130, 20), (1, 16385, 4), (2, 4096, 36), (513, 20, 8)]
+          (1, 5000, 7), (1, 9000, 20), (70, 130, 20), (1, 16385, 4), (2, 4096, 36), (513, 20, 8),
+          # many short sequences: token after token
+          (1030, 16, 36), (1030, 17, 12), (4100, 40, 8), (4100, 41, 5)]
 
 
 @pytest.mark.parametrize("B,T,C", SHAPES)
