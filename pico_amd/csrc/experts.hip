@@ -392,9 +392,11 @@ __global__ __launch_bounds__(256) void expert_combine_bwd_kernel(
     if(lane == 0) dgates[slot] = (flags & PK_ACCUM2) ? dgates[slot] + dot : dot;
 }
 
-// rows to which a workgroup each is better than a wave (us, d 768: 32 rows gathered
-// 4.0 as waves, 16 combined 5.5)
-bool few(int64_t rows) { return rows <= 1024; }
+// rows to which a workgroup each is better than a wave (d 768, 2 choices, us as
+// workgroups and as waves: gather of 16 slots 2.4 and 2.6, 1024 2.8 and 3.0, 2048 3.6 and
+// 3.5, 8192 9.0 and 8.5; combine of 8 tokens 2.6 and 3.9, 1024 3.4 and 4.5, 2048 4.5 and
+// 6.1, 4096 9.7 and 9.9)
+constexpr int64_t kFewSlots = 1024, kFewTokens = 2048;
 
 bool vec4(int64_t d, std::initializer_list<std::pair<const void*, int64_t>> xs) {
     bool v = d % 4 == 0;
@@ -482,7 +484,7 @@ extern "C" int pk_expert_gather_f32(int64_t n, int64_t d, int64_t k, int64_t E, 
     if(n == 0) return PK_OK;
     if(!offsets || !order || !x || !out || ldx < d || ldo < d)
         return pk::fail("pk_expert_gather_f32: NULL pointer or row stride < d");
-    with_rows(vec4(d, {{x, ldx}, {out, ldo}}), few(n), [&](auto v, auto l) {
+    with_rows(vec4(d, {{x, ldx}, {out, ldo}}), n <= kFewSlots, [&](auto v, auto l) {
         constexpr int V = decltype(v)::value, L = decltype(l)::value;
         expert_gather_kernel<V, L><<<(unsigned)((n * L + 255) / 256), 256, 0, pk::as_stream(stream)>>>(
             (int)n, d, (int)k, offsets + E, order, x, ldx, out, ldo);
@@ -498,7 +500,7 @@ extern "C" int pk_expert_combine_f32(int64_t R, int64_t d, int64_t k, const int3
     if(R == 0) return PK_OK;
     if(!place || !ys || !out || ldy < d || ldo < d || (c && ldc < d))
         return pk::fail("pk_expert_combine_f32: NULL pointer or row stride < d");
-    with_rows(vec4(d, {{ys, ldy}, {c, ldc}, {out, ldo}}), few(R), [&](auto v, auto l) {
+    with_rows(vec4(d, {{ys, ldy}, {c, ldc}, {out, ldo}}), R <= kFewTokens, [&](auto v, auto l) {
         constexpr int V = decltype(v)::value, L = decltype(l)::value;
         expert_combine_kernel<V, L><<<(unsigned)((R * L + 255) / 256), 256, 0, pk::as_stream(stream)>>>(
             (int)R, (int)(R * k), d, (int)k, place, gates, ys, ldy, c, ldc, out, ldo);

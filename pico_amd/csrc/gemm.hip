@@ -1532,8 +1532,10 @@ void expert_shapes(int prec, F f) {
 // the experts have many rows those last tiles often make a round of their own (1088
 // tiles on 256 CUs take 5 rounds, the 1024 of as many rows in one 4): then 256x256 tiles
 // take the whole 256 rows, without bounds where N and k allow, and a second launch of
-// smaller tiles the rest.  16384 rows of 8 experts, us: see expert_rows in
-// gemm_experts.hip.
+// smaller tiles the rest.  One launch and two, us: 16384 rows of 8 experts [768,
+// 4096] 617 and 528, [768, 2048] 337 and 263, in bf16 104 and 94; 4096 rows of 4 experts
+// [768, 4096] 177 and 146; with fewer rows an expert the same (4096 of 8 [768, 2048] 102
+// and 101, 2048 of 8 [768, 4096] 99 and 100), so one.
 ExpertShape expert_rows_shape(int prec, double groups, double m, int64_t N, double k, ExpertShape* rest) {
     ExpertShape best = {kTile128, 128, 128, 0.0};
     double c = -1.0;
