@@ -2,6 +2,7 @@
 // of the fp32 (gemm_split.h), bf16 and split-bf16 (gemm_narrow.hip) tiles over
 // groups of rows whose sizes only the device knows.
 #include <algorithm>
+#include <type_traits>
 
 #include "gemm_common.h"
 
@@ -32,16 +33,17 @@ int run(bool ta, bool tb, const ExpertParams& ep, int64_t grid, TileKind kind, b
 
 // ------------------------------------------------ a few rows to an expert
 // Y = X.W_e where every expert's weights are read for a handful of rows (tokens being
-// generated): bound by W's bytes.  A workgroup takes 4 rows of an expert and 64
-// columns; its lanes lie 16 along the columns, the others along k, 4 k at a time, so W
-// is read in runs of 256 bytes with two steps in flight, and each value is used 4
-// times in fp32 multiply-adds, which take less time than its bytes.  (bf16: operands
+// generated): bound by W's bytes.  A workgroup takes 4 rows of an expert and 64 or
+// 32 columns; its lanes lie 16 or 8 along the columns, the others along k, 4 k at a
+// time, so W is read in runs of 256 or 128 bytes with two steps in flight, and each value is
+// used 4 times in fp32 multiply-adds, which take less time than its bytes.  (bf16: operands
 // rounded first, products exact.)  The partial sums meet across the lanes, then the
 // waves, in a fixed order.
 constexpr int kThinWaves = 8, kThinRows = 4;
 
+template <int CL>
 struct ThinTile {
-    static constexpr int BM = kThinRows, BN = 64;
+    static constexpr int BM = kThinRows, BN = 4 * CL;
 };
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
@@ -55,10 +57,10 @@ __device__ __forceinline__ f32x4 rounded(f32x4 x) {
     return x;
 }
 
-template <bool BF16>
+template <bool BF16, int CL>
 __global__ __launch_bounds__(64 * kThinWaves) void experts_thin(ExpertParams p) {
-    using T = ThinTile;
-    constexpr int RM = kThinRows, CL = 16, KL = 64 / CL, STEP = 4 * KL * kThinWaves;  // k of a workgroup's step
+    using T = ThinTile<CL>;
+    constexpr int RM = kThinRows, KL = 64 / CL, STEP = 4 * KL * kThinWaves;  // k of a workgroup's step
     __shared__ float part[kThinWaves][RM][4 * CL];
     const TileJob j = tile_job<T>(p);
     if(j.skip) return;
@@ -72,47 +74,63 @@ __global__ __launch_bounds__(64 * kThinWaves) void experts_thin(ExpertParams p) 
     f32x4 acc[RM];
 #pragma unroll
     for(int r = 0; r < RM; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
-    f32x4 wv[4], xv[RM];
-    auto load = [&](int64_t k) {
-#pragma unroll
-        for(int i = 0; i < 4; ++i) wv[i] = *reinterpret_cast<const f32x4u*>(wp + (k + i) * p.ldb);
-#pragma unroll
-        for(int r = 0; r < RM; ++r) xv[r] = *reinterpret_cast<const f32x4u*>(xp[r] + k);
+    struct Step {
+        f32x4 w[4], x[RM];
     };
-    auto add = [&](const f32x4 (&a)[4], const f32x4 (&x)[RM]) {
+    auto load = [&](Step& s, int64_t k) {
+#pragma unroll
+        for(int i = 0; i < 4; ++i) s.w[i] = *reinterpret_cast<const f32x4u*>(wp + (k + i) * p.ldb);
+#pragma unroll
+        for(int r = 0; r < RM; ++r) s.x[r] = *reinterpret_cast<const f32x4u*>(xp[r] + k);
+        __builtin_amdgcn_sched_barrier(0);  // (not to be put off until they are needed)
+    };
+    auto add = [&](const Step& s) {
+        f32x4 x[RM];
+#pragma unroll
+        for(int r = 0; r < RM; ++r) x[r] = rounded<BF16>(s.x[r]);
 #pragma unroll
         for(int i = 0; i < 4; ++i) {
-            const f32x4 b = rounded<BF16>(a[i]);
+            const f32x4 b = rounded<BF16>(s.w[i]);
 #pragma unroll
             for(int r = 0; r < RM; ++r)
 #pragma unroll
                 for(int c = 0; c < 4; ++c) acc[r][c] = fmaf(x[r][i], b[c], acc[r][c]);
         }
     };
+    // the steps that K fills, two in flight, without a branch around a load: the waits
+    // would be for all of them
     int64_t k = 4 * (w * KL + lane / CL);
-    if(k + 4 <= p.K) load(k);
-    for(; k + 4 <= p.K; k += STEP) {
-        f32x4 a[4], x[RM];
-#pragma unroll
-        for(int i = 0; i < 4; ++i) a[i] = wv[i];
-#pragma unroll
-        for(int r = 0; r < RM; ++r) x[r] = rounded<BF16>(xv[r]);
-        if(k + STEP + 4 <= p.K) load(k + STEP);
-        add(a, x);
+    const int full = (int)(p.K / STEP);
+    Step a, b;
+    int left = full;
+    if(left >= 2) {
+        load(a, k);
+        load(b, k + STEP);
+        for(; left >= 4; left -= 2, k += 2 * STEP) {
+            add(a);
+            load(a, k + 2 * STEP);
+            add(b);
+            load(b, k + 3 * STEP);
+        }
+        add(a);
+        if(left == 3) load(a, k + 2 * STEP);
+        add(b);
+        if(left == 3) add(a);
+    } else if(left == 1) {
+        load(a, k);
+        add(a);
     }
+    k = (int64_t)full * STEP + 4 * (w * KL + lane / CL);
     if(k < p.K) {
-        // the last one to three k
-        f32x4 a[4], x[RM];
+        // a lane's last four k or fewer
 #pragma unroll
         for(int i = 0; i < 4; ++i) {
             const bool on = k + i < p.K;
-            a[i] = on ? *reinterpret_cast<const f32x4u*>(wp + (k + i) * p.ldb) : f32x4{0.f, 0.f, 0.f, 0.f};
+            a.w[i] = on ? *reinterpret_cast<const f32x4u*>(wp + (k + i) * p.ldb) : f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for(int r = 0; r < RM; ++r) x[r][i] = on ? xp[r][k + i] : 0.0f;
+            for(int r = 0; r < RM; ++r) a.x[r][i] = on ? xp[r][k + i] : 0.0f;
         }
-#pragma unroll
-        for(int r = 0; r < RM; ++r) x[r] = rounded<BF16>(x[r]);
-        add(a, x);
+        add(a);
     }
 #pragma unroll
     for(int o = CL; o < 64; o <<= 1)
@@ -138,14 +156,17 @@ __global__ __launch_bounds__(64 * kThinWaves) void experts_thin(ExpertParams p) 
     }
 }
 
+double thin_tiles(double groups, double m) { return groups * std::max(1.0, m / kThinRows + 0.5); }
+
 // Microseconds: W once from memory, or once for every row tile from the caches, and a
-// start.  8 experts, rows each 1 / 4 / 8 / 16, us against those of matrix-core tiles:
-// [768, 4096] 15 / 22 / 28 / 40 against 27 / 29 / 28 / 28, [2048, 768] - / 13 / 14 / 22
-// against 37 (96 tiles, each all of K).  Workgroups of 8 or 16 rows read W less often
-// but are fewer and hold more: [768, 4096] with 4 rows each 24 and 31.
+// start.  8 experts, rows each 1 / 4 / 8 / 16 / 24, us against those of matrix-core tiles:
+// [768, 4096] 17 / 18 / 20 / 31 / 45 against 28 / 27 / 27 / 28 / 28 (in bf16 18 / 18 / 22 / 36 /
+// 53 against 23 / 20 / 22 / 20 / 21), [2048, 768] 12 / 13 / 13 / 20 / 27 against 37 (96
+// tiles, each all of K).  Workgroups of 8 or 16 rows read W less often but are fewer
+// and hold more: [768, 4096] with 4 rows each 24 and 31, when 4 took 22.
 double thin_us(double groups, double m, int64_t N, int64_t K) {
-    const double mb = (double)K * (double)N * 4e-6, tiles = groups * std::max(1.0, m / kThinRows + 0.5);
-    return 4.0 + mb * std::max(groups / 6.5, tiles / 11.0);
+    const double mb = (double)K * (double)N * 4e-6;
+    return 3.0 + mb * std::max(groups / 7.0, thin_tiles(groups, m) / 11.0);
 }
 
 // dW_e (+)= the sum of the S planes [S][E][K][N], in plane order
@@ -203,16 +224,24 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     const int64_t groups = E < n ? E : n;
     ExpertShape rest;
     const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K, &rest);
-    // (the estimates are of up to 32 rows to an expert)
-    const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 63) / 64;
+    // (the estimates are of up to 32 rows to an expert; 32 columns to a workgroup where 64
+    // would leave half of the chip idle: 8 experts [2048, 768] with a row each 8.9 us, of
+    // 64 columns 11.6, with 4 rows 15.0 and 13.6; 2 experts [4096, 768] 13.2, 18.9)
+    const int cl = thin_tiles((double)groups, (double)n / groups) * (double)((N + 63) / 64) < 144.0 ? 8 : 16;
+    const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 4 * cl - 1) / (4 * cl);
     if(!TB && N >= 4 && K > 0 && n <= 32 * groups && tiles_n <= kMaxTiles / tiles_m &&
        thin_us((double)groups, (double)n / groups, N, K) < s.us) {
         ep.tiles_m = (int)tiles_m;
         ep.tiles_n = (int)tiles_n;
         const unsigned grid = (unsigned)((tiles_m * tiles_n + 7) / 8 * 8);
         hipStream_t st = pk::as_stream(stream);
-        if(precision == 1) experts_thin<true><<<grid, 64 * kThinWaves, 0, st>>>(ep);
-        else experts_thin<false><<<grid, 64 * kThinWaves, 0, st>>>(ep);
+        auto launch = [&](auto cl) {
+            constexpr int CL = decltype(cl)::value;
+            if(precision == 1) experts_thin<true, CL><<<grid, 64 * kThinWaves, 0, st>>>(ep);
+            else experts_thin<false, CL><<<grid, 64 * kThinWaves, 0, st>>>(ep);
+        };
+        if(cl == 16) launch(std::integral_constant<int, 16>());
+        else launch(std::integral_constant<int, 8>());
         return pk::launch_status("pk_gemm_experts_f32");
     }
     // `most` row tiles at most
