@@ -427,12 +427,13 @@ bool cached(int64_t C) { return C >= 4 && C <= 16384; }
 
 // the workgroups of the backward, each of which leaves a partial sum: one on every
 // CU at most (8192x4096 67 us, two 75; of short rows two: 65536x128 25, one 32), and
-// one in all where a second launch would take longer than a second turn (16x768 6.4 us,
-// two launches 6.8; of four turns 32x512 6.9 against 6.2, of eight 64x128 8.4 against
-// 5.2)
+// one in all of few values, where the launch that is saved (3 us of the host's) counts
+// for more than the turns: in a graph 16x768 6.4 us, two launches 6.8, 32x512 6.9 and
+// 6.2, 64x128 8.4 and 5.8, 64x512 10.2 and 6.3; called one by one with the forward
+// 64x128 15.5 and 18.3
 int64_t parts_of(int64_t R, int64_t C) {
     const int64_t rows = !cached(C) ? 1 : C <= 768 ? 8 : C <= 2048 ? 4 : C <= 4096 ? 2 : 1;
-    if(cached(C) && R <= 2 * rows) return 1;
+    if(cached(C) && R * C <= 16384) return 1;
     const int64_t p = (R + rows - 1) / rows;
     const int64_t most = C <= 256 ? 512 : 256;
     return p < most ? p : most;
