@@ -685,7 +685,8 @@ int pk_gated_scan_bwd_f32(int64_t B, int64_t T, int64_t C, const float* f, int64
  *   precision: 0 fp32, 1 bf16, 2 three bf16 products, as in pk_gemm_add_f32 (no
  *   fp8).  PK_ACCUM accumulates.
  *   Row strides up to 2^21 (W [K, N], and dw's X and dY: 2^24).
- * Limits: E <= 1024, k <= 64, n <= 2^25 (plan: < 2^31, products: 2^30).  What experts, offsets, order
+ * Limits: E <= 1024, k <= 64, n <= 2^25 (plan: < 2^31; products: 2^30, and
+ * at most 2^21 tiles, of 64x64 to 256x256 as their sizes ask).  What experts, offsets, order
  * and place hold is checked on the device: values out of range reach no memory out
  * of bounds (rows of overlapping experts have no defined result). */
 int pk_route_topk_f32(int64_t R, int64_t E, int64_t k, const float* logits, int64_t ldz,

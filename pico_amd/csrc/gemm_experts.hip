@@ -11,8 +11,8 @@ namespace {
 using namespace pkg;
 
 constexpr int kMaxExperts = 1024;
-// workgroups of a launch, at up to 512 threads (fewer than 2^32 in all)
-constexpr int64_t kMaxTiles = (int64_t)1 << 22;
+// workgroups of a launch, at up to 1024 threads (fewer than 2^32 in all)
+constexpr int64_t kMaxTiles = (int64_t)1 << 21;
 
 int check(const char* who, int64_t n, int64_t M, int64_t N, int64_t E, const int32_t* offsets,
           int precision) {

@@ -158,5 +158,7 @@ def test_more_threads_than_a_launch_has(L):
     # 32768 rows of 1024 experts: more tiles than a launch has, streamed or not
     _refused(L, L.pk_gemm_experts_f32(b"N", 32768, 1 << 24, 4, 1024, PTR, PTR, 4, PTR, 1 << 24, 1 << 26, PTR, 1 << 24,
                                       0, 0, None), "too large")
+    _refused(L, L.pk_gemm_experts_f32(b"T", (1 << 21) * 64, 64, 64, 1, PTR, PTR, 64, PTR, 64, 0, PTR, 64, 0, 1, None),
+             "too large")
     _refused(L, L.pk_gemm_experts_dw_f32(32768, 1 << 12, 1 << 20, 1024, PTR, PTR, 1 << 12, PTR, 1 << 20, PTR, 1 << 20,
                                          1 << 32, 0, 0, None, 0, None), "too large")
