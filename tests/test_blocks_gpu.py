@@ -149,3 +149,23 @@ def test_training_steps_captured_and_replayed(P):
         P.lib.pico_optim_sgd_free(o)
         for t in d.values():
             P.free(t)
+
+
+def test_no_tokens(P):
+    """an empty batch: empty results, and gradients of zero"""
+    d, e, k = 8, 4, 2
+    w = P.param([e, d, d], np.ones((e, d, d), np.float32))
+    g, b = P.param([d], np.ones(d, np.float32)), P.param([d], np.ones(d, np.float32))
+    with P.arena():
+        x = P.layernorm(P.tensor([0, d], np.zeros((0, d))), g, b, EPS)
+        x = P.gated_scan(x, P.tensor([0, d], np.zeros((0, d))), None, 3)
+        gates, route = P.route_topk(P.tensor([0, e], np.zeros((0, e))), k)
+        y = P.expert_combine(P.expert_matmul(P.expert_gather(x, route), w, route), gates, route, x)
+        assert P.data(y).size == 0
+        experts, offsets = P.route_to_host(route, 0, k, e)
+        assert experts.size == 0 and not offsets.any()
+        P.backward(y)
+        for t in (w, g, b):
+            assert not P.grad_value(t).any()
+    for t in (w, g, b):
+        P.free(t)

@@ -207,6 +207,16 @@ def test_token_by_token_is_the_whole_sequence(dev, B, T, C):
     _close(got, want["h"], tol["h"], "parts")
 
 
+@pytest.mark.parametrize("B,C", [(1, 1), (64, 768), (3, 41)])
+def test_state_in_place(dev, B, C):
+    """one token at a time, the new state over the old one"""
+    f, x, state, _ = _data(B, 1, C, 4)
+    want = _empty(B, C)
+    K.gated_scan_fwd(B, f, x, want, h0=state)
+    K.gated_scan_fwd(B, f, x, state, h0=state)
+    assert torch.equal(state, want)
+
+
 @pytest.mark.parametrize("T", [9, 500, 3000])
 def test_closed_and_open_gates(dev, T):
     """f = -inf starts anew at a token, f = +inf and large f hold the state, the type's
