@@ -57,37 +57,52 @@ __device__ __forceinline__ f32x4 rounded(f32x4 x) {
     return x;
 }
 
+template <bool BF16>
+__device__ __forceinline__ float rounded(float x) {
+    return BF16 ? (float)(__bf16)x : x;
+}
+
 template <bool BF16, int CL>
 __global__ __launch_bounds__(64 * kThinWaves) void experts_thin(ExpertParams p) {
     using T = ThinTile<CL>;
     constexpr int RM = kThinRows, KL = 64 / CL, STEP = 4 * KL * kThinWaves;  // k of a workgroup's step
-    __shared__ float part[kThinWaves][RM][4 * CL];
+    __shared__ alignas(16) float part[kThinWaves][RM][4 * CL];
     const TileJob j = tile_job<T>(p);
     if(j.skip) return;
     const int w = threadIdx.x / 64, lane = threadIdx.x % 64, cl = lane % CL;
     const int rows = (int)min(p.M - j.row0, (int64_t)RM);
     const int64_t col = j.col0 + 4 * cl, at = min(col, p.N - 4);
     const float* const wp = j.B + at;
-    const float* xp[RM];
-#pragma unroll
-    for(int r = 0; r < RM; ++r) xp[r] = j.A + (j.row0 + min(r, rows - 1)) * p.lda;
+    const int kl = lane / CL * 4;
+    // a wave's x, [RM][4 KL], goes through LDS of its own: read by every lane it would
+    // take as many cycles of the loads' path as W (4 experts [512, 512] 5.5 us, so 5.1; 2
+    // [4096, 768] 13.2, 12.3; 64 [768, 768] of 8 rows 36, 32.5)
+    constexpr int XV = KL / 4;
+    __shared__ alignas(16) float xs[kThinWaves][RM][4 * KL];
+    const int xr = lane / 16, xk = lane % 16 * XV;
+    const float* const xp = j.A + (j.row0 + min(xr, rows - 1)) * p.lda + xk;
     f32x4 acc[RM];
 #pragma unroll
     for(int r = 0; r < RM; ++r) acc[r] = f32x4{0.f, 0.f, 0.f, 0.f};
     struct Step {
-        f32x4 w[4], x[RM];
+        f32x4 w[4];
+        float x[XV];
     };
     auto load = [&](Step& s, int64_t k) {
 #pragma unroll
-        for(int i = 0; i < 4; ++i) s.w[i] = *reinterpret_cast<const f32x4u*>(wp + (k + i) * p.ldb);
+        for(int v = 0; v < XV; ++v) s.x[v] = xp[k + v];
 #pragma unroll
-        for(int r = 0; r < RM; ++r) s.x[r] = *reinterpret_cast<const f32x4u*>(xp[r] + k);
+        for(int i = 0; i < 4; ++i) s.w[i] = *reinterpret_cast<const f32x4u*>(wp + (k + kl + i) * p.ldb);
         __builtin_amdgcn_sched_barrier(0);  // (not to be put off until they are needed)
     };
     auto add = [&](const Step& s) {
         f32x4 x[RM];
 #pragma unroll
-        for(int r = 0; r < RM; ++r) x[r] = rounded<BF16>(s.x[r]);
+        for(int v = 0; v < XV; ++v) xs[w][xr][xk + v] = rounded<BF16>(s.x[v]);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for(int r = 0; r < RM; ++r) x[r] = *reinterpret_cast<const f32x4*>(&xs[w][r][kl]);
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for(int i = 0; i < 4; ++i) {
             const f32x4 b = rounded<BF16>(s.w[i]);
@@ -99,7 +114,7 @@ __global__ __launch_bounds__(64 * kThinWaves) void experts_thin(ExpertParams p) 
     };
     // the steps that K fills, two in flight, without a branch around a load: the waits
     // would be for all of them
-    int64_t k = 4 * (w * KL + lane / CL);
+    int64_t k = 4 * w * KL;
     const int full = (int)(p.K / STEP);
     Step a, b;
     int left = full;
@@ -120,16 +135,15 @@ __global__ __launch_bounds__(64 * kThinWaves) void experts_thin(ExpertParams p) 
         load(a, k);
         add(a);
     }
-    k = (int64_t)full * STEP + 4 * (w * KL + lane / CL);
+    k = (int64_t)full * STEP + 4 * w * KL;
     if(k < p.K) {
-        // a lane's last four k or fewer
+        // a wave's last 4 KL k or fewer
 #pragma unroll
-        for(int i = 0; i < 4; ++i) {
-            const bool on = k + i < p.K;
-            a.w[i] = on ? *reinterpret_cast<const f32x4u*>(wp + (k + i) * p.ldb) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for(int v = 0; v < XV; ++v) a.x[v] = k + xk + v < p.K ? xp[k + v] : 0.0f;
 #pragma unroll
-            for(int r = 0; r < RM; ++r) a.x[r][i] = on ? xp[r][k + i] : 0.0f;
-        }
+        for(int i = 0; i < 4; ++i)
+            a.w[i] = k + kl + i < p.K ? *reinterpret_cast<const f32x4u*>(wp + (k + kl + i) * p.ldb)
+                                     : f32x4{0.f, 0.f, 0.f, 0.f};
         add(a);
     }
 #pragma unroll
@@ -160,13 +174,13 @@ double thin_tiles(double groups, double m) { return groups * std::max(1.0, m / k
 
 // Microseconds: W once from memory, or once for every row tile from the caches, and a
 // start.  8 experts, rows each 1 / 4 / 8 / 16 / 24, us against those of matrix-core tiles:
-// [768, 4096] 17 / 18 / 20 / 31 / 45 against 28 / 27 / 27 / 28 / 28 (in bf16 18 / 18 / 22 / 36 /
-// 53 against 23 / 20 / 22 / 20 / 21), [2048, 768] 12 / 13 / 13 / 20 / 27 against 37 (96
+// [768, 4096] 18 / 18 / 19 / 28 / 40 against 28 / 27 / 27 / 28 / 29 (in bf16 18 / 18 / 20 / 30 /
+// 45 against 23 / 20 / 22 / 21 / 21), [2048, 768] 12 / 12 / 12 / 17 / 22 against 37 (96
 // tiles, each all of K).  Workgroups of 8 or 16 rows read W less often but are fewer
 // and hold more: [768, 4096] with 4 rows each 24 and 31, when 4 took 22.
 double thin_us(double groups, double m, int64_t N, int64_t K) {
     const double mb = (double)K * (double)N * 4e-6;
-    return 3.0 + mb * std::max(groups / 7.0, thin_tiles(groups, m) / 11.0);
+    return 3.0 + mb * std::max(groups / 7.0, thin_tiles(groups, m) / 16.0);
 }
 
 // dW_e (+)= the sum of the S planes [S][E][K][N], in plane order
@@ -225,8 +239,8 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     ExpertShape rest;
     const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K, &rest);
     // (the estimates are of up to 32 rows to an expert; 32 columns to a workgroup where 64
-    // would leave half of the chip idle: 8 experts [2048, 768] with a row each 8.9 us, of
-    // 64 columns 11.6, with 4 rows 15.0 and 13.6; 2 experts [4096, 768] 13.2, 18.9)
+    // would leave half of the chip idle: 8 experts [2048, 768] with a row each 8.6 us, of
+    // 64 columns 10.6, with 4 rows 14.4 and 13.7; 2 experts [4096, 768] 12.3, 16.5)
     const int cl = thin_tiles((double)groups, (double)n / groups) * (double)((N + 63) / 64) < 144.0 ? 8 : 16;
     const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 4 * cl - 1) / (4 * cl);
     if(!TB && N >= 4 && K > 0 && n <= 32 * groups && tiles_n <= kMaxTiles / tiles_m &&
