@@ -23,10 +23,9 @@ def _ptr(t):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
 
-def _raw_stream(dev):
-    """the current stream's handle on device `dev` (what torch.cuda.current_stream()
-    wraps, at 0.1 us rather than 3)"""
-    return torch._C._cuda_getCurrentRawStream(dev)
+# the current stream's handle on a device (what torch.cuda.current_stream() wraps, at
+# 0.1 us rather than 3)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _stream():
@@ -683,64 +682,74 @@ def embed_bwd(ids, dout, dtable):
 
 
 # ------------------------------------- layer norm, gated recurrence, experts
+# These are also called for a token at a time, where the checks count: each tensor is
+# looked at once.
 ACCUM3 = 4
 PRECISIONS = {"fp32": 0, "bf16": 1, "bf16x3": 2}
+_F32, _I32 = torch.float32, torch.int32
+_device = torch._C._cuda_getDevice
 
 
-def _ready(dtype, *ts):
-    """each of `ts` (None aside) is a `dtype` tensor on the current device, where the
-    launchers run; returns the device's index"""
-    dev = torch._C._cuda_getDevice()
+def _refuse(t, dtype, dev):
+    if t.dtype is not dtype or not t.is_cuda:
+        raise TypeError(f"expected a {dtype} CUDA tensor, got {t.dtype} on {t.device}")
+    if t.get_device() != dev:
+        raise ValueError("a tensor lies on another device than the current one")
+    raise ValueError("expected a contiguous tensor")
+
+
+def _dense(dev, dtype, *ts):
+    """addresses of contiguous `dtype` tensors on the current device, where the launchers
+    run (None: NULL)"""
+    at = []
     for t in ts:
-        if t is not None and (t.dtype is not dtype or t.get_device() != dev):
-            if t.dtype is not dtype or not t.is_cuda:
-                raise TypeError(f"expected a {dtype} CUDA tensor, got {t.dtype} on {t.device}")
-            raise ValueError("a tensor lies on another device than the current one")
-    return dev
+        if t is None:
+            at.append(None)
+            continue
+        if t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+            _refuse(t, dtype, dev)
+        at.append(t.data_ptr())
+    return at
 
 
-def _at(t):
-    """a tensor's address for a launcher (None: NULL)"""
-    return None if t is None else t.data_ptr()
-
-
-def _rows(t, name):
-    """row stride of a 2-D tensor with unit columns and rows that do not overlap"""
-    if t.dim() == 2:
-        rows, cols = t.shape
-        if t.is_contiguous():
-            return max(1, cols)
-        if (cols <= 1 or t.stride(1) == 1) and (rows <= 1 or t.stride(0) >= cols):
-            return max(t.stride(0), cols)
-    raise ValueError(f"{name} must be a 2-D tensor with unit column stride and rows apart")
-
-
-def _dense(*ts):
-    for t in ts:
-        if t is not None and not t.is_contiguous():
-            raise ValueError("expected a contiguous tensor")
+def _rows(dev, t, name, shape=None):
+    """address and row stride of a 2-D float32 tensor with unit columns and rows that do
+    not overlap, of `shape` if given (None: NULL)"""
+    if t is None:
+        return None, shape[1]
+    if t.dtype is not _F32 or t.get_device() != dev:
+        _refuse(t, _F32, dev)
+    size = t.shape
+    if len(size) != 2 or (shape is not None and size != shape):
+        raise ValueError(f"{name} must be a matrix{'' if shape is None else f' {list(shape)}'}, "
+                         f"got {list(size)}")
+    rows, cols = size
+    ld, unit = t.stride()
+    if (unit != 1 and cols > 1) or (ld < cols and rows > 1):
+        raise ValueError(f"{name} must have unit column stride and rows apart")
+    return t.data_ptr(), ld if rows > 1 else max(1, cols)
 
 
 def _ws(ws, dev, size, *shape):
-    """a workspace of size(*shape) bytes (ws itself when given: the launcher says
-    when it is too small) and its size"""
+    """address and size of a workspace of size(*shape) bytes (of ws when given: the
+    launcher says when it is too small), and its tensor"""
     if ws is None:
         ws = torch.empty(max(1, size(*shape)), dtype=torch.uint8, device=dev)
     elif ws.get_device() != dev or not ws.is_contiguous():
         raise ValueError("a workspace must be contiguous and on the operands' device")
-    return ws, ws.nbytes
+    return ws.data_ptr(), ws.nbytes, ws
 
 
 def layernorm_fwd(x, g, b, y, mean, rstd, eps):
     """y = (x - m) r g + b over the rows of x [R, C]; b, mean, rstd may be None"""
-    dev = _ready(torch.float32, x, g, b, y, mean, rstd)
-    _dense(x, g, b, y, mean, rstd)
+    dev = _device()
+    at = _dense(dev, _F32, x, g, b, y, mean, rstd)
     R, C = x.shape
     if g.numel() != C or (b is not None and b.numel() != C) or y.shape != x.shape or \
-            any(t is not None and t.numel() != R for t in (mean, rstd)):
+            (mean is not None and mean.numel() != R) or (rstd is not None and rstd.numel() != R):
         raise ValueError("layernorm_fwd shape mismatch")
-    check("pk_layernorm_fwd_f32", hip_lib().pk_layernorm_fwd_f32(
-        R, C, eps, _at(x), _at(g), _at(b), _at(y), _at(mean), _at(rstd), _raw_stream(dev)))
+    check("pk_layernorm_fwd_f32",
+          hip_lib().pk_layernorm_fwd_f32(R, C, eps, *at, _raw_stream(dev)))
     return y
 
 
@@ -751,86 +760,90 @@ def layernorm_bwd_workspace(R, C):
 def layernorm_bwd(x, g, mean, rstd, dy, dx, dg, db, ws=None, dx_in=None, accum_dg=False,
                   accum_db=False):
     """gradients of layernorm_fwd (a None one is skipped); dx_in is added to dx"""
-    dev = _ready(torch.float32, x, g, mean, rstd, dy, dx, dg, db, dx_in)
-    _dense(x, g, mean, rstd, dy, dx, dg, db, dx_in)
-    R, C = x.shape
-    if g.numel() != C or any(t is not None and t.shape != x.shape for t in (dy, dx, dx_in)) or \
-            any(t is not None and t.numel() != C for t in (dg, db)) or \
-            mean.numel() != R or rstd.numel() != R:
+    dev = _device()
+    at = _dense(dev, _F32, x, g, mean, rstd, dy, dx_in, dx, dg, db)
+    size = x.shape
+    R, C = size
+    if g.numel() != C or mean.numel() != R or rstd.numel() != R or dy.shape != size or \
+            (dx is not None and dx.shape != size) or (dx_in is not None and dx_in.shape != size) or \
+            (dg is not None and dg.numel() != C) or (db is not None and db.numel() != C):
         raise ValueError("layernorm_bwd shape mismatch")
-    ws, wsb = _ws(ws, dev, layernorm_bwd_workspace, R, C)
+    wp, wb, ws = _ws(ws, dev, layernorm_bwd_workspace, R, C)
     flags = (ACCUM2 if accum_dg else 0) | (ACCUM3 if accum_db else 0)
-    check("pk_layernorm_bwd_f32", hip_lib().pk_layernorm_bwd_f32(
-        R, C, _at(x), _at(g), _at(mean), _at(rstd), _at(dy), _at(dx_in), _at(dx), _at(dg),
-        _at(db), flags, _at(ws), wsb, _raw_stream(dev)))
+    check("pk_layernorm_bwd_f32",
+          hip_lib().pk_layernorm_bwd_f32(R, C, *at, flags, wp, wb, _raw_stream(dev)))
 
 
 def gated_scan_workspace(B, T, C):
     return int(hip_lib().pk_gated_scan_workspace(B, T, C))
 
 
-def _scan_layout(B, f, x, h0, *rows):
-    """(T, C) of [B*T, C] matrices"""
-    N, C = x.shape
-    if B < 1 or N % B or f.shape != x.shape or any(t is not None and t.shape != x.shape for t in rows):
-        raise ValueError("gated_scan: f, x and h must be [B*T, C]")
-    if h0 is not None and tuple(h0.shape) != (B, C):
-        raise ValueError("gated_scan: h0 must be [B, C]")
-    return N // B, C
-
-
 def gated_scan_fwd(B, f, x, h, h0=None, ws=None):
-    """h_t = s_t h_{t-1} + (1 - s_t) x_t, s = sigmoid(f), over B sequences"""
-    dev = _ready(torch.float32, f, x, h, h0)
-    _dense(h, h0)
-    T, C = _scan_layout(B, f, x, h0, h)
-    ws, wsb = _ws(ws, dev, gated_scan_workspace, B, T, C)
+    """h_t = s_t h_{t-1} + (1 - s_t) x_t, s = sigmoid(f), over B sequences of f, x, h
+    [B*T, C]"""
+    dev = _device()
+    hp, h0p = _dense(dev, _F32, h, h0)
+    size = x.shape
+    fp, ldf = _rows(dev, f, "f", size)
+    xp, ldx = _rows(dev, x, "x")
+    N, C = size
+    if B < 1 or N % B or h.shape != size or (h0 is not None and h0.shape != (B, C)):
+        raise ValueError("gated_scan: f, x and h must be [B*T, C], h0 [B, C]")
+    T = N // B
+    wp, wb, ws = _ws(ws, dev, gated_scan_workspace, B, T, C)
     check("pk_gated_scan_fwd_f32", hip_lib().pk_gated_scan_fwd_f32(
-        B, T, C, _at(f), _rows(f, "f"), _at(x), _rows(x, "x"), _at(h0), _at(h), _at(ws),
-        wsb, _raw_stream(dev)))
+        B, T, C, fp, ldf, xp, ldx, h0p, hp, wp, wb, _raw_stream(dev)))
     return h
 
 
 def gated_scan_bwd(B, f, x, h, dh, df, dx, h0=None, dh0=None, ws=None, accum_df=False,
                    accum_dx=False, accum_dh0=False):
     """gradients of gated_scan_fwd (a None one is skipped)"""
-    dev = _ready(torch.float32, f, x, h, dh, df, dx, h0, dh0)
-    _dense(h, dh, h0, dh0)
-    T, C = _scan_layout(B, f, x, h0, h, dh, df, dx)
-    if dh0 is not None and tuple(dh0.shape) != (B, C):
-        raise ValueError("gated_scan: dh0 must be [B, C]")
-    ws, wsb = _ws(ws, dev, gated_scan_workspace, B, T, C)
+    dev = _device()
+    hp, dhp, h0p, dh0p = _dense(dev, _F32, h, dh, h0, dh0)
+    size = x.shape
+    fp, ldf = _rows(dev, f, "f", size)
+    xp, ldx = _rows(dev, x, "x")
+    dfp, lddf = _rows(dev, df, "df", size)
+    dxp, lddx = _rows(dev, dx, "dx", size)
+    N, C = size
+    if B < 1 or N % B or h.shape != size or dh.shape != size or \
+            (h0 is not None and h0.shape != (B, C)) or (dh0 is not None and dh0.shape != (B, C)):
+        raise ValueError("gated_scan: f, x, h and their gradients must be [B*T, C], h0 and dh0 [B, C]")
+    T = N // B
+    wp, wb, ws = _ws(ws, dev, gated_scan_workspace, B, T, C)
     flags = (ACCUM if accum_df else 0) | (ACCUM2 if accum_dx else 0) | (ACCUM3 if accum_dh0 else 0)
     check("pk_gated_scan_bwd_f32", hip_lib().pk_gated_scan_bwd_f32(
-        B, T, C, _at(f), _rows(f, "f"), _at(x), _rows(x, "x"), _at(h0), _at(h), _at(dh),
-        _at(df), C if df is None else _rows(df, "df"), _at(dx),
-        C if dx is None else _rows(dx, "dx"), _at(dh0), flags, _at(ws), wsb, _raw_stream(dev)))
+        B, T, C, fp, ldf, xp, ldx, h0p, hp, dhp, dfp, lddf, dxp, lddx, dh0p, flags, wp, wb,
+        _raw_stream(dev)))
 
 
 def route_topk(logits, experts, gates):
     """experts [R, k] int32 and gates [R, k]: the k largest logits of each token
     and the softmax over them"""
-    dev = _ready(torch.float32, logits, gates)
-    _ready(torch.int32, experts)
-    _dense(experts, gates)
-    if experts.dim() != 2 or gates.shape != experts.shape or experts.shape[0] != logits.shape[0]:
+    dev = _device()
+    zp, ldz = _rows(dev, logits, "logits")
+    ep, = _dense(dev, _I32, experts)
+    gp, = _dense(dev, _F32, gates)
+    R, E = logits.shape
+    size = experts.shape
+    if len(size) != 2 or gates.shape != size or size[0] != R:
         raise ValueError("route_topk: experts and gates must be [R, k]")
     check("pk_route_topk_f32", hip_lib().pk_route_topk_f32(
-        logits.shape[0], logits.shape[1], experts.shape[1], _at(logits),
-        _rows(logits, "logits"), _at(experts), _at(gates), _raw_stream(dev)))
+        R, E, size[1], zp, ldz, ep, gp, _raw_stream(dev)))
 
 
 def route_topk_bwd(experts, gates, dgates, dlogits, accum=False):
-    dev = _ready(torch.float32, gates, dgates, dlogits)
-    _ready(torch.int32, experts)
-    _dense(experts, gates, dgates)
-    if gates.shape != experts.shape or dgates.shape != experts.shape or \
-            experts.shape[0] != dlogits.shape[0]:
+    dev = _device()
+    dp, ldd = _rows(dev, dlogits, "dlogits")
+    ep, = _dense(dev, _I32, experts)
+    gp, dgp = _dense(dev, _F32, gates, dgates)
+    R, E = dlogits.shape
+    size = experts.shape
+    if len(size) != 2 or gates.shape != size or dgates.shape != size or size[0] != R:
         raise ValueError("route_topk_bwd: experts, gates and dgates must be [R, k]")
     check("pk_route_topk_bwd_f32", hip_lib().pk_route_topk_bwd_f32(
-        dlogits.shape[0], dlogits.shape[1], experts.shape[1], _at(experts), _at(gates),
-        _at(dgates), _at(dlogits), _rows(dlogits, "dlogits"), ACCUM if accum else 0,
-        _raw_stream(dev)))
+        R, E, size[1], ep, gp, dgp, dp, ldd, ACCUM if accum else 0, _raw_stream(dev)))
     return dlogits
 
 
@@ -841,101 +854,103 @@ def expert_plan_workspace(n, E):
 def expert_plan(experts, offsets, order, place, ws=None):
     """the slots of experts [R, k] in expert order: offsets [E + 1], order and
     place [R*k], all int32"""
-    dev = _ready(torch.int32, experts, offsets, order, place)
-    _dense(experts, offsets, order, place)
+    dev = _device()
+    at = _dense(dev, _I32, experts, offsets, order, place)
     n, E = experts.numel(), offsets.numel() - 1
     if order.numel() != n or place.numel() != n or E < 1:
         raise ValueError("expert_plan: order and place must hold a value a slot, offsets E + 1")
-    ws, wsb = _ws(ws, dev, expert_plan_workspace, n, E)
-    check("pk_expert_plan", hip_lib().pk_expert_plan(
-        n, E, _at(experts), _at(offsets), _at(order), _at(place), _at(ws), wsb, _raw_stream(dev)))
-
-
-def _expert_rows(n, d, *ts):
-    for t in ts:
-        if t is not None and tuple(t.shape) != (n, d):
-            raise ValueError(f"expected a [{n}, {d}] matrix, got {tuple(t.shape)}")
+    wp, wb, ws = _ws(ws, dev, expert_plan_workspace, n, E)
+    check("pk_expert_plan", hip_lib().pk_expert_plan(n, E, *at, wp, wb, _raw_stream(dev)))
 
 
 def expert_gather(x, k, offsets, order, out):
     """out[r] = x[order[r] // k]; zero rows behind the last expert's"""
-    dev = _ready(torch.float32, x, out)
-    _ready(torch.int32, offsets, order)
-    _dense(offsets, order)
-    n, d = x.shape[0] * k, x.shape[1]
-    _expert_rows(n, d, out)
-    if order.numel() != n or offsets.numel() < 2:
+    dev = _device()
+    fp, op = _dense(dev, _I32, offsets, order)
+    xp, ldx = _rows(dev, x, "x")
+    R, d = x.shape
+    n = R * k
+    yp, ldo = _rows(dev, out, "out", (n, d))
+    E = offsets.numel() - 1
+    if order.numel() != n or E < 1:
         raise ValueError("expert_gather: order must hold a value a slot, offsets E + 1")
     check("pk_expert_gather_f32", hip_lib().pk_expert_gather_f32(
-        n, d, k, offsets.numel() - 1, _at(offsets), _at(order), _at(x), _rows(x, "x"),
-        _at(out), _rows(out, "out"), _raw_stream(dev)))
+        n, d, k, E, fp, op, xp, ldx, yp, ldo, _raw_stream(dev)))
     return out
 
 
 def expert_combine(place, gates, ys, out, c=None):
     """out[t] = c[t] + sum_j gates[t, j] ys[place[t, j]] (gates None: 1)"""
-    dev = _ready(torch.float32, gates, ys, out, c)
-    _ready(torch.int32, place)
-    _dense(place, gates)
-    R, d = out.shape
+    dev = _device()
+    pp, = _dense(dev, _I32, place)
+    gp, = _dense(dev, _F32, gates)
+    op, ldo = _rows(dev, out, "out")
+    size = out.shape
+    R, d = size
     n = place.numel()
+    yp, ldy = _rows(dev, ys, "ys", (n, d))
+    cp, ldc = _rows(dev, c, "c", size)
     if R == 0:
         return out
     if n % R or (gates is not None and gates.numel() != n):
         raise ValueError("expert_combine: place and gates must hold k values a token")
-    _expert_rows(n, d, ys)
-    _expert_rows(R, d, c)
     check("pk_expert_combine_f32", hip_lib().pk_expert_combine_f32(
-        R, d, n // R, _at(place), _at(gates), _at(ys), _rows(ys, "ys"), _at(c),
-        d if c is None else _rows(c, "c"), _at(out), _rows(out, "out"), _raw_stream(dev)))
+        R, d, n // R, pp, gp, yp, ldy, cp, ldc, op, ldo, _raw_stream(dev)))
     return out
 
 
 def expert_combine_bwd(offsets, order, gates, ys, dout, dys, dgates, accum_dys=False,
                        accum_dgates=False):
-    dev = _ready(torch.float32, gates, ys, dout, dys, dgates)
-    _ready(torch.int32, offsets, order)
-    _dense(offsets, order, gates, dgates)
+    dev = _device()
+    fp, op = _dense(dev, _I32, offsets, order)
+    gp, dgp = _dense(dev, _F32, gates, dgates)
+    up, ldo = _rows(dev, dout, "dout")
     R, d = dout.shape
-    n = order.numel()
+    n, E = order.numel(), offsets.numel() - 1
+    yp, ldy = _rows(dev, ys, "ys", (n, d))
+    dp, ldd = _rows(dev, dys, "dys", (n, d))
     if R == 0:
         return
-    if n % R or gates.numel() != n or (dgates is not None and dgates.numel() != n) or \
-            offsets.numel() < 2:
+    if n % R or gates.numel() != n or (dgates is not None and dgates.numel() != n) or E < 1:
         raise ValueError("expert_combine_bwd: order and gates must hold k values a token")
-    _expert_rows(n, d, ys, dys)
     flags = (ACCUM if accum_dys else 0) | (ACCUM2 if accum_dgates else 0)
     check("pk_expert_combine_bwd_f32", hip_lib().pk_expert_combine_bwd_f32(
-        R, d, n // R, offsets.numel() - 1, _at(offsets), _at(order), _at(gates), _at(ys),
-        d if ys is None else _rows(ys, "ys"), _at(dout), _rows(dout, "dout"), _at(dys),
-        d if dys is None else _rows(dys, "dys"), _at(dgates), flags, _raw_stream(dev)))
+        R, d, n // R, E, fp, op, gp, yp, ldy, up, ldo, dp, ldd, dgp, flags, _raw_stream(dev)))
 
 
-def _expert_stack(w, name):
-    """(row stride, expert stride) of w [E, rows, cols] with unit columns"""
-    if w.dim() != 3 or (w.shape[2] > 1 and w.stride(2) != 1) or \
-            (w.shape[1] > 1 and w.stride(1) < w.shape[2]):
-        raise ValueError(f"{name} must be [E, rows, cols] with unit column stride")
-    return max(w.stride(1), w.shape[2]), w.stride(0)
+def _stack(dev, t, name):
+    """address, row stride and expert stride of t [E, rows, cols] with unit columns"""
+    if t.dtype is not _F32 or t.get_device() != dev:
+        _refuse(t, _F32, dev)
+    size = t.shape
+    if len(size) != 3:
+        raise ValueError(f"{name} must be [E, rows, cols], got {list(size)}")
+    se, ld, unit = t.stride()
+    if (unit != 1 and size[2] > 1) or (ld < size[2] and size[1] > 1):
+        raise ValueError(f"{name} must have unit column stride and rows apart")
+    return t.data_ptr(), ld if size[1] > 1 else max(1, size[2]), se
 
 
 def gemm_experts(tb, x, w, offsets, y, precision="fp32", accum=False):
     """y[r] = x[r] @ op(w[e]) for every expert's rows r (op = transpose for 'T')"""
-    dev = _ready(torch.float32, x, w, y)
-    _ready(torch.int32, offsets)
-    _dense(offsets)
-    if tb not in ("N", "T"):
+    dev = _device()
+    fp, = _dense(dev, _I32, offsets)
+    wp, ldw, sw = _stack(dev, w, "w")
+    if tb == "N":
+        E, K, N = w.shape
+    elif tb == "T":
+        E, N, K = w.shape
+    else:
         raise ValueError(f"gemm_experts: the transpose flag must be 'N' or 'T' (got {tb!r})")
-    ldw, sw = _expert_stack(w, "w")
-    E, K, N = w.shape if tb == "N" else (w.shape[0], w.shape[2], w.shape[1])
+    xp, ldx = _rows(dev, x, "x")
     n = x.shape[0]
+    yp, ldy = _rows(dev, y, "y", (n, N))
     if offsets.numel() != E + 1 or x.shape[1] != K:
         raise ValueError(f"gemm_experts: x {tuple(x.shape)}, w {tuple(w.shape)} ({tb}) and "
                          f"{offsets.numel()} offsets do not fit")
-    _expert_rows(n, N, y)
     check("pk_gemm_experts_f32", hip_lib().pk_gemm_experts_f32(
-        tb.encode(), n, N, K, E, _at(offsets), _at(x), _rows(x, "x"), _at(w), ldw, sw,
-        _at(y), _rows(y, "y"), ACCUM if accum else 0, PRECISIONS[precision], _raw_stream(dev)))
+        tb.encode(), n, N, K, E, fp, xp, ldx, wp, ldw, sw, yp, ldy, ACCUM if accum else 0,
+        PRECISIONS[precision], _raw_stream(dev)))
     return y
 
 
@@ -945,20 +960,19 @@ def gemm_experts_dw_workspace(n, K, N, E):
 
 def gemm_experts_dw(x, dy, offsets, dw, precision="fp32", accum=False, ws=None):
     """dw[e] = x_e^T @ dy_e over every expert's rows"""
-    dev = _ready(torch.float32, x, dy, dw)
-    _ready(torch.int32, offsets)
-    _dense(offsets)
-    ldw, sw = _expert_stack(dw, "dw")
+    dev = _device()
+    fp, = _dense(dev, _I32, offsets)
+    wp, ldw, sw = _stack(dev, dw, "dw")
     E, K, N = dw.shape
     n = x.shape[0]
+    xp, ldx = _rows(dev, x, "x", (n, K))
+    yp, ldy = _rows(dev, dy, "dy", (n, N))
     if offsets.numel() != E + 1:
         raise ValueError("gemm_experts_dw: offsets must hold E + 1 values")
-    _expert_rows(n, K, x)
-    _expert_rows(n, N, dy)
-    ws, wsb = _ws(ws, dev, gemm_experts_dw_workspace, n, K, N, E)
+    sp, sb, ws = _ws(ws, dev, gemm_experts_dw_workspace, n, K, N, E)
     check("pk_gemm_experts_dw_f32", hip_lib().pk_gemm_experts_dw_f32(
-        n, K, N, E, _at(offsets), _at(x), _rows(x, "x"), _at(dy), _rows(dy, "dy"),
-        _at(dw), ldw, sw, ACCUM if accum else 0, PRECISIONS[precision], _at(ws), wsb, _raw_stream(dev)))
+        n, K, N, E, fp, xp, ldx, yp, ldy, wp, ldw, sw, ACCUM if accum else 0,
+        PRECISIONS[precision], sp, sb, _raw_stream(dev)))
     return dw
 
 
