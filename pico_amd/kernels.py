@@ -20,7 +20,7 @@ UNARY_OPS = {"sqrt": 0, "sin": 1, "cos": 2, "tan": 3, "tanh": 4, "log": 5}
 
 
 def _ptr(t):
-    return None if t is None else ctypes.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 # the current stream's handle on a device (what torch.cuda.current_stream() wraps, at
@@ -29,7 +29,7 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _stream():
-    return ctypes.c_void_p(_raw_stream(torch.cuda.current_device()))
+    return _raw_stream(torch.cuda.current_device())
 
 
 def _f32(*ts):
