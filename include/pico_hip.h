@@ -610,7 +610,7 @@ int pk_embed_bwd_f32(int64_t n, int64_t d, int64_t vocab, const int32_t* ids, co
 /* In the three sections below outputs overlap neither inputs nor each other, except
  * where a call says that they may.
  * ---- layer norm (no reference counterpart) -------------------------------
- * over rows of x [R, C], contiguous: y = (x - m) * r * g + b with m = mean(x),
+ * over rows of x [R, C], contiguous, C <= 2^26: y = (x - m) * r * g + b with m = mean(x),
  * r = (mean((x - m)^2) + eps)^-1/2.  g [C]; b [C] or NULL (no bias).  mean and
  * rstd [R] receive m and r for the backward; either may be NULL.
  * backward, xh = (x - m) * r:

@@ -449,7 +449,8 @@ extern "C" int pk_layernorm_fwd_f32(int64_t R, int64_t C, float eps, const float
                                     const float* b, float* y, float* mean, float* rstd,
                                     pk_stream_t stream) {
     if(R < 0 || C < 1) return pk::fail("pk_layernorm_fwd_f32: need R >= 0 and C >= 1");
-    if(R > (int64_t)INT32_MAX) return pk::fail("pk_layernorm_fwd_f32: R above 2^31 - 1");
+    if(R > (int64_t)INT32_MAX || C > (int64_t)1 << 26)
+        return pk::fail("pk_layernorm_fwd_f32: R above 2^31 - 1 or C above 2^26");
     if(R == 0) return PK_OK;
     if(!x || !g || !y) return pk::fail("pk_layernorm_fwd_f32: NULL pointer");
     hipStream_t st = pk::as_stream(stream);
@@ -485,7 +486,8 @@ extern "C" int pk_layernorm_bwd_f32(int64_t R, int64_t C, const float* x, const 
                                     const float* dx_in, float* dx, float* dg, float* db, int flags,
                                     void* workspace, size_t workspace_bytes, pk_stream_t stream) {
     if(R < 0 || C < 1) return pk::fail("pk_layernorm_bwd_f32: need R >= 0 and C >= 1");
-    if(R > (int64_t)INT32_MAX) return pk::fail("pk_layernorm_bwd_f32: R above 2^31 - 1");
+    if(R > (int64_t)INT32_MAX || C > (int64_t)1 << 26)
+        return pk::fail("pk_layernorm_bwd_f32: R above 2^31 - 1 or C above 2^26");
     const bool sums = dg || db;
     if(R > 0) {
         if(!x || !g || !mean || !rstd || !dy)

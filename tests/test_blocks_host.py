@@ -146,6 +146,10 @@ def test_products(L):
 
 def test_more_threads_than_a_launch_has(L):
     """sizes whose launch would have 2^32 threads or more"""
+    for C in ((1 << 26) + 1, 1 << 40):
+        _refused(L, L.pk_layernorm_fwd_f32(1, C, 1e-5, PTR, PTR, None, PTR, None, None, None), "2^26")
+        _refused(L, L.pk_layernorm_bwd_f32(1, C, PTR, PTR, PTR, PTR, PTR, None, PTR, None, None, 0, None, 0, None),
+                 "2^26")
     for C, R in ((3, 1 << 26), (20000, 1 << 22)):
         _refused(L, L.pk_layernorm_fwd_f32(R, C, 1e-5, PTR, PTR, None, PTR, None, None, None), "rows")
         _refused(L, L.pk_layernorm_bwd_f32(R, C, PTR, PTR, PTR, PTR, PTR, None, PTR, None, None, 0, None, 0, None),
