@@ -151,6 +151,46 @@ def test_training_steps_captured_and_replayed(P):
             P.free(t)
 
 
+def test_capture_beside_a_live_eager_graph(P):
+    """a step captured while an eager graph of the same leaves, its backward done, is kept;
+    that graph's second backward between the replays"""
+    vals = _values(3)
+    p = {k: P.param(list(t.shape), t.numpy()) for k, t in vals.items()}
+    grads = lambda: {k: P.grad_value(t) for k, t in p.items()}
+    opt = P.lib.pico_optim_sgd_init(0.0)
+    for t in p.values():
+        P.lib.pico_optim_sgd_add(opt, t)
+    with P.arena() as a:
+        eager, _ = _block(P, p)
+        P.lib.pico_optim_sgd_zero_grad(opt)
+        P.lib.pico_backward(a, eager)
+        want = grads()
+        with P.arena() as b:
+            out, _ = _block(P, p)  # the arena's blocks
+            P.lib.pico_optim_sgd_zero_grad(opt)
+            P.lib.pico_backward(b, out)
+            P.reset(b)
+            assert P.lib.pico_graph_begin() == 0
+            out, _ = _block(P, p)
+            P.lib.pico_optim_sgd_zero_grad(opt)
+            P.lib.pico_backward(b, out)
+            graph = P.lib.pico_graph_end()
+            assert graph, P.lib.pico_gpu_last_error()
+            for _ in range(3):
+                assert P.lib.pico_graph_launch(graph) == 0
+                got = grads()
+                for k in SHAPES:
+                    assert np.array_equal(got[k], want[k]), k
+                P.lib.pico_optim_sgd_zero_grad(opt)
+                P.lib.pico_backward(a, eager)
+                assert np.isfinite(P.grad_value(p["w13"])).all()
+            P.lib.pico_graph_free(graph)
+    assert not P.lib.pico_gpu_last_error()
+    P.lib.pico_optim_sgd_free(opt)
+    for t in p.values():
+        P.free(t)
+
+
 def test_no_tokens(P):
     """an empty batch: empty results, and gradients of zero"""
     d, e, k = 8, 4, 2
