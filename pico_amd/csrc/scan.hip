@@ -162,16 +162,17 @@ __device__ __forceinline__ float step(float p, float s, float v) {
     return BWD ? s * (v + p) : fmaf(s, p, v);
 }
 
-// the composed (A, H) of every chunk but the last, tile by tile as scan_tiles walks
-// them (a thread with a run of the chunk of its own read 64 rows apart: 4.1
-// TB/s)
+// the composed (A, H) of every chunk but the last, tile by tile like scan_tiles (a
+// thread with a run of the chunk of its own read 64 rows apart: 4.1 TB/s), the last tile
+// first: what is read last is what scan_tiles starts with, out of the last-level cache
+// (1x32768x256 forward 32.8 -> 27.5 us, 1x262144x256 274 -> 234, backward 436 -> 391)
 template <int V, int CL, bool BWD>
 __global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
     using Pl = Place<V, CL>;
     __shared__ float lds[2][kWaves][2][V * CL];
     const Pl at(p);
     if(!at.on) return;
-    const int64_t g0 = at.chunk * p.L + at.tl * LT, t0 = BWD ? p.T - 1 - g0 : g0;
+    const int64_t g0 = at.chunk * p.L + p.L - Pl::TT + at.tl * LT, t0 = BWD ? p.T - 1 - g0 : g0;
     const int64_t ldv = BWD ? p.C : p.ldx, df = BWD ? -p.ldf : p.ldf, dv = BWD ? -ldv : ldv;
     const float* fp = p.f + (at.b * p.T + t0) * p.ldf + at.c;
     const float* vp = (BWD ? p.dh : p.x) + (at.b * p.T + t0) * ldv + at.c;
@@ -187,8 +188,8 @@ __global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
             load<V>(fp + e * df, fr[e]);
             load<V>(vp + e * dv, vr[e]);
         }
-        fp += Pl::TT * df;
-        vp += Pl::TT * dv;
+        fp -= Pl::TT * df;
+        vp -= Pl::TT * dv;
     };
     fetch();
     int turn = 0;
@@ -215,11 +216,16 @@ __global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
                 H[i] = step<BWD>(H[i], s[e][i], vr[e][i]);
             }
         if constexpr(!decltype(last)::value) fetch();
-        through<V, CL>(A, H, carry, in, lds, turn);
+        float own[V];
 #pragma unroll
-        for(int i = 0; i < V; ++i)
+        for(int i = 0; i < V; ++i) own[i] = 0.0f;
+        through<V, CL>(A, H, own, in, lds, turn);
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            carry[i] = fmaf(all[i], own[i], carry[i]);
 #pragma unroll
             for(int q = 0; q < kWaves; ++q) all[i] *= lds[turn][q][0][at.cl * V + i];
+        }
         turn ^= 1;
     };
     for(int64_t k = Pl::TT; k < p.L; k += Pl::TT) walk(std::false_type());
@@ -469,9 +475,10 @@ Plan plan_of(int64_t B, int64_t T, int64_t C) {
     // Chunks.  Few tiles in all: one to a chunk, narrow ones, so that the chunks to
     // gather the state from are few (3x1001x333 4 lanes 24.3, 16 lanes 23.5, one chunk
     // 28.2; 1x9000x20 23.4, 8 lanes 27.8).  Else 512 workgroups: rows of 128 bytes (1x32768x256 8
-    // lanes 80.5, 16 lanes 105, 4 lanes 87.5; 1x4096x768 34.9, 39.7, 39.2), of 64 where
-    // few channels would leave chunks many (1x20000x64 40.8, 8 lanes 52.0), of 256
-    // beyond what the last-level cache holds (1x65536x512 267, 8 lanes 292)
+    // lanes 73.5, 16 lanes 101, 4 lanes 82.5; 1x4096x768 34.5, 41.9, 36.1), of 64 where
+    // few channels would leave chunks many (1x20000x64 40.5, 8 lanes 42.9), of 256
+    // beyond what the last-level cache holds (1x65536x512 260, 8 lanes 288; both in turn
+    // 286, with half as many workgroups 297)
     const int64_t tiles = groups(8) * ((T + steps(8) - 1) / steps(8));
     const int lanes = tiles <= 384 || groups(8) < 4 ? 4 : tiles >= 8192 && groups(16) >= 8 ? 16 : 8;
     const int64_t want = tiles <= 384 ? T : (512 + groups(lanes) - 1) / groups(lanes);
