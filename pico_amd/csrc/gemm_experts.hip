@@ -172,15 +172,17 @@ __global__ __launch_bounds__(64 * kThinWaves) void experts_thin(ExpertParams p) 
 
 double thin_tiles(double groups, double m) { return groups * std::max(1.0, m / kThinRows + 0.5); }
 
-// Microseconds: W once from memory, or once for every row tile from the caches, and a
-// start.  8 experts, rows each 1 / 4 / 8 / 16 / 24, us against those of matrix-core tiles:
+// Microseconds: W once from memory, or once for every row tile from the caches, a start
+// and one of every workgroup.  8 experts, rows each 1 / 4 / 8 / 16 / 24, us against those of matrix-core tiles:
 // [768, 4096] 18 / 18 / 19 / 28 / 40 against 28 / 27 / 27 / 28 / 29 (in bf16 18 / 18 / 20 / 30 /
 // 45 against 23 / 20 / 22 / 21 / 21), [2048, 768] 12 / 12 / 12 / 17 / 22 against 37 (96
-// tiles, each all of K).  Workgroups of 8 or 16 rows read W less often but are fewer
+// tiles, each all of K).  Small matrices have few tiles as well: 4 experts [512, 512] with
+// 64 / 128 rows each 7 / 12 against 13.5, one of [419, 85] 5 against 13; 8 [333, 517] with
+// 48 / 96 11 / 17 against 12, 17 [165, 641] with 48 20 against 11; in bf16 13 [152, 124] with 64 / 96 5.8 / 7.7 against 6.5.  Workgroups of 8 or 16 rows read W less often but are fewer
 // and hold more: [768, 4096] with 4 rows each 24 and 31, when 4 took 22.
-double thin_us(double groups, double m, int64_t N, int64_t K) {
-    const double mb = (double)K * (double)N * 4e-6;
-    return 3.0 + mb * std::max(groups / 7.0, thin_tiles(groups, m) / 16.0);
+double thin_us(double groups, double m, int64_t N, int64_t K, int64_t tiles_n) {
+    const double mb = (double)K * (double)N * 4e-6, tiles = thin_tiles(groups, m);
+    return 3.0 + 0.003 * tiles * (double)tiles_n + mb * std::max(groups / 7.0, tiles / 20.0);
 }
 
 // dW_e (+)= the sum of the S planes [S][E][K][N], in plane order
@@ -238,13 +240,13 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     const int64_t groups = E < n ? E : n;
     ExpertShape rest;
     const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K, &rest);
-    // (the estimates are of up to 32 rows to an expert; 32 columns to a workgroup where 64
+    // (the estimates are of up to 128 rows to an expert, 64 in bf16; 32 columns to a workgroup where 64
     // would leave half of the chip idle: 8 experts [2048, 768] with a row each 8.6 us, of
     // 64 columns 10.6, with 4 rows 14.4 and 13.7; 2 experts [4096, 768] 12.3, 16.5)
     const int cl = thin_tiles((double)groups, (double)n / groups) * (double)((N + 63) / 64) < 144.0 ? 8 : 16;
     const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 4 * cl - 1) / (4 * cl);
-    if(!TB && N >= 4 && K > 0 && n <= 32 * groups && tiles_n <= kMaxTiles / tiles_m &&
-       thin_us((double)groups, (double)n / groups, N, K) < s.us) {
+    if(!TB && N >= 4 && K > 0 && n <= (precision == 0 ? 128 : 64) * groups && tiles_n <= kMaxTiles / tiles_m &&
+       thin_us((double)groups, (double)n / groups, N, K, tiles_n) < s.us) {
         ep.tiles_m = (int)tiles_m;
         ep.tiles_n = (int)tiles_n;
         const unsigned grid = (unsigned)((tiles_m * tiles_n + 7) / 8 * 8);

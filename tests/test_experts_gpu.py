@@ -284,6 +284,7 @@ SIZES = [([1], 8, 8), ([3, 0, 2], 5, 7), ([64], 64, 64), ([0, 0, 1], 33, 65), ([
          # a few rows, streamed weights: sizes around the vectors' and steps'
          ([4, 4], 128, 64), ([5, 3, 9], 131, 68), ([1], 4, 4), ([2, 7], 130, 66), ([30, 2], 515, 6),
          ([4] * 5, 512, 260), ([3] * 9, 1030, 36), ([9, 2, 4], 769, 33), ([6] * 40, 256, 300), ([2] * 20, 385, 700),
+         ([128] * 3, 96, 85), ([36], 419, 85), ([64, 65, 0, 90], 100, 100), ([120], 515, 130),
          # more experts than a wave's lanes, tiles of several rows each
          ([45] * 70, 96, 130), ([0] * 40 + [200] * 30, 32, 40)]
 
