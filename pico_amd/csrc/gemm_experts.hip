@@ -2,6 +2,7 @@
 // of the fp32 (gemm_split.h), bf16 and split-bf16 (gemm_narrow.hip) tiles over
 // groups of rows whose sizes only the device knows.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "gemm_common.h"
@@ -170,6 +171,106 @@ __global__ __launch_bounds__(64 * kThinWaves) void experts_thin(ExpertParams p) 
     }
 }
 
+// Y = X.W_e^T of few rows, their input gradient: the sums run along W's rows.  A wave
+// takes 4 rows and 8 outputs, its lanes lie along k, 4 k each, so that every load is a
+// run of 1 KB; the lanes' sums meet at the end, each exchange halving the values a lane
+// has.
+constexpr int kThinOut = 8;
+
+template <bool BF16>
+__global__ __launch_bounds__(64 * kThinWaves) void experts_thin_t(ExpertParams p) {
+    constexpr int RM = kThinRows, C = kThinOut, STEP = 256;
+    using T = ThinTile<kThinWaves * C / 4>;
+    const TileJob j = tile_job<T>(p);
+    if(j.skip) return;
+    const int w = threadIdx.x / 64, lane = threadIdx.x % 64;
+    const int rows = (int)min(p.M - j.row0, (int64_t)RM);
+    const int64_t out = j.col0 + w * C;
+    if(out >= p.N) return;
+    const float *xp[RM], *wp[C];
+#pragma unroll
+    for(int r = 0; r < RM; ++r) xp[r] = j.A + (j.row0 + min(r, rows - 1)) * p.lda + 4 * lane;
+#pragma unroll
+    for(int c = 0; c < C; ++c) wp[c] = j.B + min(out + c, p.N - 1) * p.ldb + 4 * lane;
+    float acc[RM * C];
+#pragma unroll
+    for(int i = 0; i < RM * C; ++i) acc[i] = 0.0f;
+    struct Step {
+        f32x4 x[RM], w[C];
+    };
+    auto load = [&](Step& s, int64_t k) {
+#pragma unroll
+        for(int r = 0; r < RM; ++r) s.x[r] = *reinterpret_cast<const f32x4u*>(xp[r] + k);
+#pragma unroll
+        for(int c = 0; c < C; ++c) s.w[c] = *reinterpret_cast<const f32x4u*>(wp[c] + k);
+        __builtin_amdgcn_sched_barrier(0);  // (not to be put off until they are needed)
+    };
+    auto add = [&](const Step& s) {
+        f32x4 x[RM];
+#pragma unroll
+        for(int r = 0; r < RM; ++r) x[r] = rounded<BF16>(s.x[r]);
+#pragma unroll
+        for(int c = 0; c < C; ++c) {
+            const f32x4 b = rounded<BF16>(s.w[c]);
+#pragma unroll
+            for(int r = 0; r < RM; ++r)
+#pragma unroll
+                for(int i = 0; i < 4; ++i) acc[r * C + c] = fmaf(x[r][i], b[i], acc[r * C + c]);
+        }
+    };
+    // whole steps, two in flight
+    int left = (int)(p.K / STEP);
+    int64_t k = 0;
+    Step a, b;
+    if(left > 0) {
+        load(a, 0);
+        for(; left > 2; left -= 2, k += 2 * STEP) {
+            load(b, k + STEP);
+            add(a);
+            load(a, k + 2 * STEP);
+            add(b);
+        }
+        if(left == 2) load(b, k + STEP);
+        add(a);
+        if(left == 2) add(b);
+        k += left * STEP;
+    }
+    // the last 255 k or fewer: a lane's four, and the one lane's that has fewer
+    const int64_t rest = p.K - k - 4 * lane;
+    if(rest >= 4) {
+        load(a, k);
+        add(a);
+    } else if(rest > 0) {
+        for(int i = 0; i < (int)rest; ++i) {
+            float x[RM];
+#pragma unroll
+            for(int r = 0; r < RM; ++r) x[r] = rounded<BF16>(xp[r][k + i]);
+#pragma unroll
+            for(int c = 0; c < C; ++c) {
+                const float b = rounded<BF16>(wp[c][k + i]);
+#pragma unroll
+                for(int r = 0; r < RM; ++r) acc[r * C + c] = fmaf(x[r], b, acc[r * C + c]);
+            }
+        }
+    }
+    // lanes 2 i and 2 i + 1 end with value i
+#pragma unroll
+    for(int half = RM * C / 2; half > 0; half /= 2) {
+        const int o = 2 * half;
+        const bool up = lane & o;
+#pragma unroll
+        for(int i = 0; i < half; ++i) {
+            const float give = up ? acc[i] : acc[i + half], keep = up ? acc[i + half] : acc[i];
+            acc[i] = keep + __shfl_xor(give, o, 64);
+        }
+    }
+    const float sum = acc[0] + __shfl_xor(acc[0], 1, 64);
+    const int r = lane / 2 / C, c = lane / 2 % C;
+    if(lane % 2 || r >= rows || out + c >= p.N) return;
+    float* const y = j.C + (j.row0 + r) * p.ldc + out + c;
+    *y = j.beta != 0.0f ? *y + sum : sum;
+}
+
 double thin_tiles(double groups, double m) { return groups * std::max(1.0, m / kThinRows + 0.5); }
 
 // Microseconds: W once from memory, or once for every row tile from the caches, a start
@@ -183,6 +284,18 @@ double thin_tiles(double groups, double m) { return groups * std::max(1.0, m / k
 double thin_us(double groups, double m, int64_t N, int64_t K, int64_t tiles_n) {
     const double mb = (double)K * (double)N * 4e-6, tiles = thin_tiles(groups, m);
     return 3.0 + 0.003 * tiles * (double)tiles_n + mb * std::max(groups / 7.0, tiles / 20.0);
+}
+
+// Microseconds: W once from memory, or so many rounds of workgroups, one on a CU.  8
+// experts, [N, K] with rows each 1 / 8 / 16 / 32 / 64, us against those of matrix-core
+// tiles: [768, 4096] 20 / 22 / 34 / 50 / 96 against 66 (in bf16 22 / 23 / 40 / 61 / 119 against
+// 51), [2048, 768] 12 / 15 / 25 / 44 / 85 against 18 / 18 / 18 / 19 / 24; 2 experts [93, 1464]
+// up to 128 9 against 26.
+double thin_t_us(double groups, double m, int64_t tiles_n, int64_t N, int64_t K, bool bf16) {
+    const double wgs = thin_tiles(groups, m) * (double)tiles_n / 256.0;
+    const double rounds = std::max(1.0, 0.5 * (wgs + std::ceil(wgs)));
+    return std::max(4.0 + groups * (double)K * (double)N * 4e-6 / 6.5,
+                    1.8 + rounds * (bf16 ? 3.0 + 0.0045 * (double)K : 2.2 + 0.0035 * (double)K));
 }
 
 // dW_e (+)= the sum of the S planes [S][E][K][N], in plane order
@@ -245,6 +358,17 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     // 64 columns 10.6, with 4 rows 14.4 and 13.7; 2 experts [4096, 768] 12.3, 16.5)
     const int cl = thin_tiles((double)groups, (double)n / groups) * (double)((N + 63) / 64) < 144.0 ? 8 : 16;
     const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 4 * cl - 1) / (4 * cl);
+    const int64_t tiles_t = (N + 63) / 64;
+    if(TB && K > 0 && n <= 256 * groups && tiles_t <= kMaxTiles / tiles_m &&
+       thin_t_us((double)groups, (double)n / groups, tiles_t, N, K, precision == 1) < s.us) {
+        ep.tiles_m = (int)tiles_m;
+        ep.tiles_n = (int)tiles_t;
+        const unsigned grid = (unsigned)((tiles_m * ep.tiles_n + 7) / 8 * 8);
+        hipStream_t st = pk::as_stream(stream);
+        if(precision == 1) experts_thin_t<true><<<grid, 64 * kThinWaves, 0, st>>>(ep);
+        else experts_thin_t<false><<<grid, 64 * kThinWaves, 0, st>>>(ep);
+        return pk::launch_status("pk_gemm_experts_f32");
+    }
     if(!TB && N >= 4 && K > 0 && n <= (precision == 0 ? 128 : 64) * groups && tiles_n <= kMaxTiles / tiles_m &&
        thin_us((double)groups, (double)n / groups, N, K, tiles_n) < s.us) {
         ep.tiles_m = (int)tiles_m;
