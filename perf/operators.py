@@ -6,6 +6,7 @@
 the same outputs in float64.  Sizes are those of this repository's benchmark
 configurations (d_model 768, d_ff 2048, 8 sequences of 1024) or generic ones.
 """
+import ctypes
 import math
 
 import torch
@@ -313,6 +314,8 @@ class _Session:
         self.params = []
         self.work = self.lib.arena_init(int(work_bytes))
         self.opt = self.lib.pico_optim_sgd_init(0.01)
+        self.lib.pico_gpu_stream.restype = ctypes.c_void_p
+        self.stream = torch.cuda.ExternalStream(self.lib.pico_gpu_stream(), device=DEV)
 
     def view(self, t, grad=False):
         ptr = t.contents.grad if grad else t.contents.data
@@ -384,15 +387,23 @@ def _prepare_own(st):
 def _own_moe(st):
     c, s, v = st["case"], st["session"], st["leaves"]
     P, lib = s.P, s.lib
+    # pico has a stream of its own, which nothing orders with torch's: it starts when
+    # what torch has been given is done (it writes where that may still read), and
+    # what torch is given from here on waits for it
+    theirs, mine = s.stream, torch.cuda.current_stream()
+    theirs.wait_stream(mine)
     lib.arena_ctx_push(s.work)
-    lib.arena_reset(s.work)
-    lib.pico_optim_sgd_zero_grad(s.opt)
-    gates, route = P.route_topk(v["logits"], c["topk"])
-    gu = P.expert_matmul(P.expert_gather(v["x"], route), v["w13"], route)
-    h = P.swiglu(*P.split_cols(gu, 2))
-    y = P.expert_combine(P.expert_matmul(h, v["w2"], route), gates, route, v["x"])
-    P.backward(y)
-    lib.arena_ctx_pop()
+    try:
+        lib.arena_reset(s.work)
+        lib.pico_optim_sgd_zero_grad(s.opt)
+        gates, route = P.route_topk(v["logits"], c["topk"])
+        gu = P.expert_matmul(P.expert_gather(v["x"], route), v["w13"], route)
+        h = P.swiglu(*P.split_cols(gu, 2))
+        y = P.expert_combine(P.expert_matmul(h, v["w2"], route), gates, route, v["x"])
+        P.backward(y)
+    finally:
+        lib.arena_ctx_pop()
+        mine.wait_stream(theirs)
     return dict({"d" + n: s.view(t, grad=True) for n, t in v.items()}, y=s.view(y))
 
 
