@@ -179,8 +179,9 @@ struct PicoTensor* pico_layernorm(struct PicoTensor* x, struct PicoTensor* gain,
 /* gated linear recurrence along the tokens of each sequence, channel by channel:
  * h_t = s_t h_{t-1} + (1 - s_t) x_t, s = sigmoid(f); f, x token-major [batch*T, C]
  * (contiguous or column views), h0 [batch, C] the state before the first token
- * or NULL (zero).  f = -inf starts anew at a token.  Token by token: T = 1, and
- * h0 the h before. */
+ * or NULL (zero).  f = -inf starts anew at a token, whatever the tokens before hold,
+ * infinities and NaN too (as does f below about -87.3); f = +inf (or above 87.3) passes
+ * a token over.  Token by token: T = 1, and h0 the h before. */
 struct PicoTensor* pico_gated_scan(struct PicoTensor* f, struct PicoTensor* x,
                                    struct PicoTensor* h0, int batch);
 /* the last token of each sequence of h [batch*T, C] (contiguous or a column view), as

@@ -633,8 +633,10 @@ int pk_layernorm_bwd_f32(int64_t R, int64_t C, const float* x, const float* g, c
  *   s_t = sigmoid(f_t),  h_t = s_t*h_{t-1} + (1 - s_t)*x_t,  h before the first
  *   token = h0 [B, C], or zero when h0 is NULL
  * f, x have row strides ldf, ldx >= C (column blocks of one projection are fine);
- * h, dh are contiguous.  f = -inf starts anew (h_t = x_t), f = +inf keeps h.  One
- * token at a time is T = 1 with h0 the state so far (h may be h0).
+ * h, dh are contiguous.  One token at a time is T = 1 with h0 the state so far (h may
+ * be h0).  f = -inf starts anew: h_t = x_t, and neither values nor gradients pass, not
+ * even infinite or NaN ones.  f = +inf keeps h, whatever x_t is.  Beyond about +-87.3,
+ * where s or 1 - s is below 2^-126, they are 0 here and f acts so, too.
  * backward: with G_t = dh_t + s_{t+1}*G_{t+1},
  *   df (+)= G*(h_{t-1} - x)*s*(1 - s) (PK_ACCUM), dx (+)= (1 - s)*G (PK_ACCUM2),
  *   dh0 (+)= s_1*G_1 (PK_ACCUM3); a NULL gradient is skipped.  The gradients'

@@ -6,6 +6,10 @@
 //   G_t = dh_t + u_{t+1},  u_t = s_t G_t
 //   dx_t = (1 - s_t) G_t,  df_t = G_t (h_{t-1} - x_t) s_t (1 - s_t),  dh_0 = u_1
 //
+// A gate that is shut or open in fp32 (s or 1 - s is 0) leaves the other side out, whatever
+// that holds: with s = 0 no infinity or NaN passes from the tokens before to this one
+// and those after it, nor back with the gradients; with 1 - s = 0 none from x_t.
+//
 // Both directions are chains of p -> A p + H (forward A = s, H = q x; backward A = s,
 // H = s dh), and a run of steps is again one: (A2, H2) after (A1, H1) is
 // (A1 A2, A2 H1 + H2).  A workgroup walks its steps in tiles: a thread has 4
@@ -116,10 +120,69 @@ struct Place {
     }
 };
 
+// a b, and 0 where one of them is, whatever the other holds (the instruction has no
+// builtin; equal to a multiplication bit for bit where neither is 0)
+__device__ __forceinline__ float product(float a, float b) {
+    float r;
+    asm("v_mul_legacy_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+
+// The arithmetic of runs has two forms.  BAD is for values that may be infinite or NaN: a
+// run with a shut gate has A = -0, which leaves p out, while the product of many gates
+// that are not shut may come to +0, through which an infinity or NaN does go on.  The
+// other form multiplies by 0 like by anything else, and in it no value of a chain is
+// finite behind one that is not: the last one tells whether all has to be done again, in
+// the other form, a step at a time, after the loops (in them it takes registers or time:
+// selects throughout 8x1024x768 forward and backward 21.5 + 34.5 us, a tile at a time
+// 18.2 + 30.6, so 18.0 + 29.1).
+constexpr float kShut = -0.0f;
+__device__ __forceinline__ bool shut(float A) { return __float_as_uint(A) == 0x80000000u; }
+
+template <int V>
+__device__ __forceinline__ bool any_bad(const float (&p)[V]) {
+    float sum = 0.0f;
+#pragma unroll
+    for(int i = 0; i < V; ++i) sum = fmaf(p[i], 0.0f, sum);
+    return __any(sum != 0.0f);
+}
+
+// p behind a run of steps, and (A, H) of a run behind (a, h) of the one before it
+template <bool BAD>
+__device__ __forceinline__ float behind(float A, float H, float p) {
+    return BAD && shut(A) ? H : fmaf(A, p, H);
+}
+template <bool BAD>
+__device__ __forceinline__ void compose(float& A, float& H, float a, float h) {
+    H = behind<BAD>(A, H, h);
+    if(!BAD || !shut(A)) A *= a;
+}
+
+// one step of the chain (forward v = q x, backward dh), and one at the end of a run
+template <bool BWD, bool BAD>
+__device__ __forceinline__ float step(float p, float s, float v) {
+    if(BWD) return BAD && s == 0.0f ? 0.0f : s * (v + p);
+    return BAD && s == 0.0f ? v : fmaf(s, p, v);
+}
+template <bool BWD, bool BAD>
+__device__ __forceinline__ void extend_run(float s, float v, float& A, float& H) {
+    A = BAD && s == 0.0f ? kShut : A * s;
+    H = step<BWD, BAD>(H, s, v);
+}
+
+// dx and df of a token; returns the gradient it hands to the one before it.  (h and x may
+// be bad where the chain of the gradients is not)
+template <bool BAD>
+__device__ __forceinline__ float gradients(float G, float h, float x, float s, float q, float& dx, float& df) {
+    dx = BAD && q == 0.0f ? 0.0f : q * G;
+    df = BAD ? (s == 0.0f || q == 0.0f ? 0.0f : G * (h - x) * (s * q)) : product(G * (h - x), s * q);
+    return BAD && s == 0.0f ? 0.0f : s * G;
+}
+
 // (A, H) of the lanes' steps, in step order -> the value that reaches each lane
-// from `carry`; carry becomes the one behind the last lane.  One barrier; `turn`
-// alternates between calls.
-template <int V, int CL>
+// from `carry`; carry becomes the one behind the last lane, the same in every wave.  One
+// barrier; `turn` alternates between calls.
+template <int V, int CL, bool BAD>
 __device__ __forceinline__ void through(float (&A)[V], float (&H)[V], float (&carry)[V], float (&in)[V],
                                         float (*lds)[kWaves][2][V * CL], int turn) {
     const int lane = threadIdx.x % 64, w = threadIdx.x / 64, cl = threadIdx.x % CL;
@@ -128,20 +191,27 @@ __device__ __forceinline__ void through(float (&A)[V], float (&H)[V], float (&ca
 #pragma unroll
         for(int i = 0; i < V; ++i) {
             const float a = __shfl_up(A[i], o, 64), h = __shfl_up(H[i], o, 64);
-            if(lane >= o) {
-                H[i] = fmaf(A[i], h, H[i]);
-                A[i] *= a;
-            }
+            if(lane >= o) compose<BAD>(A[i], H[i], a, h);
         }
     }
+    typedef float Lane __attribute__((ext_vector_type(V)));
     if(lane >= 64 - CL) {
+        Lane a, h;
 #pragma unroll
         for(int i = 0; i < V; ++i) {
-            lds[turn][w][0][cl * V + i] = A[i];
-            lds[turn][w][1][cl * V + i] = H[i];
+            a[i] = A[i];
+            h[i] = H[i];
         }
+        *reinterpret_cast<Lane*>(&lds[turn][w][0][cl * V]) = a;
+        *reinterpret_cast<Lane*>(&lds[turn][w][1][cl * V]) = h;
     }
     __syncthreads();
+    Lane a[kWaves], h[kWaves];
+#pragma unroll
+    for(int q = 0; q < kWaves; ++q) {
+        a[q] = *reinterpret_cast<const Lane*>(&lds[turn][q][0][cl * V]);
+        h[q] = *reinterpret_cast<const Lane*>(&lds[turn][q][1][cl * V]);
+    }
     float own[V];
 #pragma unroll
     for(int i = 0; i < V; ++i) {
@@ -149,17 +219,11 @@ __device__ __forceinline__ void through(float (&A)[V], float (&H)[V], float (&ca
 #pragma unroll
         for(int q = 0; q < kWaves; ++q) {
             if(q == w) own[i] = carry[i];
-            carry[i] = fmaf(lds[turn][q][0][cl * V + i], carry[i], lds[turn][q][1][cl * V + i]);
+            carry[i] = behind<BAD>(a[q][i], h[q][i], carry[i]);
         }
         const float a = __shfl_up(A[i], CL, 64), h = __shfl_up(H[i], CL, 64);
-        in[i] = lane >= CL ? fmaf(a, own[i], h) : own[i];
+        in[i] = lane >= CL ? behind<BAD>(a, h, own[i]) : own[i];
     }
-}
-
-// one step of the chain
-template <bool BWD>
-__device__ __forceinline__ float step(float p, float s, float v) {
-    return BWD ? s * (v + p) : fmaf(s, p, v);
 }
 
 // the composed (A, H) of every chunk but the last, tile by tile like scan_tiles (a
@@ -167,9 +231,9 @@ __device__ __forceinline__ float step(float p, float s, float v) {
 // first: what is read last is what scan_tiles starts with, out of the last-level cache
 // (1x32768x256 forward 32.8 -> 27.5 us, 1x262144x256 274 -> 234, backward 436 -> 391)
 template <int V, int CL, bool BWD>
-__global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
+__global__ __launch_bounds__(kThreads, 4) void scan_chunks(ScanParams p) {
     using Pl = Place<V, CL>;
-    __shared__ float lds[2][kWaves][2][V * CL];
+    __shared__ alignas(16) float lds[2][kWaves][2][V * CL];
     const Pl at(p);
     if(!at.on) return;
     const int64_t g0 = at.chunk * p.L + p.L - Pl::TT + at.tl * LT, t0 = BWD ? p.T - 1 - g0 : g0;
@@ -192,48 +256,143 @@ __global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
         vp -= Pl::TT * dv;
     };
     fetch();
+    // the least s of the thread's steps
+    float least[V];
+#pragma unroll
+    for(int i = 0; i < V; ++i) least[i] = 1.0f;
     int turn = 0;
+    float A[V], H[V];
+    // (all, carry), of the tiles behind this one, with its own before them
+    auto add = [&](auto bad) {
+        constexpr bool BAD = decltype(bad)::value;
+        float own[V];
+#pragma unroll
+        for(int i = 0; i < V; ++i) own[i] = 0.0f;
+        through<V, CL, BAD>(A, H, own, in, lds, turn);
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            carry[i] = behind<BAD>(all[i], carry[i], own[i]);
+#pragma unroll
+            for(int q = kWaves - 1; q >= 0; --q)
+                if(!BAD || !shut(all[i])) all[i] *= lds[turn][q][0][at.cl * V + i];
+        }
+        turn ^= 1;
+    };
     auto walk = [&](auto last) {
-        float s[LT][V], A[V], H[V];
+        float s[LT][V];
 #pragma unroll
         for(int e = 0; e < LT; ++e)
 #pragma unroll
             for(int i = 0; i < V; ++i) {
                 float q;
                 gate(fr[e][i], s[e][i], q);
-                if(!BWD) vr[e][i] *= q;
+                if(!BWD) vr[e][i] = product(q, vr[e][i]);
             }
 #pragma unroll
         for(int i = 0; i < V; ++i) {
             A[i] = s[0][i];
             H[i] = BWD ? s[0][i] * vr[0][i] : vr[0][i];
+            least[i] = fminf(least[i], s[0][i]);
         }
 #pragma unroll
         for(int e = 1; e < LT; ++e)
 #pragma unroll
             for(int i = 0; i < V; ++i) {
-                A[i] *= s[e][i];
-                H[i] = step<BWD>(H[i], s[e][i], vr[e][i]);
+                extend_run<BWD, false>(s[e][i], vr[e][i], A[i], H[i]);
+                least[i] = fminf(least[i], s[e][i]);
             }
         if constexpr(!decltype(last)::value) fetch();
-        float own[V];
-#pragma unroll
-        for(int i = 0; i < V; ++i) own[i] = 0.0f;
-        through<V, CL>(A, H, own, in, lds, turn);
-#pragma unroll
-        for(int i = 0; i < V; ++i) {
-            carry[i] = fmaf(all[i], own[i], carry[i]);
-#pragma unroll
-            for(int q = 0; q < kWaves; ++q) all[i] *= lds[turn][q][0][at.cl * V + i];
-        }
-        turn ^= 1;
+        add(std::false_type());
     };
     for(int64_t k = Pl::TT; k < p.L; k += Pl::TT) walk(std::false_type());
     walk(std::true_type());
-    if(at.tl == 0) {
+    auto result = [&]() {
+        if(at.tl != 0) return;
         float* const o = p.ws + (at.chunk * p.B + at.b) * p.C + at.c;
         store<V>(o, all, at.skip, false);
         store<V>(o + (int64_t)p.S * p.B * p.C, carry, at.skip, false);
+    };
+    if(any_bad(carry)) {  // (the same in every wave)
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            all[i] = 1.0f;
+            carry[i] = 0.0f;
+        }
+        for(int64_t left = p.L; left > 0; left -= Pl::TT) {
+#pragma unroll
+            for(int i = 0; i < V; ++i) {
+                A[i] = 1.0f;
+                H[i] = 0.0f;
+            }
+#pragma unroll 1
+            for(int e = 0; e < LT; ++e) {
+                const int64_t g = at.chunk * p.L + left - Pl::TT + at.tl * LT + e, t = BWD ? p.T - 1 - g : g;
+                float f[V], v[V];
+                load<V>(p.f + (at.b * p.T + t) * p.ldf + at.c, f);
+                load<V>((BWD ? p.dh : p.x) + (at.b * p.T + t) * ldv + at.c, v);
+#pragma unroll
+                for(int i = 0; i < V; ++i) {
+                    float s, q;
+                    gate(f[i], s, q);
+                    extend_run<BWD, true>(s, BWD ? v[i] : product(q, v[i]), A[i], H[i]);
+                }
+            }
+            add(std::true_type());
+        }
+        result();
+        return;
+    }
+    // a shut gate leaves the product at 0
+    bool zero = false;
+#pragma unroll
+    for(int i = 0; i < V; ++i) zero |= all[i] == 0.0f;
+    if(__any(zero)) {  // (the same in every wave)
+        __shared__ int shut_at[V * CL];
+        if(threadIdx.x < V * CL) shut_at[threadIdx.x] = 0;
+        __syncthreads();
+#pragma unroll
+        for(int i = 0; i < V; ++i)
+            if(least[i] == 0.0f) shut_at[at.cl * V + i] = 1;
+        __syncthreads();
+#pragma unroll
+        for(int i = 0; i < V; ++i)
+            if(shut_at[at.cl * V + i]) all[i] = kShut;
+    }
+    result();
+}
+
+// token t of sequence b at V channels from c on, from `state` on: h and the new state, or
+// the gradients and what is handed to the token before
+template <int V, bool BWD>
+__device__ __forceinline__ void token(const ScanParams& p, int64_t b, int64_t t, int64_t c, int skip,
+                                      float (&state)[V]) {
+    const int64_t row = b * p.T + t;
+    float f[V], x[V];
+    load<V>(p.f + row * p.ldf + c, f);
+    load<V>(p.x + row * p.ldx + c, x);
+    if constexpr(!BWD) {
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            float s, q;
+            gate(f[i], s, q);
+            state[i] = step<false, true>(state[i], s, product(q, x[i]));
+        }
+        store<V>(p.out + row * p.C + c, state, skip, false);
+    } else {
+        float dh[V], h[V], df[V], dx[V];
+        load<V>(p.dh + row * p.C + c, dh);
+#pragma unroll
+        for(int i = 0; i < V; ++i) h[i] = 0.0f;
+        if(t > 0) load<V>(p.h + (row - 1) * p.C + c, h);
+        else if(p.h0) load<V>(p.h0 + b * p.C + c, h);
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            float s, q;
+            gate(f[i], s, q);
+            state[i] = gradients<true>(dh[i] + state[i], h[i], x[i], s, q, dx[i], df[i]);
+        }
+        if(p.df) store<V>(p.df + row * p.lddf + c, df, skip, p.flags & PK_ACCUM);
+        if(p.dx) store<V>(p.dx + row * p.lddx + c, dx, skip, p.flags & PK_ACCUM2);
     }
 }
 
@@ -241,10 +400,10 @@ __global__ __launch_bounds__(kThreads) void scan_chunks(ScanParams p) {
 // dh and to the next kernel (1x65536x512 backward 195 -> 167 us, 4x8192x1024 214 ->
 // 200; now 164 and 194; tensors that fit the last-level cache are better read from there: 8x1024x768
 // 30 against 37, 32x2048x256 68 against 75)
-template <int V, int CL, bool BWD, bool BIG>
+template <int V, int CL, bool BWD, bool BIG, bool ACC>
 __global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
     using Pl = Place<V, CL>;
-    __shared__ float lds[2][kWaves][2][V * CL];
+    __shared__ alignas(16) float lds[2][kWaves][2][V * CL];
     const Pl at(p);
     if(!at.on) return;
     const int64_t g0 = at.chunk * p.L, g1 = min(p.T, g0 + p.L);
@@ -296,27 +455,42 @@ __global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
     fetch(g0);
     if(at.chunk > 0) {
         // the value behind the chunks before this one
-        const int64_t m = (at.chunk + Pl::TL - 1) / Pl::TL;
-        float A[V], H[V];
+        float A[V], H[V], given[V];
 #pragma unroll
-        for(int i = 0; i < V; ++i) {
-            A[i] = 1.0f;
-            H[i] = 0.0f;
-        }
-        for(int64_t k = at.tl * m; k < min(at.tl * m + m, at.chunk); ++k) {
-            const float* o = p.ws + (k * p.B + at.b) * p.C + at.c;
-            float a[V], e[V];
-            load<V>(o, a);
-            load<V>(o + (int64_t)p.S * p.B * p.C, e);
+        for(int i = 0; i < V; ++i) given[i] = carry[i];
+        auto gather = [&](auto bad) {
+            constexpr bool BAD = decltype(bad)::value;
+            const int64_t m = (at.chunk + Pl::TL - 1) / Pl::TL;
 #pragma unroll
             for(int i = 0; i < V; ++i) {
-                H[i] = fmaf(a[i], H[i], e[i]);
-                A[i] *= a[i];
+                A[i] = 1.0f;
+                H[i] = 0.0f;
+                carry[i] = given[i];
             }
-        }
-        through<V, CL>(A, H, carry, in, lds, turn);
-        turn ^= 1;
+            for(int64_t k = at.tl * m; k < min(at.tl * m + m, at.chunk); ++k) {
+                const float* o = p.ws + (k * p.B + at.b) * p.C + at.c;
+                float a[V], e[V];
+                load<V>(o, a);
+                load<V>(o + (int64_t)p.S * p.B * p.C, e);
+#pragma unroll
+                for(int i = 0; i < V; ++i) {
+                    compose<BAD>(a[i], e[i], A[i], H[i]);
+                    A[i] = a[i];
+                    H[i] = e[i];
+                }
+            }
+            through<V, CL, BAD>(A, H, carry, in, lds, turn);
+            turn ^= 1;
+        };
+        gather(std::false_type());
+        if(any_bad(carry)) gather(std::true_type());  // (the same in every wave)
     }
+    // where the bad form would start: at the first tile, or, where the stores add to what is
+    // there and cannot be done twice, at the tile that has the first bad values
+    int64_t from = g0;
+    float reached[V];
+#pragma unroll
+    for(int i = 0; i < V; ++i) reached[i] = carry[i];
     // (the last tile apart: were its fetch a branch's, the waits for one tile's values
     // would be for the next one's as well)
     auto walk = [&](int64_t tile, auto last) {
@@ -335,7 +509,7 @@ __global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
 #pragma unroll
             for(int i = 0; i < V; ++i) {
                 gate(r.f[e][i], s[e][i], q[e][i]);
-                if(!BWD) r.x[e][i] *= q[e][i];
+                if(!BWD) r.x[e][i] = product(q[e][i], r.x[e][i]);
             }
         if(!whole) {
 #pragma unroll
@@ -356,39 +530,75 @@ __global__ __launch_bounds__(kThreads) void scan_tiles(ScanParams p) {
 #pragma unroll
         for(int e = 1; e < LT; ++e)
 #pragma unroll
-            for(int i = 0; i < V; ++i) {
-                A[i] *= s[e][i];
-                H[i] = step<BWD>(H[i], s[e][i], BWD ? r.dh[BWD ? e : 0][i] : r.x[e][i]);
-            }
-        through<V, CL>(A, H, carry, in, lds, turn);
+            for(int i = 0; i < V; ++i)
+                extend_run<BWD, false>(s[e][i], BWD ? r.dh[BWD ? e : 0][i] : r.x[e][i], A[i], H[i]);
+        through<V, CL, false>(A, H, carry, in, lds, turn);
         turn ^= 1;
+        if constexpr(ACC) {
+            if(any_bad(carry)) return false;
+            from = tile + Pl::TT;
+#pragma unroll
+            for(int i = 0; i < V; ++i) reached[i] = carry[i];
+        }
 #pragma unroll
         for(int e = 0; e < LT; ++e) {
             const int64_t g = first + e, t = BWD ? p.T - 1 - g : g;
             if(!whole && e < shift) continue;
             if constexpr(!BWD) {
 #pragma unroll
-                for(int i = 0; i < V; ++i) in[i] = step<false>(in[i], s[e][i], r.x[e][i]);
+                for(int i = 0; i < V; ++i) in[i] = step<false, false>(in[i], s[e][i], r.x[e][i]);
                 store<V>(out + t * p.C, in, at.skip, false);
             } else {
                 float df[V], dx[V];
 #pragma unroll
                 for(int i = 0; i < V; ++i) {
                     if(e == LT - 1 && t == 0 && !h0) r.h[e][i] = 0.0f;
-                    const float G = r.dh[e][i] + in[i];
-                    dx[i] = q[e][i] * G;
-                    df[i] = G * (r.h[e][i] - r.x[e][i]) * (s[e][i] * q[e][i]);
-                    in[i] = s[e][i] * G;
+                    in[i] = gradients<false>(r.dh[e][i] + in[i], r.h[e][i], r.x[e][i], s[e][i], q[e][i], dx[i],
+                                             df[i]);
                 }
                 const int64_t row = at.b * p.T + t;
-                if(p.df) store<V>(p.df + row * p.lddf + at.c, df, at.skip, p.flags & PK_ACCUM);
-                if(p.dx) store<V>(p.dx + row * p.lddx + at.c, dx, at.skip, p.flags & PK_ACCUM2);
+                if(p.df) store<V>(p.df + row * p.lddf + at.c, df, at.skip, ACC && (p.flags & PK_ACCUM));
+                if(p.dx) store<V>(p.dx + row * p.lddx + at.c, dx, at.skip, ACC && (p.flags & PK_ACCUM2));
             }
         }
+        return true;
     };
     int64_t tile = g0;
-    for(; tile + Pl::TT < g1; tile += Pl::TT) walk(tile, std::false_type());
-    walk(tile, std::true_type());
+    while(tile + Pl::TT < g1 && walk(tile, std::false_type())) tile += Pl::TT;
+    if(tile + Pl::TT >= g1) walk(tile, std::true_type());
+    const bool again = any_bad(carry);  // (the same in every wave)
+    if(again) {
+#pragma unroll
+        for(int i = 0; i < V; ++i) carry[i] = reached[i];
+    }
+    // (each step's values loaded anew: what the tiles have in flight fills the registers)
+    for(tile = from; again && tile < g1; tile += Pl::TT) {
+        const int64_t end = min(tile + (at.tl + 1) * LT, g1);
+        float A[V], H[V];
+#pragma unroll
+        for(int i = 0; i < V; ++i) {
+            A[i] = 1.0f;
+            H[i] = 0.0f;
+        }
+#pragma unroll 1
+        for(int64_t g = tile + at.tl * LT; g < end; ++g) {
+            const int64_t t = BWD ? p.T - 1 - g : g;
+            float fe[V], ve[V];
+            load<V>(f + t * p.ldf, fe);
+            load<V>(BWD ? dh + t * p.C : x + t * p.ldx, ve);
+#pragma unroll
+            for(int i = 0; i < V; ++i) {
+                float s, q;
+                gate(fe[i], s, q);
+                extend_run<BWD, true>(s, BWD ? ve[i] : product(q, ve[i]), A[i], H[i]);
+            }
+        }
+        through<V, CL, true>(A, H, carry, in, lds, turn);
+        turn ^= 1;
+#pragma unroll 1
+        for(int64_t g = tile + at.tl * LT; g < end; ++g)
+            token<V, BWD>(p, at.b, BWD ? p.T - 1 - g : g, at.c, at.skip, in);
+    }
     if(BWD && p.dh0 && at.tl == 0 && g1 == p.T)
         store<V>(p.dh0 + at.b * p.C + at.c, carry, at.skip, p.flags & PK_ACCUM3);
 }
@@ -409,39 +619,7 @@ __global__ __launch_bounds__(kThreads) void scan_serial(ScanParams p) {
 #pragma unroll
     for(int i = 0; i < V; ++i) state[i] = 0.0f;
     if(!BWD && p.h0) load<V>(p.h0 + b * p.C + c, state);
-    for(int64_t g = 0; g < p.T; ++g) {
-        const int64_t t = BWD ? p.T - 1 - g : g, row = b * p.T + t;
-        float f[V], x[V];
-        load<V>(p.f + row * p.ldf + c, f);
-        load<V>(p.x + row * p.ldx + c, x);
-        if constexpr(!BWD) {
-#pragma unroll
-            for(int i = 0; i < V; ++i) {
-                float s, q;
-                gate(f[i], s, q);
-                state[i] = step<false>(state[i], s, q * x[i]);
-            }
-            store<V>(p.out + row * p.C + c, state, skip, false);
-        } else {
-            float dh[V], h[V], df[V], dx[V];
-            load<V>(p.dh + row * p.C + c, dh);
-#pragma unroll
-            for(int i = 0; i < V; ++i) h[i] = 0.0f;
-            if(t > 0) load<V>(p.h + (row - 1) * p.C + c, h);
-            else if(p.h0) load<V>(p.h0 + b * p.C + c, h);
-#pragma unroll
-            for(int i = 0; i < V; ++i) {
-                float s, q;
-                gate(f[i], s, q);
-                const float G = dh[i] + state[i];
-                dx[i] = q * G;
-                df[i] = G * (h[i] - x[i]) * (s * q);
-                state[i] = s * G;
-            }
-            if(p.df) store<V>(p.df + row * p.lddf + c, df, skip, p.flags & PK_ACCUM);
-            if(p.dx) store<V>(p.dx + row * p.lddx + c, dx, skip, p.flags & PK_ACCUM2);
-        }
-    }
+    for(int64_t g = 0; g < p.T; ++g) token<V, BWD>(p, b, BWD ? p.T - 1 - g : g, c, skip, state);
     if(BWD && p.dh0) store<V>(p.dh0 + b * p.C + c, state, skip, p.flags & PK_ACCUM3);
 }
 
@@ -492,11 +670,19 @@ void launch(ScanParams& p, const Plan& plan, hipStream_t st) {
     p.groups = (int)((p.C + V * CL - 1) / (V * CL));
     const unsigned grid = (unsigned)((p.B * p.groups + 7) / 8 * 8);
     if(plan.S > 1) scan_chunks<V, CL, BWD><<<dim3(grid, plan.S - 1), kThreads, 0, st>>>(p);
+    auto tiles = [&](auto big, auto acc) {
+        scan_tiles<V, CL, BWD, decltype(big)::value, decltype(acc)::value>
+            <<<dim3(grid, plan.S), kThreads, 0, st>>>(p);
+    };
+    auto with = [&](auto big) {
+        if constexpr(BWD)
+            if(p.flags & (PK_ACCUM | PK_ACCUM2)) return tiles(big, std::true_type());
+        tiles(big, std::false_type());
+    };
     // (values of a tensor: between 17 and 33 million)
-    if(BWD && p.B * p.T * p.C >= (int64_t)24 << 20)
-        scan_tiles<V, CL, BWD, BWD><<<dim3(grid, plan.S), kThreads, 0, st>>>(p);
-    else
-        scan_tiles<V, CL, BWD, false><<<dim3(grid, plan.S), kThreads, 0, st>>>(p);
+    if constexpr(BWD)
+        if(p.B * p.T * p.C >= (int64_t)24 << 20) return with(std::true_type());
+    with(std::false_type());
 }
 
 template <bool BWD>

@@ -16,6 +16,7 @@ from pico_amd.pico import Pico, PicoError
 pytestmark = pytest.mark.gpu
 
 U = 2.0 ** -24
+INF = float("inf")
 
 
 @pytest.fixture(scope="module")
@@ -243,6 +244,112 @@ def test_closed_and_open_gates(dev, T):
     assert torch.equal(h.view(B, T, C)[0, -1, 12:16], h0[0, 12:16])
     assert bool(torch.isnan(h.view(B, T, C)[0, 1:, 20]).all())
     assert not bool(torch.isnan(h.view(B, T, C)[0, :1, 20]).any())
+
+
+
+# serial, one tile, tiles, chunks of one tile and of several; V of 1 and of 4 channels
+@pytest.mark.parametrize("B,T,C", [(3, 7, 20), (2, 100, 37), (2, 777, 20), (1, 1001, 33), (1, 9000, 20), (2, 3000, 3),
+                                   (8, 600, 200), (1, 40000, 64)])
+@pytest.mark.parametrize("closed", [-INF, -100.0])
+def test_a_closed_gate_keeps_bad_values_out(dev, B, T, C, closed):
+    """documents packed into one sequence, each starting with a closed gate: infinities and NaN
+    of one's tokens, gates or gradients stay in it, forward, backward and added to what is
+    there"""
+    g = torch.Generator().manual_seed(T + C)
+    f, x, h0, dh = (t.cpu() for t in _data(B, T, C, 21))
+    cuts = sorted({0, T} | set(torch.randint(1, T, (min(9, T // 2),), generator=g).tolist()))
+    f3, x3, dh3 = f.view(B, T, C), x.view(B, T, C), dh.view(B, T, C)
+    f3[:, cuts[1:-1]] = closed
+    docs = list(zip(cuts, cuts[1:]))
+    want, tol = ({k: torch.zeros(B, T, C, dtype=torch.float64) for k in ("h", "df", "dx")} for _ in range(2))
+    for n, (lo, hi) in enumerate(docs):
+        rows, bound = _reference(B, f3[:, lo:hi].reshape(-1, C), x3[:, lo:hi].reshape(-1, C), h0 if n == 0 else None,
+                                 dh3[:, lo:hi].reshape(-1, C))
+        for k in want:
+            want[k][:, lo:hi], tol[k][:, lo:hi] = (t[k].view(B, hi - lo, C) for t in (rows, bound))
+    # every other document is spoilt in every third channel
+    bad_h, bad_g = (torch.zeros(B, T, C, dtype=torch.bool) for _ in range(2))
+    for n, (lo, hi) in enumerate(docs):
+        if n % 2:
+            continue
+        at = int(torch.randint(lo, hi, (1,), generator=g))
+        cols = torch.arange(n % 3, C, 3)
+        kind = (n // 2) % 4
+        if kind == 0:
+            x3[:, at, cols] = float("nan")
+        elif kind == 1:
+            x3[:, at, cols] = INF if at % 2 else -INF
+        if kind < 2:
+            bad_h[:, at:hi, cols] = True
+        elif kind == 2:
+            dh3[:, at, cols] = float("nan")
+            bad_g[:, lo:at + 1, cols] = True
+        else:
+            dh3[:, at, cols] = -INF
+            bad_g[:, lo:at + 1, cols] = True
+    fd, xd, hd, dhd = (t.to(dev) for t in (f, x, h0, dh))
+    h, df, dx, dh0 = _empty(B * T, C), _empty(B * T, C), _empty(B * T, C), _empty(B, C)
+    K.gated_scan_fwd(B, fd, xd, h, h0=hd)
+    K.gated_scan_bwd(B, fd, xd, h, dhd, df, dx, h0=hd, dh0=dh0)
+    base = [torch.randn(B * T, C, generator=g).to(dev) for _ in range(2)]
+    acc = [t.clone() for t in base]
+    K.gated_scan_bwd(B, fd, xd, h, dhd, acc[0], acc[1], h0=hd, accum_df=True, accum_dx=True)
+    got = {"h": h, "df": df, "dx": dx}
+    # df of a document takes its h; a token's dx and df with a closed gate are dh and 0
+    spoilt = {"h": bad_h, "dx": bad_g, "df": bad_g | bad_h}
+    for k, t in got.items():
+        t = t.view(B, T, C).cpu()
+        ok = ~spoilt[k]
+        ratio = (t.double() - want[k]).abs() / (tol[k] + 1e-37)
+        assert bool((ratio[ok] <= 1).all()), (k, float(ratio[ok].nan_to_num(INF).max()))
+    assert not bool(torch.isfinite(h.view(B, T, C).cpu()[bad_h]).any())
+    assert not bool(torch.isfinite(dx.view(B, T, C).cpu()[bad_g]).any())
+    assert bool(torch.isfinite(dh0.cpu()[:, ~bad_g[0, 0]]).all())
+    # (a tile done again may round a token's gradient otherwise than in the call above: the
+    # bound is the gradient's own and u of the sum, which is at most |b| + |want| + tol)
+    for a, b, k in zip(acc, base, ("df", "dx")):
+        ok = ~spoilt[k].view(-1, C)
+        a, b, w, e = a.double().cpu()[ok], b.double().cpu()[ok], want[k].view(-1, C)[ok], tol[k].view(-1, C)[ok]
+        assert bool(((a - (b + w)).abs() <= (1 + U) * e + U * (b.abs() + w.abs()) + 1e-37).all()), k
+
+
+@pytest.mark.parametrize("B,T,C", [(3, 7, 20), (2, 777, 20), (1, 9000, 20), (2, 3000, 3)])
+@pytest.mark.parametrize("opened", [INF, 100.0])
+def test_an_open_gate_passes_bad_tokens_over(dev, B, T, C, opened):
+    """a token with f = +inf leaves the state as it is, whatever x holds, and gets no gradient"""
+    f, x, h0, dh = _data(B, T, C, 22)
+    f3, x3 = f.view(B, T, C), x.view(B, T, C)
+    at = list(range(1, T, 5)) + [T - 1]
+    f3[:, at] = opened
+    want, tol = _reference(B, f, x, h0, dh)
+    x3[:, at[::2]], x3[:, at[1::2]] = float("nan"), -INF
+    h, df, dx, dh0 = _empty(B * T, C), _empty(B * T, C), _empty(B * T, C), _empty(B, C)
+    K.gated_scan_fwd(B, f, x, h, h0=h0)
+    K.gated_scan_bwd(B, f, x, h, dh, df, dx, h0=h0, dh0=dh0)
+    for t, k in ((h, "h"), (dx, "dx"), (dh0, "dh0")):
+        _close(t, want[k], tol[k], k)
+    skipped = torch.zeros(B, T, C, dtype=torch.bool, device="cuda:0")
+    skipped[:, at] = True
+    skipped = skipped.view(-1, C)
+    assert not df[skipped].any() and not dx[skipped].any()
+    ratio = (df.double() - want["df"]).abs() / (tol["df"] + 1e-37)
+    assert bool((ratio[~skipped] <= 1).all())
+
+
+def test_bad_values_go_on_to_the_end(dev):
+    """without a closed gate an infinity or NaN reaches every token behind it, also where
+    the product of the gates between has come to 0 in fp32, and NaN gates too"""
+    T, C = 20000, 64
+    f, x, h0, dh = _data(1, T, C, 23, keep=-1.0)
+    x[5, ::2] = INF
+    f[17, 1::2] = float("nan")
+    dh[T - 9] = float("nan")
+    h, df, dx, dh0 = _empty(T, C), _empty(T, C), _empty(T, C), _empty(1, C)
+    K.gated_scan_fwd(1, f, x, h, h0=h0)
+    K.gated_scan_bwd(1, f, x, h, dh, df, dx, h0=h0, dh0=dh0)
+    assert bool(torch.isfinite(h[:5]).all()) and not bool(torch.isfinite(h[17:]).any())
+    assert bool(torch.isfinite(dx[T - 8:]).all()) and not bool(torch.isfinite(dx[:T - 8]).any())
+    assert not bool(torch.isfinite(dh0).any())
 
 
 def test_nothing(dev):
