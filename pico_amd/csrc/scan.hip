@@ -28,13 +28,16 @@ typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kThreads = 256, kWaves = kThreads / 64, LT = 4;  // LT steps a thread
 
-// s = sigmoid(f) and q = 1 - s = sigmoid(-f), each to its own last bits: the
-// smaller one is not got by subtraction.  With t = exp(-|f|) they are 1 / (1 + t) and
-// t / (1 + t).  t is 2^(-|f| log2 e) with what the exponent's product rounds off put
-// back to first order (|f| below 200, beyond which t is 0), the quotient the
-// hardware's reciprocal after one step of Newton's: both within 2 ulp, in half the
-// instructions of expf and a division, which bound the kernels (47 a value in
-// all, 8192 x 768 forward and backward 19 + 35 us; now 28).
+// s = sigmoid(f) and q = 1 - s = sigmoid(-f): with t = exp(-|f|) they are 1 / (1 + t) and
+// t / (1 + t), the smaller one not got by subtraction.  t is 2^(-|f| log2 e), log2 e in two
+// parts as in Cody and Waite's reduction, with what the exponent's product rounds off put
+// back to first order (|f| below 200, beyond which t is 0); the quotient is the
+// hardware's reciprocal after one step of Newton's.  That is half the instructions of expf
+// and a division, which bound the kernels (47 a value in all, 8192 x 768 forward and
+// backward 19 + 35 us; now 28).  With u = 2^-24, exp2 and the reciprocal within an ulp (2 u):
+// t is off by 2 u and a rounding, 1 + t by half of that at most and a rounding, so the
+// larger one by 3.5 u, the smaller by 6 u (2.0 and 4.1 at most over 4 million f).  From |f| =
+// 87.34 on, where t is below 2^-126, exp2 gives 0, and so is the smaller one.
 __device__ __forceinline__ void gate(float f, float& s, float& q) {
     constexpr float kLog2e = 1.44269502162933349609375f, kLow = 1.925963033500011079e-8f;
     float a = fabsf(f);

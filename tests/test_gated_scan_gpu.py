@@ -98,6 +98,28 @@ def test_forward_and_gradients(dev, B, T, C, state):
         assert bool((t == 7.0).all())  # nothing behind the outputs is written
 
 
+
+@pytest.mark.parametrize("lo,hi", [(0.0, 1.0), (1.0, 20.0), (20.0, 87.3), (87.3, 110.0)])
+def test_the_gates_themselves(dev, lo, hi):
+    """s and 1 - s over the range of f, read off single tokens: a state of 1 with x = 0 and
+    an empty one with x = 1.  The larger is within 3.5 u of itself (two roundings and half
+    of the exponential's 3 u, which are an ulp of the hardware's and a rounding), the
+    smaller within 6 u (those 3 u, which 1 + t takes part of back, and three roundings), or
+    0 below 2^-126"""
+    C = 1 << 20
+    g = torch.Generator(device="cuda:0").manual_seed(5)
+    f = torch.rand(1, C, device="cuda:0", generator=g) * (hi - lo) + lo
+    f[:, ::2] *= -1
+    one, zero, s, q = (torch.full((1, C), v, device="cuda:0") for v in (1.0, 0.0, 7.0, 7.0))
+    K.gated_scan_fwd(1, f, zero, s, h0=one)
+    K.gated_scan_fwd(1, f, one, q)
+    for got, want, large in ((s, torch.sigmoid(f.double()), f >= 0), (q, torch.sigmoid(-f.double()), f < 0)):
+        off = (got.double() - want).abs()
+        assert bool((off[large] <= 3.5 * U * want[large]).all())
+        assert bool((off[~large] <= 6 * U * want[~large] + 2.0 ** -126).all())
+        assert bool((got[~large & (f.abs() >= 87.34)] == 0).all())
+
+
 def _chain(a, b):
     """y_t = a_t y_{t-1} + b_t along dim 0 from zero, in log2(T) passes"""
     step = 1
