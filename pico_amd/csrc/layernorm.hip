@@ -142,18 +142,17 @@ __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void layernorm_fwd(int R, int
     }
 }
 
-// dx of every row, and the workgroup's part of dg and db in ws [P][2][C] (or, P = 1,
-// dg and db themselves): a workgroup of 8 waves walks rows 8 / W at a time, its
+// dx of every row, and the workgroup's part of dg and db in ws [P][2][C]: a workgroup of 8 waves walks rows 8 / W at a time, its
 // lanes keeping the sums of their own columns; at the end the row groups' sums meet
 // in LDS, in a fixed order.
 constexpr int kBwdWaves = 8;
-enum { kDx = 1, kSums = 2, kDirect = 4 };
+enum { kDx = 1, kSums = 2 };
 
 template <int NV, int W, bool EXACT, bool IN>
 __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
     int R, int C, const float* __restrict__ x, const float* __restrict__ g,
     const float* __restrict__ mean, const float* __restrict__ rstd, const float* __restrict__ dy,
-    const float* dxin, float* dx, float* __restrict__ ws, float* dg, float* db, int what, int flags) {
+    const float* dxin, float* dx, float* __restrict__ ws, int what) {
     constexpr int ROWS = kBwdWaves / W;
     __shared__ float part[2][ROWS][W][2];
     extern __shared__ float sums[];  // [ROWS / 2][2][C]
@@ -288,16 +287,76 @@ __global__ __launch_bounds__(64 * kBwdWaves) void layernorm_bwd(
 #pragma unroll
         for(int i = 0; i < 4; ++i) {
             if(!me.own(v, i)) continue;
-            const int c = me.at[v] + i;
-            if(what & kDirect) {
-                if(dg) dg[c] = (flags & PK_ACCUM2) ? dg[c] + sg[v][i] : sg[v][i];
-                if(db) db[c] = (flags & PK_ACCUM3) ? db[c] + sb[v][i] : sb[v][i];
-            } else {
-                float* out = ws + (int64_t)blockIdx.x * 2 * C;
-                out[c] = sg[v][i];
-                out[C + c] = sb[v][i];
-            }
+            float* const out = ws + (int64_t)blockIdx.x * 2 * C + me.at[v] + i;
+            out[0] = sg[v][i];
+            out[C] = sb[v][i];
         }
+}
+
+// ------------------------------------------------------------ few values
+// dx, dg and db in one launch, where x and dy are so few that reading them twice costs
+// less than a second launch: the first row_blocks workgroups have the rows' dx, NW waves
+// to a row, the others the sums over all rows of `cols` columns each (16 to 64, a power of
+// two, fewer of narrower rows), their threads a row apart, added in a fixed order.
+constexpr int kFewThreads = 512;
+
+template <int NW>
+__global__ __launch_bounds__(kFewThreads) void layernorm_bwd_few(
+    int R, int C, int row_blocks, int cols, const float* __restrict__ x, const float* __restrict__ g,
+    const float* __restrict__ mean, const float* __restrict__ rstd, const float* __restrict__ dy,
+    const float* dxin, float* dx, float* dg, float* db, int flags) {
+    __shared__ float part[2][kFewThreads];
+    const int t = threadIdx.x;
+    if((int)blockIdx.x < row_blocks) {
+        const int row = blockIdx.x * (kFewThreads / 64 / NW) + t / (64 * NW), at = t % (64 * NW);
+        if(NW == 1 && row >= R) return;  // (of several waves each workgroup has one row)
+        const float *xr = x + row * C, *dr = dy + row * C;
+        const float m = mean[row], r = rstd[row];
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll 2
+        for(int c = at; c < C; c += 64 * NW) {
+            const float v = g[c] * dr[c];
+            s1 += v;
+            s2 = fmaf(v, (xr[c] - m) * r, s2);
+        }
+        if constexpr(NW == 1) {
+            s1 = pk::wave_sum(s1);
+            s2 = pk::wave_sum(s2);
+        } else {
+            s1 = pk::block_sum<NW>(s1, part[0]);
+            s2 = pk::block_sum<NW>(s2, part[1]);
+        }
+        s1 /= (float)C;
+        s2 /= (float)C;
+#pragma unroll 2
+        for(int c = at; c < C; c += 64 * NW) {
+            const float v = r * (g[c] * dr[c] - s1 - (xr[c] - m) * r * s2);
+            dx[row * C + c] = dxin ? dxin[row * C + c] + v : v;
+        }
+        return;
+    }
+    const int c = ((int)blockIdx.x - row_blocks) * cols + t % cols;
+    float sg = 0.0f, sb = 0.0f;
+    if(c < C) {
+#pragma unroll 4
+        for(int row = t / cols; row < R; row += kFewThreads / cols) {
+            const float d = dy[row * C + c];
+            sg = fmaf(d, (x[row * C + c] - mean[row]) * rstd[row], sg);
+            sb += d;
+        }
+    }
+    part[0][t] = sg;
+    part[1][t] = sb;
+    for(int o = kFewThreads / 2; o >= cols; o /= 2) {
+        __syncthreads();
+        if(t < o) {
+            part[0][t] += part[0][t + o];
+            part[1][t] += part[1][t + o];
+        }
+    }
+    if(t >= cols || c >= C) return;
+    if(dg) dg[c] = (flags & PK_ACCUM2) ? dg[c] + part[0][t] : part[0][t];
+    if(db) db[c] = (flags & PK_ACCUM3) ? db[c] + part[1][t] : part[1][t];
 }
 
 // ------------------------------------- rows of fewer than 4 or too many values
@@ -429,15 +488,19 @@ void with_shape(int64_t C, F f) {
 
 bool cached(int64_t C) { return C >= 4 && C <= 16384; }
 
-// the workgroups of the backward, each of which leaves a partial sum: one on every
-// CU at most (8192x4096 67 us, two 75; of short rows two: 65536x128 25, one 32), and
-// one in all of few values, where the launch that is saved (3 us of the host's) counts
-// for more than the turns: in a graph 16x768 6.4 us, two launches 6.8, 32x512 6.9 and
-// 6.2, 64x128 8.4 and 5.8, 64x512 10.2 and 6.3; called one by one with the forward
-// 64x128 15.5 and 18.3
+// One launch for all the gradients of up to 16384 values, us in a graph, against partial
+// sums and a launch that adds them: 1x64 2.5 and 3.6, 16x768 3.0 and 7.1, 64x128 3.0 and 5.8,
+// 128x128 3.0 and 5.9, 1024x16 4.7 and 5.7, 4096x4 5.4 and 7.5, 2000x5 5.1 and 7.7; a launch
+// less is 2 us less of the host's time as well.  It would gain up to 1024 rows of 2^19
+// values (64x4096 4.6 and 9.4, 512x1024 5.0 and 7.2; 2048x64 7.3 and 6.6, 8192x8 12.1 and
+// 8.0), but a row's dx has the same bits among any number of rows above this limit.
+bool few(int64_t R, int64_t C) { return cached(C) && R * C <= 16384; }
+
+// the workgroups of the backward of more, each of which leaves a partial sum: one on every
+// CU at most (8192x4096 67 us, two 75; of short rows two: 65536x128 25, one 32)
 int64_t parts_of(int64_t R, int64_t C) {
+    if(few(R, C)) return 1;
     const int64_t rows = !cached(C) ? 1 : C <= 768 ? 8 : C <= 2048 ? 4 : C <= 4096 ? 2 : 1;
-    if(cached(C) && R * C <= 16384) return 1;
     const int64_t p = (R + rows - 1) / rows;
     const int64_t most = C <= 256 ? 512 : 256;
     return p < most ? p : most;
@@ -499,21 +562,35 @@ extern "C" int pk_layernorm_bwd_f32(int64_t R, int64_t C, const float* x, const 
     hipStream_t st = pk::as_stream(stream);
     float* ws = static_cast<float*>(workspace);
     const int64_t P = R > 0 ? parts_of(R, C) : 0;
+    if(R > 0 && !dx && !sums) return PK_OK;
+    if(R > 0 && few(R, C)) {
+        int cols = 64;
+        while(cols > 16 && kFewThreads / cols < R) cols /= 2;
+        while(cols / 2 >= C) cols /= 2;
+        const int rows = C <= 512 ? kFewThreads / 64 : 1, row_blocks = dx ? (int)((R + rows - 1) / rows) : 0;
+        const unsigned grid = (unsigned)(row_blocks + (sums ? (C + cols - 1) / cols : 0));
+        auto launch = [&](auto kernel) {
+            kernel<<<grid, kFewThreads, 0, st>>>((int)R, (int)C, row_blocks, cols, x, g, mean, rstd, dy, dx_in, dx,
+                                                 dg, db, flags);
+        };
+        if(rows > 1) launch(layernorm_bwd_few<1>);
+        else launch(layernorm_bwd_few<kFewThreads / 64>);
+        return pk::launch_status("pk_layernorm_bwd_f32");
+    }
     if(R > 0 && cached(C)) {
-        if(!dx && !sums) return PK_OK;
-        const int what = (dx ? kDx : 0) | (sums ? kSums : 0) | (P == 1 ? kDirect : 0);
+        const int what = (dx ? kDx : 0) | (sums ? kSums : 0);
         with_shape<true>(C, [&](auto nv, auto w, auto exact) {
             constexpr int N = decltype(nv)::value, W = decltype(w)::value;
             constexpr bool EXACT = decltype(exact)::value;
             const size_t lds = kBwdWaves / W / 2 * 2 * (size_t)C * sizeof(float);
             if(dx && dx_in)
                 layernorm_bwd<N, W, EXACT, true><<<(unsigned)P, 64 * kBwdWaves, lds, st>>>(
-                    (int)R, (int)C, x, g, mean, rstd, dy, dx_in, dx, ws, dg, db, what, flags);
+                    (int)R, (int)C, x, g, mean, rstd, dy, dx_in, dx, ws, what);
             else
                 layernorm_bwd<N, W, EXACT, false><<<(unsigned)P, 64 * kBwdWaves, lds, st>>>(
-                    (int)R, (int)C, x, g, mean, rstd, dy, nullptr, dx, ws, dg, db, what, flags);
+                    (int)R, (int)C, x, g, mean, rstd, dy, nullptr, dx, ws, what);
         });
-        if(sums && P > 1)
+        if(sums)
             layernorm_sum<<<(unsigned)((2 * C + 63) / 64), 64 * kSumWaves, 0, st>>>(P, C, ws, dg, db, flags);
         return pk::launch_status("pk_layernorm_bwd_f32");
     }

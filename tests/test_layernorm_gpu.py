@@ -93,6 +93,65 @@ def test_forward_and_gradients(dev, R, C, bias):
         assert bool((t == 7.0).all())  # nothing behind the outputs is written
 
 
+
+# one launch for all the gradients up to 16384 values, and just past that
+FEW = [(1, 4), (1, 16384), (4096, 4), (4097, 4), (3276, 5), (2000, 5), (1024, 16), (256, 64), (257, 64), (31, 512),
+       (31, 528), (33, 496), (15, 1024), (17, 1024), (2, 8192), (3, 5003), (29, 131)]
+
+
+@pytest.mark.parametrize("R,C", FEW)
+def test_gradients_of_few_values(dev, R, C):
+    """all three at once, each by itself, and added to what is there: the same bits"""
+    x, g, b, dy = _data(R, C, R * 3 + C)
+    want, tol = _reference(x, g, b, dy)
+    y, mean, rstd = _empty(R, C), _empty(R), _empty(R)
+    K.layernorm_fwd(x, g, b, y, mean, rstd, EPS)
+    dx, dg, db = _empty(R + 1, C), _empty(C + 1), _empty(C + 1)
+    K.layernorm_bwd(x, g, mean, rstd, dy, dx[:R], dg[:C], db[:C])
+    for t, k in ((dx[:R], "dx"), (dg[:C], "dg"), (db[:C], "db")):
+        _close(t, want[k], tol[k], k)
+    for t in (dx[R], dg[C], db[C]):
+        assert bool((t == 7.0).all())
+    for n in range(3):
+        one = [torch.full_like(t, 5.0) if i == n else None for i, t in enumerate((dx[:R], dg[:C], db[:C]))]
+        K.layernorm_bwd(x, g, mean, rstd, dy, *one)
+        assert torch.equal(one[n], (dx[:R], dg[:C], db[:C])[n])
+    base = [torch.randn_like(t) for t in (dg[:C], db[:C])]
+    acc, inplace = [t.clone() for t in base], torch.randn_like(dx[:R])
+    given = inplace.clone()
+    K.layernorm_bwd(x, g, mean, rstd, dy, inplace, *acc, dx_in=inplace, accum_dg=True, accum_db=True)
+    assert torch.equal(acc[0], base[0] + dg[:C]) and torch.equal(acc[1], base[1] + db[:C])
+    # one more rounding, of the sum
+    assert bool(((inplace - (given + dx[:R])).abs() <= 3 * U * (given.abs() + dx[:R].abs())).all())
+
+
+def test_many_short_rows_take_no_longer_than_a_square(dev):
+    """16384 values as 4096 rows of 4 and as 64 of 256, the backward in a graph: by rows one
+    after another the first would take 40 times the second"""
+    times = []
+    for R, C in ((4096, 4), (64, 256)):
+        x, g, b, dy = _data(R, C, 1)
+        y, mean, rstd, dx, dg, db = _empty(R, C), _empty(R), _empty(R), _empty(R, C), _empty(C), _empty(C)
+        ws = torch.empty(K.layernorm_bwd_workspace(R, C), dtype=torch.uint8, device="cuda:0")
+        K.layernorm_fwd(x, g, b, y, mean, rstd, EPS)
+        K.layernorm_bwd(x, g, mean, rstd, dy, dx, dg, db, ws=ws)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                K.layernorm_bwd(x, g, mean, rstd, dy, dx, dg, db, ws=ws)
+        best = 1e9
+        for _ in range(5):
+            a, z = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            graph.replay()
+            z.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(z))
+        times.append(best)
+    assert times[0] < 8 * times[1], times
+
+
 @pytest.mark.parametrize("R,C", [(64, 128), (50, 1503), (300, 768), (9, 4096), (3, 20001)])
 def test_accumulation_and_single_gradients(dev, R, C):
     x, g, b, dy = _data(R, C, 5)
