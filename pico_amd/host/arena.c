@@ -267,7 +267,7 @@ void* arena_alloc(struct Arena* a, size_t size) {
     return p;
 }
 
-void* arena_alloc_device(struct Arena* a, size_t size) {
+void* pkh_arena_alloc_with(struct Arena* a, size_t size, void* (*device_alloc)(size_t)) {
     if(!a) return NULL;
     size = (size + DEV_ALIGN - 1) & ~(size_t)(DEV_ALIGN - 1);
     if(size == 0) size = DEV_ALIGN;
@@ -283,10 +283,9 @@ void* arena_alloc_device(struct Arena* a, size_t size) {
         size_t cap = st->dev_block_bytes > size ? st->dev_block_bytes : size;
         struct PicoDeviceBlock* nb = (struct PicoDeviceBlock*)calloc(1, sizeof(*nb));
         if(!nb) return NULL;
-        nb->bottom = (unsigned char*)pkh_device_alloc(cap);
+        nb->bottom = (unsigned char*)device_alloc(cap);
         if(!nb->bottom) {
             free(nb);
-            PKH_ERR("arena: device memory exhausted (%zu bytes requested)\n", size);
             return NULL;
         }
         nb->capacity = cap;
@@ -302,6 +301,12 @@ void* arena_alloc_device(struct Arena* a, size_t size) {
     st->dev_end = b;
     void* p = b->bottom + b->used;
     b->used += size;
+    return p;
+}
+
+void* arena_alloc_device(struct Arena* a, size_t size) {
+    void* p = pkh_arena_alloc_with(a, size, pkh_device_alloc);
+    if(a && !p) PKH_ERR("arena: device memory exhausted (%zu bytes requested)\n", size);
     return p;
 }
 

@@ -24,7 +24,7 @@ static int rows_of(const struct PicoTensor* t, int64_t rows) {
 
 /* ------------------------------------------------------------- the router
  * gates [R, k] = softmax over the k largest of the E logits */
-enum { RS_ROUTE = 0, ES_WS = 1 };
+enum { RS_ROUTE = 0, ES_ARENA = 1, ES_WS = 2 };
 
 static void route_backward(struct PicoTensor* self) {
     const struct PicoRoute* r = (const struct PicoRoute*)pkh_node(self)->saved[RS_ROUTE];
@@ -129,15 +129,19 @@ struct PicoTensor* pico_expert_gather(struct PicoTensor* x, const struct PicoRou
 enum { EI_PREC = 0 };
 
 static int expert_dw(struct PicoTensor* self, const float* g, int flags, pk_stream_t stream) {
-    const struct PkNode* n = pkh_node(self);
+    struct PkNode* n = pkh_node(self);
     const struct PicoRoute* r = (const struct PicoRoute*)n->saved[RS_ROUTE];
     const struct PicoTensor *x = self->parents[0], *w = self->parents[1];
     const int64_t rows = x->shape[0], K = w->shape[1], N = w->shape[2];
+    /* (up to 64 MiB where the rows are split, so only now that there is a backward; in the
+     * node's arena, so that captured graphs share none; without it the rows are not split) */
+    const size_t ws_bytes = pk_gemm_experts_dw_workspace(rows, K, N, r->E);
+    if(ws_bytes && !n->saved[ES_WS])
+        n->saved[ES_WS] = pkh_arena_workspace_opt((struct Arena*)n->saved[ES_ARENA], ws_bytes);
     return pkh_status("pico_expert_matmul_backward",
                       pk_gemm_experts_dw_f32(rows, K, N, r->E, r->offsets, x->data, x->strides[0], g,
                                              N, w->grad, N, K * N, flags, (int)n->ival[EI_PREC],
-                                             n->saved[ES_WS],
-                                             pk_gemm_experts_dw_workspace(rows, K, N, r->E), stream));
+                                             n->saved[ES_WS], n->saved[ES_WS] ? ws_bytes : 0, stream));
 }
 
 /* dW of a parameter goes to the side stream, beside dX and what follows it, in the
@@ -207,9 +211,7 @@ struct PicoTensor* pico_expert_matmul(struct PicoTensor* x, struct PicoTensor* w
                                  N, K * N, out->data, N, 0, (int)n->ival[EI_PREC], pkh_stream());
     if(pkh_status("pico_expert_matmul", st)) return NULL;
     n->saved[RS_ROUTE] = (void*)r;
-    /* (of the node's own, so captured graphs share none; small where rows split) */
-    const size_t ws_bytes = pk_gemm_experts_dw_workspace(rows, K, N, r->E);
-    if(ws_bytes && !(n->saved[ES_WS] = arena_alloc_device(arena, ws_bytes))) return NULL;
+    n->saved[ES_ARENA] = arena;
     struct PicoTensor* ps[2] = {x, w};
     pkh_set_parents(arena, out, 2, ps, expert_matmul_backward);
     return out;

@@ -103,6 +103,10 @@ void pkh_device_free(void* p);
  * previous contents are not preserved); valid until the next call */
 void* pkh_workspace(size_t bytes);
 void* pkh_workspace_opt(size_t bytes); /* optional: NULL without a recorded error */
+/* device memory of an arena's, from `device_alloc` where its blocks have no room (arena.c) */
+void* pkh_arena_alloc_with(struct Arena* a, size_t size, void* (*device_alloc)(size_t));
+/* a workspace in an arena, for a caller with a fallback: NULL without a recorded error */
+void* pkh_arena_workspace_opt(struct Arena* a, size_t bytes);
 int pkh_is_device_ptr(const void* p);
 int pkh_copy_h2d(void* dst, const void* src, size_t bytes);
 int pkh_copy_d2h(void* dst, const void* src, size_t bytes);

@@ -318,6 +318,18 @@ void* pkh_workspace_opt(size_t bytes) {
                           "growing the GEMM workspace");
 }
 
+/* device memory without an error where there is none to be had; under capture nothing is
+ * allocated, and the capture goes on */
+static void* device_alloc_opt(size_t bytes) { return g_capturing ? NULL : device_alloc(bytes, 1); }
+
+void* pkh_arena_workspace_opt(struct Arena* a, size_t bytes) {
+    if(g_fail_opt_ws > 0) {
+        g_fail_opt_ws--;
+        return NULL;
+    }
+    return pkh_arena_alloc_with(a, bytes, device_alloc_opt);
+}
+
 int pkh_is_device_ptr(const void* p) {
     if(!p || pkh_init()) return 0;
     hipPointerAttribute_t attr;

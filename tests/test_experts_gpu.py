@@ -740,3 +740,66 @@ def test_pico_shared_weights_padding_and_two_backwards(P):
     assert not P.grad_value(zp)[30:].any()
     for t in ps:
         P.free(t)
+
+
+def test_pico_weight_gradient_workspace(P):
+    """the workspace of split weight gradients is taken by the backward, not by the forward;
+    where it cannot be had, or under capture, the rows are not split and nothing fails"""
+    R, E, kk, nn = 4096, 4, 96, 128
+    g = _gen(13)
+    z, x = torch.randn(R, E, generator=g), torch.randn(R, kk, generator=g)
+    w = torch.randn(E, kk, nn, generator=g)
+    need = K.gemm_experts_dw_workspace(R, kk, nn, E)
+    assert need > 2 << 20
+    zp, xp, wp = (P.param(list(t.shape), t.numpy()) for t in (z, x, w))
+    xr = x.double()
+
+    def check():
+        got = torch.from_numpy(P.grad_value(wp))
+        for e in range(E):
+            a = xr[offsets[e]:offsets[e + 1]]
+            want, mag = a.sum(0)[:, None].expand(kk, nn), a.abs().sum(0)[:, None].expand(kk, nn)
+            _close(got[e], want, _factor(len(a), "fp32") * mag, e)
+
+    opt = P.lib.pico_optim_sgd_init(0.0)
+    P.lib.pico_optim_sgd_add(opt, wp)
+    with P.arena(1 << 20) as arena:
+        _, route = P.route_topk(zp, 1)
+        _, offsets = P.route_to_host(route, R, 1, E)
+        before = P.memory()[0]
+        y = P.expert_matmul(xp, wp, route)
+        # its values and gradients, each in a block of its own
+        assert P.memory()[0] - before <= 2 * 4 * R * nn + 4096
+        before = P.memory()[0]
+        P.lib.pico_gpu_fail_next_workspaces(1)
+        P.backward(y)
+        P.lib.pico_gpu_fail_next_workspaces(0)
+        assert P.memory()[0] == before and not P.lib.pico_gpu_last_error()
+        check()
+        P.lib.pico_optim_sgd_zero_grad(opt)
+        y = P.expert_matmul(xp, wp, route)
+        before = P.memory()[0]
+        P.backward(y)
+        assert P.memory()[0] - before >= need
+        check()
+        # captured with no room for it: the forward's blocks are there, the workspace is not
+        with P.arena(1 << 20) as other:
+            P.expert_matmul(xp, wp, route)
+            P.reset(other)
+            P.lib.pico_optim_sgd_zero_grad(opt)
+            P.sync()
+            before = P.memory()[0]
+            assert P.lib.pico_graph_begin() == 0
+            P.lib.pico_optim_sgd_zero_grad(opt)
+            y = P.expert_matmul(xp, wp, route)
+            P.lib.pico_backward(other, y)
+            graph = P.lib.pico_graph_end()
+            assert graph, P.lib.pico_gpu_last_error()
+            assert P.memory()[0] == before
+            for _ in range(3):
+                assert P.lib.pico_graph_launch(graph) == 0
+                check()
+            P.lib.pico_graph_free(graph)
+    P.lib.pico_optim_sgd_free(opt)
+    for t in (zp, xp, wp):
+        P.free(t)
