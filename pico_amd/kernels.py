@@ -23,9 +23,11 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-# the current stream's handle on a device (what torch.cuda.current_stream() wraps, at
-# 0.1 us rather than 3)
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# the current device, and the current stream's handle on one: what torch.cuda's calls of
+# these names wrap, at 0.1 us rather than 1 and 3; where a build of torch has others, those
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _stream():
@@ -687,7 +689,6 @@ def embed_bwd(ids, dout, dtable):
 ACCUM3 = 4
 PRECISIONS = {"fp32": 0, "bf16": 1, "bf16x3": 2}
 _F32, _I32 = torch.float32, torch.int32
-_device = torch._C._cuda_getDevice
 
 
 def _refuse(t, dtype, dev):
