@@ -242,7 +242,7 @@ struct PicoTensor* pico_expert_combine(struct PicoTensor* ys, struct PicoTensor*
        (c && pkh_need_gpu("pico_expert_combine", c)))
         return NULL;
     if(!r || !rows_of(ys, r->R * r->k) || !rows_of(gates, r->R) || gates->shape[1] != r->k ||
-       (r->R > 1 && gates->strides[0] != r->k) || ys == gates) {
+       (r->R > 1 && gates->strides[0] != r->k) || pkh_one_grad(ys, gates)) {
         PKH_ERR("expert_combine expects a route, its rows [tokens*k, d] and contiguous gates "
                 "[tokens, k]!\n");
         return NULL;

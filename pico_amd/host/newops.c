@@ -230,7 +230,8 @@ struct PicoTensor* pico_layernorm(struct PicoTensor* x, struct PicoTensor* gain,
        (bias && pkh_need_gpu("pico_layernorm", bias)))
         return NULL;
     if(x->ndim < 1 || gain->numel != x->shape[x->ndim - 1] || gain->numel < 1 ||
-       (bias && bias->numel != gain->numel) || x == gain || x == bias || gain == bias ||
+       (bias && bias->numel != gain->numel) || pkh_one_grad(x, gain) || pkh_one_grad(x, bias) ||
+       pkh_one_grad(gain, bias) ||
        !contiguous(x) || !contiguous(gain) || (bias && !contiguous(bias))) {
         PKH_ERR("layernorm expects contiguous, different x [rows, C], gain [C] and bias [C] (or "
                 "NULL)!\n");
@@ -277,7 +278,7 @@ static void gated_scan_backward(struct PicoTensor* self) {
      * call each, the later ones accumulating */
     struct PicoTensor* const ps[3] = {f, x, h0};
     const int bit[3] = {PK_ACCUM, PK_ACCUM2, PK_ACCUM3};
-    const int apart = f != x && f != h0 && x != h0;
+    const int apart = !pkh_one_grad(f, x) && !pkh_one_grad(f, h0) && !pkh_one_grad(x, h0);
     for(int pass = 0; pass < (apart ? 1 : 3); pass++) {
         float* g[3] = {NULL, NULL, NULL};
         int flags = 0;

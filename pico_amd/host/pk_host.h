@@ -176,6 +176,13 @@ static inline const float* pkh_grad_base(struct PicoTensor* t) {
     }
     return pkh_grad_flag(t) ? t->grad : NULL;
 }
+/* whether a and b have one grad buffer: the same tensor, or a tensor and its only
+ * column-block view (a kernel that writes both gradients at once would lose one) */
+static inline int pkh_one_grad(const struct PicoTensor* a, const struct PicoTensor* b) {
+    if(!a || !b) return 0;
+    const struct PkNode *na = pkh_node(a), *nb = pkh_node(b);
+    return (na && na->own_grad ? na->own_grad : a->grad) == (nb && nb->own_grad ? nb->own_grad : b->grad);
+}
 static inline void pkh_grad_mark(struct PicoTensor* t) {
     struct PkNode* n = pkh_node(t);
     if(n) n->grad_live = 1;

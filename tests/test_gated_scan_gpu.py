@@ -534,3 +534,39 @@ def test_pico_shared_operands_and_refusals(P):
             with pytest.raises(PicoError):
                 P.last_token(*bad)
     P.free(t)
+
+
+def test_pico_a_tensor_and_its_only_view(P):
+    """a projection and the one column view of it share a gradient, to which each adds"""
+    B, C = 4, 6
+    f, x, h0, dh = (t.cpu() for t in _data(B, 1, C, 7))
+    v = x.double().requires_grad_()
+    s = torch.sigmoid(v)
+    ((s * h0.double() + (1 - s) * v) * dh.double()).sum().backward()
+    ((lambda u: torch.sigmoid(u) * u + (1 - torch.sigmoid(u)) * x.double())(v) * dh.double()).sum().backward()
+    leaf, sp = P.param([B, C], x.numpy()), P.param([B, C], h0.numpy())
+    one = P.param([C], np.ones(C, np.float32))
+    with P.arena():
+        for operands in (lambda t, u: (t, u, sp), lambda t, u: (t, sp, u)):
+            t = P.matmul(leaf, P.tensor([C, C], np.eye(C)))
+            f_, x_, h_ = operands(t, P.split_cols(t, 1)[0])
+            if x_ is sp:  # the token itself as the state, and another one's values
+                x_ = P.tensor([B, C], x.numpy())
+            P.backward(P.mul(P.gated_scan(f_, x_, h_, B), P.tensor([B, C], dh.numpy())))
+        got = torch.from_numpy(P.grad_value(leaf))
+        # four gradients of at most (1 + |x| + |h0|) |dh| each
+        assert bool(((got - v.grad).abs() <= 100 * U * (1 + x.abs() + h0.abs()) * dh.abs()).all())
+        row = P.matmul(P.tensor([1, C], np.ones((1, C))), P.tensor([C, C], np.eye(C)))
+        view = P.split_cols(row, 1)[0]
+        for bad in ((row, view, one), (view, row, None), (P.tensor([3, C]), row, view)):
+            with pytest.raises(PicoError):
+                P.layernorm(*bad, 1e-5)
+        col = P.matmul(P.tensor([B, C], np.ones((B, C))), P.tensor([C, 1], np.ones((C, 1))))
+        gates, route = P.route_topk(P.tensor([B, 2], np.zeros((B, 2))), 1)
+        with pytest.raises(PicoError):
+            P.expert_combine(col, P.split_cols(col, 1)[0], route, None)
+        # two views of one tensor have columns of their own
+        two = P.split_cols(P.matmul(P.tensor([B, C], np.ones((B, C))), P.tensor([C, 2 * C], np.ones((C, 2 * C)))), 2)
+        P.gated_scan(two[0], two[1], None, B)
+    for t in (leaf, sp, one):
+        P.free(t)
