@@ -353,10 +353,15 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     const int64_t groups = E < n ? E : n;
     ExpertShape rest;
     const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K, &rest);
-    // (the estimates are of up to 128 rows to an expert, 64 in bf16; 32 columns to a workgroup where 64
-    // would leave half of the chip idle: 8 experts [2048, 768] with a row each 8.6 us, of
-    // 64 columns 10.6, with 4 rows 14.4 and 13.7; 2 experts [4096, 768] 12.3, 16.5)
-    const int cl = thin_tiles((double)groups, (double)n / groups) * (double)((N + 63) / 64) < 144.0 ? 8 : 16;
+    // (the estimates are of up to 128 rows to an expert, 64 in bf16.  32 columns to a workgroup
+    // where 64 would leave much of the chip idle, by the estimated tiles of 64; [K, N], rows
+    // of each expert, us with 32 and 64, weights from memory: 96 tiles, 8 [2048, 768] of 1
+    // 14.2 and 17.3, 2 [4096, 2048] of 4 22.1 and 29.1; 128, 8 [768, 1024] of 1 8.7 and 8.9;
+    // 144, 8 [2048, 768] of 4 14.3 and 17.9, of 0 to 9 15.4 and 17.3, 16 [1024, 384] of 4 8.6
+    // and 10.1, 12 [2048, 768] of 1 19.7 and 19.5; 150, 3 [2048, 1280] of 8 13.5 and 16.3;
+    // 154, 8 [2048, 704] of 5 16.3 and 15.0; 156, 13 [2048, 768] of 1 22.6 and 20.2; 192, 8
+    // [2048, 768] of 6 18.2 and 17.0, 8 [768, 1024] of 4 8.6 and 9.1)
+    const int cl = thin_tiles((double)groups, (double)n / groups) * (double)((N + 63) / 64) <= 150.0 ? 8 : 16;
     const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 4 * cl - 1) / (4 * cl);
     const int64_t tiles_t = (N + 63) / 64;
     if(TB && K > 0 && n <= 256 * groups && tiles_t <= kMaxTiles / tiles_m &&

@@ -803,3 +803,22 @@ def test_pico_weight_gradient_workspace(P):
     P.lib.pico_optim_sgd_free(opt)
     for t in (zp, xp, wp):
         P.free(t)
+
+
+@pytest.mark.parametrize("sizes,nn", [([4] * 8, 768), ([0, 1, 2, 3, 4, 6, 7, 9], 768), ([8] * 3, 1280), ([5] * 8, 704),
+                                      ([1] * 13, 768), ([6] * 8, 770)])
+@pytest.mark.parametrize("precision", ["fp32", "bf16"])
+def test_few_rows_of_long_sums(dev, sizes, nn, precision):
+    """a few rows an expert, on both sides of where the columns of a workgroup change"""
+    kk = 2048
+    offsets, n = _offsets(sizes, extra=2)
+    g = _gen(nn + len(sizes))
+    x, w = torch.randn(n, kk, generator=g).cuda(), torch.randn(len(sizes), kk, nn, generator=g).cuda()
+    y = _empty(n, nn)
+    K.gemm_experts("N", x, w, offsets, y, precision=precision)
+    at = offsets.tolist()
+    xr, wr = _rounded(x.cpu(), precision), _rounded(w.cpu(), precision)
+    for e in range(len(sizes)):
+        r = slice(at[e], at[e + 1])
+        _close(y[r], xr[r] @ wr[e], _factor(kk, precision) * (xr[r].abs() @ wr[e].abs()), e)
+    assert not y[at[-1]:].any()
