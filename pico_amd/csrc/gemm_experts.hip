@@ -355,12 +355,14 @@ extern "C" int pk_gemm_experts_f32(char tb, int64_t n, int64_t N, int64_t K, int
     const ExpertShape s = expert_rows_shape(precision, (double)groups, (double)n / groups, N, (double)K, &rest);
     // (the estimates are of up to 128 rows to an expert, 64 in bf16.  32 columns to a workgroup
     // where 64 would leave much of the chip idle, by the estimated tiles of 64; [K, N], rows
-    // of each expert, us with 32 and 64, weights from memory: 96 tiles, 8 [2048, 768] of 1
-    // 14.2 and 17.3, 2 [4096, 2048] of 4 22.1 and 29.1; 128, 8 [768, 1024] of 1 8.7 and 8.9;
-    // 144, 8 [2048, 768] of 4 14.3 and 17.9, of 0 to 9 15.4 and 17.3, 16 [1024, 384] of 4 8.6
-    // and 10.1, 12 [2048, 768] of 1 19.7 and 19.5; 150, 3 [2048, 1280] of 8 13.5 and 16.3;
-    // 154, 8 [2048, 704] of 5 16.3 and 15.0; 156, 13 [2048, 768] of 1 22.6 and 20.2; 192, 8
-    // [2048, 768] of 6 18.2 and 17.0, 8 [768, 1024] of 4 8.6 and 9.1)
+    // of each expert, us with 32 and 64, weights from memory, as in a model of several layers:
+    // 96 tiles, 8 [2048, 768] of 1 14.2 and 17.3, 2 [4096, 2048] of 4 22.1 and 29.1; 128, 8
+    // [768, 1024] of 1 8.7 and 8.9; 144, 8 [2048, 768] of 4 14.3 and 17.9, of 0 to 9 15.4 and
+    // 17.3, 16 [1024, 384] of 4 8.6 and 10.1, 12 [2048, 768] of 1 19.7 and 19.5; 150, 3 [2048,
+    // 1280] of 8 13.5 and 16.3; 154, 8 [2048, 704] of 5 16.3 and 15.0; 156, 13 [2048, 768] of 1
+    // 22.6 and 20.2; 192, 8 [2048, 768] of 6 18.2 and 17.0.  Weights that are still in the
+    // last-level cache differ less: 144 tiles, 8 [2048, 768] of 4 11.8 and 12.5, of 0 to 9
+    // 11.9 and 11.5, 8 [768, 768] of 0 to 9 6.6 and 5.8)
     const int cl = thin_tiles((double)groups, (double)n / groups) * (double)((N + 63) / 64) <= 150.0 ? 8 : 16;
     const int64_t tiles_m = (n + kThinRows - 1) / kThinRows + groups + 1, tiles_n = (N + 4 * cl - 1) / (4 * cl);
     const int64_t tiles_t = (N + 63) / 64;
