@@ -109,6 +109,8 @@ _GPU_SIGS = {
     "pico_graph_free": (None, [c_p]),
     "pico_argmax": (ctypes.c_int, [TP, c_p]),
     "pico_gpu_synchronize": (ctypes.c_int, []),
+    "pico_gpu_stream": (c_p, []),
+    "pico_gpu_set_stream": (None, [c_p]),
     "pico_gpu_last_error": (ctypes.c_char_p, []),
     "pico_gpu_clear_error": (None, []),
     "pico_gpu_fail_next_workspaces": (None, [ctypes.c_int]),
