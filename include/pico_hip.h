@@ -679,7 +679,8 @@ int pk_gated_scan_bwd_f32(int64_t B, int64_t T, int64_t C, const float* f, int64
  *   slots.  dys or dgates may be NULL.
  * pk_gemm_experts_f32: Y[r] (+)= X[r].op(W_e) for the rows r of every expert e, X
  *   [n, K], W_e at W + e*sw: [K, N] for tb 'N', [N, K] for 'T' (row stride ldw), Y
- *   [n, N].  Rows from offsets[E] to n become zero (accumulating: are left).
+ *   [n, N].  Rows from offsets[E] to n become zero (accumulating: are left); rows before
+ *   offsets[0], which a plan has at 0, are left.
  * pk_gemm_experts_dw_f32: dW_e (+)= X_e^T.dY_e, [K, N] at dW + e*sw, an expert without
  *   rows getting zeros.  Where few tiles would leave the chip idle the rows are
  *   split, in pk_gemm_experts_dw_workspace(n, K, N, E) bytes of device workspace (0: no
