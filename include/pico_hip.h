@@ -719,6 +719,85 @@ int pk_gemm_experts_dw_f32(int64_t n, int64_t K, int64_t N, int64_t E, const int
                            int64_t ldw, int64_t sw, int flags, int precision, void* workspace,
                            size_t workspace_bytes, pk_stream_t stream);
 
+/* ---- rotary positions (no reference counterpart) --------------------------
+ * The first rot of a head's hd values are turned in rot / 2 pairs (x1, x2), pair i
+ * of the token at position p by the angle a = p * freqs[i] (radians):
+ *   y1 = m*(x1*cos a - x2*sin a),  y2 = m*(x2*cos a + x1*sin a)
+ * with m = magnitude; the other values are copied.  A pair is (i, i + rot/2) of the
+ * head, or (2i, 2i + 1) when interleaved is not 0.  Angles are computed in 64 bits
+ * (position 2^20 times 1 radian is off by 2^-24 of a turn in 32), their sine and cosine
+ * rounded once.
+ * pk_rope_freqs writes the rot / 2 frequencies into HOST memory (a program copies them to
+ * the device once): base^(-2i/rot), scaled for contexts longer than the trained one:
+ *   PK_ROPE_PLAIN: not;  PK_ROPE_LINEAR: divided by factor;
+ *   PK_ROPE_NTK: base * factor^(rot / (rot - 2)) for base (rot 2: as plain);
+ *   PK_ROPE_PARTS: a pair that turns r = length * f / (2 pi) times within the trained
+ *     length gets f * (g + (1 - g) / factor), g = (r - low) / (high - low) held to [0, 1].
+ * pk_rope_f32: y[t] = x[t] turned, x and y [N, H*hd] with row strides ldx, ldy (column
+ *   blocks of one projection are fine; y may be x).  positions [N], any int32.
+ *   PK_ACCUM: y += ...; PK_ROPE_BACKWARD: turns the other way, which maps the gradient
+ *   of y to that of x. */
+#define PK_ROPE_PLAIN 0
+#define PK_ROPE_LINEAR 1
+#define PK_ROPE_NTK 2
+#define PK_ROPE_PARTS 3
+#define PK_ROPE_BACKWARD 32
+typedef struct PkRope {
+    const double* freqs; /* device memory, rot / 2 values; not read when rot is 0 */
+    int64_t rot;         /* even, 0 to hd */
+    int interleaved;
+    double magnitude;
+} PkRope;
+int pk_rope_freqs(int64_t rot, double base, int scaling, double factor, double length, double low,
+                  double high, double* freqs);
+int pk_rope_f32(int64_t N, int64_t H, int64_t hd, const PkRope* rope, const int32_t* positions,
+                const float* x, int64_t ldx, float* y, int64_t ldy, int flags, pk_stream_t stream);
+
+/* ---- a paged cache of keys and values, held in 8 bits (no reference counterpart) ----
+ * `pages` pages of `page` (16, 32, 64 or 128) tokens.  A page holds, for each of kv_heads
+ * heads, e4m3 values times one power of two each for its keys and its values:
+ *   k [pages][kv_heads][page][hp], v [pages][kv_heads][hp][page] (tokens innermost, as
+ *   the products that read them take them), hp = pk_kv_head_size(hd): hd (1 to 256)
+ *   rounded up to 32, 64, 96, 128 or 256; k's values from hd to hp are zeros, v's rows
+ *   there are not used.  k_exp, v_exp [pages][kv_heads]: e + 127 for the factor 2^e.
+ * B sequences: table [B][width] names the pages of sequence b's tokens 0, page, 2*page..;
+ * lens [B] is how many tokens it held before the call; its new tokens are the rows
+ * offsets[b] .. offsets[b + 1] - 1 of the inputs ([B + 1], not decreasing), at the
+ * positions lens[b], lens[b] + 1, ..  All three are read on the device, so a captured
+ * graph replays with other sequences; the caller advances lens after a step's last layer.
+ * k, v, k_exp, v_exp 16-byte aligned.
+ * What they hold is checked there: rows outside [0, N), positions from width*page on and
+ * pages outside [0, pages) reach no memory out of bounds (such tokens are not kept, and
+ * count as absent when the cache is read).  Pages that sequences share are for reading only.
+ * pk_kv_append_f32 writes the new tokens' keys and values, [N, kv_heads*hd] with row
+ *   strides ldk, ldv; k turned by `rope` at its position (NULL or rot 0: as it is).  A
+ *   page's e is the smallest with all |values| <= 448 * 2^e, from -40 to 40; where it grows
+ *   the values that the page held are rounded again (exact but for those below 2^-6 of the
+ *   new scale), and where a page's first token is written it starts anew.  Infinities do
+ *   not count for e and become +-448 * 2^e, as does what is larger than that; NaN stays
+ *   NaN.  q [N, H*hd], when not NULL, is turned likewise into q_out (row strides ldq, ldqo;
+ *   q_out may be q).  Rows of no sequence are left.
+ * pk_attn_paged_f32: o[t] = softmax(scale * q[t].K^T) V over the positions up to t's own of
+ *   its sequence, which the cache holds already; q, o [N, H*hd] with row strides ldq, ldo,
+ *   head h reading the cache's head h / (H / kv_heads).  A token that finds no key gets
+ *   zeros; rows of no sequence are left.  q enters the products as two f16 values of 22
+ *   bits together, and so do the probabilities; what the cache holds is exact in f16, and
+ *   sums are fp32.  pk_attn_paged_workspace(cache, N, H) bytes of device workspace (0:
+ *   none needed).  Sums in an order that the lengths and the sizes fix. */
+typedef struct PkKvCache {
+    uint8_t *k, *v, *k_exp, *v_exp;
+    const int32_t *table, *lens, *offsets;
+    int64_t pages, kv_heads, hd, page, B, width;
+} PkKvCache;
+int64_t pk_kv_head_size(int64_t hd);
+int pk_kv_append_f32(const PkKvCache* cache, int64_t N, const float* k, int64_t ldk, const float* v,
+                     int64_t ldv, const PkRope* rope, int64_t H, const float* q, int64_t ldq,
+                     float* q_out, int64_t ldqo, pk_stream_t stream);
+size_t pk_attn_paged_workspace(const PkKvCache* cache, int64_t N, int64_t H);
+int pk_attn_paged_f32(const PkKvCache* cache, int64_t N, int64_t H, float scale, const float* q,
+                      int64_t ldq, float* o, int64_t ldo, void* workspace, size_t workspace_bytes,
+                      pk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

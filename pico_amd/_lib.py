@@ -175,6 +175,14 @@ PK_SIGNATURES = {
     "pk_gemm_experts_dw_workspace": [c_i64, c_i64, c_i64, c_i64],
     "pk_gemm_experts_dw_f32": [c_i64, c_i64, c_i64, c_i64, c_p, c_p, c_i64, c_p, c_i64, c_p, c_i64,
                                c_i64, c_int, c_int, c_p, c_size, c_p],
+    "pk_rope_freqs": [c_i64, ctypes.c_double, c_int, ctypes.c_double, ctypes.c_double,
+                      ctypes.c_double, ctypes.c_double, c_p],
+    "pk_rope_f32": [c_i64, c_i64, c_i64, c_p, c_p, c_p, c_i64, c_p, c_i64, c_int, c_p],
+    "pk_kv_head_size": [c_i64],
+    "pk_kv_append_f32": [c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64, c_p, c_i64,
+                         c_p],
+    "pk_attn_paged_workspace": [c_p, c_i64, c_i64],
+    "pk_attn_paged_f32": [c_p, c_i64, c_i64, c_f, c_p, c_i64, c_p, c_i64, c_p, c_size, c_p],
     "pk_last_error": [],
 }
 _RESTYPES = {"pk_last_error": ctypes.c_char_p, "pk_rmsnorm_bwd_workspace": c_size,
@@ -187,7 +195,8 @@ _RESTYPES = {"pk_last_error": ctypes.c_char_p, "pk_rmsnorm_bwd_workspace": c_siz
              "pk_gemm_bf16q_workspace": c_size, "pk_bf16x3q_bytes": c_size,
              "pk_gemm_bf16x3q_workspace": c_size, "pk_layernorm_bwd_workspace": c_size,
              "pk_gated_scan_workspace": c_size, "pk_expert_plan_workspace": c_size,
-             "pk_gemm_experts_dw_workspace": c_size}
+             "pk_gemm_experts_dw_workspace": c_size, "pk_kv_head_size": c_i64,
+             "pk_attn_paged_workspace": c_size}
 
 _hip = None
 

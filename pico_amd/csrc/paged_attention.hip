@@ -1,0 +1,575 @@
+// pico_amd/csrc/paged_attention.hip -- attention of new tokens over a paged cache of e4m3
+// keys and values.
+//
+// A power of two times e4m3 (4 significant bits) is exact in f16, so a product with a key
+// or a value needs no more than the other operand in f16 parts: x = hi + lo, each the
+// nearest f16, keeps 22 bits, which leaves sums of a head's length as near as fp32's own
+// rounding does.  Queries are first brought to [2^14, 2^15) by a power of two a row;
+// probabilities are taken relative to 2^7 below their running maximum: the largest stay in
+// f16's range, one of 2^-10 of it keeps the 22 bits, and smaller ones are off by 2^-32 of it.
+//
+// The scores are computed transposed, S^T = K.Q^T: a column of the result, a query, is in
+// one lane's registers and the three lanes 16 apart, and the tokens that a lane holds are
+// those that it needs as the operand of O^T = V^T.P^T, for which v is stored with its
+// tokens innermost.  So the probabilities stay where they are computed, and keys and values
+// go from memory to the matrix cores without LDS.
+//
+// The value scale 2^ev of a token's page goes into its probability's exponent, and comes
+// out of the sum of probabilities again: p = 2^(s + ev - m), l += p 2^-ev, where m is the
+// maximum of s + ev.
+#include "paged.h"
+
+namespace {
+
+using namespace pk;
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kUnit = 64;          // tokens a wave takes at a time
+constexpr int kWaves = 4;          // a workgroup's, on units in turn
+constexpr int kMinShare = kWaves;  // units a workgroup takes at least
+constexpr float kTop = 7.0f;       // probabilities are relative to 2^7 below the maximum m
+constexpr float kRaise = 8.0f;     // m is raised when a score passes it by 2^8: p <= 2^15
+constexpr float kNone = -1e30f;    // the maximum of no scores
+
+struct AttnArgs {
+    PkKvCache c;
+    int N, H, group;  // query heads, those of one head of the cache
+    float scale;      // times log2(e)
+    const float* q;
+    int64_t ldq;
+    float* o;
+    int64_t ldo;
+    float* ws;
+    int64_t W;  // workgroups
+    int vec;    // q can be read in float4
+};
+
+__device__ __forceinline__ f16x8 widen(uint32_t lo, uint32_t hi) {
+    union {
+        f16x8 v;
+        f16x2 p[4];
+    } u;
+    u.p[0] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, false));
+    u.p[1] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.0f, true));
+    u.p[2] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, false));
+    u.p[3] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.0f, true));
+    return u.v;
+}
+
+// the value of the lane 8 further in the row of 16
+__device__ __forceinline__ float across8(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
+}
+
+// a page's power of two from its byte
+__device__ __forceinline__ float power(uint8_t e) { return __uint_as_float((uint32_t)e << 23); }
+
+// 0x80 in every byte that is a NaN
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+    return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// how a sequence's work is cut: `tiles` groups of R query rows (token, head of the group)
+// for each head of the cache, each over `units` units of the sequence's tokens
+struct Cut {
+    int tiles, units;
+};
+template <int R>
+__device__ __forceinline__ Cut cut(const AttnArgs& a, const Seq& s) {
+    if(s.n == 0) return {0, 0};
+    return {(int)(((int64_t)s.n * a.group + R - 1) / R), (s.end + kUnit - 1) / kUnit};
+}
+template <int R>
+__device__ __forceinline__ int64_t units_of(const AttnArgs& a, int b) {
+    const Cut w = cut<R>(a, sequence(a.c, a.N, b));
+    return (int64_t)w.tiles * a.c.kv_heads * w.units;
+}
+// the units of the sequences before `upto`, and of all
+template <int R>
+__device__ __forceinline__ void count_units(const AttnArgs& a, int upto, int64_t& before, int64_t& all) {
+    int64_t mine = 0, mine_before = 0;
+    for(int b = threadIdx.x % kWave; b < a.c.B; b += kWave) {
+        const int64_t u = units_of<R>(a, b);
+        mine += u;
+        if(b < upto) mine_before += u;
+    }
+#pragma unroll
+    for(int o = 32; o > 0; o >>= 1) {
+        mine += __shfl_xor(mine, o, kWave);
+        mine_before += __shfl_xor(mine_before, o, kWave);
+    }
+    before = mine_before;
+    all = mine;
+}
+__device__ __forceinline__ int64_t share_of(int64_t all, int64_t W) {
+    const int64_t s = (all + W - 1) / W;
+    return s < kMinShare ? kMinShare : s;
+}
+
+// a part's maximum and sum of each row, then its weighted values
+template <int HP>
+constexpr int kPart = 32 + 16 * HP;
+
+// ------------------------------------------------- few query rows a sequence
+// The units of all sequences, heads and tiles stand in one line, which the workgroups
+// share out evenly, whatever the lengths: a workgroup takes the end of one tile's units,
+// whole tiles, and the beginning of another's; its waves take every fourth unit and join
+// in LDS.  Tiles that one workgroup covered are finished here, the others' parts are left
+// for join_kernel: the one at the beginning of a workgroup's share in its place 0, the one
+// at the end in place 1.
+// SPLIT: the 16 columns are 8 rows' high parts and their low parts; else 16 rows, for two
+// products.
+template <int HP, bool SPLIT>
+__global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(AttnArgs a) {
+    constexpr int R = SPLIT ? 8 : 16;  // query rows
+    constexpr int C = HP / 64;         // chunks of 64 values of a key; then one of 32
+    constexpr bool TAIL = HP % 64 != 0;
+    constexpr int STEPS = HP / 32, DT = HP / 16;
+    __shared__ __align__(16) float part[kWaves][R][HP + 4];
+    __shared__ float part_m[kWaves][16], part_l[kWaves][16];
+    const PkKvCache& c = a.c;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col = lane % 16, quad = lane / 16;
+    const int page = (int)c.page, kvh = (int)c.kv_heads, hd = (int)c.hd;
+
+    int64_t none, all;
+    count_units<R>(a, 0, none, all);
+    const int64_t share = share_of(all, a.W), begin = blockIdx.x * share;
+    if(begin >= all) return;
+    const int64_t end = begin + share < all ? begin + share : all;
+    int64_t at = begin;
+    int b = find_sequence((int)c.B, at, [&](int i) { return units_of<R>(a, i); });
+    Seq s = sequence(c, a.N, b);
+    Cut w = cut<R>(a, s);
+    int item = (int)(at / w.units), u0 = (int)(at - (int64_t)item * w.units);
+
+    for(int64_t now = begin; now < end;) {
+        while(item == w.tiles * kvh) {  // on to the next sequence that has any
+            ++b;
+            s = sequence(c, a.N, b);
+            w = cut<R>(a, s);
+            item = 0;
+        }
+        const int u1 = end - now < w.units - u0 ? u0 + (int)(end - now) : w.units;
+        const int h = item / w.tiles, first = (item - h * w.tiles) * R;
+        const int rows = s.n * a.group - first < R ? s.n * a.group - first : R;
+
+        // the lane's query: row `mine` of the tile, as operand of 32 values a step, the
+        // values in the order that the lane's keys come in
+        const int mine = SPLIT ? col % 8 : col;
+        const int token = (first + (mine < rows ? mine : 0)) / a.group;
+        const float* qr = a.q + (int64_t)(s.row + token) * a.ldq +
+                          (int64_t)(h * a.group + (first + (mine < rows ? mine : 0)) % a.group) * hd;
+        const int reach = s.past + token;  // the last key that it sees
+        float x[STEPS][8], amax = 0.0f;
+#pragma unroll
+        for(int st = 0; st < STEPS; ++st) {
+            const int d = TAIL && st == STEPS - 1 ? 64 * C + 8 * quad
+                                                  : 64 * (st / 2) + 16 * quad + 8 * (st % 2);
+            if(a.vec) {
+#pragma unroll
+                for(int i = 0; i < 8; i += 4) {
+                    const f32x4 v = d + i < hd ? *(const f32x4*)(qr + d + i) : f32x4{};
+#pragma unroll
+                    for(int k = 0; k < 4; ++k) x[st][i + k] = v[k];
+                }
+            } else {
+#pragma unroll
+                for(int i = 0; i < 8; ++i) x[st][i] = d + i < hd ? qr[d + i] : 0.0f;
+            }
+#pragma unroll
+            for(int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[st][i]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 16, kWave));
+        amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
+        const int eq = amax > 0.0f && amax <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
+        const float coef = ldexpf(a.scale, eq);
+        f16x8 qf[SPLIT ? 1 : 2][STEPS];
+#pragma unroll
+        for(int st = 0; st < STEPS; ++st)
+#pragma unroll
+            for(int i = 0; i < 8; ++i) {
+                const float y = mine < rows ? ldexpf(x[st][i], -eq) : 0.0f;
+                const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
+                if(SPLIT) {
+                    qf[0][st][i] = col < 8 ? hi : lo;
+                } else {
+                    qf[0][st][i] = hi;
+                    qf[SPLIT ? 0 : 1][st][i] = lo;
+                }
+            }
+
+        // the pages of a unit's tokens: 16 tokens lie on one page.  A lane's keys (tokens
+        // 16 (col / 4) + 4 t + col % 4) and its values and scores (16 quad ..) are on two.
+        auto page_of = [&](int u, int g16) {
+            const int i = (u * kUnit + 16 * g16) / page;
+            const int pid = i < c.width ? c.table[(int64_t)b * c.width + i] : -1;
+            return pid < 0 || pid >= c.pages ? -1 : pid;
+        };
+        uint4 kr[4][C > 0 ? C : 1], vr[DT];
+        uint2 kt[4];
+        auto load_keys = [&](int u, int pid) {
+            const int slot = (u * kUnit + 16 * (col / 4)) % page + col % 4;
+            const uint8_t* p = c.k + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * page + slot) * HP;
+#pragma unroll
+            for(int t = 0; t < 4; ++t) {
+#pragma unroll
+                for(int i = 0; i < C; ++i)
+                    kr[t][i] = *(const uint4*)(p + 4 * t * HP + 64 * i + 16 * quad);
+                if(TAIL) kt[t] = *(const uint2*)(p + 4 * t * HP + 64 * C + 8 * quad);
+            }
+        };
+        auto load_values = [&](int u, int pid) {
+            const int slot = (u * kUnit + 16 * quad) % page;
+            const uint8_t* p = c.v + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * HP + col) * page + slot;
+#pragma unroll
+            for(int i = 0; i < DT; ++i) vr[i] = *(const uint4*)(p + (int64_t)16 * i * page);
+        };
+
+        f32x4 acc[DT];
+#pragma unroll
+        for(int i = 0; i < DT; ++i) acc[i] = f32x4{};
+        float m = kNone, l = 0.0f;
+        int u = u0 + wave;
+        int pk = -1, pv = -1;
+        uint8_t ek = 127, ev = 127;
+        if(u < u1) {
+            pk = page_of(u, col / 4);
+            pv = page_of(u, quad);
+            load_keys(u, pk);
+            load_values(u, pv);
+            ek = c.k_exp[(int64_t)(pv < 0 ? 0 : pv) * kvh + h];
+            ev = c.v_exp[(int64_t)(pv < 0 ? 0 : pv) * kvh + h];
+        }
+        const int clear = s.past + first / a.group + 1;  // tokens that every row sees
+        for(; u < u1; u += kWaves) {
+            const int next = u + kWaves;
+            int pk_next = -1, pv_next = -1;
+            if(next < u1) {
+                pk_next = page_of(next, col / 4);
+                pv_next = page_of(next, quad);
+            }
+            f32x4 sc[4];
+#pragma unroll
+            for(int t = 0; t < 4; ++t) {
+                sc[t] = f32x4{};
+#pragma unroll
+                for(int st = 0; st < STEPS; ++st) {
+                    f16x8 kf;
+                    if(TAIL && st == STEPS - 1)
+                        kf = widen(kt[t].x, kt[t].y);
+                    else if(st % 2 == 0)
+                        kf = widen(kr[t][st / 2].x, kr[t][st / 2].y);
+                    else
+                        kf = widen(kr[t][st / 2].z, kr[t][st / 2].w);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[0][st], sc[t], 0, 0, 0);
+                    if(!SPLIT)
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[SPLIT ? 0 : 1][st], sc[t],
+                                                                       0, 0, 0);
+                }
+            }
+            const float kc = coef * power(ek), vexp = (float)((int)ev - 127), vinv = power(254 - ev);
+            const bool absent = pv < 0;
+            if(next < u1) {
+                load_keys(next, pk_next);
+                ek = c.k_exp[(int64_t)(pv_next < 0 ? 0 : pv_next) * kvh + h];
+                ev = c.v_exp[(int64_t)(pv_next < 0 ? 0 : pv_next) * kvh + h];
+            }
+            float p[16], mx = kNone;
+#pragma unroll
+            for(int t = 0; t < 4; ++t)
+#pragma unroll
+                for(int r = 0; r < 4; ++r) {
+                    float v = sc[t][r];
+                    if(SPLIT) v += across8(v);
+                    p[4 * t + r] = fmaf(v, kc, vexp);
+                }
+            const int token0 = u * kUnit + 16 * quad;
+            const bool edge = u * kUnit + kUnit > clear || __ballot(absent) != 0;
+            if(edge) {
+#pragma unroll
+                for(int i = 0; i < 16; ++i)
+                    if(absent || token0 + i > reach) p[i] = -INFINITY;
+            }
+#pragma unroll
+            for(int i = 0; i < 16; ++i) mx = fmaxf(mx, p[i]);
+            if(__ballot(mx > m + kRaise)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+                mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+                mx = fmaxf(mx, m);
+                const float down = __builtin_amdgcn_exp2f(m - mx);
+                l *= down;
+#pragma unroll
+                for(int i = 0; i < DT; ++i) acc[i] *= down;
+                m = mx;
+            }
+            float sum = 0.0f;
+            const float low = m - kTop;
+#pragma unroll
+            for(int i = 0; i < 16; ++i) {
+                p[i] = __builtin_amdgcn_exp2f(p[i] - low);
+                sum += p[i];
+            }
+            l = fmaf(sum, vinv, l);
+            f16x8 pf[2][2];
+#pragma unroll
+            for(int i = 0; i < 16; ++i) {
+                const _Float16 hi = (_Float16)p[i], lo = (_Float16)(p[i] - (float)hi);
+                if(SPLIT) {
+                    pf[0][i / 8][i % 8] = col < 8 ? hi : lo;
+                } else {
+                    pf[0][i / 8][i % 8] = hi;
+                    pf[1][i / 8][i % 8] = lo;
+                }
+            }
+            if(edge) {
+                // tokens behind the sequence's last, or on no page, may hold anything
+                const int real = absent ? 0 : held(s.end - token0, 0, 16);
+                uint32_t keep[4], nan = 0;
+#pragma unroll
+                for(int i = 0; i < 4; ++i) {
+                    const int k = held(real - 4 * i, 0, 4);
+                    keep[i] = k == 4 ? 0xffffffffu : (1u << (8 * k)) - 1u;
+                }
+#pragma unroll
+                for(int i = 0; i < DT; ++i) {
+                    vr[i].x &= keep[0];
+                    vr[i].y &= keep[1];
+                    vr[i].z &= keep[2];
+                    vr[i].w &= keep[3];
+                    nan |= nan_bytes(vr[i].x) | nan_bytes(vr[i].y) | nan_bytes(vr[i].z) | nan_bytes(vr[i].w);
+                }
+                if(__ballot(nan != 0)) {
+                    // a NaN among the values of tokens that some rows do not see, where
+                    // 0 times it must not reach them: how many of a column's NaN each row
+                    // sees, as a product of ones, and zeros in their place
+                    f16x8 seen[2];
+#pragma unroll
+                    for(int i = 0; i < 16; ++i)
+                        seen[i / 8][i % 8] = absent || token0 + i > reach ? (_Float16)0.0f : (_Float16)1.0f;
+#pragma unroll
+                    for(int i = 0; i < DT; ++i) {
+                        uint32_t word[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w}, one[4];
+#pragma unroll
+                        for(int k = 0; k < 4; ++k) {
+                            const uint32_t bits = nan_bytes(word[k]) >> 7;
+                            one[k] = bits * 0x38;  // e4m3's 1
+                            word[k] &= ~(bits * 0xff);
+                        }
+                        f32x4 count = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(one[0], one[1]), seen[0],
+                                                                             f32x4{}, 0, 0, 0);
+                        count = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(one[2], one[3]), seen[1], count,
+                                                                       0, 0, 0);
+#pragma unroll
+                        for(int r = 0; r < 4; ++r)
+                            if(count[r] > 0.0f) acc[i][r] = NAN;
+                        vr[i] = {word[0], word[1], word[2], word[3]};
+                    }
+                }
+            }
+#pragma unroll
+            for(int i = 0; i < DT; ++i) {
+                const f16x8 v0 = widen(vr[i].x, vr[i].y), v1 = widen(vr[i].z, vr[i].w);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[0][0], acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[0][1], acc[i], 0, 0, 0);
+                if(!SPLIT) {
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[1][0], acc[i], 0, 0, 0);
+                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[1][1], acc[i], 0, 0, 0);
+                }
+            }
+            if(next < u1) load_values(next, pv_next);
+            pv = pv_next;
+        }
+
+        // the waves' parts together
+        l += __shfl_xor(l, 16, kWave);
+        l += __shfl_xor(l, 32, kWave);
+#pragma unroll
+        for(int i = 0; i < DT; ++i) {
+            if(SPLIT) {
+#pragma unroll
+                for(int r = 0; r < 4; ++r) acc[i][r] += across8(acc[i][r]);
+            }
+            if(col < R) *(f32x4*)&part[wave][col][16 * i + 4 * quad] = acc[i];
+        }
+        if(lane < 16) {
+            part_m[wave][lane] = m;
+            part_l[wave][lane] = l;
+        }
+        __syncthreads();
+        const bool whole = u0 == 0 && u1 == w.units;
+        float* out = a.ws + ((int64_t)blockIdx.x * 2 + (now == begin ? 0 : 1)) * kPart<HP>;
+        for(int i = threadIdx.x; i < rows * (HP / 4); i += kWaves * kWave) {
+            const int r = i / (HP / 4), d = 4 * (i % (HP / 4));
+            float top = part_m[0][r], total = 0.0f;
+#pragma unroll
+            for(int k = 1; k < kWaves; ++k) top = fmaxf(top, part_m[k][r]);
+            f32x4 v = {};
+#pragma unroll
+            for(int k = 0; k < kWaves; ++k) {
+                const float f = __builtin_amdgcn_exp2f(part_m[k][r] - top);
+                total = fmaf(f, part_l[k][r], total);
+                v += f * *(const f32x4*)&part[k][r][d];
+            }
+            if(!whole) {
+                if(d == 0) {
+                    out[r] = top;
+                    out[16 + r] = total;
+                }
+                *(f32x4*)(out + 32 + r * HP + d) = v;
+                continue;
+            }
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // (0: no key at all)
+            float* to = a.o + (int64_t)(s.row + (first + r) / a.group) * a.ldo +
+                        (int64_t)(h * a.group + (first + r) % a.group) * hd + d;
+#pragma unroll
+            for(int k = 0; k < 4; ++k)
+                if(d + k < hd) to[k] = v[k] * inv;
+        }
+        __syncthreads();
+        now += u1 - u0;
+        u0 = 0;
+        ++item;
+    }
+}
+
+// the tiles that several workgroups have parts of: one row a workgroup, its threads on 4
+// values each of as many parts at once
+template <int HP, int R>
+__global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
+    constexpr int D4 = HP / 4, PARTS = 256 / D4;
+    __shared__ __align__(16) float sums[PARTS][HP];
+    __shared__ float totals[PARTS];
+    const PkKvCache& c = a.c;
+    const int r = (int)(blockIdx.x % R);
+    int item = (int)(blockIdx.x / R);
+    const int b = find_sequence((int)c.B, item, [&](int i) {
+        return cut<R>(a, sequence(c, a.N, i)).tiles * (int)c.kv_heads;
+    });
+    if(b < 0) return;
+    const Seq s = sequence(c, a.N, b);
+    const Cut w = cut<R>(a, s);
+    int64_t before, all;
+    count_units<R>(a, b, before, all);
+    const int64_t share = share_of(all, a.W), p0 = before + (int64_t)item * w.units;
+    const int64_t w0 = p0 / share, w1 = (p0 + w.units - 1) / share;
+    const int h = item / w.tiles, row = (item - h * w.tiles) * R + r;
+    if(w0 == w1 || row >= s.n * a.group) return;
+    auto part = [&](int64_t i) {
+        return a.ws + (i * 2 + (i == w0 && p0 != w0 * share ? 1 : 0)) * kPart<HP>;
+    };
+    float top = kNone;
+    for(int64_t i = w0 + threadIdx.x % kWave; i <= w1; i += kWave) top = fmaxf(top, part(i)[r]);
+    top = wave_max(top);
+    const int mine = threadIdx.x / D4, d = 4 * (threadIdx.x % D4);
+    f32x4 v = {};
+    float total = 0.0f;
+    if(mine < PARTS) {
+        for(int64_t i = w0 + mine; i <= w1; i += PARTS) {
+            const float* p = part(i);
+            const float f = __builtin_amdgcn_exp2f(p[r] - top);
+            total = fmaf(f, p[16 + r], total);
+            v += f * *(const f32x4*)(p + 32 + r * HP + d);
+        }
+        *(f32x4*)&sums[mine][d] = v;
+        if(d == 0) totals[mine] = total;
+    }
+    __syncthreads();
+    if(threadIdx.x >= D4) return;
+#pragma unroll
+    for(int k = 1; k < PARTS; ++k) {
+        v += *(const f32x4*)&sums[k][d];
+        total += totals[k];
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    float* to = a.o + (int64_t)(s.row + row / a.group) * a.ldo + (int64_t)(h * a.group + row % a.group) * c.hd + d;
+#pragma unroll
+    for(int k = 0; k < 4; ++k)
+        if(d + k < c.hd) to[k] = v[k] * inv;
+}
+
+// ------------------------------------------------------------------- launches
+struct Plan {
+    int rows;         // 8 or 16 query rows a tile
+    int64_t W, items; // workgroups; tiles times heads there may be
+};
+Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
+    Plan p;
+    const int64_t group = H / c->kv_heads;
+    p.rows = N * group <= 8 * c->B ? 8 : 16;
+    p.items = (N * group / p.rows + (c->B < N ? c->B : N)) * c->kv_heads;
+    p.W = 512;
+    // no more than there can be units for
+    const int64_t most = p.items * ((c->width * c->page + kUnit - 1) / kUnit + 1) / kMinShare + 1;
+    if(p.W > most) p.W = most;
+    return p;
+}
+
+int check_attn(const char* who, const PkKvCache* c, int64_t N, int64_t H) {
+    if(int st = check_cache(who, c, N)) return st;
+    if(H < 1 || H % c->kv_heads || H > (1 << 20) / c->hd)
+        return fail("%s: %lld query heads on %lld of the cache: a multiple, with H*hd up to 2^20", who,
+                    (long long)H, (long long)c->kv_heads);
+    if(N * H >= (int64_t)1 << 31)
+        return fail("%s: too many query rows, N*H up to 2^31 - 1", who);
+    return PK_OK;
+}
+
+template <int HP>
+void launch(const AttnArgs& a, const Plan& p, hipStream_t st) {
+    if(p.rows == 8) {
+        few_rows_kernel<HP, true><<<(unsigned)p.W, kWaves * kWave, 0, st>>>(a);
+        join_kernel<HP, 8><<<(unsigned)(p.items * 8), 256, 0, st>>>(a);
+    } else {
+        few_rows_kernel<HP, false><<<(unsigned)p.W, kWaves * kWave, 0, st>>>(a);
+        join_kernel<HP, 16><<<(unsigned)(p.items * 16), 256, 0, st>>>(a);
+    }
+}
+
+}  // namespace
+
+extern "C" size_t pk_attn_paged_workspace(const PkKvCache* cache, int64_t N, int64_t H) {
+    if(check_attn("pk_attn_paged_workspace", cache, N, H) || N == 0 || cache->B == 0) return 0;
+    return sizeof(float) * 2 * plan(cache, N, H).W * (32 + 16 * head_size(cache->hd));
+}
+
+extern "C" int pk_attn_paged_f32(const PkKvCache* cache, int64_t N, int64_t H, float scale,
+                                 const float* q, int64_t ldq, float* o, int64_t ldo, void* workspace,
+                                 size_t workspace_bytes, pk_stream_t stream) {
+    if(int st = check_attn("pk_attn_paged_f32", cache, N, H)) return st;
+    if(N == 0 || cache->B == 0) return PK_OK;
+    const int64_t width = H * cache->hd;
+    if(!q || !o) return fail("pk_attn_paged_f32: NULL pointer");
+    if(ldq < width || ldo < width)
+        return fail("pk_attn_paged_f32: row strides must be at least H*hd = %lld", (long long)width);
+    const size_t need = pk_attn_paged_workspace(cache, N, H);
+    if(need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
+        return fail("pk_attn_paged_f32: workspace of %zu bytes, %zu needed, 16-byte aligned",
+                    workspace ? workspace_bytes : 0, need);
+    const Plan p = plan(cache, N, H);
+    if(!grid_fits(p.items * p.rows, 256)) return fail("pk_attn_paged_f32: too many rows for one launch");
+    AttnArgs a = {};
+    a.c = *cache;
+    a.N = (int)N;
+    a.H = (int)H;
+    a.group = (int)(H / cache->kv_heads);
+    a.scale = scale * 1.4426950408889634f;
+    a.q = q;
+    a.ldq = ldq;
+    a.o = o;
+    a.ldo = ldo;
+    a.ws = (float*)workspace;
+    a.W = p.W;
+    a.vec = cache->hd % 4 == 0 && ldq % 4 == 0 && aligned16(q);
+    const hipStream_t st = as_stream(stream);
+    switch(head_size(cache->hd)) {
+        case 32: launch<32>(a, p, st); break;
+        case 64: launch<64>(a, p, st); break;
+        case 96: launch<96>(a, p, st); break;
+        case 128: launch<128>(a, p, st); break;
+        default: launch<256>(a, p, st); break;
+    }
+    return launch_status("pk_attn_paged_f32");
+}

@@ -977,6 +977,167 @@ def gemm_experts_dw(x, dy, offsets, dw, precision="fp32", accum=False, ws=None):
     return dw
 
 
+# ----------------------------- rotary positions, a paged cache, attention over it
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "parts": 3}
+ROPE_BACKWARD = 32
+_F64, _U8 = torch.float64, torch.uint8
+
+
+class PkRope(ctypes.Structure):
+    """struct PkRope (include/pico_hip.h)"""
+    _fields_ = [("freqs", ctypes.c_void_p), ("rot", ctypes.c_int64), ("interleaved", ctypes.c_int),
+                ("magnitude", ctypes.c_double)]
+
+
+class PkKvCache(ctypes.Structure):
+    """struct PkKvCache (include/pico_hip.h)"""
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("k", "v", "k_exp", "v_exp", "table", "lens", "offsets")] + \
+               [(n, ctypes.c_int64) for n in ("pages", "kv_heads", "hd", "page", "B", "width")]
+
+
+def rope_freqs(rot, base=10000.0, scaling="none", factor=1.0, length=0.0, low=1.0, high=32.0,
+               device="cuda"):
+    """the rot / 2 frequencies of rotary positions (pk_rope_freqs) as a float64 tensor;
+    scaling: none, linear, ntk or parts"""
+    out = (ctypes.c_double * max(1, rot // 2))()
+    check("pk_rope_freqs", hip_lib().pk_rope_freqs(rot, base, ROPE_SCALINGS[scaling], factor, length,
+                                                   low, high, out))
+    return torch.tensor(out[:rot // 2], dtype=_F64, device=device)
+
+
+class Rope:
+    """rotary positions for the first 2 * len(freqs) values of a head: freqs a float64
+    tensor on the device (radians a position), pairs (2i, 2i + 1) when interleaved, else
+    (i, i + len(freqs))"""
+
+    def __init__(self, freqs, interleaved=False, magnitude=1.0):
+        if freqs.dtype is not _F64 or not freqs.is_cuda or not freqs.is_contiguous() or freqs.dim() != 1:
+            raise TypeError("expected a contiguous 1-D float64 CUDA tensor of frequencies")
+        self.freqs = freqs
+        self.device = freqs.get_device()
+        self.args = PkRope(freqs.data_ptr(), 2 * freqs.numel(), int(bool(interleaved)), magnitude)
+        self.ref = ctypes.addressof(self.args)
+
+
+def _rope_ref(rope, dev):
+    if rope is None:
+        return None
+    if rope.device != dev:
+        raise ValueError("the frequencies lie on another device than the current one")
+    return rope.ref
+
+
+def _heads(size, H, name):
+    if H < 1 or size[1] % H or size[1] == 0:
+        raise ValueError(f"{name} {list(size)} does not hold {H} heads")
+    return size[1] // H
+
+
+def rope(rope, H, x, positions, y, backward=False, accum=False):
+    """y = the H heads of x [N, H*hd] turned by their positions [N] (int32); y may be x.
+    backward: turned the other way (the gradient of y to that of x)"""
+    dev = _device()
+    xp, ldx = _rows(dev, x, "x")
+    size = x.shape
+    yp, ldy = _rows(dev, y, "y", size)
+    pp, = _dense(dev, _I32, positions)
+    if positions.numel() != size[0]:
+        raise ValueError("rope: a position for every row of x")
+    flags = (ROPE_BACKWARD if backward else 0) | (ACCUM if accum else 0)
+    check("pk_rope_f32", hip_lib().pk_rope_f32(
+        size[0], H, _heads(size, H, "x"), _rope_ref(rope, dev), pp, xp, ldx, yp, ldy, flags,
+        _raw_stream(dev)))
+    return y
+
+
+def kv_head_size(hd):
+    """hd rounded up to the head size that a cache's layout has (0: larger than any)"""
+    return int(hip_lib().pk_kv_head_size(hd))
+
+
+def kv_pool(pages, kv_heads, page, hd, device="cuda"):
+    """(k, v, k_exp, v_exp): uninitialised pages of a PagedKV"""
+    hp = kv_head_size(hd)
+    return tuple(torch.empty(s, dtype=_U8, device=device) for s in (
+        (pages, kv_heads, page, hp), (pages, kv_heads, hp, page), (pages, kv_heads),
+        (pages, kv_heads)))
+
+
+class PagedKV:
+    """a paged cache of keys and values (struct PkKvCache): the pages of kv_pool, and the
+    sequences of a call: table [B, width], lens [B] and offsets [B + 1], int32.  The
+    tensors are read at each call, where they are; write into them for the next one."""
+
+    def __init__(self, k, v, k_exp, v_exp, table, lens, offsets, hd):
+        dev = k.get_device()
+        at = _dense(dev, _U8, k, v, k_exp, v_exp) + _dense(dev, _I32, table, lens, offsets)
+        if k.dim() != 4 or table.dim() != 2:
+            raise ValueError("PagedKV: k must be [pages, kv_heads, page, head], table [B, width]")
+        pages, kv_heads, page, hp = k.shape
+        B, width = table.shape
+        if hp != kv_head_size(hd) or v.shape != (pages, kv_heads, hp, page) or \
+                k_exp.shape != (pages, kv_heads) or v_exp.shape != (pages, kv_heads):
+            raise ValueError(f"PagedKV: k {list(k.shape)}, v {list(v.shape)} and their exponents do "
+                             f"not fit each other or a head size of {hd}")
+        if lens.numel() != B or offsets.numel() != B + 1:
+            raise ValueError("PagedKV: lens must hold a value a sequence, offsets B + 1")
+        self.tensors = (k, v, k_exp, v_exp, table, lens, offsets)
+        self.device, self.kv_heads, self.hd = dev, kv_heads, hd
+        self.args = PkKvCache(*at, pages, kv_heads, hd, page, B, width)
+        self.ref = ctypes.addressof(self.args)
+
+
+def _on(cache, dev):
+    if cache.device != dev:
+        raise ValueError("the cache lies on another device than the current one")
+    return cache.ref
+
+
+def kv_append(cache, k, v, rope=None, H=0, q=None, q_out=None):
+    """the new tokens' k and v [N, kv_heads*hd] into the cache, k turned by rope (None: as
+    it is); q [N, H*hd] turned likewise into q_out"""
+    dev = _device()
+    ref = _on(cache, dev)
+    kp, ldk = _rows(dev, k, "k")
+    size = k.shape
+    vp, ldv = _rows(dev, v, "v", size)
+    N = size[0]
+    if size[1] != cache.kv_heads * cache.hd:
+        raise ValueError(f"kv_append: k must be [N, {cache.kv_heads * cache.hd}], got {list(size)}")
+    qp = op = None
+    ldq = ldo = 0
+    if q is not None:
+        qp, ldq = _rows(dev, q, "q", (N, H * cache.hd))
+        op, ldo = _rows(dev, q_out, "q_out", (N, H * cache.hd))
+        if op is None:
+            raise ValueError("kv_append: q needs q_out")
+    check("pk_kv_append_f32", hip_lib().pk_kv_append_f32(
+        ref, N, kp, ldk, vp, ldv, _rope_ref(rope, dev), H, qp, ldq, op, ldo, _raw_stream(dev)))
+
+
+def attn_paged_workspace(cache, N, H):
+    return int(hip_lib().pk_attn_paged_workspace(cache.ref, N, H))
+
+
+def attn_paged(cache, H, q, o, scale=None, ws=None):
+    """o = softmax(scale q K^T) V of the new tokens' q [N, H*hd] over what the cache holds of
+    their sequences, up to themselves"""
+    dev = _device()
+    ref = _on(cache, dev)
+    qp, ldq = _rows(dev, q, "q")
+    size = q.shape
+    op, ldo = _rows(dev, o, "o", size)
+    N, hd = size[0], cache.hd
+    if size[1] != H * hd:
+        raise ValueError(f"attn_paged: q must be [N, {H * hd}], got {list(size)}")
+    wp, wb, ws = _ws(ws, dev, attn_paged_workspace, cache, N, H)
+    check("pk_attn_paged_f32", hip_lib().pk_attn_paged_f32(
+        ref, N, H, hd ** -0.5 if scale is None else scale, qp, ldq, op, ldo, wp, wb,
+        _raw_stream(dev)))
+    return o
+
+
 def device_info():
     cu, clk = ctypes.c_int(0), ctypes.c_int(0)
     arch = ctypes.create_string_buffer(64)
