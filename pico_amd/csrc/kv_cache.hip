@@ -40,13 +40,12 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, unsigned task, 
                                             float* red) {
     const PkKvCache& c = a.c;
     const int page = (int)c.page, hd = (int)c.hd, hp = a.hp;
-    int nth = (int)task;
-    const int b = find_sequence((int)c.B, nth, [&](int i) {
-        const Seq s = sequence(c, a.N, i);
-        return s.end > s.past ? (s.end - 1) / page - s.past / page + 1 : 0;
-    });
-    if(b < 0) return;
-    const Seq s = sequence(c, a.N, b);
+    int nth, b;
+    Seq s;
+    if(!locate(
+           c, a.N, [&](const Seq& t) { return t.end > t.past ? (t.end - 1) / page - t.past / page + 1 : 0; },
+           [&](int) { return (int)task; }, nth, b, s))
+        return;
     const int index = s.past / page + nth;
     const int pid = c.table[(int64_t)b * c.width + index];
     if(pid < 0 || pid >= c.pages) return;

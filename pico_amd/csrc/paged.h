@@ -24,28 +24,50 @@ __device__ __forceinline__ Seq sequence(const PkKvCache& c, int N, int b) {
     return s;
 }
 
-// the sequence in whose share of a sum over the sequences `at` falls, and where in it
-// (-1: beyond all): 64 sequences at a time, one a lane
-template <class I, class F>
-__device__ __forceinline__ int find_sequence(int B, I& at, F share) {
-    const int lane = threadIdx.x % kWave;
+// sums over the lanes up to one's own
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4 and 8 lanes
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);  // before in a row of 16
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // the last lane of row 0
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // and 2; of rows 0 and 1
+    return v;
+}
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// The sequences' shares stand in one line, whose length fits 31 bits; start(length) is a
+// place in it.  Finds the sequence there, its number `b` and the place `at` within its
+// share; false beyond the end, and where offsets that decrease make the sums wrap.  64
+// sequences at a time, one a lane; up to 64 of them take one trip to memory.
+template <class F, class G>
+__device__ __forceinline__ bool locate(const PkKvCache& c, int N, F share, G start, int& at, int& b,
+                                       Seq& s) {
+    const int lane = threadIdx.x % kWave, B = (int)c.B;
+    int all = 0;
+    if(B > kWave) {
+        for(int i = lane; i < B; i += kWave) all += share(sequence(c, N, i));
+        all = lane_of(wave_scan(all), kWave - 1);
+        at = start(all);
+        if(at >= all) return false;
+    }
     for(int base = 0; base < B; base += kWave) {
-        const I mine = base + lane < B ? share(base + lane) : 0;
-        I upto = mine;
-#pragma unroll
-        for(int o = 1; o < kWave; o <<= 1) {
-            const I other = __shfl_up(upto, o, kWave);
-            if(lane >= o) upto += other;
-        }
+        Seq mine = {};
+        if(base + lane < B) mine = sequence(c, N, base + lane);
+        const int len = base + lane < B ? share(mine) : 0, upto = wave_scan(len);
+        if(B <= kWave) at = start(lane_of(upto, kWave - 1));
         const uint64_t above = __ballot(upto > at);
         if(above) {
             const int first = __builtin_ctzll(above);
-            at -= __shfl(upto - mine, first, kWave);
-            return base + first;
+            at -= lane_of(upto - len, first);
+            b = base + first;
+            s = {lane_of(mine.row, first), lane_of(mine.n, first), lane_of(mine.past, first),
+                 lane_of(mine.end, first)};
+            return at >= 0 && at < lane_of(len, first);
         }
-        at -= __shfl(upto, kWave - 1, kWave);
+        at -= lane_of(upto, kWave - 1);
     }
-    return -1;
+    return false;
 }
 
 // the smallest e, from -40 to 40, with amax <= 448 2^e; 448 is 0.875 2^9

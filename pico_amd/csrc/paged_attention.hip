@@ -27,8 +27,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kUnit = 64;          // tokens a wave takes at a time
-constexpr int kWaves = 4;          // a workgroup's, on units in turn
-constexpr int kMinShare = kWaves;  // units a workgroup takes at least
+constexpr int kMinShare = 4;       // units a workgroup takes at least, where they share a tile
 constexpr float kTop = 7.0f;       // probabilities are relative to 2^7 below the maximum m
 constexpr float kRaise = 8.0f;     // m is raised when a score passes it by 2^8: p <= 2^15
 constexpr float kNone = -1e30f;    // the maximum of no scores
@@ -42,8 +41,8 @@ struct AttnArgs {
     float* o;
     int64_t ldo;
     float* ws;
-    int64_t W;  // workgroups
-    int vec;    // q can be read in float4
+    int W;    // workgroups that share the units of all tiles
+    int vec;  // q can be read in float4
 };
 
 __device__ __forceinline__ f16x8 widen(uint32_t lo, uint32_t hi) {
@@ -71,40 +70,16 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
     return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
-// how a sequence's work is cut: `tiles` groups of R query rows (token, head of the group)
-// for each head of the cache, each over `units` units of the sequence's tokens
-struct Cut {
-    int tiles, units;
-};
+// how a sequence's work is cut: groups of R query rows (token, head of the group) for each
+// head of the cache, each over units of the sequence's tokens
 template <int R>
-__device__ __forceinline__ Cut cut(const AttnArgs& a, const Seq& s) {
-    if(s.n == 0) return {0, 0};
-    return {(int)(((int64_t)s.n * a.group + R - 1) / R), (s.end + kUnit - 1) / kUnit};
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, const Seq& s) {
+    return (s.n * a.group + R - 1) / R;
 }
-template <int R>
-__device__ __forceinline__ int64_t units_of(const AttnArgs& a, int b) {
-    const Cut w = cut<R>(a, sequence(a.c, a.N, b));
-    return (int64_t)w.tiles * a.c.kv_heads * w.units;
-}
-// the units of the sequences before `upto`, and of all
-template <int R>
-__device__ __forceinline__ void count_units(const AttnArgs& a, int upto, int64_t& before, int64_t& all) {
-    int64_t mine = 0, mine_before = 0;
-    for(int b = threadIdx.x % kWave; b < a.c.B; b += kWave) {
-        const int64_t u = units_of<R>(a, b);
-        mine += u;
-        if(b < upto) mine_before += u;
-    }
-#pragma unroll
-    for(int o = 32; o > 0; o >>= 1) {
-        mine += __shfl_xor(mine, o, kWave);
-        mine_before += __shfl_xor(mine_before, o, kWave);
-    }
-    before = mine_before;
-    all = mine;
-}
-__device__ __forceinline__ int64_t share_of(int64_t all, int64_t W) {
-    const int64_t s = (all + W - 1) / W;
+__device__ __forceinline__ int units_of(const Seq& s) { return (s.end + kUnit - 1) / kUnit; }
+// of a line of `all` units, those of one workgroup
+__device__ __forceinline__ int share_of(int all, int W) {
+    const int s = (all + W - 1) / W;
     return s < kMinShare ? kMinShare : s;
 }
 
@@ -113,16 +88,21 @@ template <int HP>
 constexpr int kPart = 32 + 16 * HP;
 
 // ------------------------------------------------- few query rows a sequence
-// The units of all sequences, heads and tiles stand in one line, which the workgroups
-// share out evenly, whatever the lengths: a workgroup takes the end of one tile's units,
-// whole tiles, and the beginning of another's; its waves take every fourth unit and join
-// in LDS.  Tiles that one workgroup covered are finished here, the others' parts are left
-// for join_kernel: the one at the beginning of a workgroup's share in its place 0, the one
-// at the end in place 1.
+// (heads of 256 take the registers that two waves of smaller ones share)
+constexpr int waves_of(int hp, bool whole) { return whole && hp < 256 ? 8 : 4; }
+
+// A workgroup's waves take a tile's units in turn and join in LDS.  WHOLE: a workgroup to
+// a tile.  Otherwise the units of all sequences, heads and tiles stand in one line, which
+// the workgroups share out evenly, whatever the lengths: one takes the end of a tile's
+// units, whole tiles, and the beginning of another's.  Tiles that one workgroup covered
+// are finished here, the others' parts are left for join_kernel: the one at the beginning
+// of a workgroup's share in its place 0, the one at the end in place 1.
 // SPLIT: the 16 columns are 8 rows' high parts and their low parts; else 16 rows, for two
 // products.
-template <int HP, bool SPLIT>
-__global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(AttnArgs a) {
+template <int HP, bool SPLIT, bool WHOLE>
+__global__ __launch_bounds__(waves_of(HP, WHOLE) * kWave, HP == 256 ? 1 : 2)
+void few_rows_kernel(AttnArgs a) {
+    constexpr int kWaves = waves_of(HP, WHOLE);
     constexpr int R = SPLIT ? 8 : 16;  // query rows
     constexpr int C = HP / 64;         // chunks of 64 values of a key; then one of 32
     constexpr bool TAIL = HP % 64 != 0;
@@ -133,27 +113,34 @@ __global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(AttnArgs a) {
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane % 16, quad = lane / 16;
     const int page = (int)c.page, kvh = (int)c.kv_heads, hd = (int)c.hd;
+    const int shift = __builtin_ctz(page);
 
-    int64_t none, all;
-    count_units<R>(a, 0, none, all);
-    const int64_t share = share_of(all, a.W), begin = blockIdx.x * share;
-    if(begin >= all) return;
-    const int64_t end = begin + share < all ? begin + share : all;
-    int64_t at = begin;
-    int b = find_sequence((int)c.B, at, [&](int i) { return units_of<R>(a, i); });
-    Seq s = sequence(c, a.N, b);
-    Cut w = cut<R>(a, s);
-    int item = (int)(at / w.units), u0 = (int)(at - (int64_t)item * w.units);
+    int begin = 0, end = 1, at, b;
+    Seq s;
+    if(!locate(
+           c, a.N, [&](const Seq& t) { return tiles_of<R>(a, t) * kvh * (WHOLE ? 1 : units_of(t)); },
+           [&](int all) {
+               if(WHOLE) return (int)blockIdx.x;
+               const int share = share_of(all, a.W);
+               begin = (int)blockIdx.x * share;  // (at most all + share: fits)
+               end = all - begin < share ? all : begin + share;
+               return begin;
+           },
+           at, b, s))
+        return;
+    int tiles = tiles_of<R>(a, s), units = units_of(s);
+    int item = WHOLE ? at : at / units, u0 = WHOLE ? 0 : at - item * units;
 
-    for(int64_t now = begin; now < end;) {
-        while(item == w.tiles * kvh) {  // on to the next sequence that has any
-            ++b;
+    for(int now = begin; now < end;) {
+        while(item == tiles * kvh) {  // on to the next sequence that has any
+            if(++b >= c.B) return;    // (there is one, unless offsets decrease)
             s = sequence(c, a.N, b);
-            w = cut<R>(a, s);
+            tiles = tiles_of<R>(a, s);
+            units = units_of(s);
             item = 0;
         }
-        const int u1 = end - now < w.units - u0 ? u0 + (int)(end - now) : w.units;
-        const int h = item / w.tiles, first = (item - h * w.tiles) * R;
+        const int u1 = WHOLE || end - now >= units - u0 ? units : u0 + (end - now);
+        const int h = item / tiles, first = (item - h * tiles) * R;
         const int rows = s.n * a.group - first < R ? s.n * a.group - first : R;
 
         // the lane's query: row `mine` of the tile, as operand of 32 values a step, the
@@ -163,7 +150,41 @@ __global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(AttnArgs a) {
         const float* qr = a.q + (int64_t)(s.row + token) * a.ldq +
                           (int64_t)(h * a.group + (first + (mine < rows ? mine : 0)) % a.group) * hd;
         const int reach = s.past + token;  // the last key that it sees
-        float x[STEPS][8], amax = 0.0f;
+        // the pages of a unit's tokens: 16 tokens lie on one page.  A lane's keys (tokens
+        // 16 (col / 4) + 4 t + col % 4) and its values and scores (16 quad ..) are on two.
+        auto page_of = [&](int u, int g16) {
+            const int i = (u * kUnit + 16 * g16) >> shift;
+            const int pid = i < c.width ? c.table[(int64_t)b * c.width + i] : -1;
+            return pid < 0 || pid >= c.pages ? -1 : pid;
+        };
+        uint4 kr[4][C > 0 ? C : 1], vr[DT];
+        uint2 kt[4];
+        auto load_keys = [&](int u, int pid) {
+            const int slot = ((u * kUnit + 16 * (col / 4)) & (page - 1)) + col % 4;
+            const uint8_t* p = c.k + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * page + slot) * HP;
+#pragma unroll
+            for(int t = 0; t < 4; ++t) {
+#pragma unroll
+                for(int i = 0; i < C; ++i)
+                    kr[t][i] = *(const uint4*)(p + 4 * t * HP + 64 * i + 16 * quad);
+                if(TAIL) kt[t] = *(const uint2*)(p + 4 * t * HP + 64 * C + 8 * quad);
+            }
+        };
+        auto load_values = [&](int u, int pid) {
+            const int slot = (u * kUnit + 16 * quad) & (page - 1);
+            const uint8_t* p = c.v + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * HP + col) * page + slot;
+#pragma unroll
+            for(int i = 0; i < DT; ++i) vr[i] = *(const uint4*)(p + (int64_t)16 * i * page);
+        };
+
+        // (the loads that others wait for first: pages, query, then keys and values)
+        int u = u0 + wave;
+        int pk = -1, pv = -1;
+        if(u < u1) {
+            pk = page_of(u, col / 4);
+            pv = page_of(u, quad);
+        }
+        float x[STEPS][8];
 #pragma unroll
         for(int st = 0; st < STEPS; ++st) {
             const int d = TAIL && st == STEPS - 1 ? 64 * C + 8 * quad
@@ -179,9 +200,19 @@ __global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(AttnArgs a) {
 #pragma unroll
                 for(int i = 0; i < 8; ++i) x[st][i] = d + i < hd ? qr[d + i] : 0.0f;
             }
+        }
+        uint8_t ek = 127, ev = 127;
+        if(u < u1) {
+            load_keys(u, pk);
+            load_values(u, pv);
+            ek = c.k_exp[(int64_t)(pv < 0 ? 0 : pv) * kvh + h];
+            ev = c.v_exp[(int64_t)(pv < 0 ? 0 : pv) * kvh + h];
+        }
+        float amax = 0.0f;
+#pragma unroll
+        for(int st = 0; st < STEPS; ++st)
 #pragma unroll
             for(int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[st][i]));
-        }
         amax = fmaxf(amax, __shfl_xor(amax, 16, kWave));
         amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
         const int eq = amax > 0.0f && amax <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
@@ -201,48 +232,10 @@ __global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(AttnArgs a) {
                 }
             }
 
-        // the pages of a unit's tokens: 16 tokens lie on one page.  A lane's keys (tokens
-        // 16 (col / 4) + 4 t + col % 4) and its values and scores (16 quad ..) are on two.
-        auto page_of = [&](int u, int g16) {
-            const int i = (u * kUnit + 16 * g16) / page;
-            const int pid = i < c.width ? c.table[(int64_t)b * c.width + i] : -1;
-            return pid < 0 || pid >= c.pages ? -1 : pid;
-        };
-        uint4 kr[4][C > 0 ? C : 1], vr[DT];
-        uint2 kt[4];
-        auto load_keys = [&](int u, int pid) {
-            const int slot = (u * kUnit + 16 * (col / 4)) % page + col % 4;
-            const uint8_t* p = c.k + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * page + slot) * HP;
-#pragma unroll
-            for(int t = 0; t < 4; ++t) {
-#pragma unroll
-                for(int i = 0; i < C; ++i)
-                    kr[t][i] = *(const uint4*)(p + 4 * t * HP + 64 * i + 16 * quad);
-                if(TAIL) kt[t] = *(const uint2*)(p + 4 * t * HP + 64 * C + 8 * quad);
-            }
-        };
-        auto load_values = [&](int u, int pid) {
-            const int slot = (u * kUnit + 16 * quad) % page;
-            const uint8_t* p = c.v + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * HP + col) * page + slot;
-#pragma unroll
-            for(int i = 0; i < DT; ++i) vr[i] = *(const uint4*)(p + (int64_t)16 * i * page);
-        };
-
         f32x4 acc[DT];
 #pragma unroll
         for(int i = 0; i < DT; ++i) acc[i] = f32x4{};
         float m = kNone, l = 0.0f;
-        int u = u0 + wave;
-        int pk = -1, pv = -1;
-        uint8_t ek = 127, ev = 127;
-        if(u < u1) {
-            pk = page_of(u, col / 4);
-            pv = page_of(u, quad);
-            load_keys(u, pk);
-            load_values(u, pv);
-            ek = c.k_exp[(int64_t)(pv < 0 ? 0 : pv) * kvh + h];
-            ev = c.v_exp[(int64_t)(pv < 0 ? 0 : pv) * kvh + h];
-        }
         const int clear = s.past + first / a.group + 1;  // tokens that every row sees
         for(; u < u1; u += kWaves) {
             const int next = u + kWaves;
@@ -341,7 +334,7 @@ __global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(AttnArgs a) {
                     vr[i].w &= keep[3];
                     nan |= nan_bytes(vr[i].x) | nan_bytes(vr[i].y) | nan_bytes(vr[i].z) | nan_bytes(vr[i].w);
                 }
-                if(__ballot(nan != 0)) {
+                if(__builtin_expect(__ballot(nan != 0) != 0, 0)) {
                     // a NaN among the values of tokens that some rows do not see, where
                     // 0 times it must not reach them: how many of a column's NaN each row
                     // sees, as a product of ones, and zeros in their place
@@ -399,7 +392,7 @@ __global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(AttnArgs a) {
             part_l[wave][lane] = l;
         }
         __syncthreads();
-        const bool whole = u0 == 0 && u1 == w.units;
+        const bool whole = WHOLE || (u0 == 0 && u1 == units);
         float* out = a.ws + ((int64_t)blockIdx.x * 2 + (now == begin ? 0 : 1)) * kPart<HP>;
         for(int i = threadIdx.x; i < rows * (HP / 4); i += kWaves * kWave) {
             const int r = i / (HP / 4), d = 4 * (i % (HP / 4));
@@ -435,75 +428,76 @@ __global__ __launch_bounds__(kWaves * kWave) void few_rows_kernel(AttnArgs a) {
     }
 }
 
-// the tiles that several workgroups have parts of: one row a workgroup, its threads on 4
-// values each of as many parts at once
+// The tiles that several workgroups have parts of: a workgroup here stands for the one
+// there that has a tile's last part, and a wave for one of the tile's rows, its lanes on 4
+// values each of as many parts at once as there are lanes for.
 template <int HP, int R>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
-    constexpr int D4 = HP / 4, PARTS = 256 / D4;
-    __shared__ __align__(16) float sums[PARTS][HP];
-    __shared__ float totals[PARTS];
+    constexpr int D4 = HP / 4, PARTS = kWave / D4;
     const PkKvCache& c = a.c;
-    const int r = (int)(blockIdx.x % R);
-    int item = (int)(blockIdx.x / R);
-    const int b = find_sequence((int)c.B, item, [&](int i) {
-        return cut<R>(a, sequence(c, a.N, i)).tiles * (int)c.kv_heads;
-    });
-    if(b < 0) return;
-    const Seq s = sequence(c, a.N, b);
-    const Cut w = cut<R>(a, s);
-    int64_t before, all;
-    count_units<R>(a, b, before, all);
-    const int64_t share = share_of(all, a.W), p0 = before + (int64_t)item * w.units;
-    const int64_t w0 = p0 / share, w1 = (p0 + w.units - 1) / share;
-    const int h = item / w.tiles, row = (item - h * w.tiles) * R + r;
-    if(w0 == w1 || row >= s.n * a.group) return;
-    auto part = [&](int64_t i) {
-        return a.ws + (i * 2 + (i == w0 && p0 != w0 * share ? 1 : 0)) * kPart<HP>;
-    };
+    const int lane = threadIdx.x % kWave, r = blockIdx.y * 4 + threadIdx.x / kWave;
+    int share = 1, at, b;
+    Seq s;
+    if(!locate(
+           c, a.N, [&](const Seq& t) { return tiles_of<R>(a, t) * (int)c.kv_heads * units_of(t); },
+           [&](int all) {
+               share = share_of(all, a.W);
+               return (int)blockIdx.x * share;
+           },
+           at, b, s))
+        return;
+    const int tiles = tiles_of<R>(a, s), units = units_of(s), item = at / units, u0 = at - item * units;
+    if(u0 == 0 || units - u0 > share) return;  // it begins here, or has parts behind
+    const int h = item / tiles, row = (item - h * tiles) * R + r;
+    if(row >= s.n * a.group) return;
+    // the first part's workgroup, where it is in that one's place 0 if it begins its share
+    const int before = (u0 + share - 1) / share, w1 = blockIdx.x, w0 = w1 - before;
+    if(w0 < 0) return;  // (offsets that decrease)
+    const int first_place = before * share == u0 ? 0 : 1;
+    auto part = [&](int w) { return a.ws + ((int64_t)w * 2 + (w == w0 ? first_place : 0)) * kPart<HP>; };
     float top = kNone;
-    for(int64_t i = w0 + threadIdx.x % kWave; i <= w1; i += kWave) top = fmaxf(top, part(i)[r]);
+    for(int w = w0 + lane; w <= w1; w += kWave) top = fmaxf(top, part(w)[r]);
     top = wave_max(top);
-    const int mine = threadIdx.x / D4, d = 4 * (threadIdx.x % D4);
+    const int d = 4 * (lane % D4), mine = lane / D4;
     f32x4 v = {};
     float total = 0.0f;
     if(mine < PARTS) {
-        for(int64_t i = w0 + mine; i <= w1; i += PARTS) {
-            const float* p = part(i);
+#pragma unroll 4
+        for(int w = w0 + mine; w <= w1; w += PARTS) {
+            const float* p = part(w);
             const float f = __builtin_amdgcn_exp2f(p[r] - top);
             total = fmaf(f, p[16 + r], total);
             v += f * *(const f32x4*)(p + 32 + r * HP + d);
         }
-        *(f32x4*)&sums[mine][d] = v;
-        if(d == 0) totals[mine] = total;
     }
-    __syncthreads();
-    if(threadIdx.x >= D4) return;
+    f32x4 sum = v;
+    float all = total;
 #pragma unroll
     for(int k = 1; k < PARTS; ++k) {
-        v += *(const f32x4*)&sums[k][d];
-        total += totals[k];
+        all += __shfl(total, lane + k * D4, kWave);
+#pragma unroll
+        for(int i = 0; i < 4; ++i) sum[i] += __shfl(v[i], lane + k * D4, kWave);
     }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    if(mine) return;
+    const float inv = all == 0.0f ? 0.0f : 1.0f / all;
     float* to = a.o + (int64_t)(s.row + row / a.group) * a.ldo + (int64_t)(h * a.group + row % a.group) * c.hd + d;
 #pragma unroll
     for(int k = 0; k < 4; ++k)
-        if(d + k < c.hd) to[k] = v[k] * inv;
+        if(d + k < c.hd) to[k] = sum[k] * inv;
 }
 
 // ------------------------------------------------------------------- launches
 struct Plan {
-    int rows;         // 8 or 16 query rows a tile
-    int64_t W, items; // workgroups; tiles times heads there may be
+    int rows;       // 8 or 16 query rows a tile
+    int W;          // workgroups that share the units of all tiles; 0: a workgroup to a tile
+    int64_t items;  // tiles, times heads, that there may be
 };
 Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
     Plan p;
-    const int64_t group = H / c->kv_heads;
+    const int64_t group = H / c->kv_heads, units = (c->width * c->page + kUnit - 1) / kUnit;
     p.rows = N * group <= 8 * c->B ? 8 : 16;
     p.items = (N * group / p.rows + (c->B < N ? c->B : N)) * c->kv_heads;
-    p.W = 512;
-    // no more than there can be units for
-    const int64_t most = p.items * ((c->width * c->page + kUnit - 1) / kUnit + 1) / kMinShare + 1;
-    if(p.W > most) p.W = most;
+    p.W = units <= 32 || p.items * units >= (int64_t)1 << 31 ? 0 : 512;
     return p;
 }
 
@@ -517,22 +511,28 @@ int check_attn(const char* who, const PkKvCache* c, int64_t N, int64_t H) {
     return PK_OK;
 }
 
+template <int HP, bool SPLIT>
+void launch_rows(const AttnArgs& a, const Plan& p, hipStream_t st) {
+    if(!p.W) {
+        few_rows_kernel<HP, SPLIT, true><<<(unsigned)p.items, waves_of(HP, true) * kWave, 0, st>>>(a);
+        return;
+    }
+    few_rows_kernel<HP, SPLIT, false><<<(unsigned)p.W, 256, 0, st>>>(a);
+    join_kernel<HP, SPLIT ? 8 : 16><<<dim3((unsigned)p.W, SPLIT ? 2 : 4), 256, 0, st>>>(a);
+}
 template <int HP>
 void launch(const AttnArgs& a, const Plan& p, hipStream_t st) {
-    if(p.rows == 8) {
-        few_rows_kernel<HP, true><<<(unsigned)p.W, kWaves * kWave, 0, st>>>(a);
-        join_kernel<HP, 8><<<(unsigned)(p.items * 8), 256, 0, st>>>(a);
-    } else {
-        few_rows_kernel<HP, false><<<(unsigned)p.W, kWaves * kWave, 0, st>>>(a);
-        join_kernel<HP, 16><<<(unsigned)(p.items * 16), 256, 0, st>>>(a);
-    }
+    if(p.rows == 8)
+        launch_rows<HP, true>(a, p, st);
+    else
+        launch_rows<HP, false>(a, p, st);
 }
 
 }  // namespace
 
 extern "C" size_t pk_attn_paged_workspace(const PkKvCache* cache, int64_t N, int64_t H) {
     if(check_attn("pk_attn_paged_workspace", cache, N, H) || N == 0 || cache->B == 0) return 0;
-    return sizeof(float) * 2 * plan(cache, N, H).W * (32 + 16 * head_size(cache->hd));
+    return sizeof(float) * 2 * (size_t)plan(cache, N, H).W * (32 + 16 * head_size(cache->hd));
 }
 
 extern "C" int pk_attn_paged_f32(const PkKvCache* cache, int64_t N, int64_t H, float scale,
@@ -549,7 +549,7 @@ extern "C" int pk_attn_paged_f32(const PkKvCache* cache, int64_t N, int64_t H, f
         return fail("pk_attn_paged_f32: workspace of %zu bytes, %zu needed, 16-byte aligned",
                     workspace ? workspace_bytes : 0, need);
     const Plan p = plan(cache, N, H);
-    if(!grid_fits(p.items * p.rows, 256)) return fail("pk_attn_paged_f32: too many rows for one launch");
+    if(!grid_fits(p.items, 512)) return fail("pk_attn_paged_f32: too many rows for one launch");
     AttnArgs a = {};
     a.c = *cache;
     a.N = (int)N;

@@ -309,13 +309,14 @@ def test_attention_is_repeatable(dev, new):
         assert torch.equal(a, b)
 
 
-def test_attention_bad_arrays(dev):
+@pytest.mark.parametrize("past", [10, 3000])
+def test_attention_bad_arrays(dev, past):
     """lengths and offsets of any value reach nothing out of bounds"""
     rng = np.random.default_rng(15)
-    p = Pair(dev, rng, [10, 10, 10], [4, 4, 4], 16, 2, 64)
+    p = Pair(dev, rng, [past, 10, 10], [4, 4, 4], 16, 2, 64)
     q = torch.randn(12, 128, device=dev)
     for lens, offsets in (([-5, 10 ** 9, 0], [0, 4, 8, 12]), ([0, 0, 0], [-9, -3, -3, -1]),
-                          ([0, 0, 0], [12, 70, 10 ** 9, 5]), ([2 ** 31 - 1, -2 ** 31, 7], [0, 12, 3, 40])):
+                          ([0, 0, 0], [12, 70, 10 ** 9, 5]), ([9, 9, 9], [0, 12, 0, 12]), ([2 ** 31 - 1, -2 ** 31, 7], [0, 12, 3, 40])):
         p.lens_t.copy_(_i32(lens, dev))
         p.offsets_t.copy_(_i32(offsets, dev))
         o = torch.empty_like(q)
@@ -477,8 +478,9 @@ def test_refused_by_the_bindings(dev):
         K.attn_paged(p.c, 3, torch.zeros(2, 192, device=dev), torch.zeros(2, 192, device=dev))
     with pytest.raises(TypeError):
         K.attn_paged(p.c, 2, k.double(), k)
+    far = K.PagedKV(*p.t[:4], torch.full((1, 4096), -1, device=dev, dtype=torch.int32), p.lens_t, p.offsets_t, 64)
     with pytest.raises(PkError, match="workspace"):
-        K.attn_paged(p.c, 2, k, k.clone(), ws=torch.empty(16, dtype=torch.uint8, device=dev))
+        K.attn_paged(far, 2, k, k.clone(), ws=torch.empty(16, dtype=torch.uint8, device=dev))
     t = p.t
     for bad in ([t[0][:, :1].contiguous()] + t[1:], [t[0], t[0]] + t[2:], t[:2] + [t[2][:1].contiguous()] + t[3:]):
         with pytest.raises(ValueError):
