@@ -42,6 +42,7 @@ struct AttnArgs {
     int64_t ldo;
     float* ws;
     int W;    // workgroups that share the units of all tiles
+    int splits;  // workgroups to a tile of many rows
     int vec;  // q can be read in float4
 };
 
@@ -486,19 +487,347 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
         if(d + k < c.hd) to[k] = sum[k] * inv;
 }
 
+// ------------------------------------------------ many query rows a sequence
+// A workgroup takes 128 query rows of one head of the cache, a wave 32 of them as the
+// columns of 32x32 products, whose results' rows are in a lane and the one 32 further.
+// Units of 64 tokens go through LDS, still in 8 bits, two at a time: one is read while the
+// next is on its way through registers.  Keys stand in LDS in the order of the product's
+// rows, so that a lane's 16 scores are of 16 tokens in a row, on one page; rows of both are
+// 16 bytes apart from a power of two, which spreads 8 lanes' 16 bytes over all banks.
+// `splits` workgroups share a tile's units where the tiles are too few for the chip, and
+// leave their parts for finish_kernel.
+constexpr int kRows = 128;
+
+template <int HP>
+constexpr int64_t kManyPart = (int64_t)kRows * (HP + 2);
+
+template <int HP>
+__global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnArgs a) {
+    constexpr int STEPS = HP / 16, DT = HP / 32;
+    constexpr int KS = HP + 16, VS = kUnit + 16;       // bytes between rows in LDS
+    constexpr int CHUNKS = kUnit * HP / 16, LOADS = (CHUNKS + 255) / 256;  // of 16 bytes; a thread's
+    __shared__ __align__(16) uint8_t keys[2][kUnit * KS], values[2][HP * VS];
+    __shared__ __align__(16) float4 pages[2][kUnit / 16];  // 2^ek, ev, 2^-ev, whether there
+    const PkKvCache& c = a.c;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int col = lane % 32, half = lane / 32;
+    const int page = (int)c.page, kvh = (int)c.kv_heads, hd = (int)c.hd, shift = __builtin_ctz(page);
+
+    // heads of the cache in turn, so that one stays with an XCD; then parts, then tiles
+    const int h = (int)(blockIdx.x % (unsigned)kvh);
+    const int rest = (int)(blockIdx.x / (unsigned)kvh), split = rest % a.splits;
+    int at, b;
+    Seq s;
+    if(!locate(
+           c, a.N, [&](const Seq& t) { return tiles_of<kRows>(a, t); }, [&](int) { return rest / a.splits; },
+           at, b, s))
+        return;
+    const int tile = tiles_of<kRows>(a, s) - 1 - at;  // those that see the most first
+    const int first = tile * kRows + wave * 32, total = s.n * a.group;
+    const int last = (tile + 1) * kRows < total ? (tile + 1) * kRows - 1 : total - 1;
+    int units = s.past + last / a.group + 1;
+    units = ((units < s.end ? units : s.end) + kUnit - 1) / kUnit;
+    const int each = (units + a.splits - 1) / a.splits;
+    const int u0 = split * each, u1 = u0 + each < units ? u0 + each : units;
+
+    // the lane's query
+    const int row = first + col, rows = total - first < 32 ? total - first : 32;
+    const int real_row = col < rows ? row : tile * kRows;
+    const int token = real_row / a.group;
+    const float* qr = a.q + (int64_t)(s.row + token) * a.ldq + (int64_t)(h * a.group + real_row % a.group) * hd;
+    const int reach = s.past + token;
+    f16x8 qh[STEPS], ql[STEPS];
+    float coef;
+    {
+        float x[STEPS][8], amax = 0.0f;
+#pragma unroll
+        for(int st = 0; st < STEPS; ++st) {
+            const int d = 32 * (st / 2) + 16 * half + 8 * (st % 2);
+            if(a.vec) {
+#pragma unroll
+                for(int i = 0; i < 8; i += 4) {
+                    const f32x4 v = d + i < hd ? *(const f32x4*)(qr + d + i) : f32x4{};
+#pragma unroll
+                    for(int k = 0; k < 4; ++k) x[st][i + k] = v[k];
+                }
+            } else {
+#pragma unroll
+                for(int i = 0; i < 8; ++i) x[st][i] = d + i < hd ? qr[d + i] : 0.0f;
+            }
+#pragma unroll
+            for(int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[st][i]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
+        const int eq = amax > 0.0f && amax <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
+        coef = ldexpf(a.scale, eq);
+#pragma unroll
+        for(int st = 0; st < STEPS; ++st)
+#pragma unroll
+            for(int i = 0; i < 8; ++i) {
+                const float y = col < rows ? ldexpf(x[st][i], -eq) : 0.0f;
+                qh[st][i] = (_Float16)y;
+                ql[st][i] = (_Float16)(y - (float)qh[st][i]);
+            }
+    }
+
+    auto page_of = [&](int u, int g16) {
+        const int i = (u * kUnit + 16 * g16) >> shift;
+        const int pid = u < u1 && i < c.width ? c.table[(int64_t)b * c.width + i] : -1;
+        return pid < 0 || pid >= c.pages ? -1 : pid;
+    };
+    // a thread's chunks: of keys, 16 values of token e / (HP / 16); of values, 16 tokens of
+    // row e / 4, of which `real` are the sequence's
+    int pk[LOADS], pv, real = 0;
+    uint4 kr[LOADS], vr[LOADS];
+    float4 pr;
+    const int g16 = threadIdx.x % 4;
+    auto find_pages = [&](int u) {
+#pragma unroll
+        for(int i = 0; i < LOADS; ++i) pk[i] = page_of(u, (threadIdx.x + 256 * i) / (HP / 16) % kUnit / 16);
+        pv = page_of(u, g16);
+    };
+    auto load = [&](int u) {
+        const int64_t v_head = (int64_t)(pv < 0 ? 0 : pv) * kvh + h;
+#pragma unroll
+        for(int i = 0; i < LOADS; ++i) {
+            const int e = threadIdx.x + 256 * i, t = e / (HP / 16), d16 = e % (HP / 16);
+            if(e < CHUNKS) {
+                const int64_t k_head = (int64_t)(pk[i] < 0 ? 0 : pk[i]) * kvh + h;
+                kr[i] = *(const uint4*)(c.k + (k_head * page + ((u * kUnit + t) & (page - 1))) * HP + 16 * d16);
+                vr[i] = *(const uint4*)(c.v + (v_head * HP + e / 4) * page +
+                                        ((u * kUnit + 16 * g16) & (page - 1)));
+            }
+        }
+        if(threadIdx.x < 4) {
+            const uint8_t ek = c.k_exp[v_head], ev = c.v_exp[v_head];
+            pr = {power(ek), (float)((int)ev - 127), power(254 - ev), pv < 0 ? 0.0f : 1.0f};
+        }
+        real = pv < 0 ? 0 : held(s.end - u * kUnit - 16 * g16, 0, 16);
+    };
+    auto store = [&](int buf) {
+#pragma unroll
+        for(int i = 0; i < LOADS; ++i) {
+            const int e = threadIdx.x + 256 * i, t = e / (HP / 16), d16 = e % (HP / 16);
+            if(e < CHUNKS) {
+                // the row of the product that a token is: bits 4 3 2 1 0 become 3 2 4 1 0
+                const int row = (t & 32) + ((t & 12) << 1) + ((t & 16) >> 2) + (t & 3);
+                *(uint4*)&keys[buf][row * KS + 16 * d16] = kr[i];
+                if(real < 16) {  // values behind the sequence's end, or on no page, may be anything
+                    uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
+#pragma unroll
+                    for(int k = 0; k < 4; ++k) {
+                        const int n = held(real - 4 * k, 0, 4);
+                        w[k] &= n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
+                    }
+                    vr[i] = {w[0], w[1], w[2], w[3]};
+                }
+                *(uint4*)&values[buf][e / 4 * VS + 16 * g16] = vr[i];
+            }
+        }
+        if(threadIdx.x < 4) pages[buf][threadIdx.x] = pr;
+    };
+
+    f32x16 acc[DT];
+#pragma unroll
+    for(int i = 0; i < DT; ++i) acc[i] = f32x16{};
+    float m = kNone, l = 0.0f;
+    const int clear = s.past + (first < total ? first / a.group : 0) + 1;  // tokens that all rows see
+    const int reach_all = s.past + (first + rows - 1) / a.group;           // and that any does
+    find_pages(u0);
+    if(u0 < u1) {
+        load(u0);
+        store(0);
+    }
+    find_pages(u0 + 1);
+    __syncthreads();
+    for(int u = u0; u < u1; ++u) {
+        const int buf = (u - u0) & 1;
+        if(u + 1 < u1) {
+            load(u + 1);
+            find_pages(u + 2);
+        }
+#pragma unroll
+        for(int j = 0; j < 2; ++j) {
+            const int token0 = u * kUnit + 32 * j;
+            if(rows <= 0 || token0 > reach_all) continue;
+            f32x16 sc = {};
+#pragma unroll
+            for(int st = 0; st < STEPS; st += 2) {
+                const uint4 w = *(const uint4*)&keys[buf][(32 * j + col) * KS + 16 * st + 16 * half];
+                const f16x8 k0 = widen(w.x, w.y), k1 = widen(w.z, w.w);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[st], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[st + 1], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[st], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[st + 1], sc, 0, 0, 0);
+            }
+            const float4 g = pages[buf][2 * j + half];
+            const float kc = coef * g.x;
+            const bool absent = g.w == 0.0f;
+            const int mine0 = token0 + 16 * half;
+            float p[16], mx = kNone;
+#pragma unroll
+            for(int i = 0; i < 16; ++i) p[i] = fmaf(sc[i], kc, g.y);
+            const bool edge = token0 + 32 > clear || __ballot(absent) != 0;
+            if(edge) {
+#pragma unroll
+                for(int i = 0; i < 16; ++i)
+                    if(absent || mine0 + i > reach) p[i] = -INFINITY;
+            }
+#pragma unroll
+            for(int i = 0; i < 16; ++i) mx = fmaxf(mx, p[i]);
+            if(__ballot(mx > m + kRaise)) {
+                mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+                mx = fmaxf(mx, m);
+                const float down = __builtin_amdgcn_exp2f(m - mx);
+                l *= down;
+#pragma unroll
+                for(int i = 0; i < DT; ++i) acc[i] *= down;
+                m = mx;
+            }
+            const float low = m - kTop;
+            float sum = 0.0f;
+            f16x8 ph[2], pl[2];
+#pragma unroll
+            for(int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(p[i] - low);
+                sum += e;
+                ph[i / 8][i % 8] = (_Float16)e;
+                pl[i / 8][i % 8] = (_Float16)(e - (float)ph[i / 8][i % 8]);
+            }
+            l = fmaf(sum, g.z, l);
+#pragma unroll
+            for(int i = 0; i < DT; ++i) {
+                uint4 w = *(const uint4*)&values[buf][(32 * i + col) * VS + 32 * j + 16 * half];
+                if(edge) {
+                    const uint32_t nan = nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
+                    if(__builtin_expect(__ballot(nan != 0) != 0, 0)) {
+                        // (as in few_rows_kernel: the NaN that a row sees, counted)
+                        uint32_t word[4] = {w.x, w.y, w.z, w.w}, one[4];
+                        f16x8 seen[2];
+#pragma unroll
+                        for(int k = 0; k < 16; ++k)
+                            seen[k / 8][k % 8] = absent || mine0 + k > reach ? (_Float16)0.0f : (_Float16)1.0f;
+#pragma unroll
+                        for(int k = 0; k < 4; ++k) {
+                            const uint32_t bits = nan_bytes(word[k]) >> 7;
+                            one[k] = bits * 0x38;
+                            word[k] &= ~(bits * 0xff);
+                        }
+                        f32x16 count = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen(one[0], one[1]), seen[0],
+                                                                              f32x16{}, 0, 0, 0);
+                        count = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen(one[2], one[3]), seen[1], count,
+                                                                       0, 0, 0);
+#pragma unroll
+                        for(int r = 0; r < 16; ++r)
+                            if(count[r] > 0.0f) acc[i][r] = NAN;
+                        w = {word[0], word[1], word[2], word[3]};
+                    }
+                }
+                const f16x8 v0 = widen(w.x, w.y), v1 = widen(w.z, w.w);
+                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph[0], acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph[1], acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, pl[1], acc[i], 0, 0, 0);
+            }
+        }
+        if(u + 1 < u1) store(buf ^ 1);
+        __syncthreads();
+    }
+
+    l += __shfl_xor(l, 32, kWave);
+    if(col >= rows) return;
+    if(a.splits > 1) {  // (a part without units has the maximum of no scores, and zeros)
+        float* out = a.ws + (int64_t)blockIdx.x * kManyPart<HP>;
+        const int r = wave * 32 + col;
+        if(half == 0) {
+            out[r] = m;
+            out[kRows + r] = l;
+        }
+#pragma unroll
+        for(int i = 0; i < DT; ++i)
+#pragma unroll
+            for(int q = 0; q < 4; ++q)
+                *(f32x4*)(out + 2 * kRows + r * HP + 32 * i + 8 * q + 4 * half) =
+                    f32x4{acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    float* to = a.o + (int64_t)(s.row + token) * a.ldo + (int64_t)(h * a.group + row % a.group) * hd;
+#pragma unroll
+    for(int i = 0; i < DT; ++i)
+#pragma unroll
+        for(int q = 0; q < 4; ++q)
+#pragma unroll
+            for(int k = 0; k < 4; ++k) {
+                const int d = 32 * i + 8 * q + 4 * half + k;
+                if(d < hd) to[d] = acc[i][4 * q + k] * inv;
+            }
+}
+
+// the parts of many_rows_kernel's tiles together: a wave to a row
+template <int HP>
+__global__ __launch_bounds__(256) void finish_kernel(AttnArgs a) {
+    constexpr int D4 = HP / 4;
+    const PkKvCache& c = a.c;
+    const int lane = threadIdx.x % kWave, kvh = (int)c.kv_heads;
+    const int h = (int)(blockIdx.x % (unsigned)kvh);
+    const int rest = (int)(blockIdx.x / (unsigned)kvh);
+    int at, b;
+    Seq s;
+    if(!locate(
+           c, a.N, [&](const Seq& t) { return tiles_of<kRows>(a, t); }, [&](int) { return rest; }, at, b, s))
+        return;
+    const int r = blockIdx.y * 4 + threadIdx.x / kWave;
+    const int row = (tiles_of<kRows>(a, s) - 1 - at) * kRows + r;
+    if(row >= s.n * a.group) return;
+    const float* base = a.ws + ((int64_t)rest * a.splits * kvh + h) * kManyPart<HP>;
+    const int64_t apart = (int64_t)kvh * kManyPart<HP>;
+    float top = kNone, total = 0.0f;
+    for(int i = 0; i < a.splits; ++i) top = fmaxf(top, base[i * apart + r]);
+    const int d = 4 * lane;
+    f32x4 v = {};
+    for(int i = 0; i < a.splits; ++i) {
+        const float* p = base + i * apart;
+        const float f = __builtin_amdgcn_exp2f(p[r] - top);
+        total = fmaf(f, p[kRows + r], total);
+        if(lane < D4) v += f * *(const f32x4*)(p + 2 * kRows + r * HP + d);
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    float* to = a.o + (int64_t)(s.row + row / a.group) * a.ldo + (int64_t)(h * a.group + row % a.group) * c.hd + d;
+#pragma unroll
+    for(int k = 0; k < 4; ++k)
+        if(lane < D4 && d + k < c.hd) to[k] = v[k] * inv;
+}
+
 // ------------------------------------------------------------------- launches
 struct Plan {
-    int rows;       // 8 or 16 query rows a tile
-    int W;          // workgroups that share the units of all tiles; 0: a workgroup to a tile
-    int64_t items;  // tiles, times heads, that there may be
+    int rows;       // 8, 16 or 128 query rows a tile
+    int W;          // of few rows: workgroups that share the units of all tiles; 0: one to a tile
+    int splits;     // of many: workgroups to a tile
+    int64_t tiles;  // for each head of the cache, that there may be
 };
 Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
-    Plan p;
+    Plan p = {};
     const int64_t group = H / c->kv_heads, units = (c->width * c->page + kUnit - 1) / kUnit;
-    p.rows = N * group <= 8 * c->B ? 8 : 16;
-    p.items = (N * group / p.rows + (c->B < N ? c->B : N)) * c->kv_heads;
-    p.W = units <= 32 || p.items * units >= (int64_t)1 << 31 ? 0 : 512;
+    const int64_t some = c->B < N ? c->B : N;
+    p.rows = N * group <= 8 * c->B ? 8 : N * group <= 32 * c->B ? 16 : kRows;
+    p.tiles = N * group / p.rows + some;
+    if(p.rows < kRows) {
+        p.W = units <= 32 || p.tiles * c->kv_heads * units >= (int64_t)1 << 31 ? 0 : 512;
+    } else {
+        // workgroups that there are for sure, two to a CU, of 8 units at least
+        const int64_t sure = (N * group + kRows - 1) / kRows * c->kv_heads;
+        int64_t n = 512 / sure;
+        if(n > units / 8) n = units / 8;
+        p.splits = (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+    }
     return p;
+}
+size_t plan_bytes(const Plan& p, const PkKvCache* c) {
+    const size_t hp = head_size(c->hd);
+    if(p.W) return sizeof(float) * 2 * p.W * (32 + 16 * hp);
+    if(p.splits > 1) return sizeof(float) * p.tiles * c->kv_heads * p.splits * kRows * (hp + 2);
+    return 0;
 }
 
 int check_attn(const char* who, const PkKvCache* c, int64_t N, int64_t H) {
@@ -514,7 +843,8 @@ int check_attn(const char* who, const PkKvCache* c, int64_t N, int64_t H) {
 template <int HP, bool SPLIT>
 void launch_rows(const AttnArgs& a, const Plan& p, hipStream_t st) {
     if(!p.W) {
-        few_rows_kernel<HP, SPLIT, true><<<(unsigned)p.items, waves_of(HP, true) * kWave, 0, st>>>(a);
+        few_rows_kernel<HP, SPLIT, true>
+            <<<(unsigned)(p.tiles * a.c.kv_heads), waves_of(HP, true) * kWave, 0, st>>>(a);
         return;
     }
     few_rows_kernel<HP, SPLIT, false><<<(unsigned)p.W, 256, 0, st>>>(a);
@@ -522,17 +852,18 @@ void launch_rows(const AttnArgs& a, const Plan& p, hipStream_t st) {
 }
 template <int HP>
 void launch(const AttnArgs& a, const Plan& p, hipStream_t st) {
-    if(p.rows == 8)
-        launch_rows<HP, true>(a, p, st);
-    else
-        launch_rows<HP, false>(a, p, st);
+    if(p.rows == 8) return launch_rows<HP, true>(a, p, st);
+    if(p.rows == 16) return launch_rows<HP, false>(a, p, st);
+    const int64_t tiles = p.tiles * a.c.kv_heads;
+    many_rows_kernel<HP><<<(unsigned)(tiles * p.splits), 256, 0, st>>>(a);
+    if(p.splits > 1) finish_kernel<HP><<<dim3((unsigned)tiles, kRows / 4), 256, 0, st>>>(a);
 }
 
 }  // namespace
 
 extern "C" size_t pk_attn_paged_workspace(const PkKvCache* cache, int64_t N, int64_t H) {
     if(check_attn("pk_attn_paged_workspace", cache, N, H) || N == 0 || cache->B == 0) return 0;
-    return sizeof(float) * 2 * (size_t)plan(cache, N, H).W * (32 + 16 * head_size(cache->hd));
+    return plan_bytes(plan(cache, N, H), cache);
 }
 
 extern "C" int pk_attn_paged_f32(const PkKvCache* cache, int64_t N, int64_t H, float scale,
@@ -544,12 +875,13 @@ extern "C" int pk_attn_paged_f32(const PkKvCache* cache, int64_t N, int64_t H, f
     if(!q || !o) return fail("pk_attn_paged_f32: NULL pointer");
     if(ldq < width || ldo < width)
         return fail("pk_attn_paged_f32: row strides must be at least H*hd = %lld", (long long)width);
-    const size_t need = pk_attn_paged_workspace(cache, N, H);
+    const Plan p = plan(cache, N, H);
+    const size_t need = plan_bytes(p, cache);
     if(need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail("pk_attn_paged_f32: workspace of %zu bytes, %zu needed, 16-byte aligned",
                     workspace ? workspace_bytes : 0, need);
-    const Plan p = plan(cache, N, H);
-    if(!grid_fits(p.items, 512)) return fail("pk_attn_paged_f32: too many rows for one launch");
+    if(!grid_fits(p.tiles * cache->kv_heads * (p.splits > 1 ? p.splits : 1), 512))
+        return fail("pk_attn_paged_f32: too many rows for one launch");
     AttnArgs a = {};
     a.c = *cache;
     a.N = (int)N;
@@ -562,6 +894,7 @@ extern "C" int pk_attn_paged_f32(const PkKvCache* cache, int64_t N, int64_t H, f
     a.ldo = ldo;
     a.ws = (float*)workspace;
     a.W = p.W;
+    a.splits = p.splits;
     a.vec = cache->hd % 4 == 0 && ldq % 4 == 0 && aligned16(q);
     const hipStream_t st = as_stream(stream);
     switch(head_size(cache->hd)) {
