@@ -249,6 +249,73 @@ struct PicoTensor* pico_expert_matmul(struct PicoTensor* x, struct PicoTensor* w
 struct PicoTensor* pico_expert_combine(struct PicoTensor* ys, struct PicoTensor* gates,
                                        const struct PicoRoute* route, struct PicoTensor* c);
 
+/* ---- rotary positions (no reference counterpart) ----
+ * The first `rot` values of a head turn in pairs by their token's position, pair i by
+ * base^(-2i/rot) radians a position: (i, i + rot/2), or (2i, 2i + 1) when interleaved.
+ * scaling stretches the frequencies for contexts longer than the trained one: PICO_ROPE_
+ * PLAIN (not), LINEAR (divided by factor), NTK (base * factor^(rot/(rot-2))) or PARTS (a pair
+ * that turns more than `high` times in the trained `length` stays, one that turns less than
+ * `low` times is divided by factor, those between in proportion).  magnitude multiplies
+ * what is turned (0: 1).
+ * pico_rope: the heads of x [rows, n_heads*hd] (contiguous or a column view) turned by
+ * positions (int32, one a row, in host or device memory).  The rope may be freed once what
+ * was made with it is no longer used. */
+#define PICO_ROPE_PLAIN 0
+#define PICO_ROPE_LINEAR 1
+#define PICO_ROPE_NTK 2
+#define PICO_ROPE_PARTS 3
+struct PicoRopeConfig {
+    int rot;
+    int interleaved;
+    float base; /* normally 10000 */
+    int scaling;
+    float factor, length, low, high; /* low, high: normally 1 and 32 */
+    float magnitude;
+};
+struct PicoRope;
+struct PicoRope* pico_rope_init(const struct PicoRopeConfig* cfg);
+void pico_rope_free(struct PicoRope* rope);
+struct PicoTensor* pico_rope(struct PicoTensor* x, const struct PicoRope* rope,
+                             const int32_t* positions, int n_heads);
+
+/* ---- causal attention token by token (no reference counterpart) ----
+ * A cache of the keys and values of `sequences` sequences of up to max_length tokens, for
+ * every layer of a model, in 8 bits: pages of `page` (16, 32, 64 or 128) tokens, e4m3 values
+ * with a power of two for each page and head; `pages` pages for all sequences together.
+ *   pico_kv_begin(kv, new_tokens);            new_tokens [sequences], 0 for one that waits
+ *   per layer: o = pico_attention_cached(kv, layer, q, k, v, n_heads, rope)
+ * pico_kv_begin: starts a step, whose rows are the new tokens, sequence after sequence;
+ *   gives sequences the pages they need.  Returns the number of rows, or -1 (too few pages
+ *   are free, a sequence would pass max_length), the cache left as it was.  It copies to the
+ *   device, so not under graph capture: a captured step is replayed after a pico_kv_begin
+ *   with as many rows, and then works on the sequences that this one names.
+ * pico_attention_cached: puts k, v [rows, kv_heads*hd] into the layer's cache, the keys
+ *   turned by `rope` at their positions (NULL: as they are), and returns the causal
+ *   attention of q [rows, n_heads*hd], turned likewise, over all that the cache holds of
+ *   each row's sequence up to the row itself: softmax(q k^T / sqrt(hd)) v, head h reading
+ *   the cache's head h / (n_heads / kv_heads).  fp32 whatever the matmul precision, but for
+ *   the cache's 8 bits.  For inference: no gradient passes through it.
+ * pico_kv_length: tokens of a sequence, the present step's among them (-1: no such one).
+ * pico_kv_drop: forgets a sequence, whose pages are free for the next step's. */
+struct PicoKVConfig {
+    int layers;
+    int kv_heads;
+    int head_dim; /* 1 to 256 */
+    int page;
+    int pages;
+    int sequences;
+    int max_length;
+};
+struct PicoKV;
+struct PicoKV* pico_kv_init(const struct PicoKVConfig* cfg);
+int64_t pico_kv_begin(struct PicoKV* kv, const int32_t* new_tokens);
+struct PicoTensor* pico_attention_cached(struct PicoKV* kv, int layer, struct PicoTensor* q,
+                                         struct PicoTensor* k, struct PicoTensor* v, int n_heads,
+                                         const struct PicoRope* rope);
+int64_t pico_kv_length(const struct PicoKV* kv, int sequence);
+int pico_kv_drop(struct PicoKV* kv, int sequence);
+void pico_kv_free(struct PicoKV* kv);
+
 /* ---- nn (src/nn/linear.h:6-15) ---- */
 struct PicoLinear {
     int in_features;

@@ -109,6 +109,8 @@ void* pkh_arena_alloc_with(struct Arena* a, size_t size, void* (*device_alloc)(s
 void* pkh_arena_workspace_opt(struct Arena* a, size_t bytes);
 int pkh_is_device_ptr(const void* p);
 int pkh_copy_h2d(void* dst, const void* src, size_t bytes);
+/* the same for memory that is no parameter's: kept casts of parameters stay */
+int pkh_upload(void* dst, const void* src, size_t bytes);
 int pkh_copy_d2h(void* dst, const void* src, size_t bytes);
 /* device-to-device on the library's stream, not waited for */
 int pkh_copy_d2d_async(void* dst, const void* src, size_t bytes);

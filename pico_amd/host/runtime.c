@@ -343,10 +343,14 @@ int pkh_is_device_ptr(const void* p) {
 }
 
 int pkh_copy_h2d(void* dst, const void* src, size_t bytes) {
+    if(bytes) pkh_params_changed(); /* the copy may write a parameter */
+    return pkh_upload(dst, src, bytes);
+}
+
+int pkh_upload(void* dst, const void* src, size_t bytes) {
     if(pkh_init()) return -1;
     if(capture_refuses("a host-to-device copy")) return -1;
     if(bytes == 0) return 0;
-    pkh_params_changed(); /* the copy may write a parameter */
     pkh_side_join();
     hipStream_t st = (hipStream_t)pkh_stream();
     hipError_t e = hipMemcpyAsync(dst, src, bytes, hipMemcpyHostToDevice, st);

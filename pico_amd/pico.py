@@ -49,6 +49,19 @@ class PicoGPTConfig(ctypes.Structure):
                [("norm_eps", ctypes.c_float), ("init_std", ctypes.c_float)]
 
 
+class PicoRopeConfig(ctypes.Structure):
+    """struct PicoRopeConfig (include/pico_amd.h)"""
+    _fields_ = [("rot", ctypes.c_int), ("interleaved", ctypes.c_int), ("base", c_f),
+                ("scaling", ctypes.c_int)] + \
+               [(n, c_f) for n in ("factor", "length", "low", "high", "magnitude")]
+
+
+class PicoKVConfig(ctypes.Structure):
+    """struct PicoKVConfig (include/pico_amd.h)"""
+    _fields_ = [(n, ctypes.c_int) for n in ("layers", "kv_heads", "head_dim", "page", "pages",
+                                            "sequences", "max_length")]
+
+
 GPT_KEYS = ("vocab", "d_model", "n_layers", "n_heads", "d_ff", "batch", "seq_len")
 
 _SIGS = {
@@ -134,6 +147,15 @@ _GPU_SIGS = {
     "pico_expert_gather": (TP, [TP, c_p]),
     "pico_expert_matmul": (TP, [TP, TP, c_p]),
     "pico_expert_combine": (TP, [TP, TP, c_p, TP]),
+    "pico_rope_init": (c_p, [ctypes.POINTER(PicoRopeConfig)]),
+    "pico_rope_free": (None, [c_p]),
+    "pico_rope": (TP, [TP, c_p, c_p, ctypes.c_int]),
+    "pico_kv_init": (c_p, [ctypes.POINTER(PicoKVConfig)]),
+    "pico_kv_begin": (c_i64, [c_p, c_p]),
+    "pico_attention_cached": (TP, [c_p, ctypes.c_int, TP, TP, TP, ctypes.c_int, c_p]),
+    "pico_kv_length": (c_i64, [c_p, ctypes.c_int]),
+    "pico_kv_drop": (ctypes.c_int, [c_p, ctypes.c_int]),
+    "pico_kv_free": (None, [c_p]),
     "pico_set_matmul_precision": (ctypes.c_int, [ctypes.c_int]),
     "pico_get_matmul_precision": (ctypes.c_int, []),
     "pico_checkpoint_save": (ctypes.c_int, [ctypes.c_char_p, ctypes.c_int, ctypes.POINTER(TP),
@@ -338,6 +360,38 @@ class Pico:
         if self.lib.pico_route_to_host(route, e.ctypes.data_as(c_p), o.ctypes.data_as(c_p)):
             raise PicoError("pico_route_to_host failed")
         return e, o
+
+    def rope_init(self, rot, interleaved=False, base=10000.0, scaling=0, factor=1.0, length=0.0,
+                  low=1.0, high=32.0, magnitude=0.0):
+        """pico_rope_init: a rope, to be given to pico_rope_free"""
+        c = PicoRopeConfig(rot, int(interleaved), base, scaling, factor, length, low, high, magnitude)
+        r = self.lib.pico_rope_init(ctypes.byref(c))
+        if not r:
+            raise PicoError("pico_rope_init failed " +
+                            self.lib.pico_gpu_last_error().decode(errors="replace"))
+        return r
+
+    def rope(self, x, rope, positions, n_heads):
+        """positions: an int32 numpy array (staged per call) or a device pointer"""
+        p = positions if isinstance(positions, int) else self.ids(positions)
+        return self._check(self.lib.pico_rope(x, rope, p, n_heads), "pico_rope")
+
+    def kv_init(self, layers, kv_heads, head_dim, page, pages, sequences, max_length):
+        """pico_kv_init: a cache, to be given to pico_kv_free"""
+        c = PicoKVConfig(layers, kv_heads, head_dim, page, pages, sequences, max_length)
+        kv = self.lib.pico_kv_init(ctypes.byref(c))
+        if not kv:
+            raise PicoError("pico_kv_init failed " +
+                            self.lib.pico_gpu_last_error().decode(errors="replace"))
+        return kv
+
+    def kv_begin(self, kv, new_tokens):
+        """pico_kv_begin: the step's rows"""
+        a = np.ascontiguousarray(new_tokens, dtype=np.int32)
+        n = self.lib.pico_kv_begin(kv, a.ctypes.data_as(c_p))
+        if n < 0:
+            raise PicoError("pico_kv_begin failed")
+        return n
 
     def xent(self, logits, labels):
         return self._check(self.lib.pico_softmax_xent(logits, self.ids(labels)),

@@ -169,3 +169,52 @@ def test_the_oracle_rounds_to_nearest_even():
 def test_the_oracle_finds_the_exponent():
     for top, e in ((448.0, 0), (448.1, 1), (224.0, -1), (0.0, -40), (1e-30, -40), (1e30, 40), (1.0, -8)):
         assert O.exponent(np.array([top, -top / 2, np.nan, np.inf])) == e
+
+
+# --------------------------------------------------------------- pico's API
+@pytest.fixture(scope="module")
+def A():
+    from pico_amd import pico
+
+    lib = pico.amd_lib()
+    for name, (res, args) in pico._GPU_SIGS.items():
+        if "rope" in name or "kv_" in name or "cached" in name:
+            f = getattr(lib, name)
+            f.restype, f.argtypes = res, args
+    return lib
+
+
+@pytest.mark.parametrize("bad", [dict(rot=0), dict(rot=-2), dict(rot=7), dict(rot=1026), dict(base=0.0),
+                                 dict(scaling=9), dict(scaling=1, factor=0.0), dict(scaling=3, length=0.0),
+                                 dict(scaling=3, low=2.0, high=2.0), dict(magnitude=math.inf)])
+def test_pico_rope_init_refuses(A, bad):
+    from pico_amd.pico import PicoRopeConfig
+
+    f = dict(rot=8, interleaved=0, base=1e4, scaling=0, factor=2.0, length=9.0, low=1.0, high=32.0, magnitude=0.0)
+    f.update(bad)
+    c = PicoRopeConfig(*[f[n] for n, _ in PicoRopeConfig._fields_])
+    assert not A.pico_rope_init(ctypes.byref(c))
+    assert not A.pico_rope_init(None)
+    A.pico_rope_free(None)
+
+
+@pytest.mark.parametrize("bad", [dict(layers=0), dict(kv_heads=0), dict(kv_heads=4097), dict(head_dim=0),
+                                 dict(head_dim=257), dict(page=24), dict(pages=0), dict(sequences=0),
+                                 dict(sequences=(1 << 20) + 1), dict(max_length=0), dict(max_length=1 << 30)])
+def test_pico_kv_init_refuses(A, bad):
+    from pico_amd.pico import PicoKVConfig
+
+    f = dict(layers=1, kv_heads=2, head_dim=64, page=16, pages=4, sequences=2, max_length=64)
+    f.update(bad)
+    c = PicoKVConfig(*[f[n] for n, _ in PicoKVConfig._fields_])
+    assert not A.pico_kv_init(ctypes.byref(c))
+    assert not A.pico_kv_init(None)
+
+
+def test_pico_without_a_cache(A):
+    assert A.pico_kv_begin(None, None) == -1
+    assert A.pico_kv_length(None, 0) == -1
+    assert A.pico_kv_drop(None, 0) != 0
+    assert not A.pico_attention_cached(None, 0, None, None, None, 1, None)
+    assert not A.pico_rope(None, None, None, 1)
+    A.pico_kv_free(None)
