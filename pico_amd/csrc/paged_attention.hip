@@ -25,8 +25,12 @@ using namespace pk;
 
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kUnit = 64;          // tokens a wave takes at a time
+constexpr int kFew = 16;           // query rows a tile, where a sequence has few
 constexpr int kMinShare = 4;       // units a workgroup takes at least, where they share a tile
 constexpr float kTop = 7.0f;       // probabilities are relative to 2^7 below the maximum m
 constexpr float kRaise = 8.0f;     // m is raised when a score passes it by 2^8: p <= 2^15
@@ -58,17 +62,128 @@ __device__ __forceinline__ f16x8 widen(uint32_t lo, uint32_t hi) {
     return u.v;
 }
 
-// the value of the lane 8 further in the row of 16
-__device__ __forceinline__ float across8(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));
+// 8 values as their nearest f16 and the nearest f16 to what is left
+__device__ __forceinline__ void two_parts(const float* x, f16x8& hi, f16x8& lo) {
+#pragma unroll
+    for(int i = 0; i < 8; i += 2) {
+        const f16x2 h = __builtin_convertvector((f32x2{x[i], x[i + 1]}), f16x2);
+        float l0, l1;  // x - h, for which the compiler takes two instructions each
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l0) : "v"(h), "v"(x[i]));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]"
+            : "=v"(l1)
+            : "v"(h), "v"(x[i + 1]));
+        const f16x2 l = __builtin_convertvector((f32x2{l0, l1}), f16x2);
+        hi[i] = h[0];
+        hi[i + 1] = h[1];
+        lo[i] = l[0];
+        lo[i + 1] = l[1];
+    }
 }
 
 // a page's power of two from its byte
 __device__ __forceinline__ float power(uint8_t e) { return __uint_as_float((uint32_t)e << 23); }
 
 // 0x80 in every byte that is a NaN
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+__device__ __forceinline__ u32x4 nan_bytes(u32x4 w) {
     return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// a bit for every byte of 16 that is one
+__device__ __forceinline__ uint32_t nan_bits(u32x4 w) {
+    const u32x4 b = ((nan_bytes(w) >> 7) * 0x01020408u) >> 24 & 0xfu;
+    return b[0] | b[1] << 4 | b[2] << 8 | b[3] << 12;
+}
+
+// the first n of 16 bytes
+__device__ __forceinline__ u32x4 first_bytes(int n) {
+    u32x4 keep;
+#pragma unroll
+    for(int i = 0; i < 4; ++i) {
+        const int k = held(n - 4 * i, 0, 4);
+        keep[i] = k == 0 ? 0u : 0xffffffffu >> (32 - 8 * k);
+    }
+    return keep;
+}
+
+// What the reference m of a row's probabilities rises by, where their largest exponent is
+// mx: to 2^7 below mx where that is above `limit`, 2^15.  The first time, which limit =
+// kNone stands for, down too; not where there is no score yet.
+__device__ __forceinline__ float raise(float mx, float& limit) {
+    if(!(mx > kNone)) return 0.0f;
+    const float up = limit == kNone ? mx - kTop : fmaxf(mx - kTop, 0.0f);
+    limit = kTop + kRaise;
+    return up;
+}
+
+// Loads before it in the source are issued before those after it: results come in the order
+// of the loads, so one that is waited for first must not be behind others.
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
+
+// A lane's values of a query: step st's are 8 from at(st) on, those behind the head's end
+// any of it.  All loads are issued before the first is used.
+template <int STEPS, class F>
+__device__ __forceinline__ void load_query(const float* head, int hd, int vec, F at, float (&x)[STEPS][8]) {
+    if(vec) {
+#pragma unroll
+        for(int st = 0; st < STEPS; ++st)
+#pragma unroll
+            for(int i = 0; i < 8; i += 4) {
+                const int d = at(st) + i;
+                const f32x4 v = *(const f32x4*)(head + (d < hd ? d : 0));
+#pragma unroll
+                for(int k = 0; k < 4; ++k) x[st][i + k] = v[k];
+            }
+    } else {
+#pragma unroll
+        for(int st = 0; st < STEPS; ++st)
+#pragma unroll
+            for(int i = 0; i < 8; ++i) x[st][i] = head[at(st) + i < hd ? at(st) + i : 0];
+    }
+}
+
+// a query, held by lanes W apart, brought to [2^14, 2^15) by 2^-e and cut in two parts, zeros
+// behind its end; returns e.  Rows that are none become zeros.
+template <int W, int STEPS, class F>
+__device__ __forceinline__ int bring_up(float (&x)[STEPS][8], int hd, F at, bool on, f16x8 (&hi)[STEPS],
+                                        f16x8 (&lo)[STEPS]) {
+    float amax = 0.0f;
+#pragma unroll
+    for(int st = 0; st < STEPS; ++st)
+#pragma unroll
+        for(int i = 0; i < 8; ++i) {
+            if(!on || at(st) + i >= hd) x[st][i] = 0.0f;
+            amax = fmaxf(amax, fabsf(x[st][i]));
+        }
+#pragma unroll
+    for(int o = W; o < kWave; o *= 2) amax = fmaxf(amax, __shfl_xor(amax, o, kWave));
+    const int e = amax > 0.0f && amax <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
+#pragma unroll
+    for(int st = 0; st < STEPS; ++st) {
+#pragma unroll
+        for(int i = 0; i < 8; ++i) x[st][i] = ldexpf(x[st][i], -e);
+        two_parts(x[st], hi[st], lo[st]);
+    }
+    return e;
+}
+
+// Marks, in LDS, of the results that a NaN reaches: a bit for each row of a wave's tile and
+// value of the head.  mark: from the NaN (a bit each) among 16 tokens' values d of the head,
+// the rows that see them.
+__device__ __forceinline__ void clear_marks(uint32_t* marks, int words) {
+    for(int i = threadIdx.x % kWave; i < words; i += kWave) marks[i] = 0;
+}
+template <int HP>
+__device__ __forceinline__ void mark(uint32_t nan, int token0, int d, int rows, int first, int group, int past,
+                                     uint32_t* marks) {
+    for(; nan; nan &= nan - 1) {
+        const int t = token0 + __builtin_ctz(nan);
+        for(int r = 0; r < rows; ++r)
+            if(t <= past + (first + r) / group) atomicOr(&marks[r * (HP / 32) + d / 32], 1u << d % 32);
+    }
+}
+template <int HP>
+__device__ __forceinline__ bool marked(const uint32_t* marks, int r, int d) {
+    return marks[r * (HP / 32) + d / 32] >> d % 32 & 1;
 }
 
 // how a sequence's work is cut: groups of R query rows (token, head of the group) for each
@@ -86,40 +201,35 @@ __device__ __forceinline__ int share_of(int all, int W) {
 
 // a part's maximum and sum of each row, then its weighted values
 template <int HP>
-constexpr int kPart = 32 + 16 * HP;
+constexpr int kPart = kFew * (HP + 2);
 
 // ------------------------------------------------- few query rows a sequence
-// (heads of 256 take the registers that two waves of smaller ones share)
-constexpr int waves_of(int hp, bool whole) { return whole && hp < 256 ? 8 : 4; }
-
 // A workgroup's waves take a tile's units in turn and join in LDS.  WHOLE: a workgroup to
 // a tile.  Otherwise the units of all sequences, heads and tiles stand in one line, which
 // the workgroups share out evenly, whatever the lengths: one takes the end of a tile's
 // units, whole tiles, and the beginning of another's.  Tiles that one workgroup covered
 // are finished here, the others' parts are left for join_kernel: the one at the beginning
 // of a workgroup's share in its place 0, the one at the end in place 1.
-// SPLIT: the 16 columns are 8 rows' high parts and their low parts; else 16 rows, for two
-// products.
-template <int HP, bool SPLIT, bool WHOLE>
-__global__ __launch_bounds__(waves_of(HP, WHOLE) * kWave, HP == 256 ? 1 : 2)
-void few_rows_kernel(AttnArgs a) {
-    constexpr int kWaves = waves_of(HP, WHOLE);
-    constexpr int R = SPLIT ? 8 : 16;  // query rows
-    constexpr int C = HP / 64;         // chunks of 64 values of a key; then one of 32
+// Loads are issued in the order in which they are waited for, each a step before: the pages
+// of the unit after the next, the next one's keys, and its values.
+template <int HP, bool WHOLE, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kernel(AttnArgs a) {
+    constexpr int C = HP / 64;  // chunks of 64 values of a key; then one of 32
     constexpr bool TAIL = HP % 64 != 0;
     constexpr int STEPS = HP / 32, DT = HP / 16;
-    __shared__ __align__(16) float part[kWaves][R][HP + 4];
-    __shared__ float part_m[kWaves][16], part_l[kWaves][16];
+    __shared__ __align__(16) float part[WAVES][kFew][HP + 4];
+    __shared__ float part_m[WAVES][kFew], part_l[WAVES][kFew];
+    __shared__ uint32_t poisoned[WAVES][kFew * HP / 32];
     const PkKvCache& c = a.c;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane % 16, quad = lane / 16;
-    const int page = (int)c.page, kvh = (int)c.kv_heads, hd = (int)c.hd;
+    const int page = (int)c.page, kvh = (int)c.kv_heads, hd = (int)c.hd, width = (int)c.width;
     const int shift = __builtin_ctz(page);
 
     int begin = 0, end = 1, at, b;
     Seq s;
     if(!locate(
-           c, a.N, [&](const Seq& t) { return tiles_of<R>(a, t) * kvh * (WHOLE ? 1 : units_of(t)); },
+           c, a.N, [&](const Seq& t) { return tiles_of<kFew>(a, t) * kvh * (WHOLE ? 1 : units_of(t)); },
            [&](int all) {
                if(WHOLE) return (int)blockIdx.x;
                const int share = share_of(all, a.W);
@@ -129,122 +239,100 @@ void few_rows_kernel(AttnArgs a) {
            },
            at, b, s))
         return;
-    int tiles = tiles_of<R>(a, s), units = units_of(s);
+    int tiles = tiles_of<kFew>(a, s), units = units_of(s);
     int item = WHOLE ? at : at / units, u0 = WHOLE ? 0 : at - item * units;
 
     for(int now = begin; now < end;) {
-        while(item == tiles * kvh) {  // on to the next sequence that has any
-            if(++b >= c.B) return;    // (there is one, unless offsets decrease)
-            s = sequence(c, a.N, b);
-            tiles = tiles_of<R>(a, s);
-            units = units_of(s);
-            item = 0;
+        if(!WHOLE) {
+            while(item == tiles * kvh) {  // on to the next sequence that has any
+                if(++b >= c.B) return;    // (there is one, unless offsets decrease)
+                s = sequence(c, a.N, b);
+                tiles = tiles_of<kFew>(a, s);
+                units = units_of(s);
+                item = 0;
+            }
         }
         const int u1 = WHOLE || end - now >= units - u0 ? units : u0 + (end - now);
-        const int h = item / tiles, first = (item - h * tiles) * R;
-        const int rows = s.n * a.group - first < R ? s.n * a.group - first : R;
 
-        // the lane's query: row `mine` of the tile, as operand of 32 values a step, the
-        // values in the order that the lane's keys come in
-        const int mine = SPLIT ? col % 8 : col;
-        const int token = (first + (mine < rows ? mine : 0)) / a.group;
-        const float* qr = a.q + (int64_t)(s.row + token) * a.ldq +
-                          (int64_t)(h * a.group + (first + (mine < rows ? mine : 0)) % a.group) * hd;
-        const int reach = s.past + token;  // the last key that it sees
-        // the pages of a unit's tokens: 16 tokens lie on one page.  A lane's keys (tokens
-        // 16 (col / 4) + 4 t + col % 4) and its values and scores (16 quad ..) are on two.
-        auto page_of = [&](int u, int g16) {
-            const int i = (u * kUnit + 16 * g16) >> shift;
-            const int pid = i < c.width ? c.table[(int64_t)b * c.width + i] : -1;
-            return pid < 0 || pid >= c.pages ? -1 : pid;
+        // 16 tokens lie on one page, whose number and powers a lane of the wave holds for each
+        // of the wave's next units: `per` to a unit.  A lane's keys (tokens 16 (col / 4) +
+        // 4 t + col % 4) and its values and scores (16 quad ..) may be on two.
+        const int32_t* names = c.table + (int64_t)b * width;
+        const int per = page < kUnit ? kUnit / page : 1;
+        const int x_key = 16 * (col / 4) >> shift, x_value = 16 * quad >> shift;
+        const int h = item / tiles, first = (item - h * tiles) * kFew;
+        int pid, ek, ev, k = 0;
+        auto name_units = [&](int u) {
+            const int i = ((u + WAVES * (lane / per)) * kUnit + lane % per * page) >> shift;
+            pid = names[i < width ? i : 0];
+            if(i >= width || pid < 0 || pid >= c.pages) pid = -1;
+            const int64_t at = (int64_t)(pid < 0 ? 0 : pid) * kvh + h;
+            ek = c.k_exp[at];
+            ev = c.v_exp[at];
+            k = 0;
         };
-        uint4 kr[4][C > 0 ? C : 1], vr[DT];
-        uint2 kt[4];
+        auto of_unit = [&](int v, int x) { return __builtin_amdgcn_ds_bpermute(4 * (k * per + x), v); };
+        int u = u0 + wave;
+        name_units(u);
+
+        // the lane's query: a row of the tile, as operand of 32 values a step, the values in
+        // the order that the lane's keys come in
+        const int rows = s.n * a.group - first < kFew ? s.n * a.group - first : kFew;
+        const int mine = first + (col < rows ? col : 0);
+        const int token = mine / a.group;
+        const int reach = s.past + token;                 // the last key that it sees
+        const int clear = s.past + first / a.group + 1;   // tokens that every row sees
+        const float* qr = a.q + (int64_t)(s.row + token) * a.ldq +
+                          (int64_t)(h * a.group + mine - token * a.group) * hd;
+        float x[STEPS][8];
+        auto of_step = [&](int st) {
+            return TAIL && st == STEPS - 1 ? 64 * C + 8 * quad : 64 * (st / 2) + 16 * quad + 8 * (st % 2);
+        };
+        load_query(qr, hd, a.vec, of_step, x);
+        in_order();
+        __builtin_amdgcn_sched_barrier(0);
+
+        u32x4 kr[4][C > 0 ? C : 1], vr[DT];
+        u32x2 kt[4];
+        // (always the same number of loads, so that the compiler knows how many are younger
+        // than those that it waits for: where there is no unit, of one line)
         auto load_keys = [&](int u, int pid) {
             const int slot = ((u * kUnit + 16 * (col / 4)) & (page - 1)) + col % 4;
-            const uint8_t* p = c.k + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * page + slot) * HP;
+            const uint8_t* p = c.k + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * page + slot) * HP + 16 * quad;
+            if(u >= u1) p = c.k;
 #pragma unroll
             for(int t = 0; t < 4; ++t) {
 #pragma unroll
                 for(int i = 0; i < C; ++i)
-                    kr[t][i] = *(const uint4*)(p + 4 * t * HP + 64 * i + 16 * quad);
-                if(TAIL) kt[t] = *(const uint2*)(p + 4 * t * HP + 64 * C + 8 * quad);
+                    kr[t][i] = *(const u32x4*)(p + 4 * t * HP + 64 * i);
+                if(TAIL) kt[t] = *(const u32x2*)(p + 4 * t * HP + 64 * C - (u >= u1 ? 0 : 8 * quad));
+                in_order();
             }
         };
         auto load_values = [&](int u, int pid) {
             const int slot = (u * kUnit + 16 * quad) & (page - 1);
             const uint8_t* p = c.v + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * HP + col) * page + slot;
+            if(u >= u1) p = c.v;
 #pragma unroll
-            for(int i = 0; i < DT; ++i) vr[i] = *(const uint4*)(p + (int64_t)16 * i * page);
+            for(int i = 0; i < DT; ++i) vr[i] = *(const u32x4*)(p + (int64_t)16 * i * page);
+            in_order();
         };
+        int pv = of_unit(pid, x_value);
+        load_keys(u, of_unit(pid, x_key));
+        load_values(u, pv);
+        __builtin_amdgcn_sched_barrier(0);  // (nor is the query waited for before)
 
-        // (the loads that others wait for first: pages, query, then keys and values)
-        int u = u0 + wave;
-        int pk = -1, pv = -1;
-        if(u < u1) {
-            pk = page_of(u, col / 4);
-            pv = page_of(u, quad);
-        }
-        float x[STEPS][8];
-#pragma unroll
-        for(int st = 0; st < STEPS; ++st) {
-            const int d = TAIL && st == STEPS - 1 ? 64 * C + 8 * quad
-                                                  : 64 * (st / 2) + 16 * quad + 8 * (st % 2);
-            if(a.vec) {
-#pragma unroll
-                for(int i = 0; i < 8; i += 4) {
-                    const f32x4 v = d + i < hd ? *(const f32x4*)(qr + d + i) : f32x4{};
-#pragma unroll
-                    for(int k = 0; k < 4; ++k) x[st][i + k] = v[k];
-                }
-            } else {
-#pragma unroll
-                for(int i = 0; i < 8; ++i) x[st][i] = d + i < hd ? qr[d + i] : 0.0f;
-            }
-        }
-        uint8_t ek = 127, ev = 127;
-        if(u < u1) {
-            load_keys(u, pk);
-            load_values(u, pv);
-            ek = c.k_exp[(int64_t)(pv < 0 ? 0 : pv) * kvh + h];
-            ev = c.v_exp[(int64_t)(pv < 0 ? 0 : pv) * kvh + h];
-        }
-        float amax = 0.0f;
-#pragma unroll
-        for(int st = 0; st < STEPS; ++st)
-#pragma unroll
-            for(int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[st][i]));
-        amax = fmaxf(amax, __shfl_xor(amax, 16, kWave));
-        amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
-        const int eq = amax > 0.0f && amax <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
+        f16x8 qh[STEPS], ql[STEPS];
+        const int eq = bring_up<16>(x, hd, of_step, col < rows, qh, ql);
         const float coef = ldexpf(a.scale, eq);
-        f16x8 qf[SPLIT ? 1 : 2][STEPS];
-#pragma unroll
-        for(int st = 0; st < STEPS; ++st)
-#pragma unroll
-            for(int i = 0; i < 8; ++i) {
-                const float y = mine < rows ? ldexpf(x[st][i], -eq) : 0.0f;
-                const _Float16 hi = (_Float16)y, lo = (_Float16)(y - (float)hi);
-                if(SPLIT) {
-                    qf[0][st][i] = col < 8 ? hi : lo;
-                } else {
-                    qf[0][st][i] = hi;
-                    qf[SPLIT ? 0 : 1][st][i] = lo;
-                }
-            }
 
         f32x4 acc[DT];
 #pragma unroll
         for(int i = 0; i < DT; ++i) acc[i] = f32x4{};
-        float m = kNone, l = 0.0f;
-        const int clear = s.past + first / a.group + 1;  // tokens that every row sees
-        for(; u < u1; u += kWaves) {
-            const int next = u + kWaves;
-            int pk_next = -1, pv_next = -1;
-            if(next < u1) {
-                pk_next = page_of(next, col / 4);
-                pv_next = page_of(next, quad);
-            }
+        float m = 0.0f, l = 0.0f, limit = kNone;  // (of no score yet)
+        bool poison = false;
+        for(; u < u1; u += WAVES) {
+            const int next = u + WAVES;
             f32x4 sc[4];
 #pragma unroll
             for(int t = 0; t < 4; ++t) {
@@ -253,33 +341,27 @@ void few_rows_kernel(AttnArgs a) {
                 for(int st = 0; st < STEPS; ++st) {
                     f16x8 kf;
                     if(TAIL && st == STEPS - 1)
-                        kf = widen(kt[t].x, kt[t].y);
+                        kf = widen(kt[t][0], kt[t][1]);
                     else if(st % 2 == 0)
-                        kf = widen(kr[t][st / 2].x, kr[t][st / 2].y);
+                        kf = widen(kr[t][st / 2][0], kr[t][st / 2][1]);
                     else
-                        kf = widen(kr[t][st / 2].z, kr[t][st / 2].w);
-                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[0][st], sc[t], 0, 0, 0);
-                    if(!SPLIT)
-                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[SPLIT ? 0 : 1][st], sc[t],
-                                                                       0, 0, 0);
+                        kf = widen(kr[t][st / 2][2], kr[t][st / 2][3]);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[st], sc[t], 0, 0, 0);
+                    sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[st], sc[t], 0, 0, 0);
                 }
             }
-            const float kc = coef * power(ek), vexp = (float)((int)ev - 127), vinv = power(254 - ev);
+            const int ek_now = of_unit(ek, x_value), ev_now = of_unit(ev, x_value);
+            const float kc = coef * power(ek_now), vexp = (float)(ev_now - 127), vinv = power(254 - ev_now);
             const bool absent = pv < 0;
-            if(next < u1) {
-                load_keys(next, pk_next);
-                ek = c.k_exp[(int64_t)(pv_next < 0 ? 0 : pv_next) * kvh + h];
-                ev = c.v_exp[(int64_t)(pv_next < 0 ? 0 : pv_next) * kvh + h];
-            }
+            if(++k * per == kWave) name_units(next);
+            pv = of_unit(pid, x_value);
+            load_keys(next, of_unit(pid, x_key));
             float p[16], mx = kNone;
+            const float low = vexp - (m - kTop);
 #pragma unroll
             for(int t = 0; t < 4; ++t)
 #pragma unroll
-                for(int r = 0; r < 4; ++r) {
-                    float v = sc[t][r];
-                    if(SPLIT) v += across8(v);
-                    p[4 * t + r] = fmaf(v, kc, vexp);
-                }
+                for(int r = 0; r < 4; ++r) p[4 * t + r] = fmaf(sc[t][r], kc, low);
             const int token0 = u * kUnit + 16 * quad;
             const bool edge = u * kUnit + kUnit > clear || __ballot(absent) != 0;
             if(edge) {
@@ -289,92 +371,64 @@ void few_rows_kernel(AttnArgs a) {
             }
 #pragma unroll
             for(int i = 0; i < 16; ++i) mx = fmaxf(mx, p[i]);
-            if(__ballot(mx > m + kRaise)) {
+            if(__ballot(mx > limit)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-                mx = fmaxf(mx, m);
-                const float down = __builtin_amdgcn_exp2f(m - mx);
+                const float up = raise(mx, limit), down = __builtin_amdgcn_exp2f(fminf(-up, 0.0f));
+                m += up;
                 l *= down;
 #pragma unroll
                 for(int i = 0; i < DT; ++i) acc[i] *= down;
-                m = mx;
+#pragma unroll
+                for(int i = 0; i < 16; ++i) p[i] -= up;
             }
-            float sum = 0.0f;
-            const float low = m - kTop;
+            f32x4 sums = {};
 #pragma unroll
             for(int i = 0; i < 16; ++i) {
-                p[i] = __builtin_amdgcn_exp2f(p[i] - low);
-                sum += p[i];
+                p[i] = __builtin_amdgcn_exp2f(p[i]);
+                sums[i % 4] += p[i];
             }
+            const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
             l = fmaf(sum, vinv, l);
-            f16x8 pf[2][2];
-#pragma unroll
-            for(int i = 0; i < 16; ++i) {
-                const _Float16 hi = (_Float16)p[i], lo = (_Float16)(p[i] - (float)hi);
-                if(SPLIT) {
-                    pf[0][i / 8][i % 8] = col < 8 ? hi : lo;
-                } else {
-                    pf[0][i / 8][i % 8] = hi;
-                    pf[1][i / 8][i % 8] = lo;
-                }
-            }
+            f16x8 ph[2], pl[2];
+            two_parts(p, ph[0], pl[0]);
+            two_parts(p + 8, ph[1], pl[1]);
             if(edge) {
                 // tokens behind the sequence's last, or on no page, may hold anything
-                const int real = absent ? 0 : held(s.end - token0, 0, 16);
-                uint32_t keep[4], nan = 0;
-#pragma unroll
-                for(int i = 0; i < 4; ++i) {
-                    const int k = held(real - 4 * i, 0, 4);
-                    keep[i] = k == 4 ? 0xffffffffu : (1u << (8 * k)) - 1u;
-                }
+                const u32x4 keep = first_bytes(absent ? 0 : held(s.end - token0, 0, 16));
+                u32x4 nan = {};
 #pragma unroll
                 for(int i = 0; i < DT; ++i) {
-                    vr[i].x &= keep[0];
-                    vr[i].y &= keep[1];
-                    vr[i].z &= keep[2];
-                    vr[i].w &= keep[3];
-                    nan |= nan_bytes(vr[i].x) | nan_bytes(vr[i].y) | nan_bytes(vr[i].z) | nan_bytes(vr[i].w);
+                    vr[i] &= keep;
+                    nan |= nan_bytes(vr[i]);
                 }
-                if(__builtin_expect(__ballot(nan != 0) != 0, 0)) {
-                    // a NaN among the values of tokens that some rows do not see, where
-                    // 0 times it must not reach them: how many of a column's NaN each row
-                    // sees, as a product of ones, and zeros in their place
-                    f16x8 seen[2];
-#pragma unroll
-                    for(int i = 0; i < 16; ++i)
-                        seen[i / 8][i % 8] = absent || token0 + i > reach ? (_Float16)0.0f : (_Float16)1.0f;
+                if(__builtin_expect(__ballot((nan[0] | nan[1] | nan[2] | nan[3]) != 0) != 0, 0)) {
+                    // a NaN among the values of tokens that some rows do not see must not
+                    // reach them by 0 times it: zeros in its place, and the rows that do
+                    // see it are noted
+                    if(!poison) clear_marks(poisoned[wave], kFew * HP / 32);
+                    poison = true;
+                    auto* found = (volatile uint16_t*)&part[wave][0][0];
 #pragma unroll
                     for(int i = 0; i < DT; ++i) {
-                        uint32_t word[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w}, one[4];
-#pragma unroll
-                        for(int k = 0; k < 4; ++k) {
-                            const uint32_t bits = nan_bytes(word[k]) >> 7;
-                            one[k] = bits * 0x38;  // e4m3's 1
-                            word[k] &= ~(bits * 0xff);
-                        }
-                        f32x4 count = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(one[0], one[1]), seen[0],
-                                                                             f32x4{}, 0, 0, 0);
-                        count = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen(one[2], one[3]), seen[1], count,
-                                                                       0, 0, 0);
-#pragma unroll
-                        for(int r = 0; r < 4; ++r)
-                            if(count[r] > 0.0f) acc[i][r] = NAN;
-                        vr[i] = {word[0], word[1], word[2], word[3]};
+                        found[kWave * i + lane] = nan_bits(vr[i]);
+                        vr[i] &= ~((nan_bytes(vr[i]) >> 7) * 0xff);
                     }
+#pragma unroll 1
+                    for(int i = 0; i < DT; ++i)
+                        mark<HP>(found[kWave * i + lane], token0, 16 * i + col, rows, first, a.group, s.past,
+                                 poisoned[wave]);
                 }
             }
 #pragma unroll
             for(int i = 0; i < DT; ++i) {
-                const f16x8 v0 = widen(vr[i].x, vr[i].y), v1 = widen(vr[i].z, vr[i].w);
-                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[0][0], acc[i], 0, 0, 0);
-                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[0][1], acc[i], 0, 0, 0);
-                if(!SPLIT) {
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pf[1][0], acc[i], 0, 0, 0);
-                    acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pf[1][1], acc[i], 0, 0, 0);
-                }
+                const f16x8 v0 = widen(vr[i][0], vr[i][1]), v1 = widen(vr[i][2], vr[i][3]);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1], acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, pl[0], acc[i], 0, 0, 0);
+                acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, pl[1], acc[i], 0, 0, 0);
             }
-            if(next < u1) load_values(next, pv_next);
-            pv = pv_next;
+            load_values(next, pv);
         }
 
         // the waves' parts together
@@ -382,27 +436,26 @@ void few_rows_kernel(AttnArgs a) {
         l += __shfl_xor(l, 32, kWave);
 #pragma unroll
         for(int i = 0; i < DT; ++i) {
-            if(SPLIT) {
 #pragma unroll
-                for(int r = 0; r < 4; ++r) acc[i][r] += across8(acc[i][r]);
-            }
-            if(col < R) *(f32x4*)&part[wave][col][16 * i + 4 * quad] = acc[i];
+            for(int r = 0; r < 4; ++r)
+                if(poison && marked<HP>(poisoned[wave], col, 16 * i + 4 * quad + r)) acc[i][r] = NAN;
+            *(f32x4*)&part[wave][col][16 * i + 4 * quad] = acc[i];
         }
         if(lane < 16) {
-            part_m[wave][lane] = m;
+            part_m[wave][lane] = limit == kNone ? kNone : m;
             part_l[wave][lane] = l;
         }
         __syncthreads();
         const bool whole = WHOLE || (u0 == 0 && u1 == units);
         float* out = a.ws + ((int64_t)blockIdx.x * 2 + (now == begin ? 0 : 1)) * kPart<HP>;
-        for(int i = threadIdx.x; i < rows * (HP / 4); i += kWaves * kWave) {
+        for(int i = threadIdx.x; i < rows * (HP / 4); i += WAVES * kWave) {
             const int r = i / (HP / 4), d = 4 * (i % (HP / 4));
             float top = part_m[0][r], total = 0.0f;
 #pragma unroll
-            for(int k = 1; k < kWaves; ++k) top = fmaxf(top, part_m[k][r]);
+            for(int k = 1; k < WAVES; ++k) top = fmaxf(top, part_m[k][r]);
             f32x4 v = {};
 #pragma unroll
-            for(int k = 0; k < kWaves; ++k) {
+            for(int k = 0; k < WAVES; ++k) {
                 const float f = __builtin_amdgcn_exp2f(part_m[k][r] - top);
                 total = fmaf(f, part_l[k][r], total);
                 v += f * *(const f32x4*)&part[k][r][d];
@@ -410,18 +463,19 @@ void few_rows_kernel(AttnArgs a) {
             if(!whole) {
                 if(d == 0) {
                     out[r] = top;
-                    out[16 + r] = total;
+                    out[kFew + r] = total;
                 }
-                *(f32x4*)(out + 32 + r * HP + d) = v;
+                *(f32x4*)(out + 2 * kFew + r * HP + d) = v;
                 continue;
             }
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // (0: no key at all)
-            float* to = a.o + (int64_t)(s.row + (first + r) / a.group) * a.ldo +
-                        (int64_t)(h * a.group + (first + r) % a.group) * hd + d;
+            const int t = (first + r) / a.group;
+            float* to = a.o + (int64_t)(s.row + t) * a.ldo + (int64_t)(h * a.group + first + r - t * a.group) * hd + d;
 #pragma unroll
             for(int k = 0; k < 4; ++k)
                 if(d + k < hd) to[k] = v[k] * inv;
         }
+        if(WHOLE) return;
         __syncthreads();
         now += u1 - u0;
         u0 = 0;
@@ -432,7 +486,7 @@ void few_rows_kernel(AttnArgs a) {
 // The tiles that several workgroups have parts of: a workgroup here stands for the one
 // there that has a tile's last part, and a wave for one of the tile's rows, its lanes on 4
 // values each of as many parts at once as there are lanes for.
-template <int HP, int R>
+template <int HP>
 __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     constexpr int D4 = HP / 4, PARTS = kWave / D4;
     const PkKvCache& c = a.c;
@@ -440,16 +494,16 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     int share = 1, at, b;
     Seq s;
     if(!locate(
-           c, a.N, [&](const Seq& t) { return tiles_of<R>(a, t) * (int)c.kv_heads * units_of(t); },
+           c, a.N, [&](const Seq& t) { return tiles_of<kFew>(a, t) * (int)c.kv_heads * units_of(t); },
            [&](int all) {
                share = share_of(all, a.W);
                return (int)blockIdx.x * share;
            },
            at, b, s))
         return;
-    const int tiles = tiles_of<R>(a, s), units = units_of(s), item = at / units, u0 = at - item * units;
+    const int tiles = tiles_of<kFew>(a, s), units = units_of(s), item = at / units, u0 = at - item * units;
     if(u0 == 0 || units - u0 > share) return;  // it begins here, or has parts behind
-    const int h = item / tiles, row = (item - h * tiles) * R + r;
+    const int h = item / tiles, row = (item - h * tiles) * kFew + r;
     if(row >= s.n * a.group) return;
     // the first part's workgroup, where it is in that one's place 0 if it begins its share
     const int before = (u0 + share - 1) / share, w1 = blockIdx.x, w0 = w1 - before;
@@ -467,8 +521,8 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
         for(int w = w0 + mine; w <= w1; w += PARTS) {
             const float* p = part(w);
             const float f = __builtin_amdgcn_exp2f(p[r] - top);
-            total = fmaf(f, p[16 + r], total);
-            v += f * *(const f32x4*)(p + 32 + r * HP + d);
+            total = fmaf(f, p[kFew + r], total);
+            v += f * *(const f32x4*)(p + 2 * kFew + r * HP + d);
         }
     }
     f32x4 sum = v;
@@ -508,6 +562,7 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
     constexpr int CHUNKS = kUnit * HP / 16, LOADS = (CHUNKS + 255) / 256;  // of 16 bytes; a thread's
     __shared__ __align__(16) uint8_t keys[2][kUnit * KS], values[2][HP * VS];
     __shared__ __align__(16) float4 pages[2][kUnit / 16];  // 2^ek, ev, 2^-ev, whether there
+    __shared__ uint32_t poisoned[4][HP];
     const PkKvCache& c = a.c;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int col = lane % 32, half = lane / 32;
@@ -539,35 +594,10 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
     f16x8 qh[STEPS], ql[STEPS];
     float coef;
     {
-        float x[STEPS][8], amax = 0.0f;
-#pragma unroll
-        for(int st = 0; st < STEPS; ++st) {
-            const int d = 32 * (st / 2) + 16 * half + 8 * (st % 2);
-            if(a.vec) {
-#pragma unroll
-                for(int i = 0; i < 8; i += 4) {
-                    const f32x4 v = d + i < hd ? *(const f32x4*)(qr + d + i) : f32x4{};
-#pragma unroll
-                    for(int k = 0; k < 4; ++k) x[st][i + k] = v[k];
-                }
-            } else {
-#pragma unroll
-                for(int i = 0; i < 8; ++i) x[st][i] = d + i < hd ? qr[d + i] : 0.0f;
-            }
-#pragma unroll
-            for(int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[st][i]));
-        }
-        amax = fmaxf(amax, __shfl_xor(amax, 32, kWave));
-        const int eq = amax > 0.0f && amax <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
-        coef = ldexpf(a.scale, eq);
-#pragma unroll
-        for(int st = 0; st < STEPS; ++st)
-#pragma unroll
-            for(int i = 0; i < 8; ++i) {
-                const float y = col < rows ? ldexpf(x[st][i], -eq) : 0.0f;
-                qh[st][i] = (_Float16)y;
-                ql[st][i] = (_Float16)(y - (float)qh[st][i]);
-            }
+        float x[STEPS][8];
+        auto of_step = [&](int st) { return 32 * (st / 2) + 16 * half + 8 * (st % 2); };
+        load_query(qr, hd, a.vec, of_step, x);
+        coef = ldexpf(a.scale, bring_up<32>(x, hd, of_step, col < rows, qh, ql));
     }
 
     auto page_of = [&](int u, int g16) {
@@ -578,7 +608,7 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
     // a thread's chunks: of keys, 16 values of token e / (HP / 16); of values, 16 tokens of
     // row e / 4, of which `real` are the sequence's
     int pk[LOADS], pv, real = 0;
-    uint4 kr[LOADS], vr[LOADS];
+    u32x4 kr[LOADS], vr[LOADS];
     float4 pr;
     const int g16 = threadIdx.x % 4;
     auto find_pages = [&](int u) {
@@ -593,8 +623,8 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
             const int e = threadIdx.x + 256 * i, t = e / (HP / 16), d16 = e % (HP / 16);
             if(e < CHUNKS) {
                 const int64_t k_head = (int64_t)(pk[i] < 0 ? 0 : pk[i]) * kvh + h;
-                kr[i] = *(const uint4*)(c.k + (k_head * page + ((u * kUnit + t) & (page - 1))) * HP + 16 * d16);
-                vr[i] = *(const uint4*)(c.v + (v_head * HP + e / 4) * page +
+                kr[i] = *(const u32x4*)(c.k + (k_head * page + ((u * kUnit + t) & (page - 1))) * HP + 16 * d16);
+                vr[i] = *(const u32x4*)(c.v + (v_head * HP + e / 4) * page +
                                         ((u * kUnit + 16 * g16) & (page - 1)));
             }
         }
@@ -611,17 +641,10 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
             if(e < CHUNKS) {
                 // the row of the product that a token is: bits 4 3 2 1 0 become 3 2 4 1 0
                 const int row = (t & 32) + ((t & 12) << 1) + ((t & 16) >> 2) + (t & 3);
-                *(uint4*)&keys[buf][row * KS + 16 * d16] = kr[i];
-                if(real < 16) {  // values behind the sequence's end, or on no page, may be anything
-                    uint32_t w[4] = {vr[i].x, vr[i].y, vr[i].z, vr[i].w};
-#pragma unroll
-                    for(int k = 0; k < 4; ++k) {
-                        const int n = held(real - 4 * k, 0, 4);
-                        w[k] &= n == 4 ? 0xffffffffu : (1u << (8 * n)) - 1u;
-                    }
-                    vr[i] = {w[0], w[1], w[2], w[3]};
-                }
-                *(uint4*)&values[buf][e / 4 * VS + 16 * g16] = vr[i];
+                *(u32x4*)&keys[buf][row * KS + 16 * d16] = kr[i];
+                // (values behind the sequence's end, or on no page, may be anything)
+                if(real < 16) vr[i] &= first_bytes(real);
+                *(u32x4*)&values[buf][e / 4 * VS + 16 * g16] = vr[i];
             }
         }
         if(threadIdx.x < 4) pages[buf][threadIdx.x] = pr;
@@ -630,7 +653,8 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
     f32x16 acc[DT];
 #pragma unroll
     for(int i = 0; i < DT; ++i) acc[i] = f32x16{};
-    float m = kNone, l = 0.0f;
+    float m = 0.0f, l = 0.0f, limit = kNone;
+    bool poison = false;
     const int clear = s.past + (first < total ? first / a.group : 0) + 1;  // tokens that all rows see
     const int reach_all = s.past + (first + rows - 1) / a.group;           // and that any does
     find_pages(u0);
@@ -653,8 +677,8 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
             f32x16 sc = {};
 #pragma unroll
             for(int st = 0; st < STEPS; st += 2) {
-                const uint4 w = *(const uint4*)&keys[buf][(32 * j + col) * KS + 16 * st + 16 * half];
-                const f16x8 k0 = widen(w.x, w.y), k1 = widen(w.z, w.w);
+                const u32x4 w = *(const u32x4*)&keys[buf][(32 * j + col) * KS + 16 * st + 16 * half];
+                const f16x8 k0 = widen(w[0], w[1]), k1 = widen(w[2], w[3]);
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, qh[st], sc, 0, 0, 0);
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, qh[st + 1], sc, 0, 0, 0);
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[st], sc, 0, 0, 0);
@@ -665,8 +689,9 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
             const bool absent = g.w == 0.0f;
             const int mine0 = token0 + 16 * half;
             float p[16], mx = kNone;
+            const float low = g.y - (m - kTop);
 #pragma unroll
-            for(int i = 0; i < 16; ++i) p[i] = fmaf(sc[i], kc, g.y);
+            for(int i = 0; i < 16; ++i) p[i] = fmaf(sc[i], kc, low);
             const bool edge = token0 + 32 > clear || __ballot(absent) != 0;
             if(edge) {
 #pragma unroll
@@ -675,55 +700,49 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
             }
 #pragma unroll
             for(int i = 0; i < 16; ++i) mx = fmaxf(mx, p[i]);
-            if(__ballot(mx > m + kRaise)) {
+            if(__ballot(mx > limit)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-                mx = fmaxf(mx, m);
-                const float down = __builtin_amdgcn_exp2f(m - mx);
+                const float up = raise(mx, limit), down = __builtin_amdgcn_exp2f(fminf(-up, 0.0f));
+                m += up;
                 l *= down;
 #pragma unroll
                 for(int i = 0; i < DT; ++i) acc[i] *= down;
-                m = mx;
+#pragma unroll
+                for(int i = 0; i < 16; ++i) p[i] -= up;
             }
-            const float low = m - kTop;
-            float sum = 0.0f;
-            f16x8 ph[2], pl[2];
+            f32x4 sums = {};
 #pragma unroll
             for(int i = 0; i < 16; ++i) {
-                const float e = __builtin_amdgcn_exp2f(p[i] - low);
-                sum += e;
-                ph[i / 8][i % 8] = (_Float16)e;
-                pl[i / 8][i % 8] = (_Float16)(e - (float)ph[i / 8][i % 8]);
+                p[i] = __builtin_amdgcn_exp2f(p[i]);
+                sums[i % 4] += p[i];
             }
+            const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
             l = fmaf(sum, g.z, l);
+            f16x8 ph[2], pl[2];
+            two_parts(p, ph[0], pl[0]);
+            two_parts(p + 8, ph[1], pl[1]);
+            bool clean = false;  // NaN become zeros
+            auto value = [&](int i) {
+                return *(const u32x4*)&values[buf][(32 * i + col) * VS + 32 * j + 16 * half];
+            };
+            if(edge) {
+                u32x4 nan = {};
+#pragma unroll
+                for(int i = 0; i < DT; ++i) nan |= nan_bytes(value(i));
+                if(__builtin_expect(__ballot((nan[0] | nan[1] | nan[2] | nan[3]) != 0) != 0, 0)) {
+                    if(!poison) clear_marks(poisoned[wave], HP);  // (as in few_rows_kernel)
+                    poison = clean = true;
+#pragma unroll 1
+                    for(int i = 0; i < DT; ++i)
+                        mark<HP>(nan_bits(value(i)), mine0, 32 * i + col, rows, first, a.group, s.past,
+                                 poisoned[wave]);
+                }
+            }
 #pragma unroll
             for(int i = 0; i < DT; ++i) {
-                uint4 w = *(const uint4*)&values[buf][(32 * i + col) * VS + 32 * j + 16 * half];
-                if(edge) {
-                    const uint32_t nan = nan_bytes(w.x) | nan_bytes(w.y) | nan_bytes(w.z) | nan_bytes(w.w);
-                    if(__builtin_expect(__ballot(nan != 0) != 0, 0)) {
-                        // (as in few_rows_kernel: the NaN that a row sees, counted)
-                        uint32_t word[4] = {w.x, w.y, w.z, w.w}, one[4];
-                        f16x8 seen[2];
-#pragma unroll
-                        for(int k = 0; k < 16; ++k)
-                            seen[k / 8][k % 8] = absent || mine0 + k > reach ? (_Float16)0.0f : (_Float16)1.0f;
-#pragma unroll
-                        for(int k = 0; k < 4; ++k) {
-                            const uint32_t bits = nan_bytes(word[k]) >> 7;
-                            one[k] = bits * 0x38;
-                            word[k] &= ~(bits * 0xff);
-                        }
-                        f32x16 count = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen(one[0], one[1]), seen[0],
-                                                                              f32x16{}, 0, 0, 0);
-                        count = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen(one[2], one[3]), seen[1], count,
-                                                                       0, 0, 0);
-#pragma unroll
-                        for(int r = 0; r < 16; ++r)
-                            if(count[r] > 0.0f) acc[i][r] = NAN;
-                        w = {word[0], word[1], word[2], word[3]};
-                    }
-                }
-                const f16x8 v0 = widen(w.x, w.y), v1 = widen(w.z, w.w);
+                u32x4 w = value(i);
+                if(__builtin_expect(clean, 0)) w &= ~((nan_bytes(w) >> 7) * 0xff);
+                const f16x8 v0 = widen(w[0], w[1]), v1 = widen(w[2], w[3]);
                 acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, ph[0], acc[i], 0, 0, 0);
                 acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v1, ph[1], acc[i], 0, 0, 0);
                 acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v0, pl[0], acc[i], 0, 0, 0);
@@ -736,11 +755,18 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
 
     l += __shfl_xor(l, 32, kWave);
     if(col >= rows) return;
+    if(poison) {
+#pragma unroll
+        for(int i = 0; i < DT; ++i)
+#pragma unroll
+            for(int r = 0; r < 16; ++r)
+                if(marked<HP>(poisoned[wave], col, 32 * i + 8 * (r / 4) + 4 * half + r % 4)) acc[i][r] = NAN;
+    }
     if(a.splits > 1) {  // (a part without units has the maximum of no scores, and zeros)
         float* out = a.ws + (int64_t)blockIdx.x * kManyPart<HP>;
         const int r = wave * 32 + col;
         if(half == 0) {
-            out[r] = m;
+            out[r] = limit == kNone ? kNone : m;
             out[kRows + r] = l;
         }
 #pragma unroll
@@ -801,7 +827,7 @@ __global__ __launch_bounds__(256) void finish_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------- launches
 struct Plan {
-    int rows;       // 8, 16 or 128 query rows a tile
+    int rows;       // 16 or 128 query rows a tile
     int W;          // of few rows: workgroups that share the units of all tiles; 0: one to a tile
     int splits;     // of many: workgroups to a tile
     int64_t tiles;  // for each head of the cache, that there may be
@@ -810,10 +836,10 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
     Plan p = {};
     const int64_t group = H / c->kv_heads, units = (c->width * c->page + kUnit - 1) / kUnit;
     const int64_t some = c->B < N ? c->B : N;
-    p.rows = N * group <= 8 * c->B ? 8 : N * group <= 32 * c->B ? 16 : kRows;
+    p.rows = N * group <= 32 * c->B ? kFew : kRows;
     p.tiles = N * group / p.rows + some;
     if(p.rows < kRows) {
-        p.W = units <= 32 || p.tiles * c->kv_heads * units >= (int64_t)1 << 31 ? 0 : 512;
+        p.W = units <= 32 || p.tiles * c->kv_heads * units >= (int64_t)1 << 31 ? 0 : 256;
     } else {
         // workgroups that there are for sure, two to a CU, of 8 units at least
         const int64_t sure = (N * group + kRows - 1) / kRows * c->kv_heads;
@@ -825,7 +851,7 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
 }
 size_t plan_bytes(const Plan& p, const PkKvCache* c) {
     const size_t hp = head_size(c->hd);
-    if(p.W) return sizeof(float) * 2 * p.W * (32 + 16 * hp);
+    if(p.W) return sizeof(float) * 2 * p.W * kFew * (hp + 2);
     if(p.splits > 1) return sizeof(float) * p.tiles * c->kv_heads * p.splits * kRows * (hp + 2);
     return 0;
 }
@@ -840,23 +866,21 @@ int check_attn(const char* who, const PkKvCache* c, int64_t N, int64_t H) {
     return PK_OK;
 }
 
-template <int HP, bool SPLIT>
-void launch_rows(const AttnArgs& a, const Plan& p, hipStream_t st) {
-    if(!p.W) {
-        few_rows_kernel<HP, SPLIT, true>
-            <<<(unsigned)(p.tiles * a.c.kv_heads), waves_of(HP, true) * kWave, 0, st>>>(a);
-        return;
-    }
-    few_rows_kernel<HP, SPLIT, false><<<(unsigned)p.W, 256, 0, st>>>(a);
-    join_kernel<HP, SPLIT ? 8 : 16><<<dim3((unsigned)p.W, SPLIT ? 2 : 4), 256, 0, st>>>(a);
-}
 template <int HP>
 void launch(const AttnArgs& a, const Plan& p, hipStream_t st) {
-    if(p.rows == 8) return launch_rows<HP, true>(a, p, st);
-    if(p.rows == 16) return launch_rows<HP, false>(a, p, st);
     const int64_t tiles = p.tiles * a.c.kv_heads;
-    many_rows_kernel<HP><<<(unsigned)(tiles * p.splits), 256, 0, st>>>(a);
-    if(p.splits > 1) finish_kernel<HP><<<dim3((unsigned)tiles, kRows / 4), 256, 0, st>>>(a);
+    constexpr int MANY = HP == 256 ? 4 : 8;  // waves; heads of 256 take twice the registers
+    if(p.rows == kRows) {
+        many_rows_kernel<HP><<<(unsigned)(tiles * p.splits), 256, 0, st>>>(a);
+        if(p.splits > 1) finish_kernel<HP><<<dim3((unsigned)tiles, kRows / 4), 256, 0, st>>>(a);
+    } else if(p.W) {
+        few_rows_kernel<HP, false, 4><<<(unsigned)p.W, 256, 0, st>>>(a);
+        join_kernel<HP><<<dim3((unsigned)p.W, kFew / 4), 256, 0, st>>>(a);
+    } else if(tiles < 256) {
+        few_rows_kernel<HP, true, MANY><<<(unsigned)tiles, MANY * kWave, 0, st>>>(a);
+    } else {
+        few_rows_kernel<HP, true, 4><<<(unsigned)tiles, 256, 0, st>>>(a);
+    }
 }
 
 }  // namespace

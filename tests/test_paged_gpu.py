@@ -211,13 +211,14 @@ def test_attention_layouts_and_default_scale(dev):
         assert (out[:, :off] == 3.0).all() and (out[:, off + H * hd:] == 3.0).all()
 
 
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
 @pytest.mark.parametrize("new", [[1, 1, 1, 1], [30, 40, 1, 25], [150, 140, 1, 130]])
-def test_attention_over_absent_pages(dev, new):
+def test_attention_over_absent_pages(dev, new, hd):
     """pages that are none count as absent: in the middle, at the end, and all of them (a row
     without a key gets zeros); NaN in the pages that are read in their place does not matter"""
     rng = np.random.default_rng(10)
     lens = [100, 70, 40, 5]
-    p = Pair(dev, rng, lens, new, 16, 2, 64)
+    p = Pair(dev, rng, lens, new, 16, 2, hd)
     p.o.table[0, 2], p.o.table[1, (70 + new[1] - 1) // 16] = -1, 10 ** 7
     p.o.table[2, :] = -1
     p.o.table[3, 0] = 2 ** 31 - 1
@@ -226,19 +227,20 @@ def test_attention_over_absent_pages(dev, new):
         p.o.k[0], p.o.v[0] = NAN, NAN
     p.upload()
     N, H = int(p.offsets[-1]), 4
-    q = _rows(rng, N, H, 64) / 64
-    o = torch.full((N, H * 64), 5.0, device=dev)
+    q = _rows(rng, N, H, hd) / 64
+    o = torch.full((N, H * hd), 5.0, device=dev)
     K.attn_paged(p.c, H, _cuda(q.reshape(N, -1), dev), o)
     want, tol = p.o.attend(q.astype(np.float64), lens, p.offsets, H)
-    assert (np.abs(o.cpu().numpy().reshape(N, H, 64) - want) <= tol).all()
+    assert (np.abs(o.cpu().numpy().reshape(N, H, hd) - want) <= tol).all()
     assert (o[p.offsets[2]:p.offsets[3]] == 0).all()
 
 
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
 @pytest.mark.parametrize("new", [4, 50, 150])
-def test_attention_nan_reaches_the_rows_that_see_it(dev, new):
+def test_attention_nan_reaches_the_rows_that_see_it(dev, new, hd):
     """NaN among a later token's keys or values does not reach the rows before it"""
     rng = np.random.default_rng(11)
-    lens, kvh, H, hd, page = [90], 1, 2, 64, 16
+    lens, kvh, H, page = [90], 1, 2, 16
     for what in ("k", "v"):
         p = Pair(dev, rng, lens, [new], page, kvh, hd)
         t = 90 + new // 2  # this token's
