@@ -19,125 +19,149 @@ __device__ __forceinline__ uint8_t code_again(uint8_t c, float shift) {
     return (uint8_t)codes(__builtin_amdgcn_cvt_f32_fp8(c, 0) * shift, 0.0f, 0.0f, 0.0f);
 }
 
-constexpr int kThreads = 256;
-
 struct AppendArgs {
     PkKvCache c;
     int N, hp;
+    int cap;          // tokens of a page that the LDS tile holds
     unsigned halves;  // workgroups for k, and as many for v: pages that may be written to, times heads
     const float *k, *v;
     int64_t ldk, ldv;
     RopeArgs rope;
-    TurnArgs q;
-    int q_tokens, q_vec;
+    TurnArgs q;  // of the heads that a workgroup turns
+    int q_tokens, q_parts, q_heads, q_vec;
+    unsigned q_blocks;
 };
 
-// one page's new tokens of one head's keys or values.  A page's head is written to by one
+// One page's new tokens of one head's keys or values.  A page's head is written to by one
 // workgroup, which turns the new values on their way to LDS, finds the largest of them, and
 // writes their codes from there, in words of 4: k's rows are the tokens', v's the columns.
-template <bool IS_V>
+// Where the tile holds fewer tokens than are new, the values are read twice.
+template <bool IS_V, int THREADS>
 __device__ __forceinline__ void append_page(const AppendArgs& a, unsigned task, int h, float* tile,
                                             float* red) {
     const PkKvCache& c = a.c;
-    const int page = (int)c.page, hd = (int)c.hd, hp = a.hp;
+    const int page = (int)c.page, hd = (int)c.hd, hp = a.hp, shift = __builtin_ctz(page);
     int nth, b;
     Seq s;
     if(!locate(
-           c, a.N, [&](const Seq& t) { return t.end > t.past ? (t.end - 1) / page - t.past / page + 1 : 0; },
+           c, a.N,
+           [&](const Seq& t) { return t.end > t.past ? ((t.end - 1) >> shift) - (t.past >> shift) + 1 : 0; },
            [&](int) { return (int)task; }, nth, b, s))
         return;
-    const int index = s.past / page + nth;
-    const int pid = c.table[(int64_t)b * c.width + index];
-    if(pid < 0 || pid >= c.pages) return;
-    // the page's new tokens: slots [s0, s1), the first of them in row `row`
+    const int index = (s.past >> shift) + nth;
+    const int name = c.table[(int64_t)b * c.width + index];
+    // the page's new tokens: slots [s0, s1), the first of them at position p0
     const int p0 = s.past > index * page ? s.past : index * page;
     const int s0 = p0 - index * page;
     const int s1 = s.end - index * page < page ? s.end - index * page : page;
-    const int n = s1 - s0;
     const int64_t ld = IS_V ? a.ldv : a.ldk;
     const float* src = (IS_V ? a.v : a.k) + (int64_t)(s.row + p0 - s.past) * ld + (int64_t)h * hd;
-    const int64_t at = (int64_t)pid * c.kv_heads + h;
+
+    const int half = IS_V ? 0 : a.rope.half, pairs = hp / 2, apart = pairs - half;
+    const int stride = IS_V ? a.cap + 5 : hp;
+    // pair e of the tokens from slot s0 + t0 on: where its values are in the head
+    struct Pair {
+        int t, p, d1, d2;
+    };
+    auto pair_of = [&](int e) {
+        Pair q;
+        q.t = e / pairs;
+        q.p = e - q.t * pairs;
+        const bool turned = q.p < half;
+        q.d1 = turned ? (a.rope.interleaved ? 2 * q.p : q.p) : half + q.p;
+        q.d2 = turned ? (a.rope.interleaved ? q.d1 + 1 : q.p + half) : half + q.p + apart;
+        return q;
+    };
+    float x1 = 0.0f, x2 = 0.0f, amax = 0.0f;
+    auto load = [&](int e, int t0) {
+        const Pair q = pair_of(e);
+        const float* r = src + (int64_t)(t0 + q.t) * ld;
+        x1 = q.d1 < hd ? r[q.d1] : 0.0f;
+        x2 = q.d2 < hd ? r[q.d2] : 0.0f;
+    };
+    const int n = s1 - s0, parts = (n + a.cap - 1) / a.cap;
+    if((int)threadIdx.x < (n < a.cap ? n : a.cap) * pairs) load(threadIdx.x, 0);  // (beside the page's number)
+    if(name < 0 || name >= c.pages) return;
+    const int64_t at = (int64_t)name * c.kv_heads + h;
     uint8_t* exps = (IS_V ? c.v_exp : c.k_exp) + at;
     uint8_t* out = (IS_V ? c.v : c.k) + at * (int64_t)(hp * page);
     const int old = s0 ? held((int)*exps - 127, kExpMin, kExpMax) : kExpMin;
 
-    const int half = IS_V ? 0 : a.rope.half, pairs = hp / 2, apart = pairs - half;
-    const int stride = IS_V ? page + 1 : hp;
-    float amax = 0.0f;
-    for(int e = threadIdx.x; e < n * pairs; e += kThreads) {
-        const int t = e / pairs, p = e - t * pairs;
-        const bool turned = p < half;
-        const int d1 = turned ? (a.rope.interleaved ? 2 * p : p) : half + p;
-        const int d2 = turned ? (a.rope.interleaved ? d1 + 1 : p + half) : half + p + apart;
-        const float* r = src + t * ld;
-        float x1 = d1 < hd ? r[d1] : 0.0f, x2 = d2 < hd ? r[d2] : 0.0f;
-        if(turned) {
-            float co, si;
-            rope_angle(p0 + t, a.rope.freqs[p], a.rope.magnitude, co, si);
-            rope_turn(x1, x2, co, si);
+    int e = 0;
+    float scale = 1.0f;
+    for(int i = 0; i < (parts == 1 ? 1 : 2 * parts); ++i) {
+        const int t0 = (i < parts ? i : i - parts) * a.cap, tokens = n - t0 < a.cap ? n - t0 : a.cap;
+        const int c0 = s0 + t0, c1 = c0 + tokens;  // slots
+        if(i) __syncthreads();
+        for(int j = threadIdx.x; j < tokens * pairs; j += THREADS) {
+            if(i || j >= THREADS) load(j, t0);
+            const Pair q = pair_of(j);
+            if(q.p < half) {
+                float co, si;
+                rope_angle(p0 + t0 + q.t, a.rope.freqs[q.p], a.rope.magnitude, co, si);
+                rope_turn(x1, x2, co, si);
+            }
+            const float m1 = fabsf(x1), m2 = fabsf(x2);
+            if(m1 <= 3.402823466e38f) amax = fmaxf(amax, m1);  // (not infinities or NaN)
+            if(m2 <= 3.402823466e38f) amax = fmaxf(amax, m2);
+            // (v's columns are at their slots from a multiple of 4 on, so that words line up)
+            tile[IS_V ? q.d1 * stride + c0 % 4 + q.t : q.t * stride + q.d1] = x1;
+            tile[IS_V ? q.d2 * stride + c0 % 4 + q.t : q.t * stride + q.d2] = x2;
         }
-        const float m1 = fabsf(x1), m2 = fabsf(x2);
-        if(m1 <= 3.402823466e38f) amax = fmaxf(amax, m1);  // (not infinities or NaN)
-        if(m2 <= 3.402823466e38f) amax = fmaxf(amax, m2);
-        // (v's columns are at their slots, so that words of 4 tokens line up)
-        tile[IS_V ? d1 * stride + s0 + t : t * stride + d1] = x1;
-        tile[IS_V ? d2 * stride + s0 + t : t * stride + d2] = x2;
-    }
-    amax = block_max<kThreads / kWave>(amax, red);
-    const int fresh = block_exponent(amax), e = fresh > old ? fresh : old;
-    const float scale = ldexpf(1.0f, -e);
-    if(!IS_V) {
-        for(int i = 4 * (int)threadIdx.x; i < n * hp; i += 4 * kThreads) {
-            const f32x4 x = *(const f32x4*)(tile + i) * scale;
-            *(uint32_t*)(out + s0 * hp + i) = codes(x[0], x[1], x[2], x[3]);
+        if(i == parts - 1) {
+            amax = block_max<THREADS / kWave>(amax, red);
+            const int fresh = block_exponent(amax);
+            e = fresh > old ? fresh : old;
+            scale = ldexpf(1.0f, -e);
         }
-    } else {
+        if(parts > 1 && i < parts) continue;  // (the page's largest is not known yet)
+        __syncthreads();
+        if(!IS_V) {
+            for(int j = 4 * (int)threadIdx.x; j < tokens * hp; j += 4 * THREADS) {
+                const f32x4 x = *(const f32x4*)(tile + j) * scale;
+                *(uint32_t*)(out + c0 * hp + j) = codes(x[0], x[1], x[2], x[3]);
+            }
+            continue;
+        }
         // words of tokens that are all new, single bytes at the ends
-        const int w0 = s0 / 4, words = (s1 + 3) / 4 - w0;
-        for(int i = threadIdx.x; i < hd * words; i += kThreads) {
-            const int d = i / words, t = 4 * (w0 + i - d * words);
-            const float* x = tile + d * stride + t;
+        const int w0 = c0 / 4, words = (c1 + 3) / 4 - w0;
+        for(int j = threadIdx.x; j < hd * words; j += THREADS) {
+            const int d = j / words, w = j - d * words, t = 4 * (w0 + w);
+            const float* x = tile + d * stride + 4 * w;
             float y[4];
 #pragma unroll
-            for(int q = 0; q < 4; ++q) y[q] = t + q >= s0 && t + q < s1 ? x[q] * scale : 0.0f;
-            const uint32_t w = codes(y[0], y[1], y[2], y[3]);
+            for(int q = 0; q < 4; ++q) y[q] = t + q >= c0 && t + q < c1 ? x[q] * scale : 0.0f;
+            const uint32_t word = codes(y[0], y[1], y[2], y[3]);
             uint8_t* to = out + d * page + t;
-            if(t >= s0 && t + 4 <= s1) {
-                *(uint32_t*)to = w;
+            if(t >= c0 && t + 4 <= c1) {
+                *(uint32_t*)to = word;
             } else {
 #pragma unroll
                 for(int q = 0; q < 4; ++q)
-                    if(t + q >= s0 && t + q < s1) to[q] = (uint8_t)(w >> (8 * q));
+                    if(t + q >= c0 && t + q < c1) to[q] = (uint8_t)(word >> (8 * q));
             }
         }
     }
     if(e > old && s0) {  // what the page held, at its new scale
-        const float shift = ldexpf(1.0f, old - e);
-        for(int i = threadIdx.x; i < s0 * hd; i += kThreads) {
+        const float to = ldexpf(1.0f, old - e);
+        for(int i = threadIdx.x; i < s0 * hd; i += THREADS) {
             const int j = IS_V ? i / s0 * page + i % s0 : i / hd * hp + i % hd;
-            out[j] = code_again(out[j], shift);
+            out[j] = code_again(out[j], to);
         }
     }
-    // (every thread has read the old one: block_max waited for all)
+    // (every thread has read the old one: the exchange of amax waited for all)
     if(threadIdx.x == 0) *exps = (uint8_t)(e + 127);
 }
 
-__global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
-    extern __shared__ __align__(16) float tile[];
-    __shared__ float red[kThreads / kWave];
-    const unsigned block = blockIdx.x, heads = (unsigned)a.c.kv_heads;
-    if(block < a.halves) return append_page<false>(a, block / heads, (int)(block % heads), tile, red);
-    if(block < 2 * a.halves) {
-        const unsigned i = block - a.halves;
-        return append_page<true>(a, i / heads, (int)(i % heads), tile, red);
-    }
-    // queries: rows [t0, t0 + tokens), each at the position of its token
-    const int t0 = (int)(block - 2 * a.halves) * a.q_tokens;
-    const int tokens = a.N - t0 < a.q_tokens ? a.N - t0 : a.q_tokens;
+// the queries of some tokens and heads, each at the position of its token
+template <int THREADS>
+__device__ __forceinline__ void turn_queries(const AppendArgs& a, unsigned block) {
     __shared__ int place[8];
     __shared__ __align__(16) float tc[kTurnTable], ts[kTurnTable];
+    const int t0 = (int)(block / a.q_parts) * a.q_tokens, h0 = (int)(block % a.q_parts) * a.q_heads;
+    const int tokens = a.N - t0 < a.q_tokens ? a.N - t0 : a.q_tokens;
     const int lane = threadIdx.x % kWave, B = (int)a.c.B;
-    for(int t = threadIdx.x / kWave; t < tokens; t += kThreads / kWave) {
+    for(int t = threadIdx.x / kWave; t < tokens; t += THREADS / kWave) {
         // the last sequence that begins at this row or before, and whether the row is in it
         int before = 0;
         for(int base = 0; base < B; base += kWave) {
@@ -158,12 +182,30 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs a) {
         pos = place[t];
         return pos >= 0;
     };
+    TurnArgs q = a.q;  // (the last part may have fewer heads)
+    q.x += h0 * q.hd;
+    q.y += h0 * q.hd;
+    const int heads = q.H - h0 < a.q_heads ? q.H - h0 : a.q_heads;
     if(a.rope.interleaved)
-        a.q_vec ? turn_rows<4, true>(a.q, a.rope, t0, tokens, where, tc, ts)
-                : turn_rows<1, true>(a.q, a.rope, t0, tokens, where, tc, ts);
+        a.q_vec ? turn_rows<4, true>(q, a.rope, t0, tokens, heads, where, tc, ts)
+                : turn_rows<1, true>(q, a.rope, t0, tokens, heads, where, tc, ts);
     else
-        a.q_vec ? turn_rows<4, false>(a.q, a.rope, t0, tokens, where, tc, ts)
-                : turn_rows<1, false>(a.q, a.rope, t0, tokens, where, tc, ts);
+        a.q_vec ? turn_rows<4, false>(q, a.rope, t0, tokens, heads, where, tc, ts)
+                : turn_rows<1, false>(q, a.rope, t0, tokens, heads, where, tc, ts);
+}
+
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
+    extern __shared__ __align__(16) float tile[];
+    __shared__ float red[THREADS / kWave];
+    // (queries first where a few tokens' workgroups all start at once, last where they are
+    // waited for in turn)
+    const unsigned heads = (unsigned)a.c.kv_heads, pages = 2 * a.halves;
+    const unsigned block = THREADS == kWave ? (blockIdx.x + pages) % (pages + a.q_blocks) : blockIdx.x;
+    if(block >= pages) return turn_queries<THREADS>(a, block - pages);
+    if(block < a.halves)
+        return append_page<false, THREADS>(a, block / heads, (int)(block % heads), tile, red);
+    append_page<true, THREADS>(a, (block - a.halves) / heads, (int)((block - a.halves) % heads), tile, red);
 }
 
 }  // namespace
@@ -196,15 +238,29 @@ extern "C" int pk_kv_append_f32(const PkKvCache* cache, int64_t N, const float* 
     const int64_t page = cache->page, kvh = cache->kv_heads;
     // a sequence with n > 0 new tokens writes to at most n pages, and n / page + 2
     const int64_t tasks = N < N / page + 2 * cache->B ? N : N / page + 2 * cache->B;
-    int64_t blocks = 2 * tasks * kvh;
-    if(!grid_fits(blocks + N, kThreads))
-        return fail("pk_kv_append_f32: too many pages and heads for one launch");
+    // up to 2 tokens a sequence, as tokens are generated: a wave to a page's head, and a
+    // tile of 4 tokens, so that all of a step's workgroups have room at once
+    const bool few = N <= 2 * cache->B;
+    const int threads = few ? 64 : 256;
+    a.cap = few ? 4 : (int)page;
     a.halves = (unsigned)(tasks * kvh);
+    if(!grid_fits(2 * tasks * kvh + N * (q ? H : 1), threads))
+        return fail("pk_kv_append_f32: too many pages and heads for one launch");
     if(q) {
         a.q_vec = turn_args(a.q, a.rope, H, hd, q, ldq, q_out, ldqo, 0);
-        a.q_tokens = turn_tokens(N, H, a.rope.half);
-        blocks += (N + a.q_tokens - 1) / a.q_tokens;
+        a.q_tokens = few ? 1 : turn_tokens(N, H, a.rope.half);
+        // of a single token, as many heads as a wave turns with its loads in flight at once
+        a.q_heads = few ? (int)(threads * kTurnUnits / a.q.per_head.d) : (int)H;
+        a.q_heads = a.q_heads < 1 ? 1 : a.q_heads > H ? (int)H : a.q_heads;
+        a.q_parts = (int)((H + a.q_heads - 1) / a.q_heads);
+        a.q.per_token = div_by(a.q_heads);
+        a.q_blocks = (unsigned)((N + a.q_tokens - 1) / a.q_tokens * a.q_parts);
     }
-    append_kernel<<<(unsigned)blocks, kThreads, sizeof(float) * a.hp * (page + 1), as_stream(stream)>>>(a);
+    const unsigned blocks = a.q_blocks + 2 * a.halves;
+    const size_t lds = sizeof(float) * a.hp * (a.cap + 5);
+    if(few)
+        append_kernel<64><<<blocks, 64, lds, as_stream(stream)>>>(a);
+    else
+        append_kernel<256><<<blocks, 256, lds, as_stream(stream)>>>(a);
     return launch_status("pk_kv_append_f32");
 }

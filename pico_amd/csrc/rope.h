@@ -49,29 +49,30 @@ struct Div {
 inline Div div_by(int64_t d) { return {(((uint64_t)1 << 36) + d - 1) / d, (int)d}; }
 
 constexpr int kTurnTable = 512;  // angles a workgroup holds in LDS
+constexpr int kTurnUnits = 4;    // units a thread has in flight
 constexpr int kTurnHead = 1024;  // largest head, so that one token's fit there
 
-// the heads of `tokens` rows, t0 onwards, of x turned into y
+// heads of `tokens` rows, t0 onwards, of x turned into y
 struct TurnArgs {
     const float* x;
     float* y;
     int64_t ldx, ldy;
     int H, hd;
-    Div per_head, per_token;  // units of a head, heads of a token
+    Div per_head, per_token;  // units of a head, heads of a token that a workgroup takes
     int back, accum;
 };
 
 // One workgroup: the sines and cosines of the tokens' angles once, in LDS, for all heads;
-// then units of 8 values (V = 4: two float4 of a head) or of a pair (V = 1), four in
-// flight a thread, those of the first round loaded before the angles.  where(t, pos): the
+// then units of 8 values (V = 4: two float4 of a head, neighbouring threads' side by side)
+// or of a pair (V = 1), four in flight a thread, those of the first round loaded before the angles.  where(t, pos): the
 // position of token t0 + t; false leaves the row.
 template <int V, bool INTER, class P>
 __device__ __forceinline__ void turn_rows(const TurnArgs& g, const RopeArgs& r, int64_t t0,
-                                          int tokens, P where, float* tc, float* ts) {
+                                          int tokens, int heads, P where, float* tc, float* ts) {
     typedef float vec __attribute__((ext_vector_type(V)));
     const int half = r.half, rot = 2 * half, threads = blockDim.x;
-    const int total = tokens * g.H * g.per_head.d;
-    constexpr int U = 4;
+    const int total = tokens * g.per_token.d * g.per_head.d;
+    constexpr int U = kTurnUnits;
     for(int base = 0; base < total; base += threads * U) {
         vec a[U], b[U];
         int tok[U], at[U], da[U], db[U];  // where a and b are in their head; db < 0: no b
@@ -82,13 +83,16 @@ __device__ __forceinline__ void turn_rows(const TurnArgs& g, const RopeArgs& r, 
             int pos;
             if(u >= total) continue;
             const int hr = g.per_head.of(u), j = u - hr * g.per_head.d, t = g.per_token.of(hr);
-            if(!where(t, pos)) continue;
+            const int h = hr - t * g.per_token.d;
+            if(h >= heads || !where(t, pos)) continue;
             tok[i] = t;
-            at[i] = (hr - t * g.H) * g.hd;
+            at[i] = h * g.hd;
             if(V == 4) {
                 if(INTER || 8 * j >= rot) {
-                    da[i] = 8 * j;
-                    db[i] = 8 * j + 4 < g.hd ? 8 * j + 4 : -1;
+                    const int from = INTER ? 0 : rot, k = INTER ? j : j - rot / 8;
+                    da[i] = from + 4 * k;
+                    db[i] = da[i] + (g.hd - from + 7) / 8 * 4;
+                    if(db[i] >= g.hd) db[i] = -1;
                 } else {
                     da[i] = 4 * j;
                     db[i] = 4 * j + half;

@@ -17,7 +17,7 @@ __global__ __launch_bounds__(kThreads) void rope_kernel(int64_t N, int T, TurnAr
     __shared__ __align__(16) float tc[kTurnTable], ts[kTurnTable];
     const int64_t t0 = (int64_t)blockIdx.x * T;
     turn_rows<V, INTER>(
-        g, r, t0, (int)(N - t0 < T ? N - t0 : T),
+        g, r, t0, (int)(N - t0 < T ? N - t0 : T), g.H,
         [&](int t, int& pos) {
             pos = positions[t0 + t];
             return true;
