@@ -24,6 +24,19 @@ __device__ __forceinline__ Seq sequence(const PkKvCache& c, int N, int b) {
     return s;
 }
 
+// n / d for 0 <= n < 2^31: with 2^(l-1) < d <= 2^l and m = floor(2^(31+l) / d) + 1, m d
+// exceeds 2^(31+l) by d at most, which leaves n m / 2^(31+l) below the next whole number
+struct Quotient {
+    uint32_t m;
+    int s, d;
+    __device__ __forceinline__ int of(int n) const { return d == 1 ? n : (int)(__umulhi((uint32_t)n, m) >> s); }
+};
+inline Quotient quotient(int d) {
+    int l = 0;
+    while(((int64_t)1 << l) < d) ++l;
+    return {d == 1 ? 0u : (uint32_t)(((uint64_t)1 << (31 + l)) / (uint64_t)d + 1), l - 1, d};
+}
+
 // sums over the lanes up to one's own
 __device__ __forceinline__ int wave_scan(int v) {
     v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4 and 8 lanes
@@ -87,10 +100,11 @@ inline int check_cache(const char* who, const PkKvCache* c, int64_t N) {
     if(!head_size(c->hd)) return fail("%s: head size %lld: 1 to 256", who, (long long)c->hd);
     if(c->page != 16 && c->page != 32 && c->page != 64 && c->page != 128)
         return fail("%s: pages of %lld tokens: 16, 32, 64 or 128", who, (long long)c->page);
-    if(c->kv_heads < 1 || c->kv_heads > 4096 || c->pages < 1 || c->pages >= (int64_t)1 << 31 ||
+    if(c->kv_heads < 1 || c->kv_heads > 4096 || c->pages < 1 ||
+       c->pages > (((int64_t)1 << 31) - 1) / c->kv_heads ||
        c->B < 0 || c->B > (1 << 20) || c->width < 1 || c->width > (((int64_t)1 << 30) - 1) / c->page)
-        return fail("%s: kv_heads %lld, pages %lld, B %lld, width %lld: 1 to 4096 heads, 1 to 2^31 - 1 "
-                    "pages, up to 2^20 sequences of fewer than 2^30 positions",
+        return fail("%s: kv_heads %lld, pages %lld, B %lld, width %lld: 1 to 4096 heads, fewer than "
+                    "2^31 pages times heads, up to 2^20 sequences of fewer than 2^30 positions",
                     who, (long long)c->kv_heads, (long long)c->pages, (long long)c->B,
                     (long long)c->width);
     if(N < 0 || N >= (int64_t)1 << 24)

@@ -47,7 +47,8 @@ struct AttnArgs {
     float* ws;
     int W;    // workgroups that share the units of all tiles
     int splits;  // workgroups to a tile of many rows
-    int vec;  // q can be read in float4
+    int vec;  // q can be read in float4, and o written
+    Quotient by_group;
 };
 
 __device__ __forceinline__ f16x8 widen(uint32_t lo, uint32_t hi) {
@@ -115,12 +116,28 @@ __device__ __forceinline__ float raise(float mx, float& limit) {
     return up;
 }
 
+// row (token, head of the group) of a sequence -> token
+__device__ __forceinline__ int group_of(const AttnArgs& a, int row) { return a.by_group.of(row); }
+
+// the first n of 4 values
+__device__ __forceinline__ void store4(float* to, f32x4 v, int n, int vec) {
+    if(vec) {
+        if(n > 0) *(f32x4*)to = v;
+    } else {
+#pragma unroll
+        for(int k = 0; k < 4; ++k)
+            if(k < n) to[k] = v[k];
+    }
+}
+
 // Loads before it in the source are issued before those after it: results come in the order
 // of the loads, so one that is waited for first must not be behind others.
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
-// A lane's values of a query: step st's are 8 from at(st) on, those behind the head's end
-// any of it.  All loads are issued before the first is used.
+// A lane's values of a query: step st's are 8 from at(st) on.  Those behind the head's end
+// are its first, which the zeros there in the cache leave out (were the first infinite or
+// NaN, the row's scores would not be numbers anyway).  All loads are issued before the
+// first is used.
 template <int STEPS, class F>
 __device__ __forceinline__ void load_query(const float* head, int hd, int vec, F at, float (&x)[STEPS][8]) {
     if(vec) {
@@ -141,26 +158,24 @@ __device__ __forceinline__ void load_query(const float* head, int hd, int vec, F
     }
 }
 
-// a query, held by lanes W apart, brought to [2^14, 2^15) by 2^-e and cut in two parts, zeros
-// behind its end; returns e.  Rows that are none become zeros.
-template <int W, int STEPS, class F>
-__device__ __forceinline__ int bring_up(float (&x)[STEPS][8], int hd, F at, bool on, f16x8 (&hi)[STEPS],
-                                        f16x8 (&lo)[STEPS]) {
+// A query, held by lanes W apart, brought to [2^14, 2^15) by 2^-e and cut in two parts;
+// returns e.  (Below 2^-86 a query's scores are nothing beside each other: e ends there,
+// so that 2^-e is a float.)
+template <int W, int STEPS>
+__device__ __forceinline__ int bring_up(float (&x)[STEPS][8], f16x8 (&hi)[STEPS], f16x8 (&lo)[STEPS]) {
     float amax = 0.0f;
 #pragma unroll
     for(int st = 0; st < STEPS; ++st)
 #pragma unroll
-        for(int i = 0; i < 8; ++i) {
-            if(!on || at(st) + i >= hd) x[st][i] = 0.0f;
-            amax = fmaxf(amax, fabsf(x[st][i]));
-        }
+        for(int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[st][i]));
 #pragma unroll
     for(int o = W; o < kWave; o *= 2) amax = fmaxf(amax, __shfl_xor(amax, o, kWave));
-    const int e = amax > 0.0f && amax <= 3.402823466e38f ? __builtin_amdgcn_frexp_expf(amax) - 15 : 0;
+    const int e = amax > 0x1p-86f && amax <= 0x1.fffffep127f ? __builtin_amdgcn_frexp_expf(amax) - 15 : -100;
+    const float by = __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
     for(int st = 0; st < STEPS; ++st) {
 #pragma unroll
-        for(int i = 0; i < 8; ++i) x[st][i] = ldexpf(x[st][i], -e);
+        for(int i = 0; i < 8; ++i) x[st][i] *= by;
         two_parts(x[st], hi[st], lo[st]);
     }
     return e;
@@ -260,13 +275,13 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
         const int32_t* names = c.table + (int64_t)b * width;
         const int per = page < kUnit ? kUnit / page : 1;
         const int x_key = 16 * (col / 4) >> shift, x_value = 16 * quad >> shift;
-        const int h = item / tiles, first = (item - h * tiles) * kFew;
+        const int h = tiles == 1 ? item : item / tiles, first = (item - h * tiles) * kFew;
         int pid, ek, ev, k = 0;
         auto name_units = [&](int u) {
             const int i = ((u + WAVES * (lane / per)) * kUnit + lane % per * page) >> shift;
             pid = names[i < width ? i : 0];
             if(i >= width || pid < 0 || pid >= c.pages) pid = -1;
-            const int64_t at = (int64_t)(pid < 0 ? 0 : pid) * kvh + h;
+            const uint32_t at = (uint32_t)(pid < 0 ? 0 : pid) * kvh + h;
             ek = c.k_exp[at];
             ev = c.v_exp[at];
             k = 0;
@@ -279,9 +294,9 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
         // the order that the lane's keys come in
         const int rows = s.n * a.group - first < kFew ? s.n * a.group - first : kFew;
         const int mine = first + (col < rows ? col : 0);
-        const int token = mine / a.group;
-        const int reach = s.past + token;                 // the last key that it sees
-        const int clear = s.past + first / a.group + 1;   // tokens that every row sees
+        const int token = group_of(a, mine);
+        const int reach = s.past + token;                    // the last key that it sees
+        const int clear = s.past + group_of(a, first) + 1;   // tokens that every row sees
         const float* qr = a.q + (int64_t)(s.row + token) * a.ldq +
                           (int64_t)(h * a.group + mine - token * a.group) * hd;
         float x[STEPS][8];
@@ -298,7 +313,8 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
         // than those that it waits for: where there is no unit, of one line)
         auto load_keys = [&](int u, int pid) {
             const int slot = ((u * kUnit + 16 * (col / 4)) & (page - 1)) + col % 4;
-            const uint8_t* p = c.k + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * page + slot) * HP + 16 * quad;
+            const uint8_t* p = c.k + (uint64_t)((uint32_t)(pid < 0 ? 0 : pid) * kvh + h) * (uint32_t)(HP * page) +
+                               (slot * HP + 16 * quad);
             if(u >= u1) p = c.k;
 #pragma unroll
             for(int t = 0; t < 4; ++t) {
@@ -311,10 +327,11 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
         };
         auto load_values = [&](int u, int pid) {
             const int slot = (u * kUnit + 16 * quad) & (page - 1);
-            const uint8_t* p = c.v + (((int64_t)(pid < 0 ? 0 : pid) * kvh + h) * HP + col) * page + slot;
+            const uint8_t* p = c.v + (uint64_t)((uint32_t)(pid < 0 ? 0 : pid) * kvh + h) * (uint32_t)(HP * page) +
+                               (col * page + slot);
             if(u >= u1) p = c.v;
 #pragma unroll
-            for(int i = 0; i < DT; ++i) vr[i] = *(const u32x4*)(p + (int64_t)16 * i * page);
+            for(int i = 0; i < DT; ++i) vr[i] = *(const u32x4*)(p + (uint32_t)(16 * i * page));
             in_order();
         };
         int pv = of_unit(pid, x_value);
@@ -323,7 +340,7 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
         __builtin_amdgcn_sched_barrier(0);  // (nor is the query waited for before)
 
         f16x8 qh[STEPS], ql[STEPS];
-        const int eq = bring_up<16>(x, hd, of_step, col < rows, qh, ql);
+        const int eq = bring_up<16>(x, qh, ql);
         const float coef = ldexpf(a.scale, eq);
 
         f32x4 acc[DT];
@@ -374,11 +391,15 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
             if(__ballot(mx > limit)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-                const float up = raise(mx, limit), down = __builtin_amdgcn_exp2f(fminf(-up, 0.0f));
+                const bool some = __ballot(limit != kNone) != 0;  // (else there is nothing to scale)
+                const float up = raise(mx, limit);
                 m += up;
-                l *= down;
+                if(some) {
+                    const float down = __builtin_amdgcn_exp2f(fminf(-up, 0.0f));
+                    l *= down;
 #pragma unroll
-                for(int i = 0; i < DT; ++i) acc[i] *= down;
+                    for(int i = 0; i < DT; ++i) acc[i] *= down;
+                }
 #pragma unroll
                 for(int i = 0; i < 16; ++i) p[i] -= up;
             }
@@ -396,11 +417,12 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
             if(edge) {
                 // tokens behind the sequence's last, or on no page, may hold anything
                 const u32x4 keep = first_bytes(absent ? 0 : held(s.end - token0, 0, 16));
-                u32x4 nan = {};
 #pragma unroll
-                for(int i = 0; i < DT; ++i) {
-                    vr[i] &= keep;
-                    nan |= nan_bytes(vr[i]);
+                for(int i = 0; i < DT; ++i) vr[i] &= keep;
+                u32x4 nan = {};
+                if(s.n > 1) {  // (of a single token, all rows see all that are left)
+#pragma unroll
+                    for(int i = 0; i < DT; ++i) nan |= nan_bytes(vr[i]);
                 }
                 if(__builtin_expect(__ballot((nan[0] | nan[1] | nan[2] | nan[3]) != 0) != 0, 0)) {
                     // a NaN among the values of tokens that some rows do not see must not
@@ -434,13 +456,15 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
         // the waves' parts together
         l += __shfl_xor(l, 16, kWave);
         l += __shfl_xor(l, 32, kWave);
+        if(poison) {
 #pragma unroll
-        for(int i = 0; i < DT; ++i) {
+            for(int i = 0; i < DT; ++i)
 #pragma unroll
-            for(int r = 0; r < 4; ++r)
-                if(poison && marked<HP>(poisoned[wave], col, 16 * i + 4 * quad + r)) acc[i][r] = NAN;
-            *(f32x4*)&part[wave][col][16 * i + 4 * quad] = acc[i];
+                for(int r = 0; r < 4; ++r)
+                    if(marked<HP>(poisoned[wave], col, 16 * i + 4 * quad + r)) acc[i][r] = NAN;
         }
+#pragma unroll
+        for(int i = 0; i < DT; ++i) *(f32x4*)&part[wave][col][16 * i + 4 * quad] = acc[i];
         if(lane < 16) {
             part_m[wave][lane] = limit == kNone ? kNone : m;
             part_l[wave][lane] = l;
@@ -469,11 +493,9 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
                 continue;
             }
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // (0: no key at all)
-            const int t = (first + r) / a.group;
+            const int t = group_of(a, first + r);
             float* to = a.o + (int64_t)(s.row + t) * a.ldo + (int64_t)(h * a.group + first + r - t * a.group) * hd + d;
-#pragma unroll
-            for(int k = 0; k < 4; ++k)
-                if(d + k < hd) to[k] = v[k] * inv;
+            store4(to, v * inv, hd - d, a.vec);
         }
         if(WHOLE) return;
         __syncthreads();
@@ -535,10 +557,9 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     }
     if(mine) return;
     const float inv = all == 0.0f ? 0.0f : 1.0f / all;
-    float* to = a.o + (int64_t)(s.row + row / a.group) * a.ldo + (int64_t)(h * a.group + row % a.group) * c.hd + d;
-#pragma unroll
-    for(int k = 0; k < 4; ++k)
-        if(d + k < c.hd) to[k] = sum[k] * inv;
+    const int t = group_of(a, row);
+    float* to = a.o + (int64_t)(s.row + t) * a.ldo + (int64_t)(h * a.group + row - t * a.group) * c.hd + d;
+    store4(to, sum * inv, (int)c.hd - d, a.vec);
 }
 
 // ------------------------------------------------ many query rows a sequence
@@ -588,8 +609,9 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
     // the lane's query
     const int row = first + col, rows = total - first < 32 ? total - first : 32;
     const int real_row = col < rows ? row : tile * kRows;
-    const int token = real_row / a.group;
-    const float* qr = a.q + (int64_t)(s.row + token) * a.ldq + (int64_t)(h * a.group + real_row % a.group) * hd;
+    const int token = group_of(a, real_row);
+    const float* qr = a.q + (int64_t)(s.row + token) * a.ldq +
+                      (int64_t)(h * a.group + real_row - token * a.group) * hd;
     const int reach = s.past + token;
     f16x8 qh[STEPS], ql[STEPS];
     float coef;
@@ -597,7 +619,7 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
         float x[STEPS][8];
         auto of_step = [&](int st) { return 32 * (st / 2) + 16 * half + 8 * (st % 2); };
         load_query(qr, hd, a.vec, of_step, x);
-        coef = ldexpf(a.scale, bring_up<32>(x, hd, of_step, col < rows, qh, ql));
+        coef = ldexpf(a.scale, bring_up<32>(x, qh, ql));
     }
 
     auto page_of = [&](int u, int g16) {
@@ -655,7 +677,7 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
     for(int i = 0; i < DT; ++i) acc[i] = f32x16{};
     float m = 0.0f, l = 0.0f, limit = kNone;
     bool poison = false;
-    const int clear = s.past + (first < total ? first / a.group : 0) + 1;  // tokens that all rows see
+    const int clear = s.past + (first < total ? group_of(a, first) : 0) + 1;  // tokens that all rows see
     const int reach_all = s.past + (first + rows - 1) / a.group;           // and that any does
     find_pages(u0);
     if(u0 < u1) {
@@ -702,11 +724,15 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
             for(int i = 0; i < 16; ++i) mx = fmaxf(mx, p[i]);
             if(__ballot(mx > limit)) {
                 mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-                const float up = raise(mx, limit), down = __builtin_amdgcn_exp2f(fminf(-up, 0.0f));
+                const bool some = __ballot(limit != kNone) != 0;  // (else there is nothing to scale)
+                const float up = raise(mx, limit);
                 m += up;
-                l *= down;
+                if(some) {
+                    const float down = __builtin_amdgcn_exp2f(fminf(-up, 0.0f));
+                    l *= down;
 #pragma unroll
-                for(int i = 0; i < DT; ++i) acc[i] *= down;
+                    for(int i = 0; i < DT; ++i) acc[i] *= down;
+                }
 #pragma unroll
                 for(int i = 0; i < 16; ++i) p[i] -= up;
             }
@@ -778,16 +804,15 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
         return;
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    float* to = a.o + (int64_t)(s.row + token) * a.ldo + (int64_t)(h * a.group + row % a.group) * hd;
+    float* to = a.o + (int64_t)(s.row + token) * a.ldo + (int64_t)(h * a.group + row - token * a.group) * hd;
 #pragma unroll
     for(int i = 0; i < DT; ++i)
 #pragma unroll
-        for(int q = 0; q < 4; ++q)
-#pragma unroll
-            for(int k = 0; k < 4; ++k) {
-                const int d = 32 * i + 8 * q + 4 * half + k;
-                if(d < hd) to[d] = acc[i][4 * q + k] * inv;
-            }
+        for(int q = 0; q < 4; ++q) {
+            const int d = 32 * i + 8 * q + 4 * half;
+            const f32x4 v = {acc[i][4 * q], acc[i][4 * q + 1], acc[i][4 * q + 2], acc[i][4 * q + 3]};
+            store4(to + d, v * inv, hd - d, a.vec);
+        }
 }
 
 // the parts of many_rows_kernel's tiles together: a wave to a row
@@ -819,10 +844,9 @@ __global__ __launch_bounds__(256) void finish_kernel(AttnArgs a) {
         if(lane < D4) v += f * *(const f32x4*)(p + 2 * kRows + r * HP + d);
     }
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    float* to = a.o + (int64_t)(s.row + row / a.group) * a.ldo + (int64_t)(h * a.group + row % a.group) * c.hd + d;
-#pragma unroll
-    for(int k = 0; k < 4; ++k)
-        if(lane < D4 && d + k < c.hd) to[k] = v[k] * inv;
+    const int t = group_of(a, row);
+    float* to = a.o + (int64_t)(s.row + t) * a.ldo + (int64_t)(h * a.group + row - t * a.group) * c.hd + d;
+    if(lane < D4) store4(to, v * inv, (int)c.hd - d, a.vec);
 }
 
 // ------------------------------------------------------------------- launches
@@ -919,7 +943,8 @@ extern "C" int pk_attn_paged_f32(const PkKvCache* cache, int64_t N, int64_t H, f
     a.ws = (float*)workspace;
     a.W = p.W;
     a.splits = p.splits;
-    a.vec = cache->hd % 4 == 0 && ldq % 4 == 0 && aligned16(q);
+    a.vec = cache->hd % 4 == 0 && ldq % 4 == 0 && ldo % 4 == 0 && aligned16(q) && aligned16(o);
+    a.by_group = quotient(a.group);
     const hipStream_t st = as_stream(stream);
     switch(head_size(cache->hd)) {
         case 32: launch<32>(a, p, st); break;
