@@ -696,6 +696,8 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
         for(int j = 0; j < 2; ++j) {
             const int token0 = u * kUnit + 32 * j;
             if(rows <= 0 || token0 > reach_all) continue;
+            // (the waves that have products to give the matrix cores before those that do not)
+            __builtin_amdgcn_s_setprio(1);
             f32x16 sc = {};
 #pragma unroll
             for(int st = 0; st < STEPS; st += 2) {
@@ -706,6 +708,7 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[st], sc, 0, 0, 0);
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[st + 1], sc, 0, 0, 0);
             }
+            __builtin_amdgcn_s_setprio(0);
             const float4 g = pages[buf][2 * j + half];
             const float kc = coef * g.x;
             const bool absent = g.w == 0.0f;
@@ -834,9 +837,11 @@ __global__ __launch_bounds__(256) void finish_kernel(AttnArgs a) {
     const float* base = a.ws + ((int64_t)rest * a.splits * kvh + h) * kManyPart<HP>;
     const int64_t apart = (int64_t)kvh * kManyPart<HP>;
     float top = kNone, total = 0.0f;
-    for(int i = 0; i < a.splits; ++i) top = fmaxf(top, base[i * apart + r]);
+    if(lane < a.splits) top = base[lane * apart + r];  // (at most 16)
+    top = wave_max(top);
     const int d = 4 * lane;
     f32x4 v = {};
+#pragma unroll 8
     for(int i = 0; i < a.splits; ++i) {
         const float* p = base + i * apart;
         const float f = __builtin_amdgcn_exp2f(p[r] - top);
@@ -863,7 +868,7 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
     p.rows = N * group <= 32 * c->B ? kFew : kRows;
     p.tiles = N * group / p.rows + some;
     if(p.rows < kRows) {
-        p.W = units <= 32 || p.tiles * c->kv_heads * units >= (int64_t)1 << 31 ? 0 : 256;
+        p.W = units <= (c->hd <= 128 ? 32 : 16) || p.tiles * c->kv_heads * units >= (int64_t)1 << 31 ? 0 : 256;
     } else {
         // workgroups that there are for sure, two to a CU, of 8 units at least
         const int64_t sure = (N * group + kRows - 1) / kRows * c->kv_heads;
