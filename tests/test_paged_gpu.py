@@ -165,7 +165,17 @@ ATTENDS = [([0], [1], 16, 1, 1, 64), ([1, 15, 16, 17], [1, 1, 1, 1], 16, 2, 1, 6
            ([300, 0], [1, 1], 32, 1, 8, 32), ([300, 130], [1, 1], 128, 2, 16, 64), ([90], [7], 16, 3, 3, 80),
            ([0, 50], [33, 20], 16, 2, 2, 64), ([5000], [1], 128, 1, 2, 256), ([700], [4], 32, 1, 24, 256),
            ([31] * 70, [i % 3 for i in range(70)], 32, 1, 2, 7), ([0], [200], 64, 2, 1, 128), ([513], [130], 16, 1, 3, 33),
-           ([0, 0, 0], [1, 0, 5], 128, 2, 2, 64), ([100], [90], 32, 1, 2, 256)]
+           ([0, 0, 0], [1, 0, 5], 128, 2, 2, 64), ([100], [90], 32, 1, 2, 256),
+           # caches beyond 2048 tokens: units shared out evenly, tiles in parts
+           ([2300, 700, 64], [1, 1, 1], 64, 1, 3, 64), ([2100, 2500], [2, 1], 16, 1, 8, 96),
+           ([2200, 1, 0, 900], [1, 1, 0, 2], 128, 1, 1, 32), ([3000], [1], 64, 1, 16, 128), ([1500], [5], 16, 1, 7, 256),
+           ([20] * 66 + [2100], [1] * 67, 128, 1, 4, 128), ([3000], [40], 64, 1, 4, 64),
+           # tiles of 128 rows
+           ([0], [700], 64, 2, 3, 64), ([40, 0, 7], [333, 0, 400], 16, 1, 6, 128), ([5], [530], 32, 1, 8, 33),
+           ([300], [1040], 128, 4, 1, 96), ([77, 3], [500, 20], 16, 2, 4, 80), ([0], [530], 64, 1, 8, 256),
+           # and these with a tile's tokens split over workgroups
+           ([2600], [260], 64, 1, 16, 64), ([1500, 0, 900], [200, 0, 150], 16, 1, 12, 96), ([1300], [140], 32, 1, 30, 256),
+           ([2000], [129], 128, 1, 32, 32), ([1500, 1], [1, 400], 32, 1, 11, 128)]
 
 
 @pytest.mark.parametrize("lens,new,page,kvh,group,hd", ATTENDS)
@@ -226,7 +236,8 @@ def test_attention_over_absent_pages(dev, new, hd):
     if 0 not in used:
         p.o.k[0], p.o.v[0] = NAN, NAN
     p.upload()
-    N, H = int(p.offsets[-1]), 4
+    N = int(p.offsets[-1])
+    H = 12 if N > 400 else 4  # (12: tiles of 128 rows)
     q = _rows(rng, N, H, hd) / 64
     o = torch.full((N, H * hd), 5.0, device=dev)
     K.attn_paged(p.c, H, _cuda(q.reshape(N, -1), dev), o)
@@ -240,7 +251,8 @@ def test_attention_over_absent_pages(dev, new, hd):
 def test_attention_nan_reaches_the_rows_that_see_it(dev, new, hd):
     """NaN among a later token's keys or values does not reach the rows before it"""
     rng = np.random.default_rng(11)
-    lens, kvh, H, page = [90], 1, 2, 16
+    lens, kvh, page = [90], 1, 16
+    H = 32 if new == 150 else 2  # (150: tiles of 128 rows)
     for what in ("k", "v"):
         p = Pair(dev, rng, lens, [new], page, kvh, hd)
         t = 90 + new // 2  # this token's
