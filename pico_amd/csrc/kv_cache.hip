@@ -28,7 +28,7 @@ struct AppendArgs {
     int64_t ldk, ldv;
     RopeArgs rope;
     TurnArgs q;  // of the heads that a workgroup turns
-    int q_tokens, q_parts, q_heads, q_vec;
+    int q_tokens, q_parts, q_heads, q_even;
     unsigned q_blocks;
 };
 
@@ -187,15 +187,15 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, unsigned block
     q.y += h0 * q.hd;
     const int heads = q.H - h0 < a.q_heads ? q.H - h0 : a.q_heads;
     if(a.rope.interleaved)
-        a.q_vec ? turn_rows<4, true>(q, a.rope, t0, tokens, heads, where, tc, ts)
-                : turn_rows<1, true>(q, a.rope, t0, tokens, heads, where, tc, ts);
+        a.q_even ? turn_rows<true, true>(q, a.rope, t0, tokens, heads, where, tc, ts)
+                : turn_rows<false, true>(q, a.rope, t0, tokens, heads, where, tc, ts);
     else
-        a.q_vec ? turn_rows<4, false>(q, a.rope, t0, tokens, heads, where, tc, ts)
-                : turn_rows<1, false>(q, a.rope, t0, tokens, heads, where, tc, ts);
+        a.q_even ? turn_rows<true, false>(q, a.rope, t0, tokens, heads, where, tc, ts)
+                : turn_rows<false, false>(q, a.rope, t0, tokens, heads, where, tc, ts);
 }
 
 template <int THREADS>
-__global__ __launch_bounds__(THREADS) void append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(THREADS, 4) void append_kernel(AppendArgs a) {
     extern __shared__ __align__(16) float tile[];
     __shared__ float red[THREADS / kWave];
     // (queries first where a few tokens' workgroups all start at once, last where they are
@@ -244,18 +244,20 @@ extern "C" int pk_kv_append_f32(const PkKvCache* cache, int64_t N, const float* 
     const int threads = few ? 64 : 256;
     a.cap = few ? 4 : (int)page;
     a.halves = (unsigned)(tasks * kvh);
-    if(!grid_fits(2 * tasks * kvh + N * (q ? H : 1), threads))
-        return fail("pk_kv_append_f32: too many pages and heads for one launch");
+    int64_t q_blocks = 0;
     if(q) {
-        a.q_vec = turn_args(a.q, a.rope, H, hd, q, ldq, q_out, ldqo, 0);
+        a.q_even = turn_args(a.q, a.rope, H, hd, q, ldq, q_out, ldqo, 0);
         a.q_tokens = few ? 1 : turn_tokens(N, H, a.rope.half);
         // of a single token, as many heads as a wave turns with its loads in flight at once
         a.q_heads = few ? (int)(threads * kTurnUnits / a.q.per_head.d) : (int)H;
         a.q_heads = a.q_heads < 1 ? 1 : a.q_heads > H ? (int)H : a.q_heads;
         a.q_parts = (int)((H + a.q_heads - 1) / a.q_heads);
         a.q.per_token = div_by(a.q_heads);
-        a.q_blocks = (unsigned)((N + a.q_tokens - 1) / a.q_tokens * a.q_parts);
+        q_blocks = (N + a.q_tokens - 1) / a.q_tokens * a.q_parts;
     }
+    if(!grid_fits(2 * tasks * kvh + q_blocks, threads))
+        return fail("pk_kv_append_f32: too many pages and heads for one launch");
+    a.q_blocks = (unsigned)q_blocks;
     const unsigned blocks = a.q_blocks + 2 * a.halves;
     const size_t lds = sizeof(float) * a.hp * (a.cap + 5);
     if(few)

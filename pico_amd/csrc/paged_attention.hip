@@ -837,7 +837,7 @@ __global__ __launch_bounds__(256) void finish_kernel(AttnArgs a) {
     const float* base = a.ws + ((int64_t)rest * a.splits * kvh + h) * kManyPart<HP>;
     const int64_t apart = (int64_t)kvh * kManyPart<HP>;
     float top = kNone, total = 0.0f;
-    if(lane < a.splits) top = base[lane * apart + r];  // (at most 16)
+    if(lane < a.splits) top = base[lane * apart + r];  // (at most a lane each)
     top = wave_max(top);
     const int d = 4 * lane;
     f32x4 v = {};
@@ -865,22 +865,26 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
     Plan p = {};
     const int64_t group = H / c->kv_heads, units = (c->width * c->page + kUnit - 1) / kUnit;
     const int64_t some = c->B < N ? c->B : N;
-    // Tiles of 16 rows up to 96 rows a sequence on average, or 4096 of all heads together:
-    // tiles of 128 read the cache less often but are left partly empty, and are less finely
-    // shared out.  32 heads on 8 of 128 values: 16 sequences of 4000 tokens with up to 16 new
-    // ones 47 against 76 us, with up to 40 82 against 92, with up to 60 119 against 116; one
-    // sequence with 128 new ones 38 against 43.  12 heads of 64: 4 sequences of 1000 tokens
-    // with up to 128 new ones 11 against 26.
-    p.rows = N * group <= 96 * c->B || N * H <= 4096 ? kFew : kRows;
+    // Tiles of 16 rows up to 96 rows a sequence on average, or 4096 of all heads together
+    // (8192 over up to 2048 tokens): tiles of 128 read the cache less often but are left
+    // partly empty, and are less finely shared out.  32 heads on 8 of 128 values: 16
+    // sequences of 4000 tokens with up to 40 new ones 82 against 92 us, with up to 60 119
+    // against 116; one of 500 tokens with 128 new ones 11 against 33, of 300 with 256 16
+    // against 30, with 1024 81 against 63; one of 4000 with 256 61 against 59.
+    p.rows = N * group <= 96 * c->B || N * H <= (units <= 32 ? 8192 : 4096) ? kFew : kRows;
     p.tiles = N * group / p.rows + some;
     if(p.rows < kRows) {
         p.W = units <= (c->hd <= 128 ? 32 : 16) || p.tiles * c->kv_heads * units >= (int64_t)1 << 31 ? 0 : 256;
     } else {
-        // workgroups that there are for sure, two to a CU, of 8 units at least
+        // The workgroups that there are for sure: one to a CU where they get 4 units each, two
+        // where they get 8.  One sequence of 32000 tokens with 64 new ones, 3 heads of 168: 63
+        // parts a tile 65 us, 16 168; of 2000 tokens with 256, 8 parts 36, 4 57.
         const int64_t sure = (N * group + kRows - 1) / kRows * c->kv_heads;
-        int64_t n = 512 / sure;
-        if(n > units / 8) n = units / 8;
-        p.splits = (int)(n < 1 ? 1 : n > 16 ? 16 : n);
+        auto parts = [&](int64_t blocks, int64_t each) {
+            return blocks / sure < units / each ? blocks / sure : units / each;
+        };
+        const int64_t one = parts(256, 4), two = parts(512, 8), n = one > two ? one : two;
+        p.splits = (int)(n < 1 ? 1 : n > kWave ? kWave : n);
     }
     return p;
 }
@@ -939,7 +943,7 @@ extern "C" int pk_attn_paged_f32(const PkKvCache* cache, int64_t N, int64_t H, f
     if(need && (!workspace || workspace_bytes < need || !aligned16(workspace)))
         return fail("pk_attn_paged_f32: workspace of %zu bytes, %zu needed, 16-byte aligned",
                     workspace ? workspace_bytes : 0, need);
-    if(!grid_fits(p.tiles * cache->kv_heads * (p.splits > 1 ? p.splits : 1), 512))
+    if(!p.W && !grid_fits(p.tiles * cache->kv_heads * (p.splits > 1 ? p.splits : 1), 256))
         return fail("pk_attn_paged_f32: too many rows for one launch");
     AttnArgs a = {};
     a.c = *cache;

@@ -32,8 +32,7 @@ __device__ __forceinline__ void rope_turn(float& x1, float& x2, float c, float s
     x2 = x2 * c + x1 * s;
     x1 = y1;
 }
-template <class V>
-__device__ __forceinline__ void turn(V& a, int i, V& b, int j, float c, float s) {
+__device__ __forceinline__ void turn(f32x4& a, int i, f32x4& b, int j, float c, float s) {
     float p = a[i], q = b[j];
     rope_turn(p, q, c, s);
     a[i] = p;
@@ -62,51 +61,97 @@ struct TurnArgs {
     int back, accum;
 };
 
+typedef float f32x4_anywhere __attribute__((ext_vector_type(4), aligned(4)));
+// 4 values of a row of n from `at` on, or those that there are; any of the row in their
+// place behind them
+__device__ __forceinline__ f32x4 ld_in_row(const float* row, int at, int n) {
+    return __builtin_nontemporal_load((const f32x4_anywhere*)(row + (at < n - 4 ? at : n - 4)));
+}
+__device__ __forceinline__ f32x4 from_window(f32x4 v, int at, int n) {
+    const int behind = at - (n - 4);
+    if(behind > 0) {
+        if(behind & 1) v = f32x4{v[1], v[2], v[3], v[3]};
+        if(behind & 2) v = f32x4{v[2], v[3], v[3], v[3]};
+    }
+    return v;
+}
+__device__ __forceinline__ void st_first(float* to, f32x4 v, int n) {
+    if(n >= 4) {
+        __builtin_nontemporal_store((f32x4_anywhere)v, (f32x4_anywhere*)to);
+    } else {
+#pragma unroll
+        for(int k = 0; k < 3; ++k)
+            if(k < n) to[k] = v[k];
+    }
+}
+
 // One workgroup: the sines and cosines of the tokens' angles once, in LDS, for all heads;
-// then units of 8 values (V = 4: two float4 of a head, neighbouring threads' side by side)
-// or of a pair (V = 1), four in flight a thread, those of the first round loaded before the angles.  where(t, pos): the
-// position of token t0 + t; false leaves the row.
-template <int V, bool INTER, class P>
+// then units of 8 values, two times 4 in a row of a head, neighbouring threads' side by
+// side: pairs of the first half with those of the second, or what is next to each other.
+// Four units are in flight a thread, those of the first round loaded before the angles.
+// EVEN: head, halves and strides are multiples of 4 and aligned.  Where they are not, a
+// part's last 4 may be fewer; all are loaded as 4, and without a branch, so
+// that none is waited for before the others are issued (8192 tokens of 12 heads of 80, 20
+// turned: 44 us both ways, pair by pair 69; 25 at the rate of a copy).  where(t, pos): the position of token t0 + t; false leaves the row.
+template <bool EVEN, bool INTER, class P>
 __device__ __forceinline__ void turn_rows(const TurnArgs& g, const RopeArgs& r, int64_t t0,
                                           int tokens, int heads, P where, float* tc, float* ts) {
-    typedef float vec __attribute__((ext_vector_type(V)));
-    const int half = r.half, rot = 2 * half, threads = blockDim.x;
-    const int total = tokens * g.per_token.d * g.per_head.d;
-    constexpr int U = kTurnUnits;
+    const int half = r.half, rot = 2 * half, threads = blockDim.x, turned = (half + 3) / 4;
+    const int total = tokens * g.per_token.d * g.per_head.d, row = heads * g.hd;
+    if(!EVEN && row < 4) {  // (too short to load 4)
+        for(int t = threadIdx.x; t < tokens; t += threads) {
+            int pos;
+            if(!where(t, pos)) continue;
+            const float* x = g.x + (t0 + t) * g.ldx;
+            float* y = g.y + (t0 + t) * g.ldy;
+            for(int i = 0; i < row; ++i) {
+                // (the only pair of such a head is of its first two)
+                const int d = i % g.hd;
+                float a = x[i], b = 0.0f;
+                if(d < rot) {
+                    float c, s;
+                    rope_angle(pos, r.freqs[0], r.magnitude, c, s);
+                    b = x[++i];
+                    rope_turn(a, b, c, g.back ? -s : s);
+                    y[i] = g.accum ? y[i] + b : b;
+                }
+                float* to = y + (d < rot ? i - 1 : i);
+                *to = g.accum ? *to + a : a;
+            }
+        }
+        return;
+    }
+    constexpr int U = EVEN ? kTurnUnits : kTurnUnits / 2;  // (the windows' selections take registers)
     for(int base = 0; base < total; base += threads * U) {
-        vec a[U], b[U];
-        int tok[U], at[U], da[U], db[U];  // where a and b are in their head; db < 0: no b
+        f32x4 a[U], b[U];
+        // where a and b are in their head, and of how many values (b of none, where nb < 1)
+        int tok[U], at[U], da[U], db[U], na[U], nb[U];
 #pragma unroll
         for(int i = 0; i < U; ++i) {
             const int u = base + i * threads + (int)threadIdx.x;
             tok[i] = -1;
             int pos;
-            if(u >= total) continue;
-            const int hr = g.per_head.of(u), j = u - hr * g.per_head.d, t = g.per_token.of(hr);
-            const int h = hr - t * g.per_token.d;
-            if(h >= heads || !where(t, pos)) continue;
-            tok[i] = t;
+            if(EVEN && u >= total) continue;
+            const int hr = g.per_head.of(u < total ? u : 0), j = u - hr * g.per_head.d;
+            const int t = tokens == 1 ? 0 : g.per_token.of(hr), h = hr - t * g.per_token.d;
+            const bool there = u < total && h < heads && where(t, pos);
+            if(EVEN && !there) continue;
+            if(there) tok[i] = t;
             at[i] = h * g.hd;
-            if(V == 4) {
-                if(INTER || 8 * j >= rot) {
-                    const int from = INTER ? 0 : rot, k = INTER ? j : j - rot / 8;
-                    da[i] = from + 4 * k;
-                    db[i] = da[i] + (g.hd - from + 7) / 8 * 4;
-                    if(db[i] >= g.hd) db[i] = -1;
-                } else {
-                    da[i] = 4 * j;
-                    db[i] = 4 * j + half;
-                }
-            } else if(j < half) {
-                da[i] = INTER ? 2 * j : j;
-                db[i] = INTER ? 2 * j + 1 : j + half;
+            const bool pairs = !INTER && j < turned;  // of the first half and the second
+            const int from = INTER ? 0 : rot, k = INTER ? j : j - turned;
+            da[i] = pairs ? 4 * j : from + 4 * k;
+            db[i] = da[i] + (pairs ? half : (g.hd - from + 7) / 8 * 4);
+            na[i] = (pairs ? half : g.hd) - da[i];
+            nb[i] = (pairs ? rot : g.hd) - db[i];
+            const float* p = g.x + (t0 + t) * g.ldx;
+            if(EVEN) {
+                a[i] = ld_stream((const f32x4*)(p + at[i] + da[i]));
+                if(nb[i] > 0) b[i] = ld_stream((const f32x4*)(p + at[i] + db[i]));
             } else {
-                da[i] = j + half;
-                db[i] = -1;
+                a[i] = ld_in_row(p, there ? at[i] + da[i] : 0, row);
+                b[i] = ld_in_row(p, there ? at[i] + db[i] : 0, row);
             }
-            const float* p = g.x + (t0 + t) * g.ldx + at[i];
-            a[i] = ld_stream((const vec*)(p + da[i]));
-            if(db[i] >= 0) b[i] = ld_stream((const vec*)(p + db[i]));
         }
         if(base == 0) {
             for(int e = threadIdx.x; e < tokens * half; e += threads) {
@@ -124,34 +169,42 @@ __device__ __forceinline__ void turn_rows(const TurnArgs& g, const RopeArgs& r, 
         for(int i = 0; i < U; ++i) {
             if(tok[i] < 0) continue;
             const float *c = tc + tok[i] * half, *s = ts + tok[i] * half;
-            if constexpr(V == 4) {
-                if(INTER) {
-                    if(da[i] < rot) {
-                        const int e = da[i] / 2;
-                        turn(a[i], 0, a[i], 1, c[e], s[e]);
-                        turn(a[i], 2, a[i], 3, c[e + 1], s[e + 1]);
-                    }
-                    if(db[i] >= 0 && db[i] < rot) {
-                        const int e = db[i] / 2;
-                        turn(b[i], 0, b[i], 1, c[e], s[e]);
-                        turn(b[i], 2, b[i], 3, c[e + 1], s[e + 1]);
-                    }
-                } else if(da[i] < half) {
-                    const int e = da[i];
+            if(!EVEN) {
+                a[i] = from_window(a[i], at[i] + da[i], row);
+                b[i] = from_window(b[i], at[i] + db[i], row);
+            }
+            if(INTER) {
 #pragma unroll
-                    for(int q = 0; q < 4; ++q) turn(a[i], q, b[i], q, c[e + q], s[e + q]);
+                for(int k = 0; k < 4; k += 2) {
+                    const int e = (da[i] + k) / 2, f = (db[i] + k) / 2;
+                    if(da[i] + k < rot) turn(a[i], k, a[i], k + 1, c[e], s[e]);
+                    if(db[i] + k < rot) turn(b[i], k, b[i], k + 1, c[f], s[f]);
                 }
-            } else if(db[i] >= 0) {
-                const int e = INTER ? da[i] / 2 : da[i];
-                turn(a[i], 0, b[i], 0, c[e], s[e]);
+            } else if(da[i] < half) {
+                const int e = da[i];
+#pragma unroll
+                for(int k = 0; k < 4; ++k)
+                    if(EVEN || k < na[i]) turn(a[i], k, b[i], k, c[e + k], s[e + k]);
             }
-            float* p = g.y + (t0 + tok[i]) * g.ldy + at[i];
-            if(g.accum) {
-                a[i] += *(const vec*)(p + da[i]);
-                if(db[i] >= 0) b[i] += *(const vec*)(p + db[i]);
+            float *pa = g.y + (t0 + tok[i]) * g.ldy + at[i] + da[i], *pb = pa + (db[i] - da[i]);
+            if(EVEN) {
+                if(g.accum) {
+                    a[i] += *(const f32x4*)pa;
+                    if(nb[i] > 0) b[i] += *(const f32x4*)pb;
+                }
+                st_stream((f32x4*)pa, a[i]);
+                if(nb[i] > 0) st_stream((f32x4*)pb, b[i]);
+            } else {
+                if(g.accum) {
+#pragma unroll
+                    for(int k = 0; k < 4; ++k) {
+                        if(k < na[i]) a[i][k] += pa[k];
+                        if(k < nb[i]) b[i][k] += pb[k];
+                    }
+                }
+                st_first(pa, a[i], na[i]);
+                st_first(pb, b[i], nb[i]);
             }
-            st_stream((vec*)(p + da[i]), a[i]);
-            if(db[i] >= 0) st_stream((vec*)(p + db[i]), b[i]);
         }
     }
 }
@@ -163,18 +216,19 @@ inline RopeArgs rope_args(const PkRope* r) {
     if(!r) return {nullptr, 0, 0, 1.0};
     return {r->freqs, (int)(r->rot / 2), r->interleaved != 0, r->magnitude};
 }
-// whether a row is turned in float4, and the arguments for that
+// the arguments, and whether all is multiples of 4 and aligned
 inline bool turn_args(TurnArgs& g, const RopeArgs& r, int64_t H, int64_t hd, const float* x,
                       int64_t ldx, float* y, int64_t ldy, int flags) {
     const int rot = 2 * r.half;
-    const bool vec = hd % 4 == 0 && rot % (r.interleaved ? 4 : 8) == 0 && ldx % 4 == 0 &&
-                     ldy % 4 == 0 && aligned16(x) && aligned16(y);
-    g = {x, y, ldx, ldy, (int)H, (int)hd, div_by(vec ? (hd + 7) / 8 : hd - r.half), div_by(H),
+    g = {x, y, ldx, ldy, (int)H, (int)hd,
+         div_by(r.interleaved ? (hd + 7) / 8 : (r.half + 3) / 4 + (hd - rot + 7) / 8), div_by(H),
          (flags & PK_ROPE_BACKWARD) != 0, (flags & PK_ACCUM) != 0};
-    return vec;
+    return hd % 4 == 0 && rot % (r.interleaved ? 4 : 8) == 0 && ldx % 4 == 0 && ldy % 4 == 0 &&
+           aligned16(x) && aligned16(y);
 }
 // tokens a workgroup turns: as many as share a table, fewer where that leaves less than two
-// workgroups to a CU, and one where the index arithmetic would pass 2^36
+// workgroups to a CU, and one of many heads, whose
+// index arithmetic would pass 2^36
 inline int turn_tokens(int64_t N, int64_t H, int half) {
     int T = half ? kTurnTable / 2 / half : 8;
     T = T < 1 || H > 4096 ? 1 : T > 8 ? 8 : T;

@@ -11,12 +11,12 @@ using namespace pk;
 constexpr int kThreads = 256;
 
 // bound by HBM: x read and y written once; a token's angles are shared by its heads
-template <int V, bool INTER>
+template <bool EVEN, bool INTER>
 __global__ __launch_bounds__(kThreads) void rope_kernel(int64_t N, int T, TurnArgs g, RopeArgs r,
                                                         const int32_t* __restrict__ positions) {
     __shared__ __align__(16) float tc[kTurnTable], ts[kTurnTable];
     const int64_t t0 = (int64_t)blockIdx.x * T;
-    turn_rows<V, INTER>(
+    turn_rows<EVEN, INTER>(
         g, r, t0, (int)(N - t0 < T ? N - t0 : T), g.H,
         [&](int t, int& pos) {
             pos = positions[t0 + t];
@@ -67,13 +67,13 @@ extern "C" int pk_rope_f32(int64_t N, int64_t H, int64_t hd, const PkRope* rope,
         return fail("pk_rope_f32: row strides must be at least H*hd = %lld", (long long)(H * hd));
     const RopeArgs r = rope_args(rope);
     TurnArgs g;
-    const bool vec = turn_args(g, r, H, hd, x, ldx, y, ldy, flags);
+    const bool even = turn_args(g, r, H, hd, x, ldx, y, ldy, flags);
     const int T = turn_tokens(N, H, r.half);
     const unsigned grid = (unsigned)((N + T - 1) / T);
     auto go = [&](auto kernel) { kernel<<<grid, kThreads, 0, as_stream(stream)>>>(N, T, g, r, positions); };
     if(r.interleaved)
-        vec ? go(rope_kernel<4, true>) : go(rope_kernel<1, true>);
+        even ? go(rope_kernel<true, true>) : go(rope_kernel<false, true>);
     else
-        vec ? go(rope_kernel<4, false>) : go(rope_kernel<1, false>);
+        even ? go(rope_kernel<true, false>) : go(rope_kernel<false, false>);
     return launch_status("pk_rope_f32");
 }

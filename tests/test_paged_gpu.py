@@ -55,7 +55,9 @@ def _rows(rng, N, heads, hd):
 APPENDS = [([0], [1], 16, 1, 64), ([0, 5, 16], [1, 1, 1], 16, 2, 64), ([3, 0, 15, 31], [0, 40, 1, 17], 16, 3, 80),
            ([63, 64, 100], [1, 1, 200], 64, 2, 128), ([7, 127], [121, 2], 128, 2, 256), ([1], [300], 32, 1, 96),
            ([5] * 70, [i % 4 for i in range(70)], 16, 1, 32), ([9, 2], [3, 30], 32, 2, 7), ([0] * 3, [0, 0, 0], 16, 1, 32),
-           ([12], [129], 128, 1, 33), ([2], [1], 128, 16, 64)]
+           ([12], [129], 128, 1, 33), ([2], [1], 128, 16, 64),
+           # many tokens of one sequence among others that wait
+           ([5] + [0] * 99, [70] + [0] * 99, 64, 2, 64), ([37] + [3] * 40, [60] + [0] * 39 + [1], 16, 1, 256)]
 
 
 @pytest.mark.parametrize("lens,new,page,kvh,hd", APPENDS)
@@ -115,6 +117,23 @@ def test_append_one_by_one_and_at_once(dev):
         assert (a == b)[np.abs(a) >= 2.0 ** -6].all()
 
 
+def test_append_of_many_rows(dev):
+    """a million rows, whose queries have more heads than a launch has workgroups"""
+    N, H, page = 1 << 20, 32, 128
+    pages = N // page
+    pool = K.kv_pool(pages, 1, page, 1, dev)
+    table = torch.arange(pages, device=dev, dtype=torch.int32).view(1, -1)
+    c = K.PagedKV(*pool, table, _i32([0], dev), _i32([0, N], dev), 1)
+    k = torch.ones(N, 1, device=dev)
+    q = torch.arange(N * H, device=dev, dtype=torch.float32).view(N, H)
+    out = torch.zeros_like(q)
+    K.kv_append(c, k, 3 * k, None, H=H, q=q, q_out=out)
+    assert torch.equal(out, q)
+    one = torch.tensor(1.0).to(torch.float8_e4m3fn)
+    for x, e, want in ((pool[0][:, 0, :, 0], pool[2], 1.0), (pool[1][:, 0, 0, :], pool[3], 3.0)):
+        assert (x.view(one.dtype).float() * torch.exp2(e.float() - 127) == want).all()
+
+
 def test_append_odd_values(dev):
     rng = np.random.default_rng(4)
     p = Pair(dev, rng, [5], [12], 16, 2, 64)
@@ -171,11 +190,12 @@ ATTENDS = [([0], [1], 16, 1, 1, 64), ([1, 15, 16, 17], [1, 1, 1, 1], 16, 2, 1, 6
            ([2200, 1, 0, 900], [1, 1, 0, 2], 128, 1, 1, 32), ([3000], [1], 64, 1, 16, 128), ([1500], [5], 16, 1, 7, 256),
            ([20] * 66 + [2100], [1] * 67, 128, 1, 4, 128), ([3000], [40], 64, 1, 4, 64),
            # tiles of 128 rows
-           ([0], [700], 64, 2, 3, 64), ([40, 0, 7], [333, 0, 400], 16, 1, 6, 128), ([5], [530], 32, 1, 8, 33),
-           ([300], [1040], 128, 4, 1, 96), ([77, 3], [500, 20], 16, 2, 4, 80), ([0], [530], 64, 1, 8, 256),
+           ([0], [700], 64, 2, 6, 64), ([40, 0, 7], [333, 0, 400], 16, 1, 12, 128), ([5], [530], 32, 1, 16, 33),
+           ([300], [1040], 128, 8, 1, 96), ([77, 3], [500, 20], 16, 2, 8, 80), ([0], [530], 64, 1, 16, 256),
            # and these with a tile's tokens split over workgroups
-           ([2600], [260], 64, 1, 16, 64), ([1500, 0, 900], [200, 0, 150], 16, 1, 12, 96), ([1300], [140], 32, 1, 30, 256),
-           ([2000], [129], 128, 1, 32, 32), ([1500, 1], [1, 400], 32, 1, 11, 128)]
+           ([2600], [260], 64, 1, 16, 64), ([1500, 0, 900], [200, 0, 150], 16, 1, 24, 96), ([1300], [140], 32, 1, 60, 256),
+           ([2000], [129], 128, 1, 32, 32), ([1500, 1], [1, 400], 32, 1, 21, 128),
+           ([9000], [65], 128, 1, 64, 32)]
 
 
 @pytest.mark.parametrize("lens,new,page,kvh,group,hd", ATTENDS)
@@ -237,7 +257,7 @@ def test_attention_over_absent_pages(dev, new, hd):
         p.o.k[0], p.o.v[0] = NAN, NAN
     p.upload()
     N = int(p.offsets[-1])
-    H = 12 if N > 400 else 4  # (12: tiles of 128 rows)
+    H = 24 if N > 400 else 4  # (24: tiles of 128 rows)
     q = _rows(rng, N, H, hd) / 64
     o = torch.full((N, H * hd), 5.0, device=dev)
     K.attn_paged(p.c, H, _cuda(q.reshape(N, -1), dev), o)

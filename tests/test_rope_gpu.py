@@ -38,7 +38,9 @@ SHAPES = [(1, 1, 2, 2, False, 1, "none"), (1, 12, 64, 64, False, 9, "none"), (64
           (20, 3, 7, 4, False, 50, "none"), (20, 3, 7, 6, True, 50, "none"), (9, 2, 50, 50, False, 50, "none"),
           (5, 2, 256, 256, False, 4096, "none"), (3, 1, 1024, 1024, False, 999, "none"), (3, 2, 1000, 6, True, 9, "none"),
           (17, 2, 64, 0, False, 9, "none"), (5000, 4, 32, 32, True, 3000, "none"), (1030, 24, 64, 64, False, 1024, "none"),
-          (2, 5000, 8, 8, False, 4, "none")]
+          (2, 5000, 8, 8, False, 4, "none"), (40, 3, 50, 22, False, 900, "none"), (11, 5, 130, 6, True, 900, "none"),
+          (9, 4, 19, 10, True, 40, "none"), (700, 6, 128, 6, False, 900, "none"), (2, 524287, 2, 2, False, 9, "none"),
+          (3, 349525, 3, 2, True, 9, "none")]
 
 
 @pytest.mark.parametrize("N,H,hd,rot,inter,far,scaling", SHAPES)
@@ -79,15 +81,16 @@ def test_backward_is_the_transpose(dev):
     assert abs(num - want) <= 2.0 ** -18 * (dy.double().abs() * y.double().abs()).sum() / h
 
 
+@pytest.mark.parametrize("H,hd,rot", [(4, 64, 48), (4, 64, 6), (3, 45, 10)])
 @pytest.mark.parametrize("inter", [False, True])
-def test_layouts_accumulation_and_place(dev, inter):
-    N, H, hd, rot = 37, 4, 64, 48
+def test_layouts_accumulation_and_place(dev, inter, H, hd, rot):
+    N = 37
     g = torch.Generator(device=dev).manual_seed(5)
     wide = torch.randn(N, 3 * H * hd + 2, device=dev, generator=g)
     pos = torch.randint(0, 9999, (N,), device=dev, dtype=torch.int32, generator=g)
     r = K.Rope(K.rope_freqs(rot, device=dev), inter)
     want = torch.empty(N, H * hd, device=dev)
-    for off in (0, H * hd, H * hd + 1):  # (the last: not 16-byte aligned, the scalar kernel)
+    for off in (0, H * hd, H * hd + 1):  # (the last: not 16-byte aligned)
         x = wide[:, off:off + H * hd]
         K.rope(r, H, x.contiguous(), pos, want)
         out = torch.full_like(wide, 3.0)
