@@ -59,28 +59,31 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, unsigned task, 
 
     const int half = IS_V ? 0 : a.rope.half, pairs = hp / 2, apart = pairs - half;
     const int stride = IS_V ? a.cap + 5 : hp;
-    // pair e of the tokens from slot s0 + t0 on: where its values are in the head
+    // a thread has one pair of a head (one of each 64, where heads have more and threads are
+    // few), of every `abreast`th token
+    constexpr int U = THREADS == kWave ? 1 : 4;  // tokens in flight
+    const int across = pairs < THREADS ? pairs : THREADS, abreast = THREADS / across;
+    const int my_t = (int)threadIdx.x / across, my_p = (int)threadIdx.x - my_t * across;
     struct Pair {
-        int t, p, d1, d2;
+        int d1, d2;
     };
-    auto pair_of = [&](int e) {
-        Pair q;
-        q.t = e / pairs;
-        q.p = e - q.t * pairs;
-        const bool turned = q.p < half;
-        q.d1 = turned ? (a.rope.interleaved ? 2 * q.p : q.p) : half + q.p;
-        q.d2 = turned ? (a.rope.interleaved ? q.d1 + 1 : q.p + half) : half + q.p + apart;
-        return q;
+    auto pair_of = [&](int p) {
+        const bool turned = p < half;
+        const int d1 = turned ? (a.rope.interleaved ? 2 * p : p) : half + p;
+        return Pair{d1, turned ? (a.rope.interleaved ? d1 + 1 : p + half) : half + p + apart};
     };
-    float x1 = 0.0f, x2 = 0.0f, amax = 0.0f;
-    auto load = [&](int e, int t0) {
-        const Pair q = pair_of(e);
-        const float* r = src + (int64_t)(t0 + q.t) * ld;
-        x1 = q.d1 < hd ? r[q.d1] : 0.0f;
-        x2 = q.d2 < hd ? r[q.d2] : 0.0f;
+    float x1[U], x2[U], amax = 0.0f;
+    auto load = [&](const Pair& q, int t, int end) {
+#pragma unroll
+        for(int k = 0; k < U; ++k) {
+            const float* r = src + (int64_t)(t + k * abreast) * ld;
+            const bool there = t + k * abreast < end;
+            x1[k] = there && q.d1 < hd ? r[q.d1] : 0.0f;
+            x2[k] = there && q.d2 < hd ? r[q.d2] : 0.0f;
+        }
     };
     const int n = s1 - s0, parts = (n + a.cap - 1) / a.cap;
-    if((int)threadIdx.x < (n < a.cap ? n : a.cap) * pairs) load(threadIdx.x, 0);  // (beside the page's number)
+    if(my_t < abreast) load(pair_of(my_p), my_t, n < a.cap ? n : a.cap);  // (beside the page's number)
     if(name < 0 || name >= c.pages) return;
     const int64_t at = (int64_t)name * c.kv_heads + h;
     uint8_t* exps = (IS_V ? c.v_exp : c.k_exp) + at;
@@ -93,20 +96,35 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, unsigned task, 
         const int t0 = (i < parts ? i : i - parts) * a.cap, tokens = n - t0 < a.cap ? n - t0 : a.cap;
         const int c0 = s0 + t0, c1 = c0 + tokens;  // slots
         if(i) __syncthreads();
-        for(int j = threadIdx.x; j < tokens * pairs; j += THREADS) {
-            if(i || j >= THREADS) load(j, t0);
-            const Pair q = pair_of(j);
-            if(q.p < half) {
-                float co, si;
-                rope_angle(p0 + t0 + q.t, a.rope.freqs[q.p], a.rope.magnitude, co, si);
-                rope_turn(x1, x2, co, si);
+        for(int p = my_t < abreast ? my_p : pairs; p < pairs; p += across) {
+            const Pair q = pair_of(p);
+            // the angle of the next token `abreast` on by the angles' sum, in 64 bits too: 64 of
+            // these are off by 2^-46
+            double c = 0.0, s = 0.0, cs = 0.0, ss = 0.0;
+            if(p < half) {
+                rope_turns(p0 + t0 + my_t, a.rope.freqs[p], c, s);
+                if(my_t + abreast < tokens) rope_turns(abreast, a.rope.freqs[p], cs, ss);
             }
-            const float m1 = fabsf(x1), m2 = fabsf(x2);
-            if(m1 <= 3.402823466e38f) amax = fmaxf(amax, m1);  // (not infinities or NaN)
-            if(m2 <= 3.402823466e38f) amax = fmaxf(amax, m2);
-            // (v's columns are at their slots from a multiple of 4 on, so that words line up)
-            tile[IS_V ? q.d1 * stride + c0 % 4 + q.t : q.t * stride + q.d1] = x1;
-            tile[IS_V ? q.d2 * stride + c0 % 4 + q.t : q.t * stride + q.d2] = x2;
+            for(int t = my_t; t < tokens; t += U * abreast) {
+                if(i || t > my_t || p > my_p) load(q, t0 + t, t0 + tokens);
+#pragma unroll
+                for(int k = 0; k < U; ++k) {
+                    const int now = t + k * abreast;
+                    if(now >= tokens) break;
+                    if(p < half) {
+                        rope_turn(x1[k], x2[k], (float)(c * a.rope.magnitude), (float)(s * a.rope.magnitude));
+                        const double next = c * cs - s * ss;
+                        s = s * cs + c * ss;
+                        c = next;
+                    }
+                    const float m1 = fabsf(x1[k]), m2 = fabsf(x2[k]);
+                    if(m1 <= 3.402823466e38f) amax = fmaxf(amax, m1);  // (not infinities or NaN)
+                    if(m2 <= 3.402823466e38f) amax = fmaxf(amax, m2);
+                    // (v's columns are at their slots from a multiple of 4 on, so that words line up)
+                    tile[IS_V ? q.d1 * stride + c0 % 4 + now : now * stride + q.d1] = x1[k];
+                    tile[IS_V ? q.d2 * stride + c0 % 4 + now : now * stride + q.d2] = x2[k];
+                }
+            }
         }
         if(i == parts - 1) {
             amax = block_max<THREADS / kWave>(amax, red);

@@ -16,10 +16,13 @@ struct RopeArgs {
 // m cos a and m sin a of a = pos f.  In 64 bits up to the last rounding: a position of
 // 2^20 leaves a product in 32 bits off by 2^-4 radians.  The angle is taken as turns, so
 // that its whole part drops out exactly.
-__device__ __forceinline__ void rope_angle(int pos, double f, double m, float& c, float& s) {
+__device__ __forceinline__ void rope_turns(int pos, double f, double& c, double& s) {
     const double turns = (double)pos * f * 0.15915494309189533577;
+    sincospi(2.0 * (turns - rint(turns)), &s, &c);
+}
+__device__ __forceinline__ void rope_angle(int pos, double f, double m, float& c, float& s) {
     double ds, dc;
-    sincospi(2.0 * (turns - rint(turns)), &ds, &dc);
+    rope_turns(pos, f, dc, ds);
     c = (float)(dc * m);
     s = (float)(ds * m);
 }
