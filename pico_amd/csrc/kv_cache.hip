@@ -36,7 +36,10 @@ struct AppendArgs {
 // workgroup, which turns the new values on their way to LDS, finds the largest of them, and
 // writes their codes from there, in words of 4: k's rows are the tokens', v's the columns.
 // Where the tile holds fewer tokens than are new, the values are read twice.
-template <bool IS_V, int THREADS>
+// Prompts are bound by HBM: 12288 tokens of 8 heads of 128, with 32 heads of queries, 108 us
+// (4.9 TB/s).  Single tokens are bound by the way to the page, lengths, its number, its
+// power: 64 tokens 6 us.
+template <bool IS_V, int THREADS, int U>
 __device__ __forceinline__ void append_page(const AppendArgs& a, unsigned task, int h, float* tile,
                                             float* red) {
     const PkKvCache& c = a.c;
@@ -60,8 +63,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, unsigned task, 
     const int half = IS_V ? 0 : a.rope.half, pairs = hp / 2, apart = pairs - half;
     const int stride = IS_V ? a.cap + 5 : hp;
     // a thread has one pair of a head (one of each 64, where heads have more and threads are
-    // few), of every `abreast`th token
-    constexpr int U = THREADS == kWave ? 1 : 4;  // tokens in flight
+    // few), of every `abreast`th token, U of them in flight
     const int across = pairs < THREADS ? pairs : THREADS, abreast = THREADS / across;
     const int my_t = (int)threadIdx.x / across, my_p = (int)threadIdx.x - my_t * across;
     struct Pair {
@@ -212,18 +214,18 @@ __device__ __forceinline__ void turn_queries(const AppendArgs& a, unsigned block
                 : turn_rows<false, false>(q, a.rope, t0, tokens, heads, where, tc, ts);
 }
 
-template <int THREADS>
+template <int THREADS, int U>
 __global__ __launch_bounds__(THREADS, 4) void append_kernel(AppendArgs a) {
     extern __shared__ __align__(16) float tile[];
     __shared__ float red[THREADS / kWave];
     // (queries first where a few tokens' workgroups all start at once, last where they are
     // waited for in turn)
     const unsigned heads = (unsigned)a.c.kv_heads, pages = 2 * a.halves;
-    const unsigned block = THREADS == kWave ? (blockIdx.x + pages) % (pages + a.q_blocks) : blockIdx.x;
+    const unsigned block = U == 1 ? (blockIdx.x + pages) % (pages + a.q_blocks) : blockIdx.x;
     if(block >= pages) return turn_queries<THREADS>(a, block - pages);
     if(block < a.halves)
-        return append_page<false, THREADS>(a, block / heads, (int)(block % heads), tile, red);
-    append_page<true, THREADS>(a, (block - a.halves) / heads, (int)((block - a.halves) % heads), tile, red);
+        return append_page<false, THREADS, U>(a, block / heads, (int)(block % heads), tile, red);
+    append_page<true, THREADS, U>(a, (block - a.halves) / heads, (int)((block - a.halves) % heads), tile, red);
 }
 
 }  // namespace
@@ -256,11 +258,16 @@ extern "C" int pk_kv_append_f32(const PkKvCache* cache, int64_t N, const float* 
     const int64_t page = cache->page, kvh = cache->kv_heads;
     // a sequence with n > 0 new tokens writes to at most n pages, and n / page + 2
     const int64_t tasks = N < N / page + 2 * cache->B ? N : N / page + 2 * cache->B;
-    // up to 2 tokens a sequence, as tokens are generated: a wave to a page's head, and a
-    // tile of 4 tokens, so that all of a step's workgroups have room at once
-    const bool few = N <= 2 * cache->B;
-    const int threads = few ? 64 : 256;
-    a.cap = few ? 4 : (int)page;
+    // Up to 2 tokens a sequence, as tokens are generated: a wave to a page's head, and a tile
+    // of 4 tokens, so that all of a step's workgroups have room at once.  Of prompts, whose
+    // workgroups take turns: a wave too for pages of 16, most of whose time is the way to the
+    // page (8192 tokens, 8 and 16 heads of 64: 45 to 32 us; of 128: 59 to 54; 640 tokens: 7 and
+    // 8 to 10); and pages of 128 with heads of 256, which would be alone on a CU, in quarters,
+    // read twice (152 to 106 us; few of them in halves).
+    const bool few = N <= 2 * cache->B, turns = 2 * tasks * kvh > 1024;
+    const bool wave = few || (turns && page == 16 && a.hp <= 128);
+    const int threads = wave ? 64 : 256;
+    a.cap = few ? 4 : page * a.hp <= 16384 ? (int)page : (turns ? 8192 : 16384) / a.hp;
     a.halves = (unsigned)(tasks * kvh);
     int64_t q_blocks = 0;
     if(q) {
@@ -279,8 +286,10 @@ extern "C" int pk_kv_append_f32(const PkKvCache* cache, int64_t N, const float* 
     const unsigned blocks = a.q_blocks + 2 * a.halves;
     const size_t lds = sizeof(float) * a.hp * (a.cap + 5);
     if(few)
-        append_kernel<64><<<blocks, 64, lds, as_stream(stream)>>>(a);
+        append_kernel<64, 1><<<blocks, 64, lds, as_stream(stream)>>>(a);
+    else if(wave)
+        append_kernel<64, 4><<<blocks, 64, lds, as_stream(stream)>>>(a);
     else
-        append_kernel<256><<<blocks, 256, lds, as_stream(stream)>>>(a);
+        append_kernel<256, 4><<<blocks, 256, lds, as_stream(stream)>>>(a);
     return launch_status("pk_kv_append_f32");
 }

@@ -227,6 +227,13 @@ constexpr int kPart = kFew * (HP + 2);
 // of a workgroup's share in its place 0, the one at the end in place 1.
 // Loads are issued in the order in which they are waited for, each a step before: the pages
 // of the unit after the next, the next one's keys, and its values.
+// Bound by the cache's bytes where it is long: 64 sequences of 8192 tokens, 32 heads on 8 of
+// 128, 138 us (5.6 TB/s; a large copy reaches 5.1); 131072 tokens 50 (5.4), and 5 each for the
+// parts to be joined.  8 sequences of 1024 tokens, 12 heads of 64: 7 us, a launch and one
+// unit's way from length to page to key to sum.
+// Eight waves where the tiles are fewer than the CUs, as many units at once (13 sequences of
+// 1500 tokens, 4 heads of 96: 10.4 us, with four 13); heads of 256 take the registers of two
+// waves a SIMD.
 template <int HP, bool WHOLE, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kernel(AttnArgs a) {
     constexpr int C = HP / 64;  // chunks of 64 values of a key; then one of 32
@@ -571,6 +578,10 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 // 16 bytes apart from a power of two, which spreads 8 lanes' 16 bytes over all banks.
 // `splits` workgroups share a tile's units where the tiles are too few for the chip, and
 // leave their parts for finish_kernel.
+// Bound by the matrix cores at heads of 128: 2 chunks of 2048 tokens behind 6144, 32 heads on
+// 8, 725 us, 1.06 PFLOP/s of f16 products, of which a large library product reaches 1.18; at
+// heads of 64 and less by the exponentials and roundings of each score (8 chunks of 256 behind
+// 16000, 32 heads of 64: 525 us, 298 by the products).
 constexpr int kRows = 128;
 
 template <int HP>
@@ -874,6 +885,10 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
     p.rows = N * group <= 96 * c->B || N * H <= (units <= 32 ? 8192 : 4096) ? kFew : kRows;
     p.tiles = N * group / p.rows + some;
     if(p.rows < kRows) {
+        // A workgroup to a tile up to 2048 tokens, 1024 of heads of more than 128: 8 sequences of
+        // 1024, 12 heads of 64, 7.7 us, shared out 8.9 and 3.8 for the join; 4 of 1900, 8 heads of
+        // 256, 27 against 18 and 4.  256 workgroups, one to a CU, which has the loads of four waves
+        // in flight: 64 sequences of 8192 138 us, 512 of them 150.
         p.W = units <= (c->hd <= 128 ? 32 : 16) || p.tiles * c->kv_heads * units >= (int64_t)1 << 31 ? 0 : 256;
     } else {
         // The workgroups that there are for sure: one to a CU where they get 4 units each, two

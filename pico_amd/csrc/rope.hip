@@ -10,7 +10,9 @@ using namespace pk;
 
 constexpr int kThreads = 256;
 
-// bound by HBM: x read and y written once; a token's angles are shared by its heads
+// Bound by HBM: x is read and y written once, a token's angles are shared by its heads.
+// 16384 tokens of 32 heads of 128, 64 turned: 104 us (5.2 TB/s; a large copy 5.1); 8192 of 24
+// heads of 64: 20 (5.1); 64 tokens of 12 heads, as a launch and its loads take: 3.2.
 template <bool EVEN, bool INTER>
 __global__ __launch_bounds__(kThreads) void rope_kernel(int64_t N, int T, TurnArgs g, RopeArgs r,
                                                         const int32_t* __restrict__ positions) {

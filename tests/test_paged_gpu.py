@@ -57,7 +57,9 @@ APPENDS = [([0], [1], 16, 1, 64), ([0, 5, 16], [1, 1, 1], 16, 2, 64), ([3, 0, 15
            ([5] * 70, [i % 4 for i in range(70)], 16, 1, 32), ([9, 2], [3, 30], 32, 2, 7), ([0] * 3, [0, 0, 0], 16, 1, 32),
            ([12], [129], 128, 1, 33), ([2], [1], 128, 16, 64),
            # many tokens of one sequence among others that wait
-           ([5] + [0] * 99, [70] + [0] * 99, 64, 2, 64), ([37] + [3] * 40, [60] + [0] * 39 + [1], 16, 1, 256)]
+           ([5] + [0] * 99, [70] + [0] * 99, 64, 2, 64), ([37] + [3] * 40, [60] + [0] * 39 + [1], 16, 1, 256),
+           # more pages and heads than are written to at once
+           ([0, 37], [500, 700], 16, 8, 96), ([50, 3], [600, 200], 128, 60, 250)]
 
 
 @pytest.mark.parametrize("lens,new,page,kvh,hd", APPENDS)
