@@ -231,9 +231,9 @@ constexpr int kPart = kFew * (HP + 2);
 // 128, 138 us (5.6 TB/s; a large copy reaches 5.1); 131072 tokens 50 (5.4), and 5 each for the
 // parts to be joined.  8 sequences of 1024 tokens, 12 heads of 64: 7 us, a launch and one
 // unit's way from length to page to key to sum.
-// Eight waves where the tiles are fewer than the CUs, as many units at once (13 sequences of
-// 1500 tokens, 4 heads of 96: 10.4 us, with four 13); heads of 256 take the registers of two
-// waves a SIMD.
+// Eight waves, as many units at once, where the tiles are fewer than the CUs and the heads
+// leave registers for two waves a SIMD (13 sequences of 1500 tokens, 4 heads of 96: 10.5 us,
+// with four 10.9; 4 of 1900, 8 heads of 128: 16.1 and 15.4).
 template <int HP, bool WHOLE, int WAVES>
 __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kernel(AttnArgs a) {
     constexpr int C = HP / 64;  // chunks of 64 values of a key; then one of 32
@@ -886,9 +886,9 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
     p.tiles = N * group / p.rows + some;
     if(p.rows < kRows) {
         // A workgroup to a tile up to 2048 tokens, 1024 of heads of more than 128: 8 sequences of
-        // 1024, 12 heads of 64, 7.7 us, shared out 8.9 and 3.8 for the join; 4 of 1900, 8 heads of
-        // 256, 27 against 18 and 4.  256 workgroups, one to a CU, which has the loads of four waves
-        // in flight: 64 sequences of 8192 138 us, 512 of them 150.
+        // 1024, 12 heads of 64, 7.6 us, shared out and joined 12.3; 4 of 3900, 8 heads of 128, 25
+        // against 17; 4 of 1900, 8 heads of 256, 28 against 22.  256 workgroups share them, one
+        // to a CU, which the loads of four waves suffice for: 131072 tokens 49 us, 512 of them 57.
         p.W = units <= (c->hd <= 128 ? 32 : 16) || p.tiles * c->kv_heads * units >= (int64_t)1 << 31 ? 0 : 256;
     } else {
         // The workgroups that there are for sure: one to a CU where they get 4 units each, two
@@ -923,7 +923,7 @@ int check_attn(const char* who, const PkKvCache* c, int64_t N, int64_t H) {
 template <int HP>
 void launch(const AttnArgs& a, const Plan& p, hipStream_t st) {
     const int64_t tiles = p.tiles * a.c.kv_heads;
-    constexpr int MANY = HP == 256 ? 4 : 8;  // waves; heads of 256 take twice the registers
+    constexpr int MANY = HP < 128 ? 8 : 4;  // waves of few tiles
     if(p.rows == kRows) {
         many_rows_kernel<HP><<<(unsigned)(tiles * p.splits), 256, 0, st>>>(a);
         if(p.splits > 1) finish_kernel<HP><<<dim3((unsigned)tiles, kRows / 4), 256, 0, st>>>(a);
