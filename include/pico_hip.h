@@ -734,7 +734,8 @@ int pk_gemm_experts_dw_f32(int64_t n, int64_t K, int64_t N, int64_t E, const int
  *   PK_ROPE_PARTS: a pair that turns r = length * f / (2 pi) times within the trained
  *     length gets f * (g + (1 - g) / factor), g = (r - low) / (high - low) held to [0, 1].
  * pk_rope_f32: y[t] = x[t] turned, x and y [N, H*hd] with row strides ldx, ldy (column
- *   blocks of one projection are fine; y may be x).  positions [N], any int32.
+ *   blocks of one projection are fine; y may be x).  positions [N], any int32.  N below
+ *   2^24, hd up to 1024, H*hd up to 2^20.
  *   PK_ACCUM: y += ...; PK_ROPE_BACKWARD: turns the other way, which maps the gradient
  *   of y to that of x. */
 #define PK_ROPE_PLAIN 0
@@ -768,7 +769,9 @@ int pk_rope_f32(int64_t N, int64_t H, int64_t hd, const PkRope* rope, const int3
  * k, v, k_exp, v_exp 16-byte aligned.
  * What they hold is checked there: rows outside [0, N), positions from width*page on and
  * pages outside [0, pages) reach no memory out of bounds (such tokens are not kept, and
- * count as absent when the cache is read).  Pages that sequences share are for reading only.
+ * count as absent when the cache is read).  Pages that sequences share are for reading only:
+ * a page with new tokens has one place in the table.  Fewer than 2^24 rows, 2^30 positions
+ * and 2^31 pages times heads, up to 2^20 sequences, 4096 kv_heads and H*hd of 2^20.
  * pk_kv_append_f32 writes the new tokens' keys and values, [N, kv_heads*hd] with row
  *   strides ldk, ldv; k turned by `rope` at its position (NULL or rot 0: as it is).  A
  *   page's e is the smallest with all |values| <= 448 * 2^e, from -40 to 40; where it grows
