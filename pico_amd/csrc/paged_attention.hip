@@ -581,7 +581,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 // Bound by the matrix cores at heads of 128: 2 chunks of 2048 tokens behind 6144, 32 heads on
 // 8, 725 us, 1.06 PFLOP/s of f16 products, of which a large library product reaches 1.18; at
 // heads of 64 and less by the exponentials and roundings of each score (8 chunks of 256 behind
-// 16000, 32 heads of 64: 525 us, 298 by the products).
+// 16000, 32 heads of 64: 410 us, 298 by the products).
 constexpr int kRows = 128;
 
 template <int HP>
@@ -891,14 +891,19 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
         // to a CU, which the loads of four waves suffice for: 131072 tokens 49 us, 512 of them 57.
         p.W = units <= (c->hd <= 128 ? 32 : 16) || p.tiles * c->kv_heads * units >= (int64_t)1 << 31 ? 0 : 256;
     } else {
-        // The workgroups that there are for sure: one to a CU where they get 4 units each, two
-        // where they get 8.  One sequence of 32000 tokens with 64 new ones, 3 heads of 168: 63
-        // parts a tile 65 us, 16 168; of 2000 tokens with 256, 8 parts 36, 4 57.
+        // The workgroups that there are for sure: one to a CU where they get 4 units each, as
+        // many as a CU holds where they get 8.  One sequence of 32000 tokens with 64 new ones, 3
+        // heads of 168: 63 parts a tile 65 us, 16 168; of 2000 tokens with 256, 8 parts 36, 4 57;
+        // 2 of 4000 with 1024, 12 heads of 64: 4 parts 75, 2 96.  Long sequences of different
+        // lengths in parts of 40 units, 3 at least, where there are more than run at once, which
+        // levels them out: 8 up to 16000 with 256, 32 heads of 64: 4 parts 413, whole tiles 520.
         const int64_t sure = (N * group + kRows - 1) / kRows * c->kv_heads;
         auto parts = [&](int64_t blocks, int64_t each) {
             return blocks / sure < units / each ? blocks / sure : units / each;
         };
-        const int64_t one = parts(256, 4), two = parts(512, 8), n = one > two ? one : two;
+        const int64_t one = parts(256, 4), full = parts(c->hd <= 64 ? 768 : 512, 8), level = parts(2048, 40);
+        int64_t n = one > full ? one : full;
+        if(c->B > 1 && level >= 3 && level > n && level * sure >= 1024) n = level;
         p.splits = (int)(n < 1 ? 1 : n > kWave ? kWave : n);
     }
     return p;
