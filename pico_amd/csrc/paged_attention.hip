@@ -876,13 +876,15 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
     Plan p = {};
     const int64_t group = H / c->kv_heads, units = (c->width * c->page + kUnit - 1) / kUnit;
     const int64_t some = c->B < N ? c->B : N;
-    // Tiles of 16 rows up to 96 rows a sequence on average, or 4096 of all heads together
-    // (8192 over up to 2048 tokens): tiles of 128 read the cache less often but are left
-    // partly empty, and are less finely shared out.  32 heads on 8 of 128 values: 16
-    // sequences of 4000 tokens with up to 40 new ones 82 against 92 us, with up to 60 119
-    // against 116; one of 500 tokens with 128 new ones 11 against 33, of 300 with 256 16
-    // against 30, with 1024 81 against 63; one of 4000 with 256 61 against 59.
-    p.rows = N * group <= 96 * c->B || N * H <= (units <= 32 ? 8192 : 4096) ? kFew : kRows;
+    // Tiles of 16 rows up to 96 rows a sequence on average, or 4096 of all heads together;
+    // over up to 2048 tokens up to 24576 of heads of up to 64 values, 12288 of 128, 8192 of more.
+    // Tiles of 128 read the cache less often but are left partly empty, and are less finely
+    // shared out.  32 heads on 8 of 128: 16 sequences of 4000 tokens with up to 40 new ones 82
+    // against 92 us, with up to 60 119 against 116; one of 4000 with 256 61 against 59; 4 of 1900
+    // with 100 35 against 45; one with 700 40 against 36.  16 heads on 2 of 64: 16 of 1000 with 100
+    // 25 against 44, 4 of 500 with 300 17 against 28; 32 on 8: 8 of 100 with 200 26 against 19.
+    const int64_t most = units > 32 ? 4096 : c->hd <= 64 ? 24576 : c->hd <= 128 ? 12288 : 8192;
+    p.rows = N * group <= 96 * c->B || N * H <= most ? kFew : kRows;
     p.tiles = N * group / p.rows + some;
     if(p.rows < kRows) {
         // A workgroup to a tile up to 2048 tokens, 1024 of heads of more than 128: 8 sequences of

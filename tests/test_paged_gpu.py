@@ -23,10 +23,12 @@ def _i32(a, dev):
 class Pair:
     """a cache on the device and the oracle's, with the same contents"""
 
-    def __init__(self, dev, rng, lens, new, page, kvh, hd, spare=3, fill=None):
+    def __init__(self, dev, rng, lens, new, page, kvh, hd, spare=3, fill=None, width=0):
         self.dev, self.kvh, self.hd, self.page = dev, kvh, hd, page
         need = sum(-(-(a + n) // page) for a, n in zip(lens, new))
         table, self.offsets = O.layout(lens, new, page, need + spare, rng)
+        if table.shape[1] < width:
+            table = np.pad(table, ((0, 0), (0, width - table.shape[1])), constant_values=-1)
         self.lens = np.asarray(lens)
         self.o = O.Cache(need + spare, kvh, page, hd, table)
         for pool, exps in ((self.o.k, self.o.k_exp), (self.o.v, self.o.v_exp)):
@@ -192,11 +194,11 @@ ATTENDS = [([0], [1], 16, 1, 1, 64), ([1, 15, 16, 17], [1, 1, 1, 1], 16, 2, 1, 6
            ([2200, 1, 0, 900], [1, 1, 0, 2], 128, 1, 1, 32), ([3000], [1], 64, 1, 16, 128), ([1500], [5], 16, 1, 7, 256),
            ([20] * 66 + [2100], [1] * 67, 128, 1, 4, 128), ([3000], [40], 64, 1, 4, 64),
            # tiles of 128 rows
-           ([0], [700], 64, 2, 6, 64), ([40, 0, 7], [333, 0, 400], 16, 1, 12, 128), ([5], [530], 32, 1, 16, 33),
-           ([300], [1040], 128, 8, 1, 96), ([77, 3], [500, 20], 16, 2, 8, 80), ([0], [530], 64, 1, 16, 256),
+           ([0], [700], 64, 2, 18, 64), ([40, 0, 7], [333, 0, 400], 16, 1, 17, 128), ([5], [530], 32, 1, 48, 33),
+           ([300], [1040], 128, 12, 1, 96), ([77, 3], [500, 20], 16, 2, 12, 80), ([0], [530], 64, 1, 16, 256),
            # and these with a tile's tokens split over workgroups
-           ([2600], [260], 64, 1, 16, 64), ([1500, 0, 900], [200, 0, 150], 16, 1, 24, 96), ([1300], [140], 32, 1, 60, 256),
-           ([2000], [129], 128, 1, 32, 32), ([1500, 1], [1, 400], 32, 1, 21, 128),
+           ([2600], [260], 64, 1, 16, 64), ([1500, 0, 900], [200, 0, 150], 16, 1, 36, 96), ([1300], [140], 32, 1, 60, 256),
+           ([2000], [129], 128, 1, 32, 32), ([1500, 1], [1, 400], 32, 1, 31, 128),
            ([9000], [65], 128, 1, 64, 32)]
 
 
@@ -250,7 +252,8 @@ def test_attention_over_absent_pages(dev, new, hd):
     without a key gets zeros); NaN in the pages that are read in their place does not matter"""
     rng = np.random.default_rng(10)
     lens = [100, 70, 40, 5]
-    p = Pair(dev, rng, lens, new, 16, 2, hd)
+    # (tables for 4096 tokens: with many rows, tiles of 128 in parts)
+    p = Pair(dev, rng, lens, new, 16, 2, hd, width=256)
     p.o.table[0, 2], p.o.table[1, (70 + new[1] - 1) // 16] = -1, 10 ** 7
     p.o.table[2, :] = -1
     p.o.table[3, 0] = 2 ** 31 - 1
@@ -276,7 +279,7 @@ def test_attention_nan_reaches_the_rows_that_see_it(dev, new, hd):
     lens, kvh, page = [90], 1, 16
     H = 32 if new == 150 else 2  # (150: tiles of 128 rows)
     for what in ("k", "v"):
-        p = Pair(dev, rng, lens, [new], page, kvh, hd)
+        p = Pair(dev, rng, lens, [new], page, kvh, hd, width=256)  # (as above)
         t = 90 + new // 2  # this token's
         pid = p.o.table[0, t // page]
         if what == "k":
