@@ -462,6 +462,50 @@ def test_two_streams_with_workspaces_of_their_own(dev):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("new,H", [(1, 8), (300, 16)])
+def test_two_graphs_share_a_workspace(dev, new, H):
+    """replayed in turn on a stream, each leaves the other nothing that it reads"""
+    rng = np.random.default_rng(22)
+    pairs = [Pair(dev, rng, [4000 + 900 * i, 130, 2500], [new, new, new], 64, 2, 64) for i in range(2)]
+    q = torch.randn(3 * new, H * 64, device=dev) / 16
+    size = [K.attn_paged_workspace(p.c, 3 * new, H) for p in pairs]
+    assert min(size) > 0
+    ws = torch.full((max(size),), 255, dtype=torch.uint8, device=dev)  # (NaN to begin with)
+    outs, graphs = [torch.empty_like(q) for _ in pairs], []
+    for p, o in zip(pairs, outs):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            K.attn_paged(p.c, H, q, o, ws=ws)
+    for i in range(3):
+        q.copy_(torch.randn_like(q) / 16)
+        for p in pairs:
+            p.lens_t.copy_(_i32([3000 - 700 * i, 100 + i, 2500 - 64 * i], dev))
+        for g in graphs:
+            g.replay()
+        for p, o in zip(pairs, outs):
+            want = torch.empty_like(q)
+            K.attn_paged(p.c, H, q, want)
+            assert torch.equal(o, want)
+
+
+def test_pages_shared_for_reading(dev):
+    """sequences that begin alike read the same pages, and write to their own"""
+    rng = np.random.default_rng(23)
+    lens, new, kvh, H, hd, page = [64, 64, 64], [1, 20, 3], 2, 8, 64, 32
+    p = Pair(dev, rng, lens, new, page, kvh, hd)
+    p.o.table[1:, :2] = p.o.table[0, :2]
+    p.upload()
+    N = sum(new)
+    k, v, q = (_rows(rng, N, n, hd) / 8 for n in (kvh, kvh, H))
+    K.kv_append(p.c, _cuda(k.reshape(N, -1), dev), _cuda(v.reshape(N, -1), dev))
+    p.o.append(k, v, lens, p.offsets)
+    p.same()
+    o = torch.empty(N, H * hd, device=dev)
+    K.attn_paged(p.c, H, _cuda(q.reshape(N, -1), dev), o)
+    want, tol = p.o.attend(q.astype(np.float64), lens, p.offsets, H)
+    assert (np.abs(o.cpu().numpy().reshape(N, H, hd) - want) <= tol).all()
+
+
 def test_offsets_past_32_bits(dev):
     """a cache of more than 2^32 bytes of keys, its last pages in use"""
     kvh, hd, page = 16, 256, 128
