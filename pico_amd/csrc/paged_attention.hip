@@ -707,8 +707,9 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
         for(int j = 0; j < 2; ++j) {
             const int token0 = u * kUnit + 32 * j;
             if(rows <= 0 || token0 > reach_all) continue;
-            // (the waves that have products to give the matrix cores before those that do not)
-            __builtin_amdgcn_s_setprio(1);
+            // (of a SIMD's waves those that have products to give the matrix cores before those
+            // that do not; heads of 256 leave room for one)
+            if(HP < 256) __builtin_amdgcn_s_setprio(1);
             f32x16 sc = {};
 #pragma unroll
             for(int st = 0; st < STEPS; st += 2) {
@@ -719,7 +720,7 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0, ql[st], sc, 0, 0, 0);
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1, ql[st + 1], sc, 0, 0, 0);
             }
-            __builtin_amdgcn_s_setprio(0);
+            if(HP < 256) __builtin_amdgcn_s_setprio(0);
             const float4 g = pages[buf][2 * j + half];
             const float kc = coef * g.x;
             const bool absent = g.w == 0.0f;
