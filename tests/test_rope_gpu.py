@@ -40,7 +40,9 @@ SHAPES = [(1, 1, 2, 2, False, 1, "none"), (1, 12, 64, 64, False, 9, "none"), (64
           (17, 2, 64, 0, False, 9, "none"), (5000, 4, 32, 32, True, 3000, "none"), (1030, 24, 64, 64, False, 1024, "none"),
           (2, 5000, 8, 8, False, 4, "none"), (40, 3, 50, 22, False, 900, "none"), (11, 5, 130, 6, True, 900, "none"),
           (9, 4, 19, 10, True, 40, "none"), (700, 6, 128, 6, False, 900, "none"), (2, 524287, 2, 2, False, 9, "none"),
-          (3, 349525, 3, 2, True, 9, "none")]
+          (3, 349525, 3, 2, True, 9, "none"),
+          # rows of fewer than 4 values
+          (70, 1, 3, 2, False, 900, "none"), (70, 1, 3, 2, True, 900, "none"), (5, 3, 1, 0, False, 9, "none"), (600, 1, 2, 2, True, 9, "none")]
 
 
 @pytest.mark.parametrize("N,H,hd,rot,inter,far,scaling", SHAPES)
