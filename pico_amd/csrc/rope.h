@@ -64,11 +64,12 @@ struct TurnArgs {
     int back, accum;
 };
 
+// (such pieces share lines, which stay in the caches for that: 45 to 30 us at the sizes below)
 typedef float f32x4_anywhere __attribute__((ext_vector_type(4), aligned(4)));
 // 4 values of a row of n from `at` on, or those that there are; any of the row in their
 // place behind them
 __device__ __forceinline__ f32x4 ld_in_row(const float* row, int at, int n) {
-    return __builtin_nontemporal_load((const f32x4_anywhere*)(row + (at < n - 4 ? at : n - 4)));
+    return *(const f32x4_anywhere*)(row + (at < n - 4 ? at : n - 4));
 }
 __device__ __forceinline__ f32x4 from_window(f32x4 v, int at, int n) {
     const int behind = at - (n - 4);
@@ -80,7 +81,7 @@ __device__ __forceinline__ f32x4 from_window(f32x4 v, int at, int n) {
 }
 __device__ __forceinline__ void st_first(float* to, f32x4 v, int n) {
     if(n >= 4) {
-        __builtin_nontemporal_store((f32x4_anywhere)v, (f32x4_anywhere*)to);
+        *(f32x4_anywhere*)to = v;
     } else {
 #pragma unroll
         for(int k = 0; k < 3; ++k)
@@ -95,7 +96,8 @@ __device__ __forceinline__ void st_first(float* to, f32x4 v, int n) {
 // EVEN: head, halves and strides are multiples of 4 and aligned.  Where they are not, a
 // part's last 4 may be fewer; all are loaded as 4, and without a branch, so
 // that none is waited for before the others are issued (8192 tokens of 12 heads of 80, 20
-// turned: 44 us both ways, pair by pair 69; 25 at the rate of a copy).  where(t, pos): the position of token t0 + t; false leaves the row.
+// turned: 30 us both ways, pair by pair 69; 25 at the rate of a copy).
+// where(t, pos): the position of token t0 + t; false leaves the row.
 template <bool EVEN, bool INTER, class P>
 __device__ __forceinline__ void turn_rows(const TurnArgs& g, const RopeArgs& r, int64_t t0,
                                           int tokens, int heads, P where, float* tc, float* ts) {
