@@ -101,6 +101,23 @@ def test_append_turns_as_rope_does(dev, hd, rot, H, inter):
     p.same()  # (the same tokens again: the same bytes)
 
 
+@pytest.mark.parametrize("lens,new,page,kvh,hd,rot", [([100, 7], [300, 1], 128, 2, 256, 256), ([50], [900], 128, 44, 250, 100),
+                                                      ([5] + [0] * 99, [130] + [0] * 99, 64, 2, 96, 96), ([0, 37], [500, 700], 16, 8, 64, 64)])
+def test_append_turns_pages_in_parts(dev, lens, new, page, kvh, hd, rot):
+    """values that are read twice, and waves with a page each, turned as pk_rope_f32 does"""
+    rng = np.random.default_rng(hd + kvh)
+    p = Pair(dev, rng, lens, new, page, kvh, hd)
+    N = int(p.offsets[-1])
+    k, v = (_cuda(_rows(rng, N, kvh, hd).reshape(N, -1), dev) for _ in range(2))
+    pos = np.concatenate([np.arange(a, a + n) for a, n in zip(lens, new)]).astype(np.int32)
+    r = K.Rope(K.rope_freqs(rot, device=dev))
+    kt = torch.empty_like(k)
+    K.rope(r, kvh, k, _cuda(pos, dev), kt)
+    K.kv_append(p.c, k, v, r)
+    p.o.append(kt.cpu().numpy().reshape(N, kvh, hd), v.cpu().numpy().reshape(N, kvh, hd), lens, p.offsets)
+    p.same()
+
+
 def test_append_one_by_one_and_at_once(dev):
     """a page filled token by token holds what it holds filled at once where its scale does
     not grow, and values off by a step of the last rounding where it does"""
