@@ -578,10 +578,12 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
 // 16 bytes apart from a power of two, which spreads 8 lanes' 16 bytes over all banks.
 // `splits` workgroups share a tile's units where the tiles are too few for the chip, and
 // leave their parts for finish_kernel.
-// Bound by the matrix cores at heads of 128: 2 chunks of 2048 tokens behind 6144, 32 heads on
-// 8, 725 us, 1.06 PFLOP/s of f16 products, of which a large library product reaches 1.18; at
-// heads of 64 and less by the exponentials and roundings of each score (8 chunks of 256 behind
-// 16000, 32 heads of 64: 410 us, 298 by the products).
+// Heads of 128: 2 chunks of 2048 tokens behind 6144, 32 heads on 8, 720 us, 1.07 PFLOP/s of
+// f16 products, where a large library product reaches 1.18 and the matrix cores fed from
+// registers 2.1: two waves a SIMD, all that there are registers for, overlap the one's products
+// with the other's exponentials 1.6 times.  Heads of 64 and less are held by the exponentials
+// and roundings of each score (8 chunks of 256 behind 16000, 32 heads of 64: 410 us, 298 by the
+// products at the library's rate).
 constexpr int kRows = 128;
 
 template <int HP>
