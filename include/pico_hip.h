@@ -760,7 +760,8 @@ int pk_rope_f32(int64_t N, int64_t H, int64_t hd, const PkRope* rope, const int3
  *   k [pages][kv_heads][page][hp], v [pages][kv_heads][hp][page] (tokens innermost, as
  *   the products that read them take them), hp = pk_kv_head_size(hd): hd (1 to 256)
  *   rounded up to 32, 64, 96, 128 or 256; k's values from hd to hp are zeros, v's rows
- *   there are not used.  k_exp, v_exp [pages][kv_heads]: e + 127 for the factor 2^e.
+ *   there are not used.  k_exp, v_exp [pages][kv_heads]: e + 127 for the factor 2^e, e from
+ *   -40 to 40; other bytes count as the nearest of these.
  * B sequences: table [B][width] names the pages of sequence b's tokens 0, page, 2*page..;
  * lens [B] is how many tokens it held before the call; its new tokens are the rows
  * offsets[b] .. offsets[b + 1] - 1 of the inputs ([B + 1], not decreasing), at the

@@ -90,7 +90,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, unsigned task, 
     const int64_t at = (int64_t)name * c.kv_heads + h;
     uint8_t* exps = (IS_V ? c.v_exp : c.k_exp) + at;
     uint8_t* out = (IS_V ? c.v : c.k) + at * (int64_t)(hp * page);
-    const int old = s0 ? held((int)*exps - 127, kExpMin, kExpMax) : kExpMin;
+    const int old = s0 ? exponent_byte(*exps) - 127 : kExpMin;
 
     int e = 0;
     float scale = 1.0f;

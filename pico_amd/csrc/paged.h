@@ -90,6 +90,15 @@ __device__ __forceinline__ int block_exponent(float amax) {
     return held(x - (__builtin_amdgcn_frexp_mantf(amax) <= 0.875f ? 9 : 8), kExpMin, kExpMax);
 }
 
+// A page's byte, e + 127, or the nearest that there is where it is none.  (Two instructions
+// with a constant each; one with both takes a register for the length of a loop, and tiles of
+// 128 rows of heads of 64 a third wave.)
+__device__ __forceinline__ int exponent_byte(int b) {
+    int x = b > 127 + kExpMin ? b : 127 + kExpMin;
+    asm("" : "+v"(x));
+    return x < 127 + kExpMax ? x : 127 + kExpMax;
+}
+
 inline int head_size(int64_t hd) {
     return hd < 1 || hd > 256 ? 0 : hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 96 ? 96 : hd <= 128 ? 128 : 256;
 }

@@ -374,7 +374,9 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
                     sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[st], sc[t], 0, 0, 0);
                 }
             }
-            const int ek_now = of_unit(ek, x_value), ev_now = of_unit(ev, x_value);
+            // (of pages that hold no key these may be any byte, and 0 times 2^-ev has to be 0; here, not
+            // where they are loaded, which would wait for them)
+            const int ek_now = exponent_byte(of_unit(ek, x_value)), ev_now = exponent_byte(of_unit(ev, x_value));
             const float kc = coef * power(ek_now), vexp = (float)(ev_now - 127), vinv = power(254 - ev_now);
             const bool absent = pv < 0;
             if(++k * per == kWave) name_units(next);
@@ -664,8 +666,8 @@ __global__ __launch_bounds__(256, HP == 256 ? 1 : 2) void many_rows_kernel(AttnA
             }
         }
         if(threadIdx.x < 4) {
-            const uint8_t ek = c.k_exp[v_head], ev = c.v_exp[v_head];
-            pr = {power(ek), (float)((int)ev - 127), power(254 - ev), pv < 0 ? 0.0f : 1.0f};
+            const int ek = exponent_byte(c.k_exp[v_head]), ev = exponent_byte(c.v_exp[v_head]);
+            pr = {power(ek), (float)(ev - 127), power(254 - ev), pv < 0 ? 0.0f : 1.0f};
         }
         real = pv < 0 ? 0 : held(s.end - u * kUnit - 16 * g16, 0, 16);
     };

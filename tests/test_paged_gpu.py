@@ -591,3 +591,66 @@ def test_refused_by_the_bindings(dev):
         K.PagedKV(*t, p.lens_t, p.offsets_t, 65)
     with pytest.raises(TypeError):
         K.PagedKV(*t, p.lens_t.long(), p.offsets_t, 64)
+
+
+def _spare_page_0(p):
+    """a Pair whose sequences do not use page 0, and pages behind every sequence's last that
+    its table names already"""
+    t, pages = p.o.table, p.o.k.shape[0]
+    free = [i for i in range(pages) if i not in t]
+    if 0 not in free:
+        t[t == 0] = free[-1]
+    free = [i for i in range(pages) if i not in t]
+    for b in range(len(t)):
+        behind = np.flatnonzero(t[b] < 0)
+        t[b, behind[0]] = free[b % len(free)]
+    return free
+
+
+@pytest.mark.parametrize("byte", [255, 254, 0])
+@pytest.mark.parametrize("lens,new,page,kvh,group,hd", [
+    ([20, 3], [1, 1], 16, 2, 2, 64), ([40, 0, 17], [3, 0, 20], 32, 1, 4, 128), ([70], [5], 64, 1, 2, 256),
+    # units shared out evenly
+    ([2300, 700], [1, 1], 16, 1, 3, 96), ([2500], [2], 32, 2, 4, 32),
+    # tiles of 128 rows, whole and in parts
+    ([0], [650], 16, 2, 20, 64), ([2600], [260], 16, 1, 16, 64), ([1300], [140], 32, 1, 60, 256)])
+def test_powers_of_pages_without_keys(dev, lens, new, page, kvh, group, hd, byte):
+    """the exponents of pages that hold no key of a sequence may be anything: of the page that
+    is read in an absent one's place, and of those named ahead"""
+    rng = np.random.default_rng(24 + hd)
+    p = Pair(dev, rng, lens, new, page, kvh, hd)
+    for i in _spare_page_0(p):
+        p.o.k_exp[i] = p.o.v_exp[i] = byte
+    p.upload()
+    N, H = int(p.offsets[-1]), kvh * group
+    q = _rows(rng, N, H, hd)
+    o = torch.full((N, H * hd), 5.0, device=dev)
+    scale = hd ** -0.5 / 16
+    K.attn_paged(p.c, H, _cuda(q.reshape(N, -1), dev), o, scale=scale)
+    want, tol = p.o.attend(q.astype(np.float64), lens, p.offsets, H, scale)
+    assert (np.abs(o.cpu().numpy().reshape(N, H, hd) - want) <= tol + 1e-30).all()
+
+
+@pytest.mark.parametrize("new,H", [(1, 2), (150, 24)])
+def test_powers_beyond_their_range(dev, new, H):
+    """an exponent's byte beyond -40 and 40 counts as the nearest, for the attention and for
+    tokens that join such a page"""
+    rng = np.random.default_rng(25)
+    lens, kvh, hd, page = [5, 300], 1, 64, 16
+    p = Pair(dev, rng, lens, [new, new], page, kvh, hd, width=256)
+    p.o.k_exp[p.o.table[0, 0]], p.o.v_exp[p.o.table[0, 0]] = 3, 255
+    p.o.k_exp[p.o.table[1, 2]], p.o.v_exp[p.o.table[1, 2]] = 86, 168
+    p.upload()
+    for x in (p.o.k_exp, p.o.v_exp):
+        x[...] = x.clip(87, 167)
+    q = _rows(rng, 2 * new, H, hd) / 64
+    o = torch.empty(2 * new, H * hd, device=dev)
+    for _ in range(2):
+        K.attn_paged(p.c, H, _cuda(q.reshape(2 * new, -1), dev), o)
+        want, tol = p.o.attend(q.astype(np.float64), lens, p.offsets, H)
+        assert (np.abs(o.cpu().numpy().reshape(want.shape) - want) <= tol + 1e-30).all()
+        k, v = _rows(rng, 2 * new, kvh, hd), _rows(rng, 2 * new, kvh, hd)
+        K.kv_append(p.c, _cuda(k.reshape(2 * new, -1), dev), _cuda(v.reshape(2 * new, -1), dev))
+        p.o.append(k, v, lens, p.offsets)
+    for i, x in ((0, p.o.k), (1, p.o.v)):
+        np.testing.assert_array_equal(p.t[i].cpu().numpy(), x)
