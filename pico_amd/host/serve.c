@@ -113,7 +113,7 @@ struct PicoTensor* pico_rope(struct PicoTensor* x, const struct PicoRope* rope,
 struct PicoKV {
     PkKvCache* layers;
     int n_layers, S;
-    int64_t width, pages, free_pages;
+    int64_t width, max_length, pages, free_pages;
     int32_t* free_list;    /* free_pages of them */
     int64_t* length;       /* tokens of each sequence, the present step's among them */
     int32_t *words, *dev;
@@ -160,7 +160,8 @@ struct PicoKV* pico_kv_init(const struct PicoKVConfig* cfg) {
     kv->n_layers = cfg->layers;
     kv->S = cfg->sequences;
     kv->pages = kv->free_pages = cfg->pages;
-    kv->width = (cfg->max_length + cfg->page - 1) / cfg->page;
+    kv->max_length = cfg->max_length;
+    kv->width = (kv->max_length + cfg->page - 1) / cfg->page;
     kv->rows = -1;
     kv->n_words = 2 * (size_t)kv->S + 1 + (size_t)kv->S * (size_t)kv->width;
     kv->layers = (PkKvCache*)calloc((size_t)kv->n_layers, sizeof(PkKvCache));
@@ -207,9 +208,9 @@ int64_t pico_kv_begin(struct PicoKV* kv, const int32_t* new_tokens) {
     int64_t rows = 0, need = 0;
     for(int b = 0; b < kv->S; b++) {
         const int64_t n = new_tokens[b], len = kv->length[b];
-        if(n < 0 || len + n > kv->width * page) {
+        if(n < 0 || len + n > kv->max_length) {
             PKH_ERR("kv_begin: sequence %d of %lld tokens gets %lld more, up to %lld are held!\n", b,
-                    (long long)len, (long long)n, (long long)(kv->width * page));
+                    (long long)len, (long long)n, (long long)kv->max_length);
             return -1;
         }
         rows += n;

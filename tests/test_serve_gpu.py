@@ -345,3 +345,20 @@ def test_captured_step(P):
         P.lib.pico_kv_free(kv)
     for t in leaves.values():
         P.free(t)
+
+
+def test_max_length_within_a_page(P):
+    """max_length holds, though the last page has room for more"""
+    kv = P.kv_init(1, 1, 32, 16, 8, 2, 20)
+    assert P.kv_begin(kv, [19, 0]) == 19
+    for bad in ([2, 0], [0, 21], [13, 1]):
+        with pytest.raises(PicoError):
+            P.kv_begin(kv, bad)
+        assert [P.lib.pico_kv_length(kv, b) for b in (0, 1)] == [19, 0]
+    assert P.kv_begin(kv, [1, 20]) == 21
+    with pytest.raises(PicoError):
+        P.kv_begin(kv, [1, 0])
+    assert P.kv_begin(kv, [0, 0]) == 0
+    assert P.lib.pico_kv_drop(kv, 0) == 0
+    assert P.kv_begin(kv, [20, 0]) == 20
+    P.lib.pico_kv_free(kv)
