@@ -34,7 +34,8 @@ constexpr int kFew = 16;           // query rows a tile, where a sequence has fe
 constexpr int kMinShare = 4;       // units a workgroup takes at least, where they share a tile
 constexpr float kTop = 7.0f;       // probabilities are relative to 2^7 below the maximum m
 constexpr float kRaise = 8.0f;     // m is raised when a score passes it by 2^8: p <= 2^15
-constexpr float kNone = -1e30f;    // the maximum of no scores
+constexpr float kNone = -INFINITY;  // the maximum of no scores
+constexpr float kLeast = -3.402823466e38f;  // and what those of parts are relative to, where all have none
 
 struct AttnArgs {
     PkKvCache c;
@@ -483,9 +484,9 @@ __global__ __launch_bounds__(WAVES * kWave, HP < 128 ? 2 : 1) void few_rows_kern
         float* out = a.ws + ((int64_t)blockIdx.x * 2 + (now == begin ? 0 : 1)) * kPart<HP>;
         for(int i = threadIdx.x; i < rows * (HP / 4); i += WAVES * kWave) {
             const int r = i / (HP / 4), d = 4 * (i % (HP / 4));
-            float top = part_m[0][r], total = 0.0f;
+            float top = kLeast, total = 0.0f;
 #pragma unroll
-            for(int k = 1; k < WAVES; ++k) top = fmaxf(top, part_m[k][r]);
+            for(int k = 0; k < WAVES; ++k) top = fmaxf(top, part_m[k][r]);
             f32x4 v = {};
 #pragma unroll
             for(int k = 0; k < WAVES; ++k) {
@@ -541,7 +542,7 @@ __global__ __launch_bounds__(256) void join_kernel(AttnArgs a) {
     if(w0 < 0) return;  // (offsets that decrease)
     const int first_place = before * share == u0 ? 0 : 1;
     auto part = [&](int w) { return a.ws + ((int64_t)w * 2 + (w == w0 ? first_place : 0)) * kPart<HP>; };
-    float top = kNone;
+    float top = kLeast;
     for(int w = w0 + lane; w <= w1; w += kWave) top = fmaxf(top, part(w)[r]);
     top = wave_max(top);
     const int d = 4 * (lane % D4), mine = lane / D4;
@@ -852,7 +853,7 @@ __global__ __launch_bounds__(256) void finish_kernel(AttnArgs a) {
     if(row >= s.n * a.group) return;
     const float* base = a.ws + ((int64_t)rest * a.splits * kvh + h) * kManyPart<HP>;
     const int64_t apart = (int64_t)kvh * kManyPart<HP>;
-    float top = kNone, total = 0.0f;
+    float top = kLeast, total = 0.0f;
     if(lane < a.splits) top = base[lane * apart + r];  // (at most a lane each)
     top = wave_max(top);
     const int d = 4 * lane;

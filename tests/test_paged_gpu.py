@@ -654,3 +654,24 @@ def test_powers_beyond_their_range(dev, new, H):
         p.o.append(k, v, lens, p.offsets)
     for i, x in ((0, p.o.k), (1, p.o.v)):
         np.testing.assert_array_equal(p.t[i].cpu().numpy(), x)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256])
+@pytest.mark.parametrize("past,new,H", [(0, 1, 1), (40, 1, 3), (100, 20, 2), (3000, 1, 2), (0, 660, 40), (2600, 200, 32)])
+def test_attention_of_scores_far_below_zero(dev, past, new, H, hd):
+    """scores of -1e35 are scores: a single key's row is its value, and a row of equal keys,
+    whose scores' last bits decide between them, lies between the values that it sees"""
+    rng = np.random.default_rng(26)
+    p = Pair(dev, rng, [past], [new], 16, 1, hd)
+    p.o.k[..., :hd], p.o.k_exp[...], p.o.v_exp[...] = 0x38, 150, 120  # keys of 2^23
+    p.upload()
+    q = np.full((new, H, hd), -1e28, np.float32)
+    o = torch.empty(new, H * hd, device=dev)
+    K.attn_paged(p.c, H, _cuda(q.reshape(new, -1), dev), o, scale=1.0 / hd)
+    v = p.o.dense(0, past + new, 0)[1]
+    lo, hi = (f.accumulate(v)[past:, None] for f in (np.minimum, np.maximum))
+    # numerator and denominator are sums of L terms of weights of 22 bits, and a division is
+    # rounded
+    tol = (2.0 ** -21 + 2 * (past + new + 8) * 2.0 ** -24) * np.maximum(np.abs(lo), np.abs(hi))
+    got = o.cpu().numpy().reshape(new, H, hd)
+    assert (got >= lo - tol).all() and (got <= hi + tol).all()
