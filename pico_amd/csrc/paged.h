@@ -118,7 +118,7 @@ inline int check_cache(const char* who, const PkKvCache* c, int64_t N) {
                     (long long)c->width);
     if(N < 0 || N >= (int64_t)1 << 24)
         return fail("%s: N %lld: 0 to 2^24 - 1 rows", who, (long long)N);
-    if(!c->k || !c->v || !c->k_exp || !c->v_exp || !c->table || !c->lens || !c->offsets)
+    if(!c->k || !c->v || !c->k_exp || !c->v_exp || (c->B > 0 && (!c->table || !c->lens || !c->offsets)))
         return fail("%s: NULL pointer in the cache", who);
     if(!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_exp) || !aligned16(c->v_exp))
         return fail("%s: k, v and their exponents must be 16-byte aligned", who);

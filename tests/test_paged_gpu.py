@@ -675,3 +675,16 @@ def test_attention_of_scores_far_below_zero(dev, past, new, H, hd):
     tol = (2.0 ** -21 + 2 * (past + new + 8) * 2.0 ** -24) * np.maximum(np.abs(lo), np.abs(hi))
     got = o.cpu().numpy().reshape(new, H, hd)
     assert (got >= lo - tol).all() and (got <= hi + tol).all()
+
+
+def test_a_cache_of_no_sequence(dev):
+    """an empty batch: nothing is written, and rows of no sequence are left"""
+    pool = K.kv_pool(2, 1, 16, 64, dev)
+    for t in pool:
+        t.fill_(7)
+    c = K.PagedKV(*pool, torch.empty(0, 4, dtype=torch.int32, device=dev), _i32([], dev), _i32([0], dev), 64)
+    x = torch.full((3, 64), 2.0, device=dev)
+    K.kv_append(c, x, x)
+    K.attn_paged(c, 1, torch.zeros_like(x), x)
+    assert K.attn_paged_workspace(c, 3, 1) == 0
+    assert (x == 2.0).all() and all((t == 7).all() for t in pool)

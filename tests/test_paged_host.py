@@ -141,6 +141,14 @@ def test_attention_refused(L):
     assert L.pk_attn_paged_workspace(_cache(), 0, 4) == 0
 
 
+def test_no_sequences_need_no_arrays(L):
+    c = _cache(B=0, table=None, lens=None, offsets=None)
+    assert L.pk_kv_append_f32(c, 4, PTR, 128, PTR, 128, None, 0, None, 0, None, 0, None) == 0
+    assert L.pk_attn_paged_f32(c, 4, 4, 1.0, PTR, 256, PTR, 256, None, 0, None) == 0
+    assert L.pk_attn_paged_workspace(c, 4, 4) == 0
+    assert L.pk_kv_append_f32(_cache(B=0, k=None), 4, PTR, 128, PTR, 128, None, 0, None, 0, None, 0, None) == EINVAL
+
+
 def test_head_sizes():
     assert [K.kv_head_size(h) for h in (0, -1, 1, 32, 33, 64, 65, 96, 97, 128, 129, 256, 257)] == \
         [0, 0, 32, 32, 64, 64, 96, 96, 128, 128, 256, 256, 0]
