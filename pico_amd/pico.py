@@ -372,7 +372,9 @@ class Pico:
         return r
 
     def rope(self, x, rope, positions, n_heads):
-        """positions: an int32 numpy array (staged per call) or a device pointer"""
+        """positions: an int32 numpy array (staged per call), one a row, or a device pointer"""
+        if not isinstance(positions, int) and np.size(positions) != x.contents.shape[0]:
+            raise ValueError(f"rope: {np.size(positions)} positions for {x.contents.shape[0]} rows")
         p = positions if isinstance(positions, int) else self.ids(positions)
         return self._check(self.lib.pico_rope(x, rope, p, n_heads), "pico_rope")
 
@@ -386,8 +388,10 @@ class Pico:
         return kv
 
     def kv_begin(self, kv, new_tokens):
-        """pico_kv_begin: the step's rows"""
+        """pico_kv_begin: the step's rows; new_tokens: a count for each sequence"""
         a = np.ascontiguousarray(new_tokens, dtype=np.int32)
+        if kv and (self.lib.pico_kv_length(kv, a.size - 1) < 0 or self.lib.pico_kv_length(kv, a.size) >= 0):
+            raise ValueError(f"kv_begin: {a.size} counts, not one for each sequence of the cache")
         n = self.lib.pico_kv_begin(kv, a.ctypes.data_as(c_p))
         if n < 0:
             raise PicoError("pico_kv_begin failed")

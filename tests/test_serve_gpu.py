@@ -362,3 +362,21 @@ def test_max_length_within_a_page(P):
     assert P.lib.pico_kv_drop(kv, 0) == 0
     assert P.kv_begin(kv, [20, 0]) == 20
     P.lib.pico_kv_free(kv)
+
+
+def test_arrays_of_another_length(P):
+    """fewer positions than rows, or counts than sequences, are not read past their end"""
+    kv, rope = P.kv_init(1, 1, 32, 16, 8, 2, 64), P.rope_init(32)
+    with P.arena():
+        x = P.tensor([3, 32], np.zeros((3, 32)))
+        for pos in ([0, 1], [], [0, 1, 2, 3], np.zeros((2, 3))):
+            with pytest.raises(ValueError):
+                P.rope(x, rope, pos, 1)
+        assert P.shape(P.rope(x, rope, [[0], [1], [2]], 1)) == (3, 32)
+    for new in ([1], [], [1, 1, 1]):
+        with pytest.raises(ValueError):
+            P.kv_begin(kv, new)
+        assert [P.lib.pico_kv_length(kv, b) for b in (0, 1)] == [0, 0]
+    assert P.kv_begin(kv, np.array([2, 1], np.int64)) == 3
+    P.lib.pico_rope_free(rope)
+    P.lib.pico_kv_free(kv)
