@@ -688,3 +688,61 @@ def test_a_cache_of_no_sequence(dev):
     K.attn_paged(c, 1, torch.zeros_like(x), x)
     assert K.attn_paged_workspace(c, 3, 1) == 0
     assert (x == 2.0).all() and all((t == 7).all() for t in pool)
+
+
+def _guarded(t, byte=0xa5, rows=64):
+    """(t's copy in the middle of a larger tensor, that tensor)"""
+    big = torch.full((t.shape[0] + 2 * rows, *t.shape[1:]), byte, dtype=t.dtype, device=t.device)
+    big[rows:-rows] = t
+    return big[rows:-rows], big
+
+
+@pytest.mark.parametrize("new,width", [(4, 0), (4, 256), (50, 256)])  # tiles of 16 rows, shared ones, of 128
+@pytest.mark.parametrize("lens,offsets", [((-5, 10 ** 9, 7), (0, 1, 2, 3)), ((0, 0, 0), (-9, -3, 2 / 3, 10 ** 9)),
+                                          ((2, 30, 0), (1, 2, 2, 5 / 2)), ((0, 30, 0), (3, 70, 10 ** 9, 5)), ((9, 9, 9), (0, 3, 0, 3)),
+                                          ((2 ** 31 - 1, -2 ** 31, 7), (0, 3, 1, 40))])
+def test_bad_arrays_reach_nothing_else(dev, new, width, lens, offsets):
+    """lengths and offsets of any value: what lies around the operands and between them stays
+    as it is, and of offsets that do not decrease, rows inside the inputs come out right"""
+    rng = np.random.default_rng(27)
+    kvh, H, hd, page = 16, 32, 64, 16
+    p = Pair(dev, rng, [40, 10, 23], [new] * 3, page, kvh, hd, width=width)
+    N, cap = 3 * new, p.o.table.shape[1] * page
+    offsets = [int(x * new) if abs(x) < 100 else x for x in offsets]  # (given in sequences' rows)
+    pools = [_guarded(t) for t in p.t[:4]]
+    p.t = [t for t, _ in pools] + p.t[4:]
+    lens_t, offsets_t = _i32(lens, dev), _i32(offsets, dev)
+    p.c = K.PagedKV(*p.t, lens_t, offsets_t, hd)
+    row = np.clip(offsets[:-1], 0, N)
+    n = np.clip(offsets[1:], row, N) - row
+    past = np.clip(lens, 0, cap)
+    rising = list(offsets) == sorted(offsets)
+    mine = sorted({i for a, m in zip(row, n) for i in range(a, a + m)})  # rows of a sequence
+
+    wide, out = (torch.full((N + 64, H * hd + 16), x, device=dev) for x in (float("nan"), 5.0))
+    q, o = wide[32:-32, 8:-8], out[32:-32, 8:-8]
+    qv = _rows(rng, N, H, hd) / 64
+    q.copy_(_cuda(qv.reshape(N, -1), dev))
+    K.attn_paged(p.c, H, q, o)
+    got = o.cpu().numpy().reshape(N, H, hd)
+    o[mine] = 5.0
+    assert (out == 5.0).all()
+    held = np.clip(offsets, 0, N)
+    if rising:
+        want, tol = p.o.attend(qv.astype(np.float64), past, held, H)
+        assert (np.abs(got - want) <= tol)[mine].all()
+
+    k, v = _rows(rng, N, kvh, hd), _rows(rng, N, kvh, hd)
+    turned = torch.full_like(wide, 5.0)
+    K.kv_append(p.c, _cuda(k.reshape(N, -1), dev), _cuda(v.reshape(N, -1), dev), None, H=H, q=q,
+                q_out=turned[32:-32, 8:-8])
+    inside = turned[32:-32, 8:-8]
+    if rising:
+        assert torch.equal(inside[mine], q[mine])
+    inside[mine] = 5.0
+    assert (turned == 5.0).all()
+    for t, big in pools:
+        assert (big[:64] == 0xa5).all() and (big[-64:] == 0xa5).all()
+    if rising:
+        p.o.append(k, v, past, held)
+        p.same()
