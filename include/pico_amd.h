@@ -284,7 +284,8 @@ struct PicoTensor* pico_rope(struct PicoTensor* x, const struct PicoRope* rope,
  * with a power of two for each page and head; `pages` pages for all sequences together.
  *   pico_kv_begin(kv, new_tokens);            new_tokens [sequences], 0 for one that waits
  *   per layer: o = pico_attention_cached(kv, layer, q, k, v, n_heads, rope)
- * pico_kv_begin: starts a step, whose rows are the new tokens, sequence after sequence;
+ * pico_kv_begin: starts a step, whose rows are the new tokens, sequence after sequence, and
+ *   which count as held from then on (pico_attention_cached of every layer writes them);
  *   gives sequences the pages they need.  Returns the number of rows, or -1 (too few pages
  *   are free, a sequence would pass max_length), the cache left as it was.  It copies to the
  *   device, so not under graph capture: a captured step is replayed after a pico_kv_begin
@@ -296,7 +297,8 @@ struct PicoTensor* pico_rope(struct PicoTensor* x, const struct PicoRope* rope,
  *   the cache's head h / (n_heads / kv_heads).  fp32 whatever the matmul precision, but for
  *   the cache's 8 bits.  For inference: no gradient passes through it.
  * pico_kv_length: tokens of a sequence, the present step's among them (-1: no such one).
- * pico_kv_drop: forgets a sequence, whose pages are free for the next step's. */
+ * pico_kv_drop: forgets a sequence, whose pages are free for the next step's.  It ends the
+ *   present step: pico_attention_cached is refused until the next pico_kv_begin. */
 struct PicoKVConfig {
     int layers;
     int kv_heads;

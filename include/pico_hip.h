@@ -725,7 +725,7 @@ int pk_gemm_experts_dw_f32(int64_t n, int64_t K, int64_t N, int64_t E, const int
  *   y1 = m*(x1*cos a - x2*sin a),  y2 = m*(x2*cos a + x1*sin a)
  * with m = magnitude; the other values are copied.  A pair is (i, i + rot/2) of the
  * head, or (2i, 2i + 1) when interleaved is not 0.  Angles are computed in 64 bits
- * (position 2^20 times 1 radian is off by 2^-24 of a turn in 32), their sine and cosine
+ * (position 2^20 times 1 radian is off by 2^-4 radians in 32), their sine and cosine
  * rounded once.
  * pk_rope_freqs writes the rot / 2 frequencies into HOST memory (a program copies them to
  * the device once): base^(-2i/rot), scaled for contexts longer than the trained one:
@@ -785,8 +785,9 @@ int pk_rope_f32(int64_t N, int64_t H, int64_t hd, const PkRope* rope, const int3
  *   its sequence, which the cache holds already; q, o [N, H*hd] with row strides ldq, ldo,
  *   head h reading the cache's head h / (H / kv_heads).  A token that finds no key gets
  *   zeros; rows of no sequence are left.  q enters the products as two f16 values of 22
- *   bits together, and so do the probabilities; what the cache holds is exact in f16, and
- *   sums are fp32.  pk_attn_paged_workspace(cache, N, H) bytes of device workspace (0:
+ *   bits together, and so do the probabilities (times their pages' 2^e) down to 2^-10 of a
+ *   row's largest; those below are off by up to 2^-32 of that.  What the cache holds is exact
+ *   in f16, and sums are fp32.  pk_attn_paged_workspace(cache, N, H) bytes of device workspace (0:
  *   none needed).  Sums in an order that the lengths and the sizes fix. */
 typedef struct PkKvCache {
     uint8_t *k, *v, *k_exp, *v_exp;

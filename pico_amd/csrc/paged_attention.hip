@@ -889,6 +889,8 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
     // against 92 us, with up to 60 119 against 116; one of 4000 with 256 61 against 59; 4 of 1900
     // with 100 35 against 45; one with 700 40 against 36.  16 heads on 2 of 64: 16 of 1000 with 100
     // 25 against 44, 4 of 500 with 300 17 against 28; 32 on 8: 8 of 100 with 200 26 against 19.
+    // The average is over all of the table's sequences, those that wait too: 1500 tokens behind
+    // 4000, 32 heads on 8 of 128, take 254 us alone and 489 among 64 sequences.
     const int64_t most = units > 32 ? 4096 : c->hd <= 64 ? 24576 : c->hd <= 128 ? 12288 : 8192;
     p.rows = N * group <= 96 * c->B || N * H <= most ? kFew : kRows;
     p.tiles = N * group / p.rows + some;
@@ -905,6 +907,8 @@ Plan plan(const PkKvCache* c, int64_t N, int64_t H) {
         // 2 of 4000 with 1024, 12 heads of 64: 4 parts 75, 2 96.  Long sequences of different
         // lengths in parts of 40 units, 3 at least, where there are more than run at once, which
         // levels them out: 8 up to 16000 with 256, 32 heads of 64: 4 parts 413, whole tiles 520.
+        // The parts are of what the table has room for, the lengths are not known here: 2 prompts
+        // of 256 tokens, 32 heads on 8 of 128, take 26 us with tables of 512 tokens, 74 of 131072.
         const int64_t sure = (N * group + kRows - 1) / kRows * c->kv_heads;
         auto parts = [&](int64_t blocks, int64_t each) {
             return blocks / sure < units / each ? blocks / sure : units / each;

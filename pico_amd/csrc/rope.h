@@ -27,8 +27,8 @@ __device__ __forceinline__ void rope_angle(int pos, double f, double m, float& c
     s = (float)(ds * m);
 }
 
-// (x1, x2) turned; each product rounded by itself, as the formula stands, so that a value
-// does not depend on which kernel turned it
+// (x1, x2) turned; each product rounded by itself, as the formula stands, so that the same
+// sine and cosine give the same value in every kernel
 __device__ __forceinline__ void rope_turn(float& x1, float& x2, float c, float s) {
 #pragma clang fp contract(off)
     const float y1 = x1 * c - x2 * s;
